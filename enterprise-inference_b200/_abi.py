@@ -115,6 +115,14 @@ SIGNATURES = {
     "b200_paged_attn_static_scratch_bytes": (_i64, []),
     "b200_paged_attn_decode_static": (C.c_int, [_vp, _i64, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32,
                                                 _i32, _i32, _f32, _vp]),
+    "b200_rope_kv_append_fp8": (C.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _vp]),
+    "b200_paged_attn_fp8_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "b200_paged_attn_decode_fp8": (C.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp,
+                                             _i64, _vp]),
+    "b200_paged_attn_prefill_fp8": (C.c_int, [_vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _i32, _f32,
+                                              _vp, _i64, _vp]),
+    "b200_verify_drafts_workspace_bytes": (_i64, [_i32, _i32]),
+    "b200_verify_drafts": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
     "b200_silu_mul": (C.c_int, [_vp, _vp, _i32, _i32, _vp]),
     "b200_argmax": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
     "b200_sample": (C.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

@@ -269,6 +269,60 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
                                   int64_t ldo, int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
                                   int32_t block_size, int32_t max_ctx_len, float scale, void* stream);
 
+/* ---- an 8-bit paged cache, and drafted decoding over it ------------------------------------------------------------
+ * The cache of a layer, caller-owned: k_codes, v_codes [n_blocks][n_kv_heads][block_size][128] e4m3, k_exps, v_exps
+ * [n_blocks][n_kv_heads][block_size] uint8.  A value is code * 2^(byte - 127): one exponent per token and kv head, the
+ * smallest e >= -100 with max |x| <= 448 * 2^e (every value is an exact bf16; relative error of a normal code at most
+ * 2^-4).  Byte 255: the row held an inf or a NaN; its codes are NaN.  129 bytes a row where bf16 takes 256.
+ * block_size is 16, 32, 64 or a multiple of 128; n_blocks * n_kv_heads * block_size < 2^31.  Codes are 16-byte aligned.
+ *
+ * (a4+a5) b200_rope_kv_append_fp8: NeoX RoPE of the q and k heads of qkv [T][ld] in fp32 with one rounding (where
+ * b200_rope_kv_append follows the image's bf16 arithmetic); q rows go to q_out [T][ldq] (which may be qkv itself: q is then
+ * rotated in place), k and v rows are quantised into the cache at slot_mapping[t].  qkv's k and v columns keep what they
+ * hold.  A row whose slot is negative or behind the cache is not stored (its q is rotated).  Slots of one call differ.
+ *
+ * (a6) b200_paged_attn_decode_fp8: attention of rows by themselves; b200_paged_attn_prefill_fp8: the same results for steps in
+ * which neighbouring rows belong to one sequence (drafts under verification, chunks of prompts): they share its keys and
+ * values.  Arguments as b200_paged_attn_decode / _prefill; up to 16 query heads to a kv head; scores, sums and softmax in
+ * fp32, weights of at least eight significant bits, one rounding of the result.  A row sees ctx_lens[t] tokens of its
+ * sequence (no more than bt_stride blocks of them): none gives zeros.  What lies behind them in a block is never looked at.  A block id outside
+ * [0, n_blocks) stands for keys and values of zero.  max_rows: a HOST bound on the rows of one sequence that follow one
+ * another in this step (0: not known): it only chooses the kernels.  The workspace has no state between calls.
+ *
+ * b200_verify_drafts: which drafted tokens the target keeps, and the token that follows them (speculative sampling: what comes
+ * out is distributed as the target's own draws).  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1 of target_logits
+ * (bf16 [n_rows][ldt]); row r gives the probabilities at the place of draft_tokens[r], a sequence's last row those behind
+ * its last draft (its draft_tokens entry is not read).  draft_logits (bf16 [n_rows][ldd], last rows not read): what the drafts
+ * were drawn from; NULL: a drafter without probabilities (each draft taken as certain).  With p, q the softmax of target and
+ * draft row over the sequence's temperature (filtered logits are -inf in both; NaN and +inf are not expected):
+ *   draft x is kept while uniforms[r][0] * q(x) < p(x); the first row r that is not, or the last one, draws the token
+ *   min { i : sum over j <= i of w_j > uniforms[r][1] * sum of w },  w = max(p - q, 0) for a refused draft (p where that
+ *   leaves nothing), p behind the last one; sums in 64 bits.
+ * temperature[s] <= 0 (or temperature NULL, uniforms then unused): a draft is kept if it is the row's argmax (ties: the lowest
+ * index), and the token is the argmax.  A draft outside [0, vocab) is refused; a row of nothing but -inf refuses and yields token 0.
+ * uniforms [n_rows][2] in [0, 1).  out_tokens[n_rows]: per sequence the kept drafts, the drawn token, then -1; out_accepted[s]:
+ * drafts kept.  A sequence without rows gets out_accepted 0; rows of no sequence stay as they are. */
+B200_API int b200_rope_kv_append_fp8(const void* qkv, int64_t ld, const int32_t* positions, const int32_t* slot_mapping,
+                            const void* cos_sin, void* q_out, int64_t ldq, void* k_codes, void* v_codes, void* k_exps,
+                            void* v_exps, int64_t n_blocks, int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
+                            int32_t block_size, void* stream);
+B200_API int64_t b200_paged_attn_fp8_workspace_bytes(int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads);
+B200_API int b200_paged_attn_decode_fp8(const void* q, int64_t ldq, const void* k_codes, const void* v_codes,
+                               const void* k_exps, const void* v_exps, int64_t n_blocks, const int32_t* block_table,
+                               int32_t bt_stride, const int32_t* row_to_seq, const int32_t* ctx_lens, void* out, int64_t ldo,
+                               int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t block_size, float scale,
+                               void* workspace, int64_t workspace_bytes, void* stream);
+B200_API int b200_paged_attn_prefill_fp8(const void* q, int64_t ldq, const void* k_codes, const void* v_codes,
+                                const void* k_exps, const void* v_exps, int64_t n_blocks, const int32_t* block_table,
+                                int32_t bt_stride, const int32_t* row_to_seq, const int32_t* ctx_lens, void* out, int64_t ldo,
+                                int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads, int32_t block_size,
+                                int32_t max_rows, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+B200_API int64_t b200_verify_drafts_workspace_bytes(int32_t n_rows, int32_t vocab);
+B200_API int b200_verify_drafts(const void* target_logits, int64_t ldt, const void* draft_logits, int64_t ldd,
+                       const int32_t* draft_tokens, const int32_t* row_starts, const float* temperature,
+                       const float* uniforms, int32_t n_seqs, int32_t n_rows, int32_t vocab, int32_t* out_tokens,
+                       int32_t* out_accepted, void* workspace, int64_t workspace_bytes, void* stream);
+
 /* (a8) out[T][I] = bf16(bf16(silu(g))*u), gu = [T][2I] gate|up ([V22] activation.py:137-141). */
 B200_API int b200_silu_mul(const void* gu, void* out, int32_t n_tokens, int32_t intermediate, void* stream);
 

@@ -1,0 +1,553 @@
+"""Drafted decoding over an 8-bit cache, operator by operator and together, against kv8_util's plain forms in 64 bits."""
+import pytest
+import torch
+
+import kv8_util as K
+from conftest import pkg
+
+pytestmark = pytest.mark.gpu
+DEV, BF, I32 = "cuda", torch.bfloat16, torch.int32
+
+
+def _lib():
+    abi = pkg("_abi")
+    return abi.lib(), abi.check
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _cos_sin(n):
+    ang = torch.arange(n).double()[:, None] * (500000.0 ** (-torch.arange(0, 128, 2).double() / 128))[None]
+    return torch.cat([ang.cos(), ang.sin()], 1).to(BF)
+
+
+def append(qkv, pos, slots, cos_sin, q_out, cache, hq, stream=None):
+    lib, check = _lib()
+    check(lib.b200_rope_kv_append_fp8(qkv.data_ptr(), qkv.stride(0), pos.data_ptr(), slots.data_ptr(), cos_sin.data_ptr(), q_out.data_ptr(), q_out.stride(0),
+                                      cache.k.data_ptr(), cache.v.data_ptr(), cache.ke.data_ptr(), cache.ve.data_ptr(), cache.n_blocks, qkv.shape[0], hq,
+                                      cache.hkv, cache.block, stream))
+
+
+def attend(q, cache, seq, ctx, out, hq, most=None, scale=128 ** -0.5, ws=None, stream=None):
+    """most None: rows by themselves."""
+    lib, check = _lib()
+    T = ctx.shape[0]
+    size = int(lib.b200_paged_attn_fp8_workspace_bytes(T, hq, cache.hkv))
+    ws = torch.full((size,), 0xff, dtype=torch.uint8, device=DEV) if ws is None else ws
+    lead = (q.data_ptr(), q.stride(0), cache.k.data_ptr(), cache.v.data_ptr(), cache.ke.data_ptr(), cache.ve.data_ptr(), cache.n_blocks, cache.bt.data_ptr(),
+            cache.bt.shape[1], _ptr(seq), ctx.data_ptr(), out.data_ptr(), out.stride(0), T, hq, cache.hkv, cache.block)
+    if most is None:
+        check(lib.b200_paged_attn_decode_fp8(*lead, scale, ws.data_ptr(), size, stream))
+    else:
+        check(lib.b200_paged_attn_prefill_fp8(*lead, most, scale, ws.data_ptr(), size, stream))
+    return ws
+
+
+def check_attention(out, q, cache, seq, ctx, scale=128 ** -0.5):
+    """Result rounded to bf16 (2^-8 of itself), weights of eight significant bits (2^-8 of each one's share) from scores and exponentials in fp32 (scores
+    below 64: 2^-12), the smallest weights of a tile in steps of 2^-22 (with codes up to 448 under 128 keys: 2^-14 of the largest value)."""
+    out, q = out.double().cpu(), q.cpu()
+    for t in range(len(ctx)):
+        want, share, top = K.attention(q[t], cache.rows[seq[t]], ctx[t], scale)
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * share + 2.0 ** -14 * top
+        off = (out[t] - want).abs() - bound
+        assert (off <= 0).all(), (t, ctx[t], float(off.max()), int(off.argmax()))
+
+
+# ---- appending -------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,hq,hkv,block", [(1, 32, 8, 128), (5, 4, 1, 16), (67, 40, 8, 64), (33, 7, 7, 32), (130, 28, 4, 256), (1, 1, 1, 128)])
+def test_append_quantises_what_rope_gives(T, hq, hkv, block):
+    g = torch.Generator().manual_seed(T * 31 + hq)
+    cache = K.Cache([], hkv, block, g, spare=(T + block - 1) // block + 2)
+    slots = torch.randperm(cache.n_blocks * block, generator=g)[:T].to(I32)
+    if T > 4:
+        slots[1], slots[3] = -1, cache.n_blocks * block   # rows that are not stored
+    pos = torch.randint(0, 4000, (T,), generator=g).to(I32)
+    x = torch.randn(T, hq + 2 * hkv, 128, generator=g) * torch.exp2(torch.randn(T, hq + 2 * hkv, 1, generator=g) * 4)
+    x[0, -1] = 0                                            # a row of zeros
+    if T > 30:
+        x[5, hq, 3], x[6, hq + hkv, 70], x[7, hq, 1] = float("inf"), float("nan"), float("-inf")
+        x[8, hq + hkv] *= 2.0 ** -130                       # below the smallest exponent
+        x[9, hq + hkv] = 3e38
+        x[10, hq + hkv] = 448 * 2.0 ** -5                   # a power of two times 448 takes that power
+        x[11, hq + hkv, :5] = torch.tensor([449.0, 450.0, -452.0, 17.0, 2.0 ** -12])
+    x, cos_sin = x.to(BF), _cos_sin(4000)
+    want_q = K.rope(x[:, :hq], pos, cos_sin).to(BF)
+    rows = torch.cat([K.rope(x[:, hq:hq + hkv], pos, cos_sin), x[:, hq + hkv:].float()], 1)
+    codes, exps = K.quantise(rows)
+    keep = {n: getattr(cache, n).clone() for n in ("k", "v", "ke", "ve")}
+    for t in range(T):
+        if 0 <= slots[t] < cache.n_blocks * block:
+            b, o = int(slots[t]) // block, int(slots[t]) % block
+            keep["k"][b, :, o], keep["ke"][b, :, o] = codes[t, :hkv], exps[t, :hkv]
+            keep["v"][b, :, o], keep["ve"][b, :, o] = codes[t, hkv:], exps[t, hkv:]
+    cache.to(DEV)
+    wide = torch.full((T, (hq + 2 * hkv) * 128 + 24), 7.0, dtype=BF)   # rows with something behind them
+    wide[:, :(hq + 2 * hkv) * 128] = x.reshape(T, -1)
+    qkv, before = wide.to(DEV), wide.clone()
+    q_out = torch.full((T, hq * 128 + 8), -3.0, dtype=BF, device=DEV)
+    dev = [t.to(DEV) for t in (pos, slots, cos_sin)]
+    append(qkv, *dev, q_out, cache, hq)
+    torch.cuda.synchronize()
+    for n, want in keep.items():
+        assert torch.equal(getattr(cache, n).cpu(), want), n
+    assert torch.equal(q_out[:, :hq * 128].cpu().reshape(T, hq, 128).view(torch.int16), want_q.view(torch.int16)) and bool((q_out[:, hq * 128:] == -3).all())
+    assert torch.equal(qkv.cpu().view(torch.int16), before.view(torch.int16))
+    append(qkv, *dev, qkv, cache, hq)   # q in place; k and v columns stay
+    torch.cuda.synchronize()
+    got = qkv.cpu()
+    assert torch.equal(got[:, :hq * 128].reshape(T, hq, 128).view(torch.int16), want_q.view(torch.int16))
+    assert torch.equal(got[:, hq * 128:].contiguous().view(torch.int16), before[:, hq * 128:].contiguous().view(torch.int16))
+    for n, want in keep.items():
+        assert torch.equal(getattr(cache, n).cpu(), want), n
+    # what is read back is within half a step of four significant bits, and a bf16
+    back = K.values(codes, exps)
+    fine = torch.isfinite(back)
+    assert ((back - rows.double()).abs() <= 2.0 ** -4 * rows.double().abs() + torch.exp2(exps.double() - 127)[..., None] * 2.0 ** -10)[fine].all()
+    assert torch.equal(back[fine], back[fine].to(BF).double())
+
+
+# ---- attention -------------------------------------------------------------------------------------------------------------
+
+def _rows(T, heads, g, size=2.0):
+    return (torch.randn(T, heads, 128, generator=g) * size).to(BF)
+
+
+def _on_device(q, extra=0):
+    T, heads, _ = q.shape
+    wide = torch.full((T, heads * 128 + extra), float("nan"), dtype=BF, device=DEV)
+    wide[:, :heads * 128] = q.reshape(T, -1).to(DEV)
+    return wide
+
+
+EDGES = [0, 1, 2, 15, 16, 17, 31, 33, 63, 64, 65, 127, 128, 129, 255, 256, 257, 500, 901]
+
+
+@pytest.mark.parametrize("hq,hkv,block", [(4, 1, 128), (32, 8, 128), (40, 8, 16), (8, 8, 32), (28, 4, 64), (32, 2, 256), (16, 8, 128), (64, 8, 128), (1, 1, 128), (13, 1, 128)])
+def test_rows_by_themselves(hq, hkv, block):
+    g = torch.Generator().manual_seed(hq * 100 + hkv + block)
+    cache = K.Cache(EDGES, hkv, block, g)
+    T = len(EDGES)
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q, 24), torch.full((T + 1, hq * 128 + 8), -5.0, dtype=BF, device=DEV)
+    ctx = torch.tensor(EDGES, dtype=I32, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, None, ctx, out, hq)
+    torch.cuda.synchronize()
+    assert bool((out[:, hq * 128:] == -5).all()) and bool((out[T] == -5).all())   # nothing but the rows themselves
+    check_attention(out[:T, :hq * 128].reshape(T, hq, 128), q, cache, list(range(T)), EDGES)
+
+
+@pytest.mark.parametrize("hq,hkv,ctxs", [(32, 8, [20011]), (8, 1, [70001, 3]), (64, 8, [9000, 1, 0, 5000, 700]), (16, 16, [4097])])
+def test_few_rows_over_long_contexts(hq, hkv, ctxs):
+    """Contexts cut into parts that are joined again."""
+    g = torch.Generator().manual_seed(hq + len(ctxs))
+    cache = K.Cache(ctxs, hkv, 128, g)
+    T = len(ctxs)
+    q = _rows(T, hq, g, 3.0)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, None, torch.tensor(ctxs, dtype=I32, device=DEV), out, hq)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hq, 128), q, cache, list(range(T)), ctxs)
+
+
+def _step(parts, before):
+    seq = [s for s, n in enumerate(parts) for _ in range(n)]
+    ctx = [b + i + 1 for n, b in zip(parts, before) for i in range(n)]
+    return seq, ctx
+
+
+STEPS = {
+    "drafts": ([5] * 7, [0, 1, 120, 126, 250, 700, 1300]),
+    "one row each": ([1] * 6, [0, 5, 127, 128, 300, 1000]),
+    "short and long": ([1, 3, 8, 9, 1, 70, 1, 33, 2], [900, 126, 0, 513, 63, 100, 1, 700, 0]),
+    "a chunk": ([300], [0]),
+    "a chunk behind a context": ([131], [1000]),
+    "long chunks": ([257, 190, 140], [77, 0, 1025]),
+}
+
+
+@pytest.mark.parametrize("name", sorted(STEPS))
+@pytest.mark.parametrize("hq,hkv,block", [(32, 8, 128), (8, 1, 16), (10, 2, 64), (3, 3, 128), (16, 1, 32), (28, 4, 128)])
+def test_rows_of_runs(name, hq, hkv, block):
+    parts, before = STEPS[name]
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(len(name) + hq * 7 + hkv)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, block, g)
+    T = len(seq)
+    q = _rows(T, hq, g)
+    qd = _on_device(q, 8)
+    cache.to(DEV)
+    sd, cd = torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV)
+    for most in (max(parts), 0):
+        out = torch.full((T + 1, hq * 128 + 16), -5.0, dtype=BF, device=DEV)
+        attend(qd, cache, sd, cd, out, hq, most)
+        torch.cuda.synchronize()
+        assert bool((out[:, hq * 128:] == -5).all()) and bool((out[T] == -5).all())
+        check_attention(out[:T, :hq * 128].reshape(T, hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("most", [None, 40])
+def test_contexts_that_do_not_rise_and_rows_without_any(most):
+    """A row's context is its own: padded rows see nothing, neighbouring rows of one sequence see what they say."""
+    hq, hkv = 8, 2
+    g = torch.Generator().manual_seed(5)
+    cache = K.Cache([900, 300], hkv, 128, g)
+    seq = [0] * 30 + [1] * 12
+    ctx = [900, 0, 3, 129, 128, 0, 0, 700, 1, 256] * 3 + [0] * 6 + [300, -4, 10, 11, 12, 0]
+    q = _rows(42, hq, g)
+    qd, out = _on_device(q), torch.full((42, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(42, hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("most", [None, 64])
+def test_scales_of_every_size(most):
+    """Rows of keys and values thousands of times larger than their neighbours, value rows of zeros, scores far apart, a negative scale."""
+    hq, hkv, n = 8, 2, 700
+    g = torch.Generator().manual_seed(9)
+    cache = K.Cache([n], hkv, 128, g, spread=5.0)
+    for h in range(hkv):   # some value rows of zeros, in the cache and in the oracle's copy
+        for t in range(0, n, 7):
+            b, o = int(cache.bt[0, t // 128]), t % 128
+            cache.v[b, h, o] = 0
+            cache.ve[b, h, o] = 27
+            cache.rows[0][1][t, h] = 0
+    T = 40
+    seq, ctx = [0] * T, list(range(n - T + 1, n + 1))
+    q = _rows(T, hq, g, 0.3)
+    q[3] = 0
+    qd = _on_device(q)
+    cache.to(DEV)
+    for scale in (128 ** -0.5, -0.02, 0.0):
+        out = torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+        attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most, scale)
+        torch.cuda.synchronize()
+        got, qc = out.double().cpu().reshape(T, hq, 128), q
+        for t in range(T):
+            want, share, top = K.attention(qc[t], cache.rows[0], ctx[t], scale)
+            # scores up to some thousands: fp32 holds them to 2^-23 of themselves, which the weights take as a relative error
+            k = cache.rows[0][0][:ctx[t]].repeat_interleave(hq // hkv, 1)
+            s = (torch.einsum("hd,chd->hc", q[t].double().abs(), k.abs()) * abs(scale)).amax(-1, keepdim=True)
+            bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12 + 2 * s * 2.0 ** -22) * share + 2.0 ** -14 * top
+            assert ((got[t] - want).abs() <= bound).all(), (t, scale)
+
+
+@pytest.mark.parametrize("most", [None, 64])
+def test_keys_that_are_not_numbers_reach_the_rows_that_see_them(most):
+    hq, hkv = 4, 1
+    g = torch.Generator().manual_seed(13)
+    cache = K.Cache([300], hkv, 128, g)
+    b, o = int(cache.bt[0, 1]), 200 - 128
+    cache.ke[b, 0, o], cache.k[b, 0, o] = 255, 0x7f
+    T = 64
+    ctx = list(range(170, 170 + T))
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.zeros(T, hq * 128, dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.zeros(T, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    sees = torch.tensor([c > 200 for c in ctx])
+    got = out.cpu().reshape(T, hq, 128)
+    assert bool(torch.isnan(got[sees]).all()) and bool(torch.isfinite(got[~sees]).all())
+
+
+@pytest.mark.parametrize("most", [None, 64])
+@pytest.mark.parametrize("block", [16, 128])
+def test_block_ids_outside_the_cache_stand_for_zeros(most, block):
+    hq, hkv = 8, 2
+    g = torch.Generator().manual_seed(17)
+    cache = K.Cache([400, 400], hkv, block, g)
+    for s, at, bad in ((0, 1, -1), (0, 2, 2 ** 31 - 1), (1, 0, cache.n_blocks), (1, 2, -2 ** 31)):
+        cache.bt[s, at] = bad
+        for x in cache.rows[s]:
+            x[at * block:(at + 1) * block] = 0
+    T = 40
+    seq, ctx = [0] * 20 + [1] * 20, list(range(380, 400)) + list(range(1, 400, 20))
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hq, 128), q, cache, seq, ctx)
+
+
+def test_contexts_end_with_the_block_table():
+    hq, hkv = 8, 2
+    g = torch.Generator().manual_seed(19)
+    cache = K.Cache([384], hkv, 128, g)
+    cache.bt = cache.bt[:, :3].contiguous()
+    q = _rows(3, hq, g)
+    cache.to(DEV)
+    for most in (None, 3):
+        qd, out = _on_device(q), torch.full((3, hq * 128), float("nan"), dtype=BF, device=DEV)
+        attend(qd, cache, torch.zeros(3, dtype=I32, device=DEV), torch.tensor([384, 385, 2 ** 31 - 1], dtype=I32, device=DEV), out, hq, most)
+        torch.cuda.synchronize()
+        check_attention(out.reshape(3, hq, 128), q, cache, [0] * 3, [384] * 3)
+
+
+@pytest.mark.parametrize("most", [None, 5, 0])
+def test_attention_in_graphs_and_on_other_streams(most):
+    """Captured once, replayed over new inputs; two streams at a time with a workspace each; the same bits every time."""
+    hq, hkv = 32, 8
+    parts, before = [5] * 12, [40 * i * i % 3000 for i in range(12)]
+    if most == 0:
+        parts[3], before[3] = 150, 20
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(23)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 128, g).to(DEV)
+    T = len(seq)
+    sd, cd = torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV)
+    q1, q2 = _rows(T, hq, g), _rows(T, hq, g)
+    want = []
+    for q in (q1, q2):
+        out = torch.empty(T, hq * 128, dtype=BF, device=DEV)
+        attend(_on_device(q), cache, sd, cd, out, hq, most)
+        torch.cuda.synchronize()
+        want.append(out.clone())
+    check_attention(want[0].reshape(T, hq, 128), q1, cache, seq, ctx)
+    qd, out = _on_device(q1), torch.zeros(T, hq * 128, dtype=BF, device=DEV)
+    side = torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        ws = attend(qd, cache, sd, cd, out, hq, most, ws=None, stream=torch.cuda.current_stream().cuda_stream)
+    for q, w in ((q1, want[0]), (q2, want[1]), (q1, want[0])):
+        qd.copy_(q.reshape(T, -1))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.view(torch.int16), w.view(torch.int16))
+    del ws
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs, qs = [torch.zeros(T, hq * 128, dtype=BF, device=DEV) for _ in range(2)], [_on_device(q1), _on_device(q2)]
+    lib, _ = _lib()
+    size = int(lib.b200_paged_attn_fp8_workspace_bytes(T, hq, hkv))
+    spaces = [torch.zeros(size, dtype=torch.uint8, device=DEV) for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        for i, st in enumerate(streams):
+            attend(qs[i], cache, sd, cd, outs[i], hq, most, ws=spaces[i], stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(outs[i].view(torch.int16), want[i].view(torch.int16))
+
+
+# ---- checking drafts -------------------------------------------------------------------------------------------------------
+
+def check_drafts(target, draft, tokens, starts, temperature, uniforms, vocab=None, stream=None):
+    lib, check = _lib()
+    n, V = target.shape[0], vocab or target.shape[1]
+    size = int(lib.b200_verify_drafts_workspace_bytes(n, V))
+    ws = torch.full((max(size, 16),), 0xff, dtype=torch.uint8, device=DEV)
+    out = torch.full((n,), -9, dtype=I32, device=DEV)
+    kept = torch.full((len(starts) - 1,), -9, dtype=I32, device=DEV)
+    keep = [tokens.to(I32).to(DEV), torch.tensor(starts, dtype=I32, device=DEV), None if temperature is None else temperature.float().to(DEV),
+            None if uniforms is None else uniforms.float().contiguous().to(DEV)]
+    check(lib.b200_verify_drafts(target.data_ptr(), target.stride(0), _ptr(draft), draft.stride(0) if draft is not None else 0, keep[0].data_ptr(),
+                                 keep[1].data_ptr(), _ptr(keep[2]), _ptr(keep[3]), len(starts) - 1, n, V, out.data_ptr(), kept.data_ptr(), ws.data_ptr(), size,
+                                 stream))
+    torch.cuda.synchronize()
+    return out.long().cpu(), kept.long().cpu()
+
+
+def _drafts(parts, V, g, noise=0.5, near=True):
+    n = sum(parts)
+    target = (torch.randn(n, V, generator=g) * 2.5).to(BF)
+    draft = (target.float() + torch.randn(n, V, generator=g) * noise).to(BF)
+    gumbel = -torch.log(-torch.log(torch.rand(n, V, generator=g).clamp(1e-9, 1 - 1e-7)))
+    tokens = ((draft.float() if near else torch.zeros(n, V)) + gumbel).argmax(1)
+    starts = [0]
+    for p in parts:
+        starts.append(starts[-1] + p)
+    return target, draft, tokens, starts
+
+
+@pytest.mark.parametrize("V", [1, 2, 7, 300, 1024, 1027, 5000, 16032, 40001])
+@pytest.mark.parametrize("probs", [True, False])
+def test_drafts_kept_and_drawn(V, probs):
+    g = torch.Generator().manual_seed(V * 2 + probs)
+    parts = [5, 1, 0, 3, 9, 2, 0, 6]
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    temperature = torch.tensor([1.0, 0.7, 1.0, 0.0, 0.9, 2.5, 1.0, 0.3])
+    uniforms = torch.rand(len(tokens), 2, generator=g)
+    uniforms[0], uniforms[5, 1], uniforms[3, 1] = 0.0, 0.0, 1 - 2.0 ** -24
+    want, kept, margins = K.verify(target, draft if probs else None, tokens, starts, temperature, uniforms)
+    assert all(m > 1e-5 for m in margins)   # no decision of these inputs is nearer to its limit than the roundings it may have
+    got = check_drafts(target.to(DEV), draft.to(DEV) if probs else None, tokens, starts, temperature, uniforms)
+    assert torch.equal(got[1], kept)
+    assert torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("V", [1024, 33333])
+def test_greedy_drafts(V):
+    """No temperatures: kept while they are the first of the largest logits."""
+    g = torch.Generator().manual_seed(V)
+    parts = [6] * 9 + [1]
+    target, _, tokens, starts = _drafts(parts, V, g)
+    best = target.double().argmax(1)
+    for r in range(len(tokens)):
+        tie = int(torch.randint(0, V, (1,), generator=g))
+        target[r, tie] = target[r].max()          # a second largest entry: the lowest index counts
+        tokens[r] = min(tie, int(best[r])) if r % 4 else max(tie, int(best[r]))
+    want, kept, _ = K.verify(target, None, tokens, starts, None, None)
+    got = check_drafts(target.to(DEV), None, tokens, starts, None, None)
+    assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+    assert 0 < int(kept.sum()) < len(tokens) - 10
+
+
+def test_filtered_and_empty_rows():
+    """Logits of -inf: filtered ones, all but one, all of them; drafts outside the vocabulary; distributions that are the same."""
+    V, g = 3001, torch.Generator().manual_seed(3)
+    parts = [4] * 10
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    inf = float("-inf")
+    for x in (target, draft):
+        x[0:8] = torch.where(torch.rand(8, V, generator=g) < 0.99, inf, x[0:8].float()).to(BF)   # few tokens left, each row its own
+    target[8:12] = inf
+    target[8:12, 17] = -3.0                      # one token left
+    tokens[8:11] = torch.tensor([17, 17, 5])
+    target[13] = inf                             # nothing left under a draft
+    tokens[12:16] = target[12:16].double().argmax(1)
+    target[19] = inf                             # nothing left behind the last draft
+    draft[16:20] = target[16:20]
+    tokens[20], tokens[25], tokens[28] = -1, V, 2 ** 31 - 1
+    draft[32:34] = inf                           # a drafter that gives nothing any probability
+    draft[36:39] = target[36:39]                 # the target's own distribution: everything is kept
+    temperature = torch.full((10,), 0.8)
+    temperature[5] = 0.0
+    uniforms = torch.rand(40, 2, generator=g)
+    uniforms[12:19, 0] = 0.0
+    for d in (draft, None):
+        want, kept, margins = K.verify(target, d, tokens, starts, temperature, uniforms)
+        assert all(m > 1e-5 for m in margins if m > 0)
+        got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
+        assert torch.equal(got[1], kept), (got[1], kept)
+        assert torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("shift", [0, 1, 3, 8])
+def test_rows_at_any_stride_and_address(shift):
+    V, g = 2051, torch.Generator().manual_seed(shift)
+    parts = [3, 4, 1, 5]
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    uniforms, temperature = torch.rand(len(tokens), 2, generator=g), torch.tensor([1.0, 0.5, 1.0, 0.0])
+    want, kept, margins = K.verify(target, draft, tokens, starts, temperature, uniforms)
+    assert all(m > 1e-5 for m in margins)
+    big = [torch.full((len(tokens), V + 13 + shift), float("nan"), dtype=BF, device=DEV) for _ in range(2)]
+    views = []
+    for b, x, at in zip(big, (target, draft), (shift, 5)):
+        b[:, at:at + V] = x.to(DEV)
+        views.append(b[:, at:at + V])
+    got = check_drafts(*views, tokens, starts, temperature, uniforms, V)
+    assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+def test_rows_of_no_sequence_stay():
+    V, g = 512, torch.Generator().manual_seed(1)
+    target, draft, tokens, starts = _drafts([2, 3, 4], V, g)
+    uniforms = torch.rand(9, 2, generator=g)
+    got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts[:3], torch.ones(2), uniforms)
+    want, kept, _ = K.verify(target[:5], draft[:5], tokens[:5], starts[:3], torch.ones(2), uniforms)
+    assert torch.equal(got[0][:5], want) and bool((got[0][5:] == -9).all()) and torch.equal(got[1], kept)
+
+
+def test_what_comes_out_is_distributed_as_the_target():
+    """One row and the one behind it, 20000 sequences with numbers of their own over 12 tokens: counts within 5 standard deviations."""
+    V, n, g = 12, 20000, torch.Generator().manual_seed(8)
+    target, draft = (torch.randn(2, V, generator=g) * 1.5).to(BF), (torch.randn(2, V, generator=g) * 1.5).to(BF)
+    p = torch.softmax(target.double(), 1)
+    x = torch.multinomial(torch.softmax(draft[0].double(), 0), n, True, generator=g)
+    tokens = torch.stack([x, torch.zeros_like(x)], 1).reshape(-1)
+    out, kept = check_drafts(target.repeat(n, 1).to(DEV), draft.repeat(n, 1).to(DEV), tokens, list(range(0, 2 * n + 1, 2)), torch.ones(n),
+                             torch.rand(2 * n, 2, generator=g))
+    first, second = out.reshape(n, 2)[:, 0], out.reshape(n, 2)[:, 1]
+    both = second[second >= 0]
+    assert int(kept.sum()) == len(both)
+    for got, want, m in ((first, p[0], n), (both, p[1], len(both))):
+        counts = torch.bincount(got, minlength=V).double()
+        assert ((counts - m * want).abs() <= 5 * (m * want * (1 - want)).sqrt() + 1).all()
+
+
+# ---- together --------------------------------------------------------------------------------------------------------------
+
+def test_a_drafted_step():
+    """Rows appended, attended, turned into logits and checked, over several steps that keep what was kept: one graph, and the cache of a program that
+    quantises by itself."""
+    hq, hkv, block, V, per, S = 8, 2, 64, 700, 4, 6
+    g = torch.Generator().manual_seed(77)
+    lens = torch.tensor([3, 60, 61, 127, 200, 0])
+    total = 300
+    cache = K.Cache([int(n) for n in lens], hkv, block, g, spare=0)
+    need = (total + block - 1) // block
+    # every sequence owns its blocks from the start
+    n_blocks = S * need
+    k, v = (torch.full((n_blocks, hkv, block, 128), 0x7f, dtype=torch.uint8) for _ in range(2))
+    ke, ve = (torch.full((n_blocks, hkv, block), 255, dtype=torch.uint8) for _ in range(2))
+    bt = torch.randperm(n_blocks, generator=g).reshape(S, need).to(I32)
+    for s in range(S):
+        for b in range((int(lens[s]) + block - 1) // block):
+            for dst, src in ((k, cache.k), (v, cache.v), (ke, cache.ke), (ve, cache.ve)):
+                dst[bt[s, b]] = src[cache.bt[s, b]]
+    cache.k, cache.v, cache.ke, cache.ve, cache.bt, cache.n_blocks = k, v, ke, ve, bt, n_blocks
+    cache.to(DEV)
+    history = [[x.clone() for x in r] for r in cache.rows]
+    cos_sin, head = _cos_sin(total), torch.randn(hq * 128, V, generator=g) * 0.3
+    cs, hd = cos_sin.to(DEV), head.to(DEV)
+    T = S * per
+    n_w = (hq + 2 * hkv) * 128
+    qkv = torch.zeros(T, n_w, dtype=BF, device=DEV)
+    q, att = (torch.zeros(T, hq * 128, dtype=BF, device=DEV) for _ in range(2))
+    pos, slots, ctx, tokens = (torch.zeros(T, dtype=I32, device=DEV) for _ in range(4))
+    seq = torch.arange(S).repeat_interleave(per)
+    sd, starts = seq.to(I32).to(DEV), torch.arange(0, T + 1, per).to(I32).to(DEV)
+    temp, uni = torch.full((S,), 0.9).to(DEV), torch.zeros(T, 2, device=DEV)
+    logits, out, kept = torch.zeros(T, V, dtype=BF, device=DEV), torch.zeros(T, dtype=I32, device=DEV), torch.zeros(S, dtype=I32, device=DEV)
+    lib, check = _lib()
+    wa = torch.zeros(int(lib.b200_paged_attn_fp8_workspace_bytes(T, hq, hkv)), dtype=torch.uint8, device=DEV)
+    wv = torch.zeros(max(16, int(lib.b200_verify_drafts_workspace_bytes(T, V))), dtype=torch.uint8, device=DEV)
+
+    def step(stream):
+        append(qkv, pos, slots, cs, q, cache, hq, stream)
+        attend(q, cache, sd, ctx, att, hq, per, ws=wa, stream=stream)
+        logits.copy_((att.float() @ hd).to(BF))
+        check(lib.b200_verify_drafts(logits.data_ptr(), V, None, 0, tokens.data_ptr(), starts.data_ptr(), temp.data_ptr(), uni.data_ptr(), S, T, V, out.data_ptr(),
+                                     kept.data_ptr(), wv.data_ptr(), wv.numel(), stream))
+
+    slots.fill_(-1)
+    step(None)   # rows that are not stored and see nothing: warms the library up
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(torch.cuda.current_stream().cuda_stream)
+    lens = lens.clone()
+    for it in range(4):
+        x = torch.randn(T, hq + 2 * hkv, 128, generator=g).to(BF)
+        p = lens[seq] + torch.arange(T) % per
+        sl = cache.bt.cpu()[seq, p // block].long() * block + p % block
+        u = torch.rand(T, 2, generator=g)
+        u[:, 0] *= 0.02                          # some drafts are kept
+        drafts = torch.randint(0, V, (T,), generator=g)
+        for dst, src in ((qkv, x.reshape(T, -1)), (pos, p), (slots, sl), (ctx, p + 1), (tokens, drafts), (uni, u)):
+            dst.copy_(src)
+        graph.replay()
+        torch.cuda.synchronize()
+        rows = torch.cat([K.rope(x[:, hq:hq + hkv], p, cos_sin), x[:, hq + hkv:].float()], 1)
+        vals = K.values(*K.quantise(rows))
+        want_q = K.rope(x[:, :hq], p, cos_sin).to(BF)
+        assert torch.equal(q.cpu().reshape(T, hq, 128).view(torch.int16), want_q.view(torch.int16))
+        cache.rows = []
+        for s in range(S):
+            n = int(lens[s])
+            cache.rows.append([torch.cat([history[s][i][:n], vals[seq == s][:, i * hkv:(i + 1) * hkv]]) for i in range(2)])
+        check_attention(att.reshape(T, hq, 128), want_q, cache, seq.tolist(), (p + 1).tolist())
+        want, took, margins = K.verify(logits.cpu(), None, drafts, list(range(0, T + 1, per)), temp.cpu(), u)
+        assert all(m > 1e-5 for m in margins)
+        assert torch.equal(out.long().cpu(), want) and torch.equal(kept.long().cpu(), took)
+        for s in range(S):
+            history[s] = cache.rows[s]
+        lens = lens + took + 1                   # refused rows are overwritten by the next step
