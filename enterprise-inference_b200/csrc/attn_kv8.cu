@@ -1,68 +1,96 @@
-// Paged attention over the 8-bit cache (kv8.cuh): a warp per (row, kv head) walks the context token by token, all G query heads at once.
-#include "kv8.cuh"
+// Host side of the attention over the 8-bit cache: maps, workspace, routes, and the joining of parts.
+#include <algorithm>
+
+#include "attn_kv8.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int kMostHeads = 16;
-
-__device__ __forceinline__ void codes4(uint32_t c, float (&x)[4]) {
-  const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c & 0xffffu), __NV_E4M3),
-                    hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c >> 16), __NV_E4M3);
-  const float2 a = __half22float2(__half2(lo)), b = __half22float2(__half2(hi));
-  x[0] = a.x, x[1] = a.y, x[2] = b.x, x[3] = b.y;
-}
-
-__global__ void __launch_bounds__(32) paged_attn_fp8_kernel(const Kv8Attn a) {
+// an item that several CTAs share, column by column: out = sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m)
+__global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Params p) {
   pdl_wait();
   pdl_launch_dependents();
-  const int t = blockIdx.x, kvh = blockIdx.y, lane = threadIdx.x, G = a.hq / a.hkv;
-  const int seq = a.row_to_seq ? a.row_to_seq[t] : t;
-  const int ctx = (int)min((int64_t)a.ctx_lens[t], (int64_t)a.bt_stride * a.block_size);
-  float q[kMostHeads][4], o[kMostHeads][4] = {}, m[kMostHeads], l[kMostHeads] = {};
-#pragma unroll
-  for (int g = 0; g < kMostHeads; ++g) {
-    m[g] = -INFINITY;
-    if (g >= G) continue;
-    const uint2 v = *reinterpret_cast<const uint2*>(a.q + (int64_t)t * a.ldq + (kvh * G + g) * kHeadDim + 4 * lane);
-    q[g][0] = bf16lo(v.x), q[g][1] = bf16hi(v.x), q[g][2] = bf16lo(v.y), q[g][3] = bf16hi(v.y);
-  }
-  for (int j = 0; j < ctx; ++j) {
-    const int blk = a.block_table[(int64_t)seq * a.bt_stride + j / a.block_size];
-    float k[4] = {}, v[4] = {}, ks = 0.f, vs = 0.f;
-    if (blk >= 0 && blk < a.n_blocks) {
-      const int64_t cell = ((int64_t)blk * a.hkv + kvh) * a.block_size + j % a.block_size;
-      codes4(*reinterpret_cast<const uint32_t*>(a.kc + cell * kHeadDim + 4 * lane), k);
-      codes4(*reinterpret_cast<const uint32_t*>(a.vc + cell * kHeadDim + 4 * lane), v);
-      ks = kv8_scale(a.ke[cell]);
-      vs = kv8_scale(a.ve[cell]);
+  const Kv8Cut cut = p.cuts[blockIdx.x];
+  const int G = p.hq / p.hkv, d = threadIdx.x;
+  if (cut.parts < 2) return;
+  for (int c = blockIdx.y; c < cut.nrows * G; c += gridDim.y) {
+    auto part = [&](int i) { return p.part + ((int64_t)(2 * (blockIdx.x + i) + (i == 0)) * kKv8Cols + c) * kKv8PartFloats; };
+    float m = -INFINITY, l = 0.f, a = 0.f;
+    for (int i = 0; i < cut.parts; ++i) m = fmaxf(m, part(i)[128]);
+    for (int i = 0; i < cut.parts; ++i) {
+      const float* x = part(i);
+      const float f = m == -INFINITY ? 1.f : tc::exp2_fast(x[128] - m);
+      l += x[129] * f;
+      a += x[d] * f;
     }
-#pragma unroll
-    for (int g = 0; g < kMostHeads; ++g) {
-      if (g >= G) continue;
-      const float s = warp_sum(q[g][0] * k[0] + q[g][1] * k[1] + q[g][2] * k[2] + q[g][3] * k[3]) * ks * a.scale;
-      const float mn = fmaxf(m[g], s), f = mn == -INFINITY ? 1.f : expf(m[g] - mn), p = mn == -INFINITY ? 0.f : expf(s - mn);
-      m[g] = mn;
-      l[g] = l[g] * f + p;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) o[g][i] = o[g][i] * f + p * (v[i] * vs);
-    }
+    p.out[(int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim + d] = __float2bfloat16_rn(l == 0.f ? 0.f : a / l);
   }
-#pragma unroll
-  for (int g = 0; g < kMostHeads; ++g) {
-    if (g >= G) continue;
-    const float inv = l[g] == 0.f ? 0.f : 1.f / l[g];
-    *reinterpret_cast<uint2*>(a.out + (int64_t)t * a.ldo + (kvh * G + g) * kHeadDim + 4 * lane) =
-        make_uint2(pack_bf16(o[g][0] * inv, o[g][1] * inv), pack_bf16(o[g][2] * inv, o[g][3] * inv));
-  }
+}
+
+constexpr int64_t kCutBytes = (kNumSMs * sizeof(Kv8Cut) + 255) / 256 * 256;
+constexpr int64_t kPartBytes = (int64_t)kNumSMs * 2 * kKv8Cols * kKv8PartFloats * 4;
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                  const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static const EncodeTiledFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess)
+      return reinterpret_cast<EncodeTiledFn>(p);
+    cudaGetLastError();
+    return EncodeTiledFn(nullptr);
+  }();
+  return fn;
 }
 
 }  // namespace
 
-int64_t paged_attn_fp8_workspace_bytes(int T, int hq, int hkv) { return 16; }
+// encoded anew by every call (1 us): a map that is kept would go by the cache's address
+int kv8_maps(const Kv8Attn& a, int box_rows, Kv8Maps* m) {
+  const EncodeTiledFn fn = encode_fn();
+  B200_REQUIRE(fn != nullptr, B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t cells = (cuuint64_t)a.n_blocks * a.hkv * a.block_size, dims[2] = {kHeadDim, cells}, stride[1] = {kHeadDim};
+  const cuuint32_t box[2] = {kHeadDim, (cuuint32_t)box_rows}, one[2] = {1, 1};
+  CUresult r = CUDA_SUCCESS;
+  const std::pair<CUtensorMap*, const uint8_t*> codes[2] = {{&m->k, a.kc}, {&m->v, a.vc}};
+  for (int i = 0; i < 2 && r == CUDA_SUCCESS; ++i)
+    r = fn(codes[i].first, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(codes[i].second), dims, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  B200_REQUIRE(r == CUDA_SUCCESS, B200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %lld rows", (int)r, (long long)cells);
+  return B200_OK;
+}
+
+int64_t paged_attn_fp8_workspace_bytes(int T, int hq, int hkv) { return kCutBytes + kPartBytes; }
 
 int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaStream_t s) {
-  B200_CUDA(launch(paged_attn_fp8_kernel, dim3(a.T, a.hkv), dim3(32), 0, s, a));
+  Kv8Maps maps;
+  if (const int rc = kv8_maps(a, std::min(a.block_size, kKv8Tile), &maps)) return rc;
+  const int G = a.hq / a.hkv;
+  Kv8Params p = {};
+  p.q = a.q;
+  p.ldq = a.ldq;
+  p.block_table = a.block_table;
+  p.row_to_seq = a.row_to_seq;
+  p.ctx_lens = a.ctx_lens;
+  p.ke = a.ke;
+  p.ve = a.ve;
+  p.out = a.out;
+  p.ldo = a.ldo;
+  p.cuts = static_cast<Kv8Cut*>(ws);
+  p.part = reinterpret_cast<float*>(static_cast<char*>(ws) + kCutBytes);
+  p.status = wait_status_word();
+  p.n_blocks = a.n_blocks;
+  p.bt_stride = a.bt_stride;
+  p.T = a.T;
+  p.hq = a.hq;
+  p.hkv = a.hkv;
+  p.block_size = a.block_size;
+  p.scale2 = a.scale * 1.4426950408889634f;
+  p.group_rows = most == 1 ? 1 : most > 0 && most * G <= kKv8Cols ? most : kKv8Cols / G;
+  if (const int rc = kv8_cols_launch(maps, p, p.group_rows * G, kNumSMs, s)) return rc;
+  const PdlScope join;
+  B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs, std::min(p.group_rows * G, 8)), dim3(128), 0, s, p));
   return B200_OK;
 }
 

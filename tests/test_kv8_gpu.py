@@ -239,13 +239,14 @@ def test_scales_of_every_size(most):
             assert ((got[t] - want).abs() <= bound).all(), (t, scale)
 
 
-@pytest.mark.parametrize("most", [None, 64])
-def test_keys_that_are_not_numbers_reach_the_rows_that_see_them(most):
+@pytest.mark.parametrize("most", [None, 6, 64])
+@pytest.mark.parametrize("keys", [True, False])
+def test_rows_that_are_not_numbers_reach_the_rows_that_see_them(most, keys):
     hq, hkv = 4, 1
     g = torch.Generator().manual_seed(13)
     cache = K.Cache([300], hkv, 128, g)
     b, o = int(cache.bt[0, 1]), 200 - 128
-    cache.ke[b, 0, o], cache.k[b, 0, o] = 255, 0x7f
+    (cache.ke if keys else cache.ve)[b, 0, o], (cache.k if keys else cache.v)[b, 0, o] = 255, 0x7f
     T = 64
     ctx = list(range(170, 170 + T))
     q = _rows(T, hq, g)
