@@ -7,23 +7,30 @@ namespace b200 {
 namespace {
 
 // an item that several CTAs share, column by column: out = sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m)
-__global__ void __launch_bounds__(128) kv8_join_kernel(const Kv8Params p) {
+// (a warp a column, four entries a lane)
+__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Params p) {
   pdl_wait();
   pdl_launch_dependents();
   const Kv8Cut cut = p.cuts[blockIdx.x];
-  const int G = p.hq / p.hkv, d = threadIdx.x;
+  const int G = p.hq / p.hkv, lane = threadIdx.x & 31;
   if (cut.parts < 2) return;
-  for (int c = blockIdx.y; c < cut.nrows * G; c += gridDim.y) {
+  for (int c = blockIdx.y * 8 + (threadIdx.x >> 5); c < cut.nrows * G; c += 8 * gridDim.y) {
     auto part = [&](int i) { return p.part + ((int64_t)(2 * (blockIdx.x + i) + (i == 0)) * kKv8Cols + c) * kKv8PartFloats; };
-    float m = -INFINITY, l = 0.f, a = 0.f;
-    for (int i = 0; i < cut.parts; ++i) m = fmaxf(m, part(i)[128]);
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < cut.parts; i += 32) m = fmaxf(m, part(i)[128]);
+    m = warp_max(m);
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
     for (int i = 0; i < cut.parts; ++i) {
       const float* x = part(i);
       const float f = m == -INFINITY ? 1.f : tc::exp2_fast(x[128] - m);
+      const float4 v = reinterpret_cast<const float4*>(x)[lane];
       l += x[129] * f;
-      a += x[d] * f;
+      a.x += v.x * f, a.y += v.y * f, a.z += v.z * f, a.w += v.w * f;
     }
-    p.out[(int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim + d] = __float2bfloat16_rn(l == 0.f ? 0.f : a / l);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    *reinterpret_cast<uint2*>(p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim + 4 * lane) =
+        make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
   }
 }
 
@@ -64,6 +71,8 @@ int kv8_maps(const Kv8Attn& a, int box_rows, Kv8Maps* m) {
 int64_t paged_attn_fp8_workspace_bytes(int T, int hq, int hkv) { return kCutBytes + kPartBytes; }
 
 int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaStream_t s) {
+  B200_REQUIRE((int64_t)a.T * a.hkv * (((int64_t)a.bt_stride * a.block_size + kKv8Tile - 1) / kKv8Tile) < 0x7fffffffll, B200_ERR_UNSUPPORTED,
+               "paged_attn_fp8: %d rows of up to %lld tokens", a.T, (long long)a.bt_stride * a.block_size);
   Kv8Maps maps;
   if (const int rc = kv8_maps(a, std::min(a.block_size, kKv8Tile), &maps)) return rc;
   const int G = a.hq / a.hkv;
@@ -90,7 +99,7 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
   p.group_rows = most == 1 ? 1 : most > 0 && most * G <= kKv8Cols ? most : kKv8Cols / G;
   if (const int rc = kv8_cols_launch(maps, p, p.group_rows * G, kNumSMs, s)) return rc;
   const PdlScope join;
-  B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs, std::min(p.group_rows * G, 8)), dim3(128), 0, s, p));
+  B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs, (p.group_rows * G + 7) / 8), dim3(256), 0, s, p));
   return B200_OK;
 }
 

@@ -7,7 +7,7 @@ namespace b200 {
 
 constexpr int kKv8Tile = 128;          // tokens of a tile
 constexpr int kKv8Cols = 32;           // (row, head) pairs of a group at most
-constexpr int kKv8PartFloats = 130;    // of a pair in a part: 128 sums, their maximum (log2 domain), the denominator
+constexpr int kKv8PartFloats = 132;    // of a pair in a part: 128 sums, their maximum (log2 domain), the denominator
 
 // rows [row0, row0 + nrows) of one sequence that share its keys and values; nrows 0: none
 struct Kv8Group {
@@ -47,13 +47,28 @@ __device__ __forceinline__ int kv8_ctx(const Kv8Params& p, int row) {
   return (int)min((int64_t)__ldg(p.ctx_lens + row), (int64_t)p.bt_stride * p.block_size);
 }
 
+// the warp's largest value; NaN if one is
+__device__ __forceinline__ float warp_max_f32(float v) {
+  float m;
+  asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
+  return m;
+}
+
 namespace tc {
 
-// `bytes` (a multiple of 16) between 16-byte aligned addresses
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src), "r"(bytes),
-               "r"(smem_u32(bar))
-               : "memory");
+// has the phase completed?  (mbar_try may wait for a while)
+__device__ __forceinline__ bool mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n"
+      ".reg .pred p;\n"
+      "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+      "selp.u32 %0, 1, 0, p;\n"
+      "}\n"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;   // one answer for the warp
 }
 // D += A B, e4m3 operands in shared memory
 __device__ __forceinline__ void mma_f8_ss(uint32_t one, uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc, uint32_t acc) {

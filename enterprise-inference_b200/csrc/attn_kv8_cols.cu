@@ -25,26 +25,31 @@ using namespace tc;
 
 constexpr int kSlotBytes = kKv8Tile * 128;   // a tile of keys or of values: 16 KiB
 constexpr int kTable = 96;                   // items of a CTA that are described at a time
-constexpr int kExpBytes = 2 * kKv8Tile;      // a tile's exponents: keys', values'
-constexpr int kStageWarps = 4;               // TMA, MMA, queries, table
+constexpr int kFacs = 2;                     // tiles whose factors are kept
+constexpr int kFacBytes = kKv8Tile * 8 + 16; // a token's (key factor, value factor); the tile's factor, whether a token is dead
+constexpr int kStageWarps = 4;               // keys, MMA, queries, values
 
 struct Kv8Item {
   int row0, nrows, seq, kvh, tile0, tile1, ctx, ends;   // ends: 1 begins in an earlier CTA, 2 goes on in the next
 };
 
+#ifndef B200_CG
+#define B200_CG(NC) ((NC) >= 16 ? 4 : (NC) >= 4 ? 2 : (NC))
+#endif
 template <int NC>
 struct Cols {
   static constexpr int NP = NC < 8 ? 8 : NC;               // columns of either term: N = 2 NP is a multiple of 16
-  static constexpr int CG = NC >= 4 ? 4 : NC;              // groups of four softmax warps that share the columns
+  static constexpr int CG = B200_CG(NC);              // groups of four softmax warps that share the columns
   static constexpr int NCG = NC / CG;
-  static constexpr int kThreads = (kStageWarps + 4 * CG) * 32;
+  static constexpr int kSpare = kStageWarps + 4 * CG;      // the warp behind them makes the tokens' factors
+  static constexpr int kThreads = (kSpare + 1) * 32;
   static constexpr int kOperand = 2 * NP * 128;            // queries, or weights, of an item or tile
   static constexpr int kSlots = NP <= 16 ? 12 : 10;          // even: keys and values in turn
-  static constexpr int kExps = kSlots / 2 + 3;             // tiles whose exponents are kept: a ring ahead of the scores, and two behind them
+  static constexpr int kBars = (2 * kSlots + 15 + kFacs + 1) & ~1;
   static constexpr uint32_t kTmem = 8 * NP;                // S, S, O, O
-  static constexpr int kSmem = 1024 + kSlots * kSlotBytes + 4 * kOperand + kExps * kExpBytes + kTable * (int)sizeof(Kv8Item) + (2 * kSlots + 16 + kExps) * 8 +
-                               (4 * 32 + CG * 4 * NCG + CG * 2 * 4 * (NCG + 1)) * 4 + 256;
-  static_assert(kSmem <= 232448, "shared memory");
+  static constexpr int kSmem = 1024 + kSlots * kSlotBytes + 4 * kOperand + kFacs * kFacBytes + kTable * (int)sizeof(Kv8Item) +
+                               kBars * 8 + (4 * 32 + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + 64;
+  static_assert(kSmem + 8 * (kThreads + kThreads / 32) <= 232448, "shared memory");
 };
 
 // byte (row r, byte b) of an operand in rows of 128 bytes
@@ -75,8 +80,8 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   unsigned char* qs = ring + kSlots * kSlotBytes;          // [2] queries of an item
   unsigned char* ws = qs + 2 * C::kOperand;                // [2] weights of a tile
-  unsigned char* exps = ws + 2 * C::kOperand;              // [kExps][keys', values']
-  Kv8Item* table = reinterpret_cast<Kv8Item*>(exps + C::kExps * kExpBytes);
+  unsigned char* facs = ws + 2 * C::kOperand;              // [kFacs]
+  Kv8Item* table = reinterpret_cast<Kv8Item*>(facs + kFacs * kFacBytes);
   uint64_t* full = reinterpret_cast<uint64_t*>(table + kTable);   // [kSlots]: K, V, K, V, ...
   uint64_t* freed = full + kSlots;
   uint64_t* s_full = freed + kSlots;                       // [2]
@@ -85,15 +90,15 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   uint64_t* q_ready = o_full + 2;
   uint64_t* q_free = q_ready + 2;
   uint64_t* q_info = q_free + 2;                           // [4]: an item's scales, for the softmax warps (who may be three items behind)
-  uint64_t* e_full = q_info + 4;                           // [kExps]
-  uint64_t* last = e_full + C::kExps;
-  float* q_scale = reinterpret_cast<float*>(last + 1);     // [4 items][32]
-  float* x_sum = q_scale + 4 * 32;                         // [CG][4][NCG]
-  int* x_max = reinterpret_cast<int*>(x_sum + CG * 4 * NCG);   // [CG][2][4][NCG + 1]
-  int* shared_int = x_max + CG * 2 * 4 * (NCG + 1);        // 0: tensor memory, 1: a wait ran out, 2: items in the table, 3: next group, 4..: where the share starts
+  uint64_t* f_full = q_info + 4;                           // [kFacs]
+  uint64_t* last = f_full + kFacs;
+  float* q_scale = reinterpret_cast<float*>(full + C::kBars);   // [4 items][32]; from here on in whole 16 bytes
+  float* x_sum = q_scale + 4 * 32;                         // [CG][2][NCG][4 warps]
+  float* x_max = x_sum + CG * 2 * NCG * 4;                 // [CG][2][NCG][4 warps]
+  int* shared_int = reinterpret_cast<int*>(x_max + CG * 2 * NCG * 4);        // 0: tensor memory, 1: a wait ran out, 2, 3: the share's first and last item
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Waits wait(reinterpret_cast<uint32_t*>(shared_int + 1), p.status);
-  __shared__ int64_t scan_warp[kThreads / 32];
+  __shared__ uint64_t scan_warp[kThreads / 32], scan_thread[kThreads];
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kSlots; ++s) mbar_init(full + s, 1), mbar_init(freed + s, 1);
@@ -105,7 +110,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       mbar_init(q_free + s, 1);
     }
     for (int s = 0; s < 4; ++s) mbar_init(q_info + s, 1);
-    for (int s = 0; s < C::kExps; ++s) mbar_init(e_full + s, 1);
+    for (int s = 0; s < kFacs; ++s) mbar_init(f_full + s, 1);
     mbar_init(last, 1);
     shared_int[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -119,122 +124,98 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   pdl_wait();
   pdl_launch_dependents();
 
-  // ---- the CTA's share of the tiles ----
+  // ---- the CTA's share of the tiles: a thread counts its groups' (32 bits hold them: the host's check) ----
   const int n_groups = p.groups ? p.groups[-1].row0 : p.T, each = (n_groups + kThreads - 1) / kThreads;
-  int64_t sum = 0;   // tiles of this thread's groups
-  for (int i = threadIdx.x * each; i < min((int)(threadIdx.x + 1) * each, n_groups); ++i) sum += group_tiles(find_group(p, i));
-  int64_t before = sum;
+  const int g0 = min((int)threadIdx.x * each, n_groups), g1 = min(g0 + each, n_groups);
+  Kv8Group own = {0, 0, 0, 0};
+  uint64_t sum = 0;   // groups that see something << 32 | their tiles
+  for (int i = g0; i < g1; ++i) {
+    own = find_group(p, i);
+    const uint32_t nt = group_tiles(own);
+    sum += (uint64_t)(nt > 0) << 32 | nt;
+  }
+  uint64_t before = sum;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t v = __shfl_up_sync(0xffffffffu, before, o);
+    const uint64_t v = __shfl_up_sync(0xffffffffu, before, o);
     if (lane >= o) before += v;
   }
   if (lane == 31) scan_warp[warp] = before;
   before -= sum;
-  __syncthreads();
-  int64_t total = 0;
-  for (int w = 0; w < kThreads / 32; ++w) {
-    if (w < warp) before += scan_warp[w];
-    total += scan_warp[w];
-  }
-  const int64_t tiles = total * p.hkv, share = (tiles + gridDim.x - 1) / gridDim.x;
-  const int64_t begin = min(tiles, share * blockIdx.x), end = min(tiles, begin + share);
-  const int n_tiles = (int)(end - begin);
-  if (begin < end && begin >= before * p.hkv && begin < (before + sum) * p.hkv) {   // one thread's groups hold the first tile
-    int i = threadIdx.x * each;
-    for (;; ++i) {
-      const int nt = group_tiles(find_group(p, i));
-      if (begin < (before + nt) * p.hkv) break;
-      before += nt;
-    }
-    shared_int[3] = i;
-    *reinterpret_cast<int64_t*>(shared_int + 4) = before * p.hkv;
-  }
   if (threadIdx.x == 0) p.cuts[blockIdx.x].parts = 0;
+  __syncthreads();
+  uint64_t warps = lane < kThreads / 32 ? scan_warp[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const uint64_t v = __shfl_up_sync(0xffffffffu, warps, o);
+    if (lane >= o) warps += v;
+  }
+  const uint64_t in_front = __shfl_sync(0xffffffffu, warps, max(warp - 1, 0));
+  if (warp > 0) before += in_front;
+  const uint32_t tiles = (uint32_t)__shfl_sync(0xffffffffu, warps, 31) * p.hkv, share = (tiles + gridDim.x - 1) / gridDim.x;
+  const uint32_t begin = min(tiles, share * blockIdx.x), end = min(tiles, begin + share);
+  scan_thread[threadIdx.x] = before;
+  // the groups of this thread that the share touches: f(group, its first tile, tiles of a head, items in front of it)
+  auto own_groups = [&](auto f) {
+    uint64_t at = scan_thread[threadIdx.x];
+    for (int i = g0; i < g1; ++i) {
+      const Kv8Group g = each == 1 ? own : find_group(p, i);
+      const uint32_t nt = group_tiles(g), base = (uint32_t)at * p.hkv;
+      if (nt > 0 && base < end && base + nt * p.hkv > begin) f(g, base, nt, (int)(at >> 32) * p.hkv);
+      at += (uint64_t)(nt > 0) << 32 | nt;
+    }
+  };
+  own_groups([&](const Kv8Group& g, uint32_t base, uint32_t nt, int items) {
+    if (begin >= base) shared_int[2] = items + (int)((begin - base) / nt);                                  // the share's first item
+    if (end <= base + nt * p.hkv) shared_int[3] = items + (int)((end - 1 - base) / nt);                     // its last
+  });
+  __syncthreads();
+  const int first_item = shared_int[2], n_items = begin < end ? shared_int[3] - first_item + 1 : 0;
+  // items [from, from + kTable) of the share, by all threads
+  auto fill_table = [&](int from) {
+    own_groups([&](const Kv8Group& g, uint32_t base, uint32_t nt, int items) {
+      const int h1 = min(p.hkv, (int)((end - base + nt - 1) / nt));
+      for (int h = begin > base ? (int)((begin - base) / nt) : 0; h < h1; ++h) {
+        const int at = items + h - first_item - from;
+        if (at < 0 || at >= kTable) continue;
+        Kv8Item w = {g.row0, g.nrows, g.seq, h, 0, (int)nt, g.ctx, 0};
+        const uint32_t b = base + h * nt;
+        if (b < begin) w.tile0 = (int)(begin - b), w.ends |= 1;
+        if (b + nt > end) {
+          w.tile1 = (int)(end - b), w.ends |= 2;
+          if (!(w.ends & 1)) p.cuts[blockIdx.x] = {g.row0, g.nrows, h, (int)((b + nt - 1) / share) - (int)blockIdx.x + 1};
+        }
+        table[at] = w;
+      }
+    });
+  };
+  if (n_items > 0) fill_table(0);
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = (uint32_t)shared_int[0];
-
-  // table of the next items, by warp 3 (all threads come here); false: there are none
-  int64_t table_base = n_tiles > 0 ? *reinterpret_cast<int64_t*>(shared_int + 4) : 0;   // flat index of the next group's first tile (warp 3's is kept up to date)
-  int table_group = shared_int[3], table_skip = 0;   // items of that group that are in earlier tables
-  bool table_done = n_tiles == 0;
+  // how many items the next table has (0: there is none); all threads come here
+  int described = 0;
   auto next_table = [&]() {
-    __syncthreads();
-    if (warp == 3) {
-      int count = 0;
-      while (!table_done && count < kTable) {
-        const int i = table_group + lane;
-        Kv8Group g = {0, 0, 0, 0};
-        if (i < n_groups) g = find_group(p, i);
-        const int nt = group_tiles(g);
-        int at = nt;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, at, o);
-          if (lane >= o) at += v;
-        }
-        const int64_t base = table_base + (int64_t)(at - nt) * p.hkv;   // this group's first tile
-        // kv heads [h0, h1) whose tiles are in the share
-        int h0 = 0, h1 = 0;
-        if (nt > 0) {
-          h0 = (int)min((int64_t)p.hkv, max((int64_t)0, (begin - base) / nt));
-          h1 = (int)min((int64_t)p.hkv, max((int64_t)0, (end - base + nt - 1) / nt));
-          if (lane == 0) h0 = max(h0, table_skip);
-          h1 = max(h1, h0);
-        }
-        const int mine = h1 - h0;
-        int pos = mine;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int v = __shfl_up_sync(0xffffffffu, pos, o);
-          if (lane >= o) pos += v;
-        }
-        const int all = __shfl_sync(0xffffffffu, pos, 31);
-        pos += count - mine;
-        for (int h = h0; h < h1 && pos + h - h0 < kTable; ++h) {
-          Kv8Item w = {g.row0, g.nrows, g.seq, h, 0, nt, g.ctx, 0};
-          const int64_t b = base + (int64_t)h * nt;
-          if (b < begin) w.tile0 = (int)(begin - b), w.ends |= 1;
-          if (b + nt > end) {
-            w.tile1 = (int)(end - b), w.ends |= 2;
-            if (!(w.ends & 1)) p.cuts[blockIdx.x] = {g.row0, g.nrows, h, (int)((b + nt - 1) / share) - (int)blockIdx.x + 1};
-          }
-          table[pos + h - h0] = w;
-        }
-        if (count + all > kTable) {   // full inside this lane's group: the next table goes on there
-          const unsigned over = __ballot_sync(0xffffffffu, pos + mine > kTable);
-          const int who = __ffs(over) - 1;
-          table_skip = __shfl_sync(0xffffffffu, h0 + kTable - pos, who);
-          table_base = __shfl_sync(0xffffffffu, base, who);
-          table_group += who;
-          count = kTable;
-        } else {
-          count += all;
-          table_base += (int64_t)__shfl_sync(0xffffffffu, at, 31) * p.hkv;
-          table_group += 32;
-          table_skip = 0;
-          table_done = table_base >= end || table_group >= n_groups;
-        }
-      }
-      if (lane == 0) shared_int[2] = count;
+    const int from = described;
+    described += kTable;
+    if (from > 0 && from < n_items) {
+      __syncthreads();
+      fill_table(from);
+      __syncthreads();
     }
-    __syncthreads();
-    return shared_int[2];
+    return min(max(n_items - from, 0), kTable);
   };
 
-  if (warp == 0) {
-    // ===== TMA: a tile's keys with all its exponents, its values =====
-    const bool issuer = elect_one();
-    if (issuer) {
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
-      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
-    }
+  if (warp == 0 || warp == 3) {
+    // ===== TMA: warp 0 keys, warp 3 values =====
+    const bool issuer = elect_one(), values = warp == 3;
+    const CUtensorMap* map = values ? &maps.v : &maps.k;
+    if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     const int box = min(p.block_size, kKv8Tile), per_tile = kKv8Tile / box;   // boxes of a tile
     const int cells = (int)(p.n_blocks * p.hkv * p.block_size);
-    int slot = 0, exp_slot = 0;
-    uint32_t ph = 1, eph = 1;
+    int slot = values ? 1 : 0;
+    uint32_t ph = 1;
     bool stop = false;
     for (int count; (count = next_table()) > 0;) {
       for (int it = 0; it < count && !stop; ++it) {
@@ -247,50 +228,24 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           const int tok = b * box, blk = __ldg(bt + tok / p.block_size);
           return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
         };
-        int have = cell_of(b0 + lane), next = cell_of(b0 + 32 + lane);
+        int have = cell_of(b0 + lane), next = b0 + 32 < b1 ? cell_of(b0 + 32 + lane) : 0;
         for (int b = b0; b < b1 && !(stop = wait.stop()); b += per_tile) {
           if (b - b0 && ((b - b0) & 31) == 0) have = next, next = cell_of(b + 32 + lane);
-          const int n = min(per_tile, b1 - b);
-          wait(freed + slot, ph);
-          unsigned char* eb = exps + exp_slot * kExpBytes;   // (its tile of a ring ago is long done: the keys' ring is shorter)
-          const unsigned lanes = (n == 32 ? 0xffffffffu : (1u << n) - 1u) << ((b - b0) & 31);
-          const unsigned outside = __ballot_sync(0xffffffffu, have == cells) & lanes;   // boxes outside the cache: no exponents to fetch
-          if (issuer) {
-            for (unsigned o = outside; o; o &= o - 1) {
-              const int i = __ffs(o) - 1 - ((b - b0) & 31);
-              for (int j = 0; j < box; j += 4) *reinterpret_cast<uint32_t*>(eb + i * box + j) = *reinterpret_cast<uint32_t*>(eb + kKv8Tile + i * box + j) = 0u;
-            }
-            mbar_expect_tx(full + slot, n * box * 128);
-            mbar_expect_tx(e_full + exp_slot, (n - __popc(outside)) * box * 2);
-          }
-          __syncwarp();
-          for (int i = 0; i < n; ++i) {
-            const int cell = __shfl_sync(0xffffffffu, have, (b - b0 + i) & 31);
-            if (issuer) {
-              tma_load_2d(ring + slot * kSlotBytes + i * box * 128, &maps.k, 0, cell, full + slot);
-              if (cell != cells) {
-                bulk_load(eb + i * box, p.ke + cell, box, e_full + exp_slot);
-                bulk_load(eb + kKv8Tile + i * box, p.ve + cell, box, e_full + exp_slot);
-              }
-            }
-          }
-          if (++slot == kSlots) slot = 0, ph ^= 1;
-          if (++exp_slot == C::kExps) exp_slot = 0, eph ^= 1;
+          const int n = min(per_tile, b1 - b), first = (b - b0) & 31;
           wait(freed + slot, ph);
           if (issuer) mbar_expect_tx(full + slot, n * box * 128);
           __syncwarp();
           for (int i = 0; i < n; ++i) {
-            const int cell = __shfl_sync(0xffffffffu, have, (b - b0 + i) & 31);
-            if (issuer) tma_load_2d(ring + slot * kSlotBytes + i * box * 128, &maps.v, 0, cell, full + slot);
+            const int cell = __shfl_sync(0xffffffffu, have, first + i);
+            if (issuer) tma_load_2d(ring + slot * kSlotBytes + i * box * 128, map, 0, cell, full + slot);
           }
-          if (++slot == kSlots) slot = 0, ph ^= 1;
+          slot += 2;
+          if (slot >= kSlots) slot -= kSlots, ph ^= 1;
         }
       }
     }
-    if (wait.stop()) {   // the loads in flight: a slot's last one filled it in this round of the ring or in the one before
-      for (int s = 0; s < kSlots; ++s) wait.drain(full + s, s < slot ? ph ^ 1 : ph);
-      for (int s = 0; s < C::kExps; ++s) wait.drain(e_full + s, s < exp_slot ? eph ^ 1 : eph);
-    }
+    if (wait.stop())   // the loads in flight: a slot's last one filled it in this round of the ring or in the one before
+      for (int s = values ? 1 : 0; s < kSlots; s += 2) wait.drain(full + s, s < slot ? ph ^ 1 : ph);
   } else if (warp == 1) {
     // ===== MMA: the scores of tile n + 1, of the next item if need be, then tile n's second product =====
     const uint32_t one = elect_one() ? 1u : 0u, tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -314,9 +269,12 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     for (int count; (count = __shfl_sync(0xffffffffu, next_table(), 0)) > 0;) {
       for (int it = 0; it < count; ++it, ++item) {
         const int nt = __shfl_sync(0xffffffffu, table[it].tile1 - table[it].tile0, 0);
+        // what is not there yet is not waited for before what is: the previous tile's product
+        if (pending && !mbar_test(q_ready + (item & 1), (item >> 1) & 1)) product(n - 1), pending = false;
         wait(q_ready + (item & 1), (item >> 1) & 1);
         const uint64_t dq = desc_q + (uint64_t)(((item & 1) * C::kOperand) >> 4);
         for (int i = 0; i < nt; ++i, ++n) {
+          if (pending && !mbar_test(full + slot, ph)) product(n - 1), pending = false;
           wait(full + slot, ph);
           fence_after();
           const uint64_t dk = desc_ring + (uint64_t)((slot * kSlotBytes) >> 4);
@@ -343,40 +301,54 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     // ===== queries: 16 lanes a pair, scaled to [128, 256), in two terms =====
     const int G = p.hq / p.hkv;
     int item = 0;
+    if (!p.groups)   // rows that see nothing: zeros, by the CTAs in turn
+      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
+        if (__ldg(p.ctx_lens + r) <= 0)
+          for (int i = lane; i < p.hq * kHeadDim / 8; i += 32) *reinterpret_cast<uint4*>(p.out + (int64_t)r * p.ldo + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
     for (int count; (count = next_table()) > 0;) {
       for (int it = 0; it < count; ++it, ++item) {
         const Kv8Item w = table[it];
         if (item >= 2) wait(q_free + (item & 1), ((item >> 1) - 1) & 1);
         unsigned char* qb = qs + (item & 1) * C::kOperand;
         const int ncol = w.nrows * G, d = (lane & 15) * 8;
-        for (int c = lane >> 4; c < ((ncol + 1) & ~1); c += 2) {
-          uint4 v = make_uint4(0u, 0u, 0u, 0u);
-          if (c < ncol) v = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)(w.row0 + c / G) * p.ldq + (w.kvh * G + c % G) * kHeadDim + d));
-          const uint32_t x[4] = {v.x, v.y, v.z, v.w};
-          uint32_t m = 0;   // the largest magnitude, as bf16 bits
+        constexpr int U = NC < 8 ? (NC + 1) / 2 : 4;   // pairs of columns that are asked for at a time
+        for (int c1 = 0; c1 < ncol; c1 += 2 * U) {
+          uint4 v[U];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) m = max(m, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
-#pragma unroll
-          for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-          const uint32_t e = max(m >> 7, 8u);   // biased exponent
-          const float f = __uint_as_float((261u - min(e, 254u)) << 23);
-          uint32_t hi[2], lo[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            hi[j] = lo[j] = 0u;
-#pragma unroll
-            for (int k = 0; k < 2; ++k) {
-              const float a = bf16lo(x[2 * j + k]) * f, b = bf16hi(x[2 * j + k]) * f;
-              const uint32_t h = e == 255u ? 0x7f7fu : e4m3x2(a, b);
-              const float2 r = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
-              hi[j] |= h << (16 * k);
-              lo[j] |= e4m3x2((a - r.x) * 16.f, (b - r.y) * 16.f) << (16 * k);
-            }
+          for (int u = 0; u < U; ++u) {
+            const int c = c1 + 2 * u + (lane >> 4);
+            v[u] = make_uint4(0u, 0u, 0u, 0u);
+            if (c < ncol) v[u] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)(w.row0 + c / G) * p.ldq + (w.kvh * G + c % G) * kHeadDim + d));
           }
-          if (c < ncol) {
-            *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = make_uint2(hi[0], hi[1]);
-            *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = make_uint2(lo[0], lo[1]);
-            if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = __uint_as_float((min(e, 254u) - 7u) << 23) * p.scale2;
+#pragma unroll
+          for (int u = 0; u < U; ++u) {
+            const int c = c1 + 2 * u + (lane >> 4);
+            const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+            uint32_t m = 0;   // the largest magnitude, as bf16 bits
+#pragma unroll
+            for (int j = 0; j < 4; ++j) m = max(m, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const uint32_t e = max(m >> 7, 8u);   // biased exponent
+            const float f = __uint_as_float((261u - min(e, 254u)) << 23);
+            uint32_t hi[2], lo[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              hi[j] = lo[j] = 0u;
+#pragma unroll
+              for (int k = 0; k < 2; ++k) {
+                const float a = bf16lo(x[2 * j + k]) * f, b = bf16hi(x[2 * j + k]) * f;
+                const uint32_t h = e == 255u ? 0x7f7fu : e4m3x2(a, b);
+                const float2 r = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
+                hi[j] |= h << (16 * k);
+                lo[j] |= e4m3x2((a - r.x) * 16.f, (b - r.y) * 16.f) << (16 * k);
+              }
+            }
+            if (c < ncol) {
+              *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = make_uint2(hi[0], hi[1]);
+              *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = make_uint2(lo[0], lo[1]);
+              if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = __uint_as_float((min(e, 254u) - 7u) << 23) * p.scale2;
+            }
           }
         }
         fence_async_smem();
@@ -384,60 +356,164 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         if (lane == 0) mbar_arrive(q_ready + (item & 1)), mbar_arrive(q_info + (item & 3));
       }
     }
-  } else if (warp == 3) {
-    // ===== rows that see nothing: zeros, by the CTAs in turn =====
-    if (!p.groups)
-      for (int r = blockIdx.x; r < p.T; r += gridDim.x)
-        if (__ldg(p.ctx_lens + r) <= 0)
-          for (int i = lane; i < p.hq * kHeadDim / 8; i += 32) *reinterpret_cast<uint4*>(p.out + (int64_t)r * p.ldo + 8 * i) = make_uint4(0u, 0u, 0u, 0u);
-    while (next_table() > 0) {
+  } else if (warp == C::kSpare) {
+    // ===== factors: a token's 2^key exponent, and 256 * 2^(value exponent - the tile's largest); four tokens a lane.  The exponents are fetched four
+    // tiles ahead, their places in the cache eight (bulk copies of 128 bytes took the issuing warp 400 cycles each) =====
+    constexpr int D = 4;
+    const int stride = p.hkv * p.block_size;
+    int n = 0;
+    for (int count; (count = next_table()) > 0;) {
+      // the tiles in order: the block of this lane's tokens, asked for, and their cells in it (-1: behind the context, or the table)
+      int it_c = -1, i_c = 0, end_c = 0, ctx_c = 0, kvh_c = 0, blk_c = 0, off_c = 0;
+      const int32_t* bt_c = p.block_table;
+      auto place = [&](int& blk, int& cell) {
+        if (i_c == end_c && it_c < count) {
+          if (++it_c < count) {
+            const Kv8Item w = table[it_c];
+            const int tok = w.tile0 * kKv8Tile + 4 * lane;
+            i_c = w.tile0, end_c = w.tile1, ctx_c = w.ctx, kvh_c = w.kvh;
+            bt_c = p.block_table + (int64_t)w.seq * p.bt_stride;
+            blk_c = tok / p.block_size, off_c = tok - blk_c * p.block_size;
+          } else {
+            ctx_c = 0;
+          }
+        }
+        const bool in = i_c * kKv8Tile + 4 * lane < ctx_c;
+        blk = __ldg(in ? bt_c + blk_c : p.block_table);
+        cell = in ? kvh_c * p.block_size + off_c : -1;
+        ++i_c;
+        off_c += kKv8Tile;
+        while (off_c >= p.block_size) off_c -= p.block_size, ++blk_c;
+      };
+      auto fetch = [&](int blk, int cell, uint32_t& k4, uint32_t& v4) {
+        const bool in = cell >= 0 && blk >= 0 && blk < p.n_blocks;   // (outside the cache: zeros)
+        const int c = in ? blk * stride + cell : 0;
+        k4 = v4 = 0u;
+        if (in) k4 = __ldg(reinterpret_cast<const uint32_t*>(p.ke + c)), v4 = __ldg(reinterpret_cast<const uint32_t*>(p.ve + c));
+      };
+      int blk[D], cell[D];
+      uint32_t k4[D], v4[D];
+#pragma unroll
+      for (int d = 0; d < D; ++d) place(blk[d], cell[d]);
+#pragma unroll
+      for (int d = 0; d < D; ++d) fetch(blk[d], cell[d], k4[d], v4[d]);
+#pragma unroll
+      for (int d = 0; d < D; ++d) place(blk[d], cell[d]);
+      int it = 0, i = table[0].tile0;
+      while (it < count) {
+#pragma unroll
+        for (int d = 0; d < D; ++d) {
+          if (it >= count) break;
+          const int left = table[it].ctx - i * kKv8Tile - 4 * lane;   // tokens of this lane's four
+          // a value row that is not a number: the columns that see it are none either (its key's factor), the others must not meet it
+          uint32_t ve[4], m = 1u;
+          bool none = false;
+          float kf[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            ve[j] = (v4[d] >> (8 * j)) & 255u;
+            kf[j] = __uint_as_float(j < left && ve[j] == 255u ? 0x7fffffffu : ((k4[d] >> (8 * j)) & 255u) << 23);   // (2^-127 counts as nothing)
+            if (j >= left) ve[j] = 255u;
+            if (ve[j] == 255u) none = true;
+            else m = max(m, ve[j]);
+          }
+          fetch(blk[d], cell[d], k4[d], v4[d]);
+          place(blk[d], cell[d]);
+          m = __reduce_max_sync(0xffffffffu, m);
+          none = __any_sync(0xffffffffu, none);
+          float vf[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vf[j] = ve[j] == 255u ? -0.f : __uint_as_float((uint32_t)max((int)(ve[j] - m) + 135, 0) << 23);
+          // the slot is tile n - 2's until that one's weights are ready
+          if (n >= kFacs) wait(w_ready + (n & 1), ((n - 2) >> 1) & 1);
+          float* f = reinterpret_cast<float*>(facs + (n & (kFacs - 1)) * kFacBytes);
+          reinterpret_cast<float4*>(f)[2 * lane] = make_float4(kf[0], vf[0], kf[1], vf[1]);
+          reinterpret_cast<float4*>(f)[2 * lane + 1] = make_float4(kf[2], vf[2], kf[3], vf[3]);
+          if (lane == 0) {
+            f[2 * kKv8Tile] = __uint_as_float((uint32_t)max((int)m - 8, 1) << 23);
+            reinterpret_cast<int*>(f)[2 * kKv8Tile + 1] = none;
+          }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(f_full + (n & (kFacs - 1)));
+          ++n;
+          if (++i == table[it].tile1 && ++it < count) i = table[it].tile0;
+        }
+      }
     }
   } else {
     // ===== softmax: a thread owns a token of the scores and an entry of the result; the columns are dealt to CG groups of four warps =====
     const int grp = (warp - kStageWarps) >> 2, quad = warp & 3, tau = quad * 32 + lane, G = p.hq / p.hkv, c0 = grp * NCG;
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + c0;
-    int* xm = x_max + grp * 2 * 4 * (NCG + 1);
-    float* xs = x_sum + grp * 4 * NCG;
-    int n = 0, item = 0, v_slot = 1, exp_slot = 0;
-    uint32_t ph = 0, eph = 0;
+    float* xm = x_max + grp * 2 * NCG * 4;
+    float* xs = x_sum + grp * 2 * NCG * 4;
+    int n = 0, item = 0, v_slot = 1;
+    uint32_t ph = 0;
+    float mu[NCG], l[NCG], acc[NCG], keep[NCG], take[NCG];   // keep, take: what becomes of the sums, and of the previous tile's product
+    auto fold = [&](int m) {                                   // tile m's product
+      wait(o_full + (m & 1), (m >> 1) & 1);
+      fence_after();
+      uint32_t hi[NCG], lo[NCG];
+      ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP, hi);
+      ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP + NP, lo);
+      ld_wait<NCG>(hi);
+#pragma unroll
+      for (int j = 0; j < NCG; ++j) {
+        asm volatile("" : "+r"(lo[j]));
+        acc[j] = acc[j] * keep[j] + fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])) * take[j];
+      }
+    };
+    // an item's results: its last product, then the denominators (every token's share)
+    auto finish = [&](const Kv8Item& w, const float (&mu0)[NCG], const float (&l0)[NCG], int last_tile) {
+      float* xt = xs + (item & 1) * NCG * 4;
+#pragma unroll
+      for (int j = 0; j < NCG; ++j) {
+        const float v = warp_sum(l0[j]);
+        if (lane == 0) xt[j * 4 + quad] = v;
+      }
+      fold(last_tile);
+      asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
+      const int ncol = w.nrows * G;
+#pragma unroll
+      for (int j = 0; j < NCG; ++j) {
+        const int c = c0 + j;
+        if (c < ncol) {
+          const float4 x = reinterpret_cast<const float4*>(xt)[j];
+          const float sum_l = (x.x + x.y) + (x.z + x.w);
+          if (w.ends == 0) {
+            p.out[(int64_t)(w.row0 + c / G) * p.ldo + (w.kvh * G + c % G) * kHeadDim + tau] = __float2bfloat16_rn(sum_l == 0.f ? 0.f : __fdividef(acc[j], sum_l));
+          } else {
+            float* dst = p.part + ((int64_t)(2 * blockIdx.x + ((w.ends & 1) ? 0 : 1)) * kKv8Cols + c) * kKv8PartFloats;
+            dst[tau] = acc[j];
+            if (tau == 0) dst[128] = mu0[j], dst[129] = sum_l;
+          }
+        }
+        acc[j] = 0.f;
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < NCG; ++j) acc[j] = 0.f;
     for (int count; (count = next_table()) > 0;) {
       for (int it = 0; it < count; ++it, ++item) {
         const Kv8Item w = table[it];
         const int ncol = w.nrows * G;
         int ctx[NCG];
-        float qf[NCG], mu[NCG], l[NCG], acc[NCG], keep[NCG], take[NCG];   // keep, take: what becomes of the sums, and of the previous tile's product
+        float qf[NCG], mu_before[NCG], l_before[NCG];
         wait(q_info + (item & 3), (item >> 2) & 1);
 #pragma unroll
         for (int j = 0; j < NCG; ++j) {
           const bool live = c0 + j < ncol;
           ctx[j] = !live ? 0 : w.nrows == 1 ? w.ctx : kv8_ctx(p, w.row0 + (c0 + j) / G);
           qf[j] = live ? q_scale[(item & 3) * 32 + c0 + j] : 0.f;
+          mu_before[j] = mu[j], l_before[j] = l[j];
           mu[j] = -INFINITY;
-          l[j] = acc[j] = 0.f;
+          l[j] = 0.f;
         }
-        auto fold = [&](int m) {   // tile m's product
-          wait(o_full + (m & 1), (m >> 1) & 1);
-          fence_after();
-          uint32_t hi[NCG], lo[NCG];
-          ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP, hi);
-          ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP + NP, lo);
-          ld_wait<NCG>(hi);
-#pragma unroll
-          for (int j = 0; j < NCG; ++j) {
-            asm volatile("" : "+r"(lo[j]));
-            acc[j] = acc[j] * keep[j] + fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])) * take[j];
-          }
-        };
         for (int i = w.tile0; i < w.tile1; ++i, ++n) {
-          const int tok = i * kKv8Tile + tau, n_valid = w.ctx - i * kKv8Tile;
-          wait(e_full + exp_slot, eph);
-          uint32_t ve = exps[exp_slot * kExpBytes + kKv8Tile + tau];
-          // a value row that is not a number: the columns that see it are none either, the others must not meet it
-          const float ks = ve == 255u ? __uint_as_float(0x7fffffffu) : kv8_scale(exps[exp_slot * kExpBytes + tau]);
-          const bool dead = tau >= n_valid || ve == 255u;
-          if (dead) ve = 0u;
-          int* xt = xm + (n & 1) * 4 * (NCG + 1);
-          const uint32_t vw = __reduce_max_sync(0xffffffffu, ve);
+          const int tok = i * kKv8Tile + tau;
+          wait(f_full + (n & (kFacs - 1)), (n / kFacs) & 1);
+          const float* f = reinterpret_cast<const float*>(facs + (n & (kFacs - 1)) * kFacBytes);
+          const float2 kv = reinterpret_cast<const float2*>(f)[tau], vr = reinterpret_cast<const float2*>(f)[kKv8Tile];
+          float* xt = xm + (n & 1) * NCG * 4;
           wait(s_full + (n & 1), (n >> 1) & 1);
           fence_after();
           uint32_t hi[NCG], lo[NCG];
@@ -448,28 +524,23 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
 #pragma unroll
           for (int j = 0; j < NCG; ++j) {
             asm volatile("" : "+r"(lo[j]));
-            s[j] = tok < ctx[j] ? fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])) * (ks * qf[j]) : -INFINITY;
-            const float m = warp_max_redux(s[j]);
-            if (lane == 0) xt[quad * (NCG + 1) + j] = __float_as_int(m);
+            s[j] = tok < ctx[j] ? fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])) * (kv.x * qf[j]) : -INFINITY;
+            const float m = warp_max_f32(s[j]);
+            if (lane == 0) xt[j * 4 + quad] = m;
           }
-          if (lane == 0) xt[quad * (NCG + 1) + NCG] = (int)vw;
           asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
-          const int vmax = max(max(xt[NCG], xt[2 * NCG + 1]), max(xt[3 * NCG + 2], xt[4 * NCG + 3]));
-          // 256 * 2^(ve - vmax), and what it is relative to
-          const float vf = dead ? 0.f : __uint_as_float((uint32_t)max((int)ve - vmax + 127 + 8, 0) << 23);
-          const float vr = __uint_as_float((uint32_t)max(vmax - 8, 1) << 23);
           float wt[NCG], keep1[NCG], take1[NCG];
 #pragma unroll
           for (int j = 0; j < NCG; ++j) {
-            const float mt = fmaxf(fmaxf(__int_as_float(xt[j]), __int_as_float(xt[NCG + 1 + j])),
-                                   fmaxf(__int_as_float(xt[2 * (NCG + 1) + j]), __int_as_float(xt[3 * (NCG + 1) + j])));
+            const float4 x = reinterpret_cast<const float4*>(xt)[j];
+            const float mt = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
             const bool none = mt == -INFINITY;   // a column whose row does not see this tile
             const float mn = fmaxf(mu[j], mt), e = none ? 0.f : exp2_fast(s[j] - mt), b = none ? 0.f : exp2_fast(mt - mn);
             keep1[j] = mn == -INFINITY ? 1.f : exp2_fast(mu[j] - mn);
-            take1[j] = b * vr;
+            take1[j] = b * vr.x;
             l[j] = l[j] * keep1[j] + e * b;
             mu[j] = mn;
-            wt[j] = none ? 0.f : e * vf;
+            wt[j] = e * kv.y;
           }
           unsigned char* wb = ws + (n & 1) * C::kOperand;
 #pragma unroll
@@ -485,10 +556,10 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
               wb[operand_off(NP + c0 + j + 1, tau)] = (unsigned char)(g >> 8);
             }
           }
-          if (grp == 0 && __any_sync(0xffffffffu, dead)) {
+          if (grp == 0 && __float_as_int(vr.y) != 0) {
             // value rows behind the context may hold anything, and 0 * NaN = NaN: zero them under their zero weights
             wait(full + v_slot, ph);
-            if (dead) {
+            if (__float_as_uint(kv.y) == 0x80000000u) {
               unsigned char* vb = ring + v_slot * kSlotBytes + tau * 128;
 #pragma unroll
               for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vb + c * 16) = make_uint4(0u, 0u, 0u, 0u);
@@ -499,35 +570,14 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           __syncwarp();
           if (lane == 0) mbar_arrive(w_ready + (n & 1));
           if (i > w.tile0) fold(n - 1);
+          else if (it > 0) finish(table[it - 1], mu_before, l_before, n - 1);   // the item before, while this one's first product runs
 #pragma unroll
           for (int j = 0; j < NCG; ++j) keep[j] = keep1[j], take[j] = take1[j];
           v_slot += 2;
           if (v_slot >= kSlots) v_slot -= kSlots, ph ^= 1;
-          if (++exp_slot == C::kExps) exp_slot = 0, eph ^= 1;
         }
-        fold(n - 1);
-        // the denominators: every token's share
-#pragma unroll
-        for (int j = 0; j < NCG; ++j) {
-          const float v = warp_sum(l[j]);
-          if (lane == 0) xs[quad * NCG + j] = v;
-        }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
-#pragma unroll
-        for (int j = 0; j < NCG; ++j) {
-          const int c = c0 + j;
-          if (c >= ncol) continue;
-          const float sum_l = (xs[j] + xs[NCG + j]) + (xs[2 * NCG + j] + xs[3 * NCG + j]);
-          if (w.ends == 0) {
-            p.out[(int64_t)(w.row0 + c / G) * p.ldo + (w.kvh * G + c % G) * kHeadDim + tau] = __float2bfloat16_rn(sum_l == 0.f ? 0.f : acc[j] / sum_l);
-          } else {
-            float* dst = p.part + ((int64_t)(2 * blockIdx.x + ((w.ends & 1) ? 0 : 1)) * kKv8Cols + c) * kKv8PartFloats;
-            dst[tau] = acc[j];
-            if (tau == 0) dst[128] = mu[j], dst[129] = sum_l;
-          }
-        }
-        asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");   // xs is written again
       }
+      finish(table[count - 1], mu, l, n - 1);
     }
     fence_before();
   }

@@ -1,136 +1,379 @@
-// Check of drafted tokens against the target's probabilities (b200_verify_drafts): a CTA takes a sequence, its rows in order, in 64 bits.
+// Check of drafted tokens against the target's probabilities (b200_verify_drafts), two launches.
+//
+// stats: a CTA takes a slice of a logit row (target rows, and the rows that drafts were drawn from) and leaves its largest logit, the first place of it and the sum
+// of 2^((l - max) log2e / T) relative to it, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  Bound by the rows' bytes, closely
+// followed by instructions (about six an entry at 12 entries a cycle and SM).
+// draw: a cluster of eight CTAs takes a sequence: the kept drafts from the slices' sums, then the token from the one row that draws it.  A draw next to a border of
+// the cumulated weights has to come out as in exact arithmetic (128 k borders: sums that are off by 1e-9 pick another token once in 4000 draws), so weights and
+// sums are fp64 there: 2^t by a table of 256 powers and a cubic, relative error below 2e-13, ten fp64 operations a weight.  Each CTA owns an eighth of the
+// row in chunks of 256 entries; sums are taken in a fixed order, chunk by chunk.
+#include <cooperative_groups.h>
+
+#include <algorithm>
+
 #include "kv8.cuh"
+#include "tc.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int kVerifyThreads = 1024;
+namespace cg = cooperative_groups;
 
-__device__ __forceinline__ double block_sum(double v, double* sh) {
+constexpr int kStatThreads = 256, kSlice = 8192;
+constexpr int kDrawThreads = 512, kDrawCtas = 8, kChunk = 256, kMostChunks = 512;
+constexpr int kMostVocab = kDrawCtas * kMostChunks * kChunk;
+
+struct Stat {
+  float m, s;
+  int at, pad;
+};
+
+// eight entries from index i on (-inf behind the end), 16 bytes at a time where the address allows it
+__device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int i, int n) {
+  const __nv_bfloat16* p = row + i;
+  if (i + 8 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) return ld_stream(p);
+  uint32_t w[4];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
-  __syncthreads();
-  double t = 0;
-  for (int i = 0; i < kVerifyThreads / 32; ++i) t += sh[i];
-  __syncthreads();
-  return t;
+  for (int j = 0; j < 4; ++j) {
+    const uint32_t a = i + 2 * j < n ? __bfloat16_as_ushort(p[2 * j]) : 0xff80u, b = i + 2 * j + 1 < n ? __bfloat16_as_ushort(p[2 * j + 1]) : 0xff80u;
+    w[j] = a | b << 16;
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
 }
-// largest value of a row and its first place
-__device__ __forceinline__ float row_max(const __nv_bfloat16* l, int vocab, int* at, float* shv, int* shi) {
-  float m = -INFINITY;
-  int i0 = 0x7fffffff;
-  for (int i = threadIdx.x; i < vocab; i += kVerifyThreads) {
-    const float v = __bfloat162float(l[i]);
-    if (v > m || i0 == 0x7fffffff) m = v, i0 = i;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float v = __shfl_xor_sync(0xffffffffu, m, o);
-    const int i = __shfl_xor_sync(0xffffffffu, i0, o);
-    if (v > m || (v == m && i < i0)) m = v, i0 = i;
-  }
-  if ((threadIdx.x & 31) == 0) shv[threadIdx.x >> 5] = m, shi[threadIdx.x >> 5] = i0;
-  __syncthreads();
-  for (int w = 0; w < kVerifyThreads / 32; ++w)
-    if (shv[w] > m || (shv[w] == m && shi[w] < i0)) m = shv[w], i0 = shi[w];
-  __syncthreads();
-  *at = i0;
-  return m;
+__device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
 }
 
-__global__ void __launch_bounds__(kVerifyThreads)
-verify_kernel(const __nv_bfloat16* target, int64_t ldt, const __nv_bfloat16* draft, int64_t ldd, const int32_t* tokens, const int32_t* starts,
-              const float* temperature, const float* uniforms, int n_rows, int vocab, int32_t* out, int32_t* accepted) {
-  __shared__ double sh[kVerifyThreads / 32], part[kVerifyThreads];
-  __shared__ float shv[32];
-  __shared__ int shi[32], found;
+__global__ void __launch_bounds__(kStatThreads)
+verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const __nv_bfloat16* __restrict__ draft, int64_t ldd, const int32_t* __restrict__ starts,
+                    const float* __restrict__ temperature, int n_seqs, int vocab, Stat* __restrict__ stats) {
+  __shared__ int found;
+  __shared__ float sh_m[kStatThreads / 32], sh_s[kStatThreads / 32];
+  __shared__ int sh_at[kStatThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
-  const int s = blockIdx.x, r0 = max(starts[s], 0), r1 = min(starts[s + 1], n_rows);
-  const double temp = temperature ? (double)temperature[s] : 0.0;
-  int taken = 0, token = -1;
-  for (int r = r0; r < r1; ++r) {
-    const bool last = r == r1 - 1;
-    const __nv_bfloat16* l = target + (int64_t)r * ldt;
-    const __nv_bfloat16* d = draft ? draft + (int64_t)r * ldd : nullptr;
-    const int x = last ? -1 : tokens[r];
-    int best;
-    const float m = row_max(l, vocab, &best, shv, shi);
-    if (!(temp > 0.0) || m == -INFINITY) {
-      token = best;
-      if (best == x && m > -INFINITY) {
-        if (threadIdx.x == 0) out[r0 + taken] = x;
-        ++taken;
-        continue;
-      }
-      break;
-    }
-    double z = 0, zd = 0;
-    float md = 0;
-    for (int i = threadIdx.x; i < vocab; i += kVerifyThreads) z += exp((double)(__bfloat162float(l[i]) - m) / temp);
-    z = block_sum(z, sh);
-    if (d && !last) {
-      int at;
-      md = row_max(d, vocab, &at, shv, shi);
-      for (int i = threadIdx.x; i < vocab && md > -INFINITY; i += kVerifyThreads) zd += exp((double)(__bfloat162float(d[i]) - md) / temp);
-      zd = block_sum(zd, sh);
-    }
-    auto p = [&](int i) { return exp((double)(__bfloat162float(l[i]) - m) / temp) / z; };
-    auto q = [&](int i) {
-      if (last) return 0.0;
-      if (!d) return i == x ? 1.0 : 0.0;
-      return zd > 0 ? exp((double)(__bfloat162float(d[i]) - md) / temp) / zd : 0.0;
-    };
-    if (!last && x >= 0 && x < vocab && (double)uniforms[2 * r] * q(x) < p(x)) {
-      if (threadIdx.x == 0) out[r0 + taken] = x;
-      ++taken;
-      continue;
-    }
-    const int per = (vocab + kVerifyThreads - 1) / kVerifyThreads, i0 = min((int)threadIdx.x * per, vocab), i1 = min(i0 + per, vocab);
-    for (int pass = 0; pass < 2; ++pass) {   // what is left of p; p itself where nothing is
-      auto w = [&](int i) { return pass ? p(i) : fmax(p(i) - q(i), 0.0); };
-      double own = 0;
-      for (int i = i0; i < i1; ++i) own += w(i);
-      part[threadIdx.x] = own;
-      if (threadIdx.x == 0) found = 0x7fffffff;
-      __syncthreads();
-      double before = 0, all = 0;
-      for (int i = 0; i < kVerifyThreads; ++i) {
-        if (i == (int)threadIdx.x) before = all;
-        all += part[i];
-      }
-      const double limit = (double)uniforms[2 * r + 1] * all;
-      double c = before;
-      for (int i = i0; i < i1; ++i) {
-        c += w(i);
-        if (c > limit) {
-          atomicMin(&found, i);
-          break;
+  const int slice = blockIdx.x, row = blockIdx.y, which = blockIdx.z;
+  if (threadIdx.x == 0) found = -1;
+  __syncthreads();
+  for (int s = threadIdx.x; s < n_seqs; s += kStatThreads)
+    if (starts[s] <= row && row < starts[s + 1]) found = s;
+  __syncthreads();
+  const int seq = found;
+  if (seq < 0) return;
+  const float temp = temperature ? temperature[seq] : 0.f;
+  if (which && (!(temp > 0.f) || row == starts[seq + 1] - 1)) return;   // no probabilities asked for
+  const __nv_bfloat16* l = which ? draft + (int64_t)row * ldd : target + (int64_t)row * ldt;
+  // entries from i0 on in groups of eight that start at 16-byte addresses (slice 0: the entries in front of the first such address as well)
+  const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7);
+  const int i0 = slice * kSlice, i1 = min(vocab, i0 + kSlice), a0 = i0 - shift;
+  float m = -INFINITY, s = 0.f;
+  int at = 0x7fffffff;
+  const float c = temp > 0.f ? 1.4426950408889634f / temp : 0.f;
+  constexpr int U = 4;
+  for (int g0 = threadIdx.x * 8; g0 < kSlice + 8; g0 += U * kStatThreads * 8) {
+    uint4 v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = a0 + g0 + u * kStatThreads * 8;
+      v[u] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+      if (i >= i0 && i + 8 <= i1) {
+        v[u] = ld_stream(l + i);
+      } else if (i + 8 > i0 && i < i1) {   // a group that crosses the slice's ends: its entries one by one
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const int k = i + 2 * j;
+          const uint32_t x = k >= i0 && k < i1 ? __bfloat16_as_ushort(l[k]) : 0xff80u, y = k + 1 >= i0 && k + 1 < i1 ? __bfloat16_as_ushort(l[k + 1]) : 0xff80u;
+          w[j] = x | y << 16;
         }
+        v[u] = make_uint4(w[0], w[1], w[2], w[3]);
       }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
+      const uint32_t h = max2(max2(w[0], w[1]), max2(w[2], w[3]));
+      const float top = fmaxf(bf16lo(h), bf16hi(h));
+      if (top > m) {
+        s *= tc::exp2_fast((m - top) * c);   // (m = -inf: s is 0)
+        m = top;
+        at = a0 + g0 + u * kStatThreads * 8;
+      }
+      if (temp > 0.f && m > -INFINITY) {
+        float e = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) e += tc::exp2_fast((bf16lo(w[j]) - m) * c) + tc::exp2_fast((bf16hi(w[j]) - m) * c);
+        s += e;
+      }
+    }
+  }
+  // the first place of the thread's largest entry
+  if (m > -INFINITY) {
+    for (int k = max(at, i0);; ++k)
+      if (__bfloat162float(l[k]) == m) {
+        at = k;
+        break;
+      }
+  }
+  auto join = [](float& m1, float& s1, int& at1, float m2, float s2, int at2, float c1) {
+    const float mn = fmaxf(m1, m2);
+    if (mn > -INFINITY) s1 = s1 * tc::exp2_fast((m1 - mn) * c1) + s2 * tc::exp2_fast((m2 - mn) * c1);
+    if (m2 > m1 || (m2 == m1 && at2 < at1)) at1 = at2;
+    m1 = mn;
+  };
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1)
+    join(m, s, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), __shfl_xor_sync(0xffffffffu, at, o), c);
+  if ((threadIdx.x & 31) == 0) sh_m[threadIdx.x >> 5] = m, sh_s[threadIdx.x >> 5] = s, sh_at[threadIdx.x >> 5] = at;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kStatThreads / 32; ++w) join(m, s, at, sh_m[w], sh_s[w], sh_at[w], c);
+    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {m, s, at, 0};
+  }
+}
+
+// a bf16 as a double by its bits (zero and denormals come out as 2^-127 to 2^-126, -inf as -2^128: nothing beside any logit that counts)
+__device__ __forceinline__ double bf16_double(uint32_t h) {
+  return __hiloint2double((int)((h & 0x8000u) << 16 | (((h & 0x7fffu) << 13) + (896u << 20))), 0);
+}
+// 2^t for t <= 0: t = n / 256 + r, 2^(n / 256) = 2^(n >> 8) table[n & 255], 2^r = 1 + r q(r), |r| <= 1 / 512, terms ln2^k / k! (the first left out: 1.4e-13)
+__device__ __forceinline__ double exp2_table(double t, const double* table) {
+  if (t < -1000.0) return 0.0;
+  const double u = t + 26388279066624.0;   // 1.5 * 2^44: n in the low bits
+  const double r = t - (u - 26388279066624.0);
+  const int n = __double2loint(u);
+  double q = fma(r, 0.05550410866482158, 0.24022650695910072);
+  q = fma(q, r, 0.6931471805599453);
+  const double b = table[n & 255], e = fma(b * r, q, b);
+  return __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
+}
+__device__ __forceinline__ double warp_sum_double(double v) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  return v;
+}
+
+__global__ void __launch_bounds__(kDrawThreads, 3) __cluster_dims__(kDrawCtas, 1, 1)
+verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const __nv_bfloat16* __restrict__ draft, int64_t ldd,
+                   const int32_t* __restrict__ tokens, const int32_t* __restrict__ starts, const float* __restrict__ temperature,
+                   const float* __restrict__ uniforms, int n_rows, int vocab, int n_slices, const Stat* __restrict__ stats, int32_t* __restrict__ out,
+                   int32_t* __restrict__ accepted) {
+  __shared__ double table[256], chunk_sum[kMostChunks], warp_part[2][kDrawThreads / 32], mine[2], shared_w;
+  __shared__ int sh_refused, sh_best, sh_chunk;
+  __shared__ float sh_m[2];
+  const cg::cluster_group cluster = cg::this_cluster();
+  const int rank = (int)cluster.block_rank(), s = blockIdx.x / kDrawCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (tid < 256) table[tid] = exp2(tid / 256.0);
+  pdl_wait();
+  pdl_launch_dependents();
+  const int r0 = min(max(starts[s], 0), n_rows), r1 = min(max(starts[s + 1], r0), n_rows);
+  const float temp = temperature ? temperature[s] : 0.f;
+  const bool greedy = !(temp > 0.f);
+  const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temp;
+  if (tid == 0) sh_refused = max(r1 - r0 - 1, 0);
+  __syncthreads();
+  // a warp a row: the slices' statistics, and whether the draft is refused
+  for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
+    double z[2] = {0.0, 0.0};
+    float m[2];
+    int at = 0x7fffffff;
+    const bool last = r == r1 - 1;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      m[k] = -INFINITY;
+      if (k && (greedy || last || !draft)) continue;
+      const Stat* st = stats + ((int64_t)r * 2 + k) * n_slices;
+      for (int i = lane; i < n_slices; i += 32) m[k] = fmaxf(m[k], st[i].m);
+      m[k] = warp_max(m[k]);
+      for (int i = lane; i < n_slices; i += 32) {
+        if (m[k] > -INFINITY) z[k] += (double)st[i].s * exp2_table(((double)st[i].m - (double)m[k]) * c, table);
+        if (!k && st[i].m == m[0]) at = min(at, st[i].at);
+      }
+      z[k] = warp_sum_double(z[k]);
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (m[0] == -INFINITY) at = 0;
+    const int x = last ? -1 : tokens[r];
+    bool ok = !last && x >= 0 && x < vocab && m[0] > -INFINITY;
+    if (ok && greedy) {
+      ok = x == at;
+    } else if (ok) {
+      const double p = exp2_table((bf16_double(__bfloat16_as_ushort(target[(int64_t)r * ldt + x])) - (double)m[0]) * c, table) / z[0];
+      double q = 1.0;
+      if (draft) q = m[1] > -INFINITY ? exp2_table((bf16_double(__bfloat16_as_ushort(draft[(int64_t)r * ldd + x])) - (double)m[1]) * c, table) / z[1] : 0.0;
+      ok = (double)uniforms[2 * r] * q < p;
+    }
+    if (!ok && lane == 0) atomicMin(&sh_refused, r - r0);
+  }
+  __syncthreads();
+  const int taken = sh_refused, row = r0 + taken;
+  const bool any = r1 > r0, last = row == r1 - 1;
+  // the row that draws: its largest logits again
+  if (any && warp == 0) {
+    int at = 0x7fffffff;
+    float m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      if (k && (greedy || last || !draft)) continue;
+      const Stat* st = stats + ((int64_t)row * 2 + k) * n_slices;
+      for (int i = lane; i < n_slices; i += 32) m[k] = fmaxf(m[k], st[i].m);
+      m[k] = warp_max(m[k]);
+      if (!k)
+        for (int i = lane; i < n_slices; i += 32)
+          if (st[i].m == m[0]) at = min(at, st[i].at);
+    }
+    at = __reduce_min_sync(0xffffffffu, at);
+    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = m[0] > -INFINITY ? at : 0;
+  }
+  __syncthreads();
+  if (rank == 0) {
+    if (tid == 0) accepted[s] = taken;
+    for (int r = r0 + tid; r < r1; r += kDrawThreads)
+      if (r != row) out[r] = r < row ? tokens[r] : -1;
+    if (any && tid == 0 && (greedy || sh_m[0] == -INFINITY)) out[row] = sh_best;
+  }
+  if (!any || greedy || sh_m[0] == -INFINITY) return;   // (the cluster's CTAs all leave here)
+
+  const __nv_bfloat16* l = target + (int64_t)row * ldt;
+  const bool residual = !last, probs = residual && draft && sh_m[1] > -INFINITY;
+  const __nv_bfloat16* d = probs ? draft + (int64_t)row * ldd : nullptr;
+  const int x = residual && !draft ? tokens[row] : -1;   // a certain draft: what is left has nothing of it
+  const double mp = (double)sh_m[0] * c, mq = probs ? (double)sh_m[1] * c : 0.0;
+  const int n_chunks = (vocab + kChunk - 1) / kChunk, per = (n_chunks + kDrawCtas - 1) / kDrawCtas;
+  const int ch0 = min(n_chunks, rank * per), ch1 = min(n_chunks, ch0 + per);
+  auto weight = [&](uint32_t h, double m) { return exp2_table(fma(bf16_double(h), c, -m), table); };
+  // the CTA's two sums -> the cluster's, in rank order; before: what the ranks in front have
+  auto cluster_sum = [&](double a, double b, double* all, double* before) {
+    if (tid == 0) mine[0] = a, mine[1] = b;
+    cluster.sync();
+    double t[2] = {0.0, 0.0};
+    for (int k = 0; k < kDrawCtas; ++k) {
+      const double* other = cluster.map_shared_rank(mine, k);
+      if (k == rank && before) *before = t[0];
+      t[0] += other[0], t[1] += other[1];
+    }
+    cluster.sync();   // (nobody writes again, or leaves, while another reads)
+    all[0] = t[0], all[1] = t[1];
+  };
+  double zp = 1.0, zq = 1.0;
+  if (probs) {
+    double a = 0.0, b = 0.0;
+    for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
+      const int i = ch * kChunk + 8 * lane;
+      if (i >= vocab) continue;
+      const uint4 v = load8(l, i, vocab), w = load8(d, i, vocab);
+      const uint32_t p4[4] = {v.x, v.y, v.z, v.w}, q4[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        a += weight(p4[j] & 0xffffu, mp) + weight(p4[j] >> 16, mp);
+        b += weight(q4[j] & 0xffffu, mq) + weight(q4[j] >> 16, mq);
+      }
+    }
+    a = warp_sum_double(a), b = warp_sum_double(b);
+    if (lane == 0) warp_part[0][warp] = a, warp_part[1][warp] = b;
+    __syncthreads();
+    a = b = 0.0;
+    for (int w = 0; w < kDrawThreads / 32; ++w) a += warp_part[0][w], b += warp_part[1][w];
+    double z[2];
+    cluster_sum(a, b, z, nullptr);
+    zp = 1.0 / z[0], zq = 1.0 / z[1];
+  }
+  for (int pass = residual ? 0 : 1; pass < 2; ++pass) {   // what the draft leaves of p; p itself behind the last draft, and where nothing is left
+    auto weights8 = [&](int i, double (&w)[8]) {
+      if (i >= vocab) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = 0.0;
+        return;
+      }
+      const uint4 v = load8(l, i, vocab);
+      const uint32_t p4[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+      for (int j = 0; j < 8; ++j) w[j] = weight(j & 1 ? p4[j >> 1] >> 16 : p4[j >> 1] & 0xffffu, mp) * zp;
+      if (pass) return;
+      if (probs) {
+        const uint4 q = load8(d, i, vocab);
+        const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int j = 0; j < 8; ++j) w[j] = fmax(w[j] - weight(j & 1 ? q4[j >> 1] >> 16 : q4[j >> 1] & 0xffffu, mq) * zq, 0.0);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j == x) w[j] = 0.0;
+    };
+    for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
+      double w[8];
+      weights8(ch * kChunk + 8 * lane, w);
+      const double t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+      if (lane == 0) chunk_sum[ch - ch0] = t;
+    }
+    __syncthreads();
+    if (tid == 0) {   // sums of the chunks in their order
+      double t = 0.0;
+      for (int i = 0; i < ch1 - ch0; ++i) t += chunk_sum[i], chunk_sum[i] = t;
+      shared_w = t;
+    }
+    __syncthreads();
+    double all[2], before = 0.0;
+    cluster_sum(shared_w, 0.0, all, &before);
+    if (all[0] == 0.0) continue;   // nothing left (pass 0): the cluster agrees
+    const double limit = (double)uniforms[2 * row + 1] * all[0];
+    if (tid == 0) sh_chunk = 0x7fffffff;
+    __syncthreads();
+    if (before + shared_w > limit && !(before > limit)) {   // the CTA that holds the border (each adds up the same numbers: there is one)
+      for (int i = tid; i < ch1 - ch0; i += kDrawThreads)
+        if (before + chunk_sum[i] > limit) atomicMin(&sh_chunk, i);
       __syncthreads();
-      token = found;
-      __syncthreads();
-      if (all > 0) break;
+      if (warp == 0) {
+        const int at = min(sh_chunk, ch1 - ch0 - 1), i = (ch0 + at) * kChunk + 8 * lane;
+        double w[8], t = 0.0;
+        weights8(i, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) t += w[j];
+        double front = t;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const double v = __shfl_up_sync(0xffffffffu, front, o);
+          if (lane >= o) front += v;
+        }
+        front += before + (at > 0 ? chunk_sum[at - 1] : 0.0) - t;
+        int token = 0x7fffffff, some = -1;   // the first entry above the limit; the last of any weight
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          front += w[j];
+          if (w[j] > 0.0) {
+            some = i + j;
+            if (front > limit && token == 0x7fffffff) token = i + j;
+          }
+        }
+        token = __reduce_min_sync(0xffffffffu, token);
+        some = __reduce_max_sync(0xffffffffu, some);
+        if (lane == 0) out[row] = token == 0x7fffffff ? some : token;
+      }
     }
     break;
   }
-  if (threadIdx.x == 0) {
-    accepted[s] = taken;
-    for (int r = r0 + taken; r < r1; ++r) out[r] = r == r0 + taken ? token : -1;
-  }
 }
+
+int slices(int vocab) { return (vocab + kSlice - 1) / kSlice; }
 
 }  // namespace
 
-int64_t verify_drafts_workspace_bytes(int n_rows, int vocab) { return 0; }
+int64_t verify_drafts_workspace_bytes(int n_rows, int vocab) { return (int64_t)n_rows * 2 * slices(vocab) * (int64_t)sizeof(Stat); }
 
 int verify_drafts(const __nv_bfloat16* target, int64_t ldt, const __nv_bfloat16* draft, int64_t ldd, const int32_t* tokens, const int32_t* starts,
                   const float* temperature, const float* uniforms, int n_seqs, int n_rows, int vocab, int32_t* out, int32_t* accepted, void* ws,
                   int64_t ws_bytes, cudaStream_t s) {
-  B200_CUDA(launch(verify_kernel, dim3(n_seqs), dim3(kVerifyThreads), 0, s, target, ldt, draft, ldd, tokens, starts, temperature, uniforms, n_rows, vocab, out,
-                   accepted));
+  B200_REQUIRE(vocab <= kMostVocab, B200_ERR_UNSUPPORTED, "verify_drafts: vocab=%d (at most %d)", vocab, kMostVocab);
+  B200_REQUIRE(n_rows <= 65535, B200_ERR_UNSUPPORTED, "verify_drafts: %d rows (at most 65535)", n_rows);
+  Stat* stats = static_cast<Stat*>(ws);
+  if (n_rows > 0)
+    B200_CUDA(launch(verify_stats_kernel, dim3(slices(vocab), n_rows, draft && temperature ? 2 : 1), dim3(kStatThreads), 0, s, target, ldt, draft, ldd, starts,
+                     temperature, n_seqs, vocab, stats));
+  const PdlScope draw(n_rows > 0);
+  B200_CUDA(launch(verify_draw_kernel, dim3(n_seqs * kDrawCtas), dim3(kDrawThreads), 0, s, target, ldt, draft, ldd, tokens, starts, temperature, uniforms, n_rows,
+                   vocab, slices(vocab), stats, out, accepted));
   return B200_OK;
 }
 

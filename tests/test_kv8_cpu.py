@@ -69,10 +69,13 @@ def _verify(**kw):
 @pytest.mark.parametrize("kw", [{"target": None}, {"tokens": None}, {"starts": None}, {"out": None}, {"kept": None}, {"uni": None}, {"S": -1}, {"n": -1}, {"V": 0},
                                 {"ldt": 999}, {"ldd": 999}, {"ws": None}, {"size": 8}, {"ws": BUF + 4}])
 def test_verify_refuses(kw):
-    if set(kw) & {"ws", "size"} and _lib().b200_verify_drafts_workspace_bytes(7, 1000) == 0:
-        pytest.skip("nothing to keep")
     assert _verify(**kw) == -1
     assert b"verify_drafts" in _lib().b200_last_error()
+
+
+def test_verify_has_limits():
+    assert _verify(V=2 ** 20 + 1, ldt=2 ** 21, ldd=2 ** 21) == -3 and b"1048576" in _lib().b200_last_error()
+    assert _verify(n=65536) == -3 and b"65535" in _lib().b200_last_error()
 
 
 def test_verify_of_no_sequences_is_nothing():
