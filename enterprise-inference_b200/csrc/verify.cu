@@ -1,17 +1,19 @@
 // Check of drafted tokens against the target's probabilities (b200_verify_drafts), two launches.
 //
 // stats: a CTA takes a slice of a logit row (target rows, and the rows that drafts were drawn from) and leaves its largest logit, the first place of it and the sum
-// of 2^((l - max) log2e / T) relative to it, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  Bound by the rows' bytes, closely
-// followed by instructions (about six an entry at 12 entries a cycle and SM).
+// of 2^(l c - f), c = log2e / T, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  f is the largest l c as a whole number,
+// so that l c - f is rounded once.  Bound by the rows' bytes, closely followed by the exponentials (12 entries a cycle and SM, of 16).
 // draw: a cluster of eight CTAs takes a sequence: the kept drafts from the slices' sums, then the token from the one row that draws it.  A draw next to a border of
 // the cumulated weights has to come out as in exact arithmetic (128 k borders: sums that are off by 1e-9 pick another token once in 4000 draws), so weights and
-// sums are fp64 there: 2^t by a table of 256 powers and a cubic, relative error below 2e-13, ten fp64 operations a weight.  Each CTA owns an eighth of the
-// row in chunks of 256 entries; sums are taken in a fixed order, chunk by chunk.
+// sums are fp64 there: 2^t by a table of 16 powers and a polynomial of degree 5, relative error below 2e-13, twelve fp64 operations a weight (256 powers and a cubic
+// are ten, but 32 lanes that look up 256 doubles meet in the banks of shared memory; 16 fill them exactly).  Each CTA owns an eighth of the
+// row in chunks of 256 entries, the target's fetched once into shared memory; sums are taken in a fixed order, chunk by chunk.
 #include <cooperative_groups.h>
 
 #include <algorithm>
 
 #include "kv8.cuh"
+#include "f32x2.cuh"
 #include "tc.cuh"
 
 namespace b200 {
@@ -19,26 +21,32 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kStatThreads = 256, kSlice = 8192;
-constexpr int kDrawThreads = 512, kDrawCtas = 8, kChunk = 256, kMostChunks = 512;
-constexpr int kMostVocab = kDrawCtas * kMostChunks * kChunk;
+constexpr int kStatThreads = 256, kLeastSlice = 2048;
+constexpr int kDrawThreads = 256, kDrawCtas = 8, kChunk = 256, kMostChunks = 192;
+constexpr int kMostVocab = kDrawCtas * kMostChunks * kChunk, kMostPart = kMostChunks * kChunk * 2;
 
 struct Stat {
-  float m, s;
-  int at, pad;
+  float m, f, s;
+  int at;
 };
+constexpr int kKnownRows = 64;   // rows of a sequence whose largest logits are kept
 
 // eight entries from index i on (-inf behind the end), 16 bytes at a time where the address allows it
+__device__ __forceinline__ bool whole8(const __nv_bfloat16* row, int i, int n) { return i + 8 <= n && (reinterpret_cast<uintptr_t>(row + i) & 15) == 0; }
 __device__ __forceinline__ uint4 load8(const __nv_bfloat16* row, int i, int n) {
-  const __nv_bfloat16* p = row + i;
-  if (i + 8 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0) return ld_stream(p);
+  if (whole8(row, i, n)) return ld_ro(row + i);
   uint32_t w[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const uint32_t a = i + 2 * j < n ? __bfloat16_as_ushort(p[2 * j]) : 0xff80u, b = i + 2 * j + 1 < n ? __bfloat16_as_ushort(p[2 * j + 1]) : 0xff80u;
+    const int k = i + 2 * j;
+    const uint32_t a = k < n ? __bfloat16_as_ushort(row[k]) : 0xff80u, b = k + 1 < n ? __bfloat16_as_ushort(row[k + 1]) : 0xff80u;
     w[j] = a | b << 16;
   }
   return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void fetch8(uint4* dst, const __nv_bfloat16* row, int i, int n) {   // -> shared memory
+  if (whole8(row, i, n)) f2::cp16(dst, row + i);
+  else *dst = load8(row, i, n);
 }
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -48,12 +56,10 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 
 __global__ void __launch_bounds__(kStatThreads)
 verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const __nv_bfloat16* __restrict__ draft, int64_t ldd, const int32_t* __restrict__ starts,
-                    const float* __restrict__ temperature, int n_seqs, int vocab, Stat* __restrict__ stats) {
+                    const float* __restrict__ temperature, int n_seqs, int vocab, int slice_len, Stat* __restrict__ stats) {
   __shared__ int found;
-  __shared__ float sh_m[kStatThreads / 32], sh_s[kStatThreads / 32];
-  __shared__ int sh_at[kStatThreads / 32];
+  __shared__ Stat sh[kStatThreads / 32];
   pdl_wait();
-  pdl_launch_dependents();
   const int slice = blockIdx.x, row = blockIdx.y, which = blockIdx.z;
   if (threadIdx.x == 0) found = -1;
   __syncthreads();
@@ -65,14 +71,14 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
   const float temp = temperature ? temperature[seq] : 0.f;
   if (which && (!(temp > 0.f) || row == starts[seq + 1] - 1)) return;   // no probabilities asked for
   const __nv_bfloat16* l = which ? draft + (int64_t)row * ldd : target + (int64_t)row * ldt;
-  // entries from i0 on in groups of eight that start at 16-byte addresses (slice 0: the entries in front of the first such address as well)
+  // entries from i0 on in groups of eight that start at 16-byte addresses (the slice's ends may lie inside a group)
   const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7);
-  const int i0 = slice * kSlice, i1 = min(vocab, i0 + kSlice), a0 = i0 - shift;
-  float m = -INFINITY, s = 0.f;
+  const int i0 = slice * slice_len, i1 = min(vocab, i0 + slice_len), a0 = i0 - shift;
+  float m = -INFINITY, f = 0.f, s = 0.f;
   int at = 0x7fffffff;
   const float c = temp > 0.f ? 1.4426950408889634f / temp : 0.f;
   constexpr int U = 4;
-  for (int g0 = threadIdx.x * 8; g0 < kSlice + 8; g0 += U * kStatThreads * 8) {
+  for (int g0 = threadIdx.x * 8; a0 + g0 < i1; g0 += U * kStatThreads * 8) {
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -97,18 +103,21 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
       const uint32_t h = max2(max2(w[0], w[1]), max2(w[2], w[3]));
       const float top = fmaxf(bf16lo(h), bf16hi(h));
       if (top > m) {
-        s *= tc::exp2_fast((m - top) * c);   // (m = -inf: s is 0)
+        const float fn = rintf(top * c);
+        s *= tc::exp2_fast(f - fn);   // (nothing yet: s is 0, f too)
+        f = fn;
         m = top;
         at = a0 + g0 + u * kStatThreads * 8;
       }
-      if (temp > 0.f && m > -INFINITY) {
-        float e = 0.f;
+      if (temp > 0.f) {   // (-inf alone so far: 2^-inf)
+        float e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e += tc::exp2_fast((bf16lo(w[j]) - m) * c) + tc::exp2_fast((bf16hi(w[j]) - m) * c);
-        s += e;
+        for (int j = 0; j < 4; ++j) e[j] = tc::exp2_fast(fmaf(bf16lo(w[j]), c, -f)) + tc::exp2_fast(fmaf(bf16hi(w[j]), c, -f));
+        s += (e[0] + e[1]) + (e[2] + e[3]);
       }
     }
   }
+  pdl_launch_dependents();   // (before the rows are read the next launch's CTAs would only take their places: 112 -> 141 us)
   // the first place of the thread's largest entry
   if (m > -INFINITY) {
     for (int k = max(at, i0);; ++k)
@@ -117,37 +126,43 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
         break;
       }
   }
-  auto join = [](float& m1, float& s1, int& at1, float m2, float s2, int at2, float c1) {
-    const float mn = fmaxf(m1, m2);
-    if (mn > -INFINITY) s1 = s1 * tc::exp2_fast((m1 - mn) * c1) + s2 * tc::exp2_fast((m2 - mn) * c1);
-    if (m2 > m1 || (m2 == m1 && at2 < at1)) at1 = at2;
-    m1 = mn;
+  auto join = [](float& m1, float& f1, float& s1, int& at1, float m2, float f2, float s2, int at2) {
+    if (m2 > -INFINITY) {
+      const float fn = m1 > -INFINITY ? fmaxf(f1, f2) : f2;
+      s1 = s1 * tc::exp2_fast(m1 > -INFINITY ? f1 - fn : 0.f) + s2 * tc::exp2_fast(f2 - fn);
+      f1 = fn;
+      if (m2 > m1 || (m2 == m1 && at2 < at1)) m1 = m2, at1 = at2;
+    }
   };
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1)
-    join(m, s, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, s, o), __shfl_xor_sync(0xffffffffu, at, o), c);
-  if ((threadIdx.x & 31) == 0) sh_m[threadIdx.x >> 5] = m, sh_s[threadIdx.x >> 5] = s, sh_at[threadIdx.x >> 5] = at;
+    join(m, f, s, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, f, o), __shfl_xor_sync(0xffffffffu, s, o),
+         __shfl_xor_sync(0xffffffffu, at, o));
+  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = {m, f, s, at};
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kStatThreads / 32; ++w) join(m, s, at, sh_m[w], sh_s[w], sh_at[w], c);
-    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {m, s, at, 0};
+    for (int w = 1; w < kStatThreads / 32; ++w) join(m, f, s, at, sh[w].m, sh[w].f, sh[w].s, sh[w].at);
+    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {m, f, s, at};
   }
 }
 
 // a bf16 as a double by its bits (zero and denormals come out as 2^-127 to 2^-126, -inf as -2^128: nothing beside any logit that counts)
-__device__ __forceinline__ double bf16_double(uint32_t h) {
-  return __hiloint2double((int)((h & 0x8000u) << 16 | (((h & 0x7fffu) << 13) + (896u << 20))), 0);
+__device__ __forceinline__ double float_double(uint32_t f) {   // f: the value's fp32 bits
+  return __hiloint2double((int)(((f >> 3) & 0x0fffffffu) + 0x38000000u | (f & 0x80000000u)), 0);
 }
-// 2^t for t <= 0: t = n / 256 + r, 2^(n / 256) = 2^(n >> 8) table[n & 255], 2^r = 1 + r q(r), |r| <= 1 / 512, terms ln2^k / k! (the first left out: 1.4e-13)
+__device__ __forceinline__ double bf16_double(uint32_t h) { return float_double(h << 16); }
+// 2^t for t <= 0 (or little more): t = n / 16 + r, 2^(n / 16) = 2^(n >> 4) table[n & 15], 2^r = 1 + r q(r), |r| <= 1 / 32, terms ln2^k / k! (the first left out: 1.5e-13)
 __device__ __forceinline__ double exp2_table(double t, const double* table) {
-  if (t < -1000.0) return 0.0;
-  const double u = t + 26388279066624.0;   // 1.5 * 2^44: n in the low bits
-  const double r = t - (u - 26388279066624.0);
+  const double u = t + 422212465065984.0;   // 1.5 * 2^48: n in the low bits
+  const double r = t - (u - 422212465065984.0);
   const int n = __double2loint(u);
-  double q = fma(r, 0.05550410866482158, 0.24022650695910072);
+  double q = fma(r, 0.0013333558146428441, 0.009618129107628477);
+  q = fma(q, r, 0.05550410866482158);
+  q = fma(q, r, 0.24022650695910072);
   q = fma(q, r, 0.6931471805599453);
-  const double b = table[n & 255], e = fma(b * r, q, b);
-  return __hiloint2double(__double2hiint(e) + ((n >> 8) << 20), __double2loint(e));
+  const double b = table[n & 15], e = fma(b * r, q, b);
+  const bool none = (uint32_t)__double2hiint(t) > 0xc08f4000u;   // t < -1000
+  return __hiloint2double(none ? 0 : __double2hiint(e) + ((n >> 4) << 20), none ? 0 : __double2loint(e));
 }
 __device__ __forceinline__ double warp_sum_double(double v) {
 #pragma unroll
@@ -155,77 +170,85 @@ __device__ __forceinline__ double warp_sum_double(double v) {
   return v;
 }
 
-__global__ void __launch_bounds__(kDrawThreads, 3) __cluster_dims__(kDrawCtas, 1, 1)
+__global__ void __launch_bounds__(kDrawThreads, 4) __cluster_dims__(kDrawCtas, 1, 1)
 verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const __nv_bfloat16* __restrict__ draft, int64_t ldd,
                    const int32_t* __restrict__ tokens, const int32_t* __restrict__ starts, const float* __restrict__ temperature,
                    const float* __restrict__ uniforms, int n_rows, int vocab, int n_slices, const Stat* __restrict__ stats, int32_t* __restrict__ out,
                    int32_t* __restrict__ accepted) {
-  __shared__ double table[256], chunk_sum[kMostChunks], warp_part[2][kDrawThreads / 32], mine[2], shared_w;
-  __shared__ int sh_refused, sh_best, sh_chunk;
-  __shared__ float sh_m[2];
+  extern __shared__ __align__(16) unsigned char row_smem[];   // the CTA's part of the target row
+  __shared__ double table[16], chunk_sum[kMostChunks], warp_part[2][kDrawThreads / 32], mine[2], shared_w;
+  __shared__ int sh_refused, sh_best, sh_chunk, known_at[kKnownRows];
+  __shared__ float sh_m[2], known_m[kKnownRows][2];
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), s = blockIdx.x / kDrawCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid < 256) table[tid] = exp2(tid / 256.0);
+  if (tid < 16) table[tid] = exp2(tid / 16.0);
   pdl_wait();
   pdl_launch_dependents();
   const int r0 = min(max(starts[s], 0), n_rows), r1 = min(max(starts[s + 1], r0), n_rows);
   const float temp = temperature ? temperature[s] : 0.f;
   const bool greedy = !(temp > 0.f);
-  const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temp;
+  const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temp, cf = greedy ? 0.0 : (double)(1.4426950408889634f / temp);   // cf: what the sums have
   if (tid == 0) sh_refused = max(r1 - r0 - 1, 0);
   __syncthreads();
-  // a warp a row: the slices' statistics, and whether the draft is refused
-  for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
-    double z[2] = {0.0, 0.0};
-    float m[2];
-    int at = 0x7fffffff;
-    const bool last = r == r1 - 1;
+  // a row's largest logits and their first place, from the slices (by a warp)
+  auto row_stats = [&](int r, float (&m)[2], float (&f)[2], double (&z)[2], int& at, bool sums) {
+    at = 0x7fffffff;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      m[k] = -INFINITY;
-      if (k && (greedy || last || !draft)) continue;
+      m[k] = -INFINITY, f[k] = -INFINITY, z[k] = 0.0;
+      if (k && (greedy || r == r1 - 1 || !draft)) continue;
       const Stat* st = stats + ((int64_t)r * 2 + k) * n_slices;
-      for (int i = lane; i < n_slices; i += 32) m[k] = fmaxf(m[k], st[i].m);
-      m[k] = warp_max(m[k]);
       for (int i = lane; i < n_slices; i += 32) {
-        if (m[k] > -INFINITY) z[k] += (double)st[i].s * exp2_table(((double)st[i].m - (double)m[k]) * c, table);
-        if (!k && st[i].m == m[0]) at = min(at, st[i].at);
+        const Stat x = st[i];
+        if (x.m > -INFINITY) f[k] = fmaxf(f[k], x.f);
+        if (!k && (x.m > m[0] || (x.m == m[0] && x.at < at))) at = x.at;
+        m[k] = fmaxf(m[k], x.m);
       }
+      const float own = m[k];
+      m[k] = warp_max(own), f[k] = warp_max(f[k]);
+      if (!k) at = __reduce_min_sync(0xffffffffu, own == m[0] ? at : 0x7fffffff);
+      if (!sums || !(m[k] > -INFINITY)) continue;
+      for (int i = lane; i < n_slices; i += 32)
+        if (st[i].m > -INFINITY) z[k] += (double)st[i].s * exp2_table((double)st[i].f - (double)f[k], table);
       z[k] = warp_sum_double(z[k]);
     }
-    at = __reduce_min_sync(0xffffffffu, at);
     if (m[0] == -INFINITY) at = 0;
+  };
+  // a warp a row: is the draft refused?
+  for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
+    double z[2];
+    float m[2], f[2];
+    int at;
+    const bool last = r == r1 - 1;
     const int x = last ? -1 : tokens[r];
-    bool ok = !last && x >= 0 && x < vocab && m[0] > -INFINITY;
+    bool ok = !last && x >= 0 && x < vocab;
+    // (asked for before the sums are there)
+    const uint32_t lx = ok ? __bfloat16_as_ushort(target[(int64_t)r * ldt + x]) : 0u, dx = ok && draft ? __bfloat16_as_ushort(draft[(int64_t)r * ldd + x]) : 0u;
+    const double u = ok && !greedy ? (double)uniforms[2 * r] : 0.0;
+    row_stats(r, m, f, z, at, !greedy);
+    if (lane == 0 && r - r0 < kKnownRows) known_m[r - r0][0] = m[0], known_m[r - r0][1] = m[1], known_at[r - r0] = at;
+    ok = ok && m[0] > -INFINITY;
     if (ok && greedy) {
       ok = x == at;
     } else if (ok) {
-      const double p = exp2_table((bf16_double(__bfloat16_as_ushort(target[(int64_t)r * ldt + x])) - (double)m[0]) * c, table) / z[0];
-      double q = 1.0;
-      if (draft) q = m[1] > -INFINITY ? exp2_table((bf16_double(__bfloat16_as_ushort(draft[(int64_t)r * ldd + x])) - (double)m[1]) * c, table) / z[1] : 0.0;
-      ok = (double)uniforms[2 * r] * q < p;
+      const double p = exp2_table(fma(bf16_double(lx), cf, -(double)f[0]), table) / z[0];
+      const double q = !draft ? 1.0 : m[1] > -INFINITY ? exp2_table(fma(bf16_double(dx), cf, -(double)f[1]), table) / z[1] : 0.0;
+      ok = u * q < p;
     }
     if (!ok && lane == 0) atomicMin(&sh_refused, r - r0);
   }
   __syncthreads();
   const int taken = sh_refused, row = r0 + taken;
   const bool any = r1 > r0, last = row == r1 - 1;
-  // the row that draws: its largest logits again
-  if (any && warp == 0) {
-    int at = 0x7fffffff;
-    float m[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int k = 0; k < 2; ++k) {
-      if (k && (greedy || last || !draft)) continue;
-      const Stat* st = stats + ((int64_t)row * 2 + k) * n_slices;
-      for (int i = lane; i < n_slices; i += 32) m[k] = fmaxf(m[k], st[i].m);
-      m[k] = warp_max(m[k]);
-      if (!k)
-        for (int i = lane; i < n_slices; i += 32)
-          if (st[i].m == m[0]) at = min(at, st[i].at);
-    }
-    at = __reduce_min_sync(0xffffffffu, at);
-    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = m[0] > -INFINITY ? at : 0;
+  // the row that draws: its largest logits
+  if (any && taken < kKnownRows) {
+    if (tid == 0) sh_m[0] = known_m[taken][0], sh_m[1] = known_m[taken][1], sh_best = known_at[taken];
+  } else if (any && warp == 0) {
+    double z[2];
+    float m[2], f[2];
+    int at;
+    row_stats(row, m, f, z, at, false);
+    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = at;
   }
   __syncthreads();
   if (rank == 0) {
@@ -240,10 +263,18 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   const bool residual = !last, probs = residual && draft && sh_m[1] > -INFINITY;
   const __nv_bfloat16* d = probs ? draft + (int64_t)row * ldd : nullptr;
   const int x = residual && !draft ? tokens[row] : -1;   // a certain draft: what is left has nothing of it
-  const double mp = (double)sh_m[0] * c, mq = probs ? (double)sh_m[1] * c : 0.0;
+  double mp = (double)sh_m[0] * c, mq = probs ? (double)sh_m[1] * c : 0.0;
   const int n_chunks = (vocab + kChunk - 1) / kChunk, per = (n_chunks + kDrawCtas - 1) / kDrawCtas;
   const int ch0 = min(n_chunks, rank * per), ch1 = min(n_chunks, ch0 + per);
-  auto weight = [&](uint32_t h, double m) { return exp2_table(fma(bf16_double(h), c, -m), table); };
+  // the CTA's entries, -inf behind the end (a thread reads back what it wrote: its eight of every 16th chunk)
+  uint4* part_p = reinterpret_cast<uint4*>(row_smem);
+  for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
+    const int i = ch * kChunk + 8 * lane, at = (ch - ch0) * (kChunk / 8) + lane;
+    fetch8(part_p + at, l, i, vocab);
+  }
+  f2::cp_wait_all();
+  // entry j of eight, relative to 2^m
+  auto weight = [&](const uint32_t* w, int j, double m) { return exp2_table(fma(float_double(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16), c, -m), table); };
   // the CTA's two sums -> the cluster's, in rank order; before: what the ranks in front have
   auto cluster_sum = [&](double a, double b, double* all, double* before) {
     if (tid == 0) mine[0] = a, mine[1] = b;
@@ -257,19 +288,13 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     cluster.sync();   // (nobody writes again, or leaves, while another reads)
     all[0] = t[0], all[1] = t[1];
   };
-  double zp = 1.0, zq = 1.0;
   if (probs) {
     double a = 0.0, b = 0.0;
     for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
-      const int i = ch * kChunk + 8 * lane;
-      if (i >= vocab) continue;
-      const uint4 v = load8(l, i, vocab), w = load8(d, i, vocab);
+      const uint4 v = part_p[(ch - ch0) * (kChunk / 8) + lane], w = load8(d, ch * kChunk + 8 * lane, vocab);
       const uint32_t p4[4] = {v.x, v.y, v.z, v.w}, q4[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        a += weight(p4[j] & 0xffffu, mp) + weight(p4[j] >> 16, mp);
-        b += weight(q4[j] & 0xffffu, mq) + weight(q4[j] >> 16, mq);
-      }
+      for (int j = 0; j < 8; ++j) a += weight(p4, j, mp), b += weight(q4, j, mq);
     }
     a = warp_sum_double(a), b = warp_sum_double(b);
     if (lane == 0) warp_part[0][warp] = a, warp_part[1][warp] = b;
@@ -278,25 +303,24 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     for (int w = 0; w < kDrawThreads / 32; ++w) a += warp_part[0][w], b += warp_part[1][w];
     double z[2];
     cluster_sum(a, b, z, nullptr);
-    zp = 1.0 / z[0], zq = 1.0 / z[1];
+    mp += log2(z[0]), mq += log2(z[1]);   // from here on probabilities
   }
   for (int pass = residual ? 0 : 1; pass < 2; ++pass) {   // what the draft leaves of p; p itself behind the last draft, and where nothing is left
-    auto weights8 = [&](int i, double (&w)[8]) {
-      if (i >= vocab) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = 0.0;
-        return;
-      }
-      const uint4 v = load8(l, i, vocab);
+    auto weights8 = [&](int ch, double (&w)[8]) {
+      const int at = (ch - ch0) * (kChunk / 8) + lane, i = ch * kChunk + 8 * lane;
+      const uint4 v = part_p[at];
       const uint32_t p4[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = weight(j & 1 ? p4[j >> 1] >> 16 : p4[j >> 1] & 0xffffu, mp) * zp;
+      for (int j = 0; j < 8; ++j) w[j] = weight(p4, j, mp);
       if (pass) return;
       if (probs) {
         const uint4 q = load8(d, i, vocab);
         const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
-        for (int j = 0; j < 8; ++j) w[j] = fmax(w[j] - weight(j & 1 ? q4[j >> 1] >> 16 : q4[j >> 1] & 0xffffu, mq) * zq, 0.0);
+        for (int j = 0; j < 8; ++j) {
+          const double left = w[j] - weight(q4, j, mq);
+          w[j] = left > 0.0 ? left : 0.0;
+        }
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j)
@@ -304,15 +328,31 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     };
     for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
       double w[8];
-      weights8(ch * kChunk + 8 * lane, w);
+      weights8(ch, w);
       const double t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
       if (lane == 0) chunk_sum[ch - ch0] = t;
     }
     __syncthreads();
-    if (tid == 0) {   // sums of the chunks in their order
-      double t = 0.0;
-      for (int i = 0; i < ch1 - ch0; ++i) t += chunk_sum[i], chunk_sum[i] = t;
-      shared_w = t;
+    if (warp == 0) {   // running sums of the chunks: kMostChunks / 32 neighbours a lane, then over the lanes
+      constexpr int N = kMostChunks / 32;
+      double t[N], sum = 0.0;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const int at = lane * N + i;
+        sum += at < ch1 - ch0 ? chunk_sum[at] : 0.0;
+        t[i] = sum;
+      }
+      double front = sum;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double v = __shfl_up_sync(0xffffffffu, front, o);
+        if (lane >= o) front += v;
+      }
+      const double prev = __shfl_up_sync(0xffffffffu, front, 1), base = lane ? prev : 0.0;
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (lane * N + i < ch1 - ch0) chunk_sum[lane * N + i] = base + t[i];
+      if (lane == 31) shared_w = front;
     }
     __syncthreads();
     double all[2], before = 0.0;
@@ -323,12 +363,12 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     __syncthreads();
     if (before + shared_w > limit && !(before > limit)) {   // the CTA that holds the border (each adds up the same numbers: there is one)
       for (int i = tid; i < ch1 - ch0; i += kDrawThreads)
-        if (before + chunk_sum[i] > limit) atomicMin(&sh_chunk, i);
+        if (before + chunk_sum[i] > limit) atomicMin(&sh_chunk, i);   // (rounding may leave none: the last)
       __syncthreads();
       if (warp == 0) {
         const int at = min(sh_chunk, ch1 - ch0 - 1), i = (ch0 + at) * kChunk + 8 * lane;
         double w[8], t = 0.0;
-        weights8(i, w);
+        weights8(ch0 + at, w);   // (another warp's entries: the barriers in between)
 #pragma unroll
         for (int j = 0; j < 8; ++j) t += w[j];
         double front = t;
@@ -356,11 +396,19 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   }
 }
 
-int slices(int vocab) { return (vocab + kSlice - 1) / kSlice; }
+// slices of a row: 24 CTAs an SM, each of at least kLeastSlice entries
+int slice_length(int n_rows, int vocab) {
+  const int64_t want = std::max<int64_t>(1, kNumSMs * 24 / std::max(1, 2 * n_rows));
+  return (int)std::max<int64_t>(kLeastSlice, ((vocab + want - 1) / want + 7) / 8 * 8);
+}
+int slices(int n_rows, int vocab) {
+  const int len = slice_length(n_rows, vocab);
+  return (vocab + len - 1) / len;
+}
 
 }  // namespace
 
-int64_t verify_drafts_workspace_bytes(int n_rows, int vocab) { return (int64_t)n_rows * 2 * slices(vocab) * (int64_t)sizeof(Stat); }
+int64_t verify_drafts_workspace_bytes(int n_rows, int vocab) { return (int64_t)n_rows * 2 * slices(n_rows, vocab) * (int64_t)sizeof(Stat); }
 
 int verify_drafts(const __nv_bfloat16* target, int64_t ldt, const __nv_bfloat16* draft, int64_t ldd, const int32_t* tokens, const int32_t* starts,
                   const float* temperature, const float* uniforms, int n_seqs, int n_rows, int vocab, int32_t* out, int32_t* accepted, void* ws,
@@ -368,12 +416,15 @@ int verify_drafts(const __nv_bfloat16* target, int64_t ldt, const __nv_bfloat16*
   B200_REQUIRE(vocab <= kMostVocab, B200_ERR_UNSUPPORTED, "verify_drafts: vocab=%d (at most %d)", vocab, kMostVocab);
   B200_REQUIRE(n_rows <= 65535, B200_ERR_UNSUPPORTED, "verify_drafts: %d rows (at most 65535)", n_rows);
   Stat* stats = static_cast<Stat*>(ws);
+  const int n = slices(n_rows, vocab), per = ((vocab + kChunk - 1) / kChunk + kDrawCtas - 1) / kDrawCtas, smem = per * kChunk * 2;
+  static bool done[64] = {};
+  B200_CUDA(ensure_dynamic_smem(verify_draw_kernel, kMostPart, done));
   if (n_rows > 0)
-    B200_CUDA(launch(verify_stats_kernel, dim3(slices(vocab), n_rows, draft && temperature ? 2 : 1), dim3(kStatThreads), 0, s, target, ldt, draft, ldd, starts,
-                     temperature, n_seqs, vocab, stats));
+    B200_CUDA(launch(verify_stats_kernel, dim3(n, n_rows, draft && temperature ? 2 : 1), dim3(kStatThreads), 0, s, target, ldt, draft, ldd, starts,
+                     temperature, n_seqs, vocab, slice_length(n_rows, vocab), stats));
   const PdlScope draw(n_rows > 0);
-  B200_CUDA(launch(verify_draw_kernel, dim3(n_seqs * kDrawCtas), dim3(kDrawThreads), 0, s, target, ldt, draft, ldd, tokens, starts, temperature, uniforms, n_rows,
-                   vocab, slices(vocab), stats, out, accepted));
+  B200_CUDA(launch(verify_draw_kernel, dim3(n_seqs * kDrawCtas), dim3(kDrawThreads), (size_t)smem, s, target, ldt, draft, ldd, tokens, starts, temperature, uniforms, n_rows,
+                   vocab, n, stats, out, accepted));
   return B200_OK;
 }
 

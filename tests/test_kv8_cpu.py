@@ -74,7 +74,7 @@ def test_verify_refuses(kw):
 
 
 def test_verify_has_limits():
-    assert _verify(V=2 ** 20 + 1, ldt=2 ** 21, ldd=2 ** 21) == -3 and b"1048576" in _lib().b200_last_error()
+    assert _verify(V=393217, ldt=2 ** 21, ldd=2 ** 21) == -3 and b"393216" in _lib().b200_last_error()
     assert _verify(n=65536) == -3 and b"65535" in _lib().b200_last_error()
 
 
