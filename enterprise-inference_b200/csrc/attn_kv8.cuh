@@ -1,5 +1,6 @@
 // Attention over the 8-bit cache: what its kernels (attn_kv8_cols.cu, attn_kv8_rows.cu) and their host side (attn_kv8.cu) share.
 #pragma once
+#include "f32x2.cuh"
 #include "kv8.cuh"
 #include "tc.cuh"
 
@@ -12,6 +13,15 @@ constexpr int kKv8PartFloats = 132;    // of a pair in a part: 128 sums, their m
 // rows [row0, row0 + nrows) of one sequence that share its keys and values; nrows 0: none
 struct Kv8Group {
   int row0, nrows, seq, ctx;   // ctx: the longest context, within the block table
+};
+
+// work of the rows kernel: rows of one sequence over the cache tiles [tile0, tile1); `parts` neighbours from item `first` on share the rows
+struct Kv8Rows {
+  int row0, nrows, seq, ctx, tile0, tile1, first, parts;
+};
+// what a plan found; its groups come right behind
+struct Kv8Head {
+  int groups, items, pad[2];
 };
 
 // CTA a's last item continues in `parts` - 1 further CTAs
@@ -29,6 +39,9 @@ struct Kv8Params {
   const Kv8Group* groups;      // a plan's groups (groups[-1].row0 of them), or null: found among the rows themselves
   float* part;                 // [CTA][2][pairs][kKv8PartFloats]: of an item that began in an earlier CTA, of one that goes on in the next
   Kv8Cut* cuts;                // [CTA]
+  const Kv8Head* head;         // of a plan
+  const Kv8Rows* items;
+  float* part_rows;            // [item x kv head][128 pairs][kKv8PartFloats], of items in parts
   uint32_t* status;
   int64_t n_blocks;
   int bt_stride, T, hq, hkv, block_size, group_rows;   // group_rows: rows of a group at most
@@ -42,9 +55,39 @@ struct Kv8Maps {
 int kv8_maps(const Kv8Attn& a, int box_rows, Kv8Maps* m);
 
 int kv8_cols_launch(const Kv8Maps& m, const Kv8Params& p, int cols, int grid, cudaStream_t s);
+int kv8_rows_launch(const Kv8Maps& m, const Kv8Params& p, int grid, cudaStream_t s);
 
 __device__ __forceinline__ int kv8_ctx(const Kv8Params& p, int row) {
   return (int)min((int64_t)__ldg(p.ctx_lens + row), (int64_t)p.bt_stride * p.block_size);
+}
+
+// byte (row r, byte b) of an operand in rows of 128 bytes, 128-byte swizzle
+__device__ __forceinline__ int operand_off(int r, int b) { return (r >> 3) * 1024 + (r & 7) * 128 + ((((b >> 4) ^ r) & 7) << 4) + (b & 15); }
+
+// eight entries (16 bytes) of a query whose entries 16 neighbouring lanes have: scaled by a power of two to [128, 256), as e4m3 and LO times what that rounding left;
+// returns the factor that undoes the scaling.  With LO = 16 both terms are exact down to 2^-14 of the largest entry, with 1 to 2^-10, and off by at most 2^-23
+// (2^-19) of it below.
+template <int LO>
+__device__ __forceinline__ float split_query(const uint4 v, uint2& hi, uint2& lo) {
+  const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+  uint32_t m = 0;   // the largest magnitude, as bf16 bits
+#pragma unroll
+  for (int j = 0; j < 4; ++j) m = max(m, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  const uint32_t e = max(m >> 7, 8u);   // biased exponent; 255: not a number
+  const float f = __uint_as_float((261u - min(e, 254u)) << 23);
+  uint32_t h4[4], l4[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = bf16lo(x[j]) * f, b = bf16hi(x[j]) * f;
+    h4[j] = e == 255u ? 0x7f7fu : e4m3x2(a, b);
+    const float2 r = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h4[j], __NV_E4M3)));
+    l4[j] = e4m3x2((a - r.x) * (float)LO, (b - r.y) * (float)LO);
+  }
+  hi = make_uint2(h4[0] | h4[1] << 16, h4[2] | h4[3] << 16);
+  lo = make_uint2(l4[0] | l4[1] << 16, l4[2] | l4[3] << 16);
+  return __uint_as_float((min(e, 254u) - 7u) << 23);
 }
 
 // the warp's largest value; NaN if one is

@@ -52,9 +52,6 @@ struct Cols {
   static_assert(kSmem + 8 * (kThreads + kThreads / 32) <= 232448, "shared memory");
 };
 
-// byte (row r, byte b) of an operand in rows of 128 bytes
-__device__ __forceinline__ int operand_off(int r, int b) { return (r >> 3) * 1024 + (r & 7) * 128 + ((((b >> 4) ^ r) & 7) << 4) + (b & 15); }
-
 // group i: of the plan, or the one that starts at row i
 __device__ __forceinline__ Kv8Group find_group(const Kv8Params& p, int i) {
   if (p.groups) return p.groups[i];
@@ -98,6 +95,14 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   int* shared_int = reinterpret_cast<int*>(x_max + CG * 2 * NCG * 4);        // 0: tensor memory, 1: a wait ran out, 2, 3: the share's first and last item
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Waits wait(reinterpret_cast<uint32_t*>(shared_int + 1), p.status);
+  if (p.groups) {
+    pdl_wait();
+    if (p.groups[-1].row0 == 0) {   // a plan without groups
+      if (threadIdx.x == 0) p.cuts[blockIdx.x].parts = 0;
+      pdl_launch_dependents();
+      return;
+    }
+  }
   __shared__ uint64_t scan_warp[kThreads / 32], scan_thread[kThreads];
 
   if (threadIdx.x == 0) {
@@ -323,31 +328,12 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int c = c1 + 2 * u + (lane >> 4);
-            const uint32_t x[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-            uint32_t m = 0;   // the largest magnitude, as bf16 bits
-#pragma unroll
-            for (int j = 0; j < 4; ++j) m = max(m, max(x[j] & 0x7fffu, (x[j] >> 16) & 0x7fffu));
-#pragma unroll
-            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-            const uint32_t e = max(m >> 7, 8u);   // biased exponent
-            const float f = __uint_as_float((261u - min(e, 254u)) << 23);
-            uint32_t hi[2], lo[2];
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              hi[j] = lo[j] = 0u;
-#pragma unroll
-              for (int k = 0; k < 2; ++k) {
-                const float a = bf16lo(x[2 * j + k]) * f, b = bf16hi(x[2 * j + k]) * f;
-                const uint32_t h = e == 255u ? 0x7f7fu : e4m3x2(a, b);
-                const float2 r = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
-                hi[j] |= h << (16 * k);
-                lo[j] |= e4m3x2((a - r.x) * 16.f, (b - r.y) * 16.f) << (16 * k);
-              }
-            }
+            uint2 hi, lo;
+            const float back = split_query<16>(v[u], hi, lo);
             if (c < ncol) {
-              *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = make_uint2(hi[0], hi[1]);
-              *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = make_uint2(lo[0], lo[1]);
-              if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = __uint_as_float((min(e, 254u) - 7u) << 23) * p.scale2;
+              *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = hi;
+              *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = lo;
+              if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = back * p.scale2;
             }
           }
         }
