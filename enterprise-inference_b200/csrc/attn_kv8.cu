@@ -42,19 +42,17 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Params p, int ba
     }
     return;
   }
-  const int slot = block - kNumSMs;
-  if (slot >= p.head->items * p.hkv) return;
-  const Kv8Rows w = p.items[slot / p.hkv];
-  if (w.parts < 2 || w.first != slot / p.hkv) return;
-  const int64_t step = (int64_t)p.hkv * 128 * kKv8PartFloats;
-  for (int c = blockIdx.y * 8 + warp; c < w.nrows * G; c += 8 * gridDim.y) {
-    const float* x = p.part_rows + ((int64_t)slot * 128 + c) * kKv8PartFloats;
-    join_parts(x, x + step, step, w.parts, p.out + (int64_t)(w.row0 + c / G) * p.ldo + (slot % p.hkv * G + c % G) * kHeadDim);
+  const Kv8Cut cut = p.cuts_rows[block - kNumSMs];
+  if (cut.parts < 2) return;
+  const int64_t step = 2ll * 128 * kKv8PartFloats;
+  for (int c = blockIdx.y * 8 + warp; c < cut.nrows * G; c += 8 * gridDim.y) {
+    const float* x = p.part_rows + (2 * (int64_t)(block - kNumSMs) * 128 + c) * kKv8PartFloats;
+    join_parts(x + 128 * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
   }
 }
 
 // ---- plan: rows -> runs of one sequence -> groups of few pairs (columns kernel) and items of a tile of pairs or two (rows kernel).  One CTA. ----
-constexpr int kPlanThreads = 1024, kLeastPart = 4;   // tiles of a part at least
+constexpr int kPlanThreads = 1024;
 
 // exclusive scan over the CTA of two counts; returns the totals
 __device__ __forceinline__ int2 plan_scan(int& a, int& b, int2* sh) {
@@ -79,13 +77,34 @@ __device__ __forceinline__ int2 plan_scan(int& a, int& b, int2* sh) {
   return make_int2(__shfl_sync(0xffffffffu, w.x, 31), __shfl_sync(0xffffffffu, w.y, 31));
 }
 
-__global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params p, int short_rows, Kv8Head* head, Kv8Group* groups, Kv8Rows* items, int* starts) {
+// block 0: the plan; the others: the rows kernel's queries, as two e4m3 terms and a factor each (16 lanes a query)
+__global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params p, int short_rows, Kv8Head* head, Kv8Group* groups, Kv8Group* rows, int* runs,
+                                                                uint8_t* q_hi, uint8_t* q_lo, float* q_scale) {
   __shared__ int2 sh[32];
-  __shared__ Kv8Rows whole[kNumSMs];
-  __shared__ int sh_length;
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = 128 / (p.hq / p.hkv);
+  if (blockIdx.x > 0) {
+    const int64_t pairs = (int64_t)p.T * p.hq, step = (int64_t)(gridDim.x - 1) * (kPlanThreads / 16);
+    for (int64_t i0 = (int64_t)(blockIdx.x - 1) * (kPlanThreads / 16); i0 < pairs; i0 += step) {
+      const int64_t i = i0 + (tid >> 4);
+      const bool in = i < pairs;
+      const int row = in ? (int)(i / p.hq) : 0, h = in ? (int)(i % p.hq) : 0, d = (tid & 15) * 8;
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)row * p.ldq + h * kHeadDim + d));
+      uint32_t m = query_max(v);
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+      const uint32_t e = query_exponent(m);
+      uint2 hi, lo;
+      split_query<1>(v, e, hi, lo);
+      if (in) {
+        *reinterpret_cast<uint2*>(q_hi + i * kHeadDim + d) = hi;
+        *reinterpret_cast<uint2*>(q_lo + i * kHeadDim + d) = lo;
+        if (d == 0) q_scale[i] = fmaxf(query_back(e) * fabsf(p.scale2), 1e-37f);   // (a scale of zero: keys behind the context are still -inf)
+      }
+    }
+    return;
+  }
   auto seq_of = [&](int r) { return p.row_to_seq ? __ldg(p.row_to_seq + r) : r; };
   // the runs' first rows
   int n_runs = 0;
@@ -94,19 +113,20 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
     const int flag = r < p.T && (r == 0 || seq_of(r) != seq_of(r - 1));
     int at = flag, none = 0;
     const int n = plan_scan(at, none, sh).x;
-    if (flag) starts[n_runs + at] = r;
+    if (flag) runs[n_runs + at] = r;
     n_runs += n;
   }
   __syncthreads();
-  auto run_rows = [&](int i) { return i < n_runs ? (i + 1 < n_runs ? starts[i + 1] : p.T) - starts[i] : 0; };
-  // items of two tiles of pairs where that leaves every SM one
+  auto run_rows = [&](int i) { return i < n_runs ? (i + 1 < n_runs ? runs[i + 1] : p.T) - runs[i] : 0; };
+  // items of two tiles of pairs where that leaves every SM one, and most of them are full
   int n1 = 0, n2 = 0;
   for (int i = tid; i < n_runs; i += kPlanThreads) {
     const int n = run_rows(i);
     if (n > short_rows) n1 += (n + R - 1) / R, n2 += (n + 2 * R - 1) / (2 * R);
   }
   const int2 both = plan_scan(n1, n2, sh);
-  const int per = both.y * p.hkv >= kNumSMs ? 2 * R : R;
+  const bool two = both.y * p.hkv >= kNumSMs && 2 * both.x >= 3 * both.y;
+  const int per = two ? 2 * R : R;
   int n_groups = 0, n_items = 0;
   for (int i0 = 0; i0 < n_runs; i0 += kPlanThreads) {
     const int i = i0 + tid, n = run_rows(i);
@@ -114,64 +134,76 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
     int ga = n > 0 && n <= short_rows, it = mine;
     const bool group = ga;
     const int2 all = plan_scan(ga, it, sh);
-    if (group) groups[n_groups + ga] = {starts[i], n, seq_of(starts[i]), 0};
-    for (int k = 0; k < mine; ++k) items[n_items + it + k] = {starts[i] + k * per, min(per, n - k * per), seq_of(starts[i]), 0, 0, 0, n_items + it + k, 1};
+    if (group) groups[n_groups + ga] = {runs[i], n, seq_of(runs[i]), 0};
+    for (int k = 0; k < mine; ++k) rows[n_items + it + k] = {runs[i] + k * per, min(per, n - k * per), seq_of(runs[i]), 0};
     n_groups += all.x, n_items += all.y;
   }
   __syncthreads();
   // the longest context of each; zeros for rows of which none sees anything
   for (int i = warp; i < n_groups + n_items; i += kPlanThreads / 32) {
-    const bool group = i < n_groups;
-    const int row0 = group ? groups[i].row0 : items[i - n_groups].row0, n = group ? groups[i].nrows : items[i - n_groups].nrows;
+    Kv8Group* const g = i < n_groups ? groups + i : rows + i - n_groups;
+    const int row0 = g->row0, n = g->nrows;
     int ctx = 0;
     for (int r = lane; r < n; r += 32) ctx = max(ctx, kv8_ctx(p, row0 + r));
     ctx = __reduce_max_sync(0xffffffffu, ctx);
-    if (lane == 0) {
-      if (group) groups[i].ctx = ctx;
-      else items[i - n_groups].ctx = ctx, items[i - n_groups].tile1 = (ctx + kKv8Tile - 1) / kKv8Tile;
-    }
+    if (lane == 0) g->ctx = ctx;
     if (ctx <= 0)
       for (int r = 0; r < n; ++r)
         for (int c = lane; c < p.hq * kHeadDim / 8; c += 32) *reinterpret_cast<uint4*>(p.out + (int64_t)(row0 + r) * p.ldo + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
   }
+  const int n_list = n_items * p.hkv + 2 * kNumSMs + 1;   // places that the list may use, and the one behind them
+  for (int i = tid; i < n_list; i += kPlanThreads) p.items[i].cta = -1;
+  if (tid < kNumSMs) p.starts[tid] = -1, p.cuts_rows[tid].parts = 0;
   __syncthreads();
-  // fewer items than SMs: their contexts in parts, as short as lets every SM have one part at most
-  const int room = kNumSMs / p.hkv;
-  if (n_items > 0 && n_items < room) {
-    if (tid < n_items) whole[tid] = items[tid];
-    __syncthreads();
-    if (warp == 0) {
-      int lo = kLeastPart, hi = 1;
-      for (int i = lane; i < n_items; i += 32) hi = max(hi, whole[i].tile1);
-      hi = max(lo, __reduce_max_sync(0xffffffffu, hi));
-      while (lo < hi) {   // the smallest length whose parts fit
-        const int mid = (lo + hi) / 2;
-        int n = 0;
-        for (int i = lane; i < n_items; i += 32) n += max(1, (whole[i].tile1 + mid - 1) / mid);
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (n <= room) hi = mid;
-        else lo = mid + 1;
+  if (two) {
+    // whole items, the longest contexts (the last rows) first, every other round backwards
+    const int n = n_items * p.hkv, rounds = (n + kNumSMs - 1) / kNumSMs;
+    for (int i = tid; i < n; i += kPlanThreads) {
+      const int round = i / kNumSMs, k = i % kNumSMs, cta = round & 1 ? kNumSMs - 1 - k : k, u = n - 1 - i;
+      const Kv8Group g = rows[u / p.hkv];
+      // a CTA's items have places of their own: one a round, and one behind them (the last round may have nothing for it)
+      p.items[cta * (rounds + 1) + round] = {g.row0, g.nrows, g.seq, g.ctx, 0, (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile, u % p.hkv, cta, 1, 0, {0, 0}};
+      if (round == 0) p.starts[cta] = cta * (rounds + 1);
+    }
+  } else {
+    // one tile of pairs: the flattened list of (item, kv head, tile) in equal shares
+    int tiles = 0, none = 0;
+    for (int i = tid; i < n_items; i += kPlanThreads) tiles += (max(rows[i].ctx, 0) + kKv8Tile - 1) / kKv8Tile;
+    const int total = plan_scan(tiles, none, sh).x * p.hkv, share = max(1, (total + kNumSMs - 1) / kNumSMs);
+    int front = 0;
+    for (int i0 = 0; i0 < n_items; i0 += kPlanThreads) {
+      const int i = i0 + tid;
+      Kv8Group g = {0, 0, 0, 0};
+      if (i < n_items) g = rows[i];
+      const int nt = (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile;
+      int base = nt;
+      none = 0;
+      const int all = plan_scan(base, none, sh).x;
+      base = (front + base) * p.hkv;
+      front += all;
+      for (int h = 0; h < p.hkv && nt > 0; ++h, base += nt) {
+        const int k0 = base / share, k1 = (base + nt - 1) / share;
+        for (int k = k0; k <= k1; ++k) {
+          const int from = max(base, k * share), to = min(base + nt, (k + 1) * share), place = i * p.hkv + h + k;
+          p.items[place] = {g.row0, g.nrows, g.seq, g.ctx, from - base, to - base, h, k, k1 - k0 + 1, 2 * k + (k == k0 ? 1 : 0), {0, 0}};
+          if (from == k * share) p.starts[k] = place;
+          if (k == k0 && k1 > k0) p.cuts_rows[k] = {g.row0, g.nrows, h, k1 - k0 + 1};
+        }
       }
-      if (lane == 0) sh_length = lo;
     }
-    __syncthreads();
-    const int length = sh_length, parts = tid < n_items ? max(1, (whole[tid].tile1 + length - 1) / length) : 0;
-    int at = parts, none = 0;
-    const int n = plan_scan(at, none, sh).x;
-    for (int k = 0; k < parts; ++k) {
-      Kv8Rows w = whole[tid];
-      w.tile0 = k * length, w.tile1 = min(w.tile1, (k + 1) * length), w.first = at, w.parts = parts;
-      items[at + k] = w;
-    }
-    n_items = n;
   }
-  if (tid == 0) *head = {n_groups, n_items, {0, 0}};
+  if (tid == 0) *head = {n_groups, {0, 0, 0}};
 }
 
 constexpr int kShortPairs = 8;    // (row, head) pairs of a group of the columns kernel in steps of longer runs
 constexpr int64_t kCutBytes = (kNumSMs * sizeof(Kv8Cut) + 255) / 256 * 256;
-constexpr int64_t kPartBytes = (int64_t)kNumSMs * 2 * kKv8Cols * kKv8PartFloats * 4, kPartRowsBytes = (int64_t)kNumSMs * 128 * kKv8PartFloats * 4;
-int64_t plan_bytes(int T) { return (int64_t)sizeof(Kv8Head) + (int64_t)T * sizeof(Kv8Group) + ((int64_t)T + kNumSMs) * sizeof(Kv8Rows) + (int64_t)T * 4; }
+constexpr int64_t kPartBytes = (int64_t)kNumSMs * 2 * kKv8Cols * kKv8PartFloats * 4, kPartRowsBytes = (int64_t)kNumSMs * 2 * 128 * kKv8PartFloats * 4;
+// places of the list of items: one for each and one for each CTA, or (whole items) a round's for every CTA and one behind them
+int64_t list_places(int T, int hkv) { return (int64_t)T * hkv + 3 * kNumSMs; }
+int64_t plan_bytes(int T, int hkv) {
+  return (2 * kCutBytes + (int64_t)sizeof(Kv8Head) + 2ll * T * sizeof(Kv8Group) + list_places(T, hkv) * sizeof(Kv8Rows) + (int64_t)T * 4 + 255) / 256 * 256;
+}
+int64_t query_bytes(int T, int hq) { return (int64_t)T * hq * kHeadDim; }   // of a term; a 32nd of it the factors
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
                                   const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -204,7 +236,19 @@ int kv8_maps(const Kv8Attn& a, int box_rows, Kv8Maps* m) {
   return B200_OK;
 }
 
-int64_t paged_attn_fp8_workspace_bytes(int T, int hq, int hkv) { return kCutBytes + kPartBytes + kPartRowsBytes + plan_bytes(T); }
+// [rows][heads][128] bytes of a query's term, boxes of n rows by the heads of a kv head
+int kv8_query_map(const uint8_t* q, int T, int hq, int G, int n, CUtensorMap* m) {
+  const EncodeTiledFn fn = encode_fn();
+  B200_REQUIRE(fn != nullptr, B200_ERR_CUDA, "cuTensorMapEncodeTiled is not available from the driver");
+  const cuuint64_t dims[3] = {kHeadDim, (cuuint64_t)hq, (cuuint64_t)T}, stride[2] = {kHeadDim, (cuuint64_t)hq * kHeadDim};
+  const cuuint32_t box[3] = {kHeadDim, (cuuint32_t)G, (cuuint32_t)n}, one[3] = {1, 1, 1};
+  const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<uint8_t*>(q), dims, stride, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  B200_REQUIRE(r == CUDA_SUCCESS, B200_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d) for %d rows of %d queries", (int)r, T, hq);
+  return B200_OK;
+}
+
+int64_t paged_attn_fp8_workspace_bytes(int T, int hq, int hkv) { return kCutBytes + kPartBytes + kPartRowsBytes + plan_bytes(T, hkv) + 2 * query_bytes(T, hq) + query_bytes(T, hq) / 32; }
 
 int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaStream_t s) {
   B200_REQUIRE((int64_t)a.T * a.hkv * (((int64_t)a.bt_stride * a.block_size + kKv8Tile - 1) / kKv8Tile) < 0x7fffffffll, B200_ERR_UNSUPPORTED,
@@ -241,20 +285,30 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
     B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs, (most * G + 7) / 8), dim3(256), 0, s, p, 0));
     return B200_OK;
   }
-  Kv8Head* const head = reinterpret_cast<Kv8Head*>(w + kCutBytes + kPartBytes + kPartRowsBytes);
-  Kv8Group* const groups = reinterpret_cast<Kv8Group*>(head + 1);
-  Kv8Rows* const items = reinterpret_cast<Kv8Rows*>(groups + a.T);
+  char* at = w + kCutBytes + kPartBytes + kPartRowsBytes;
+  p.cuts_rows = reinterpret_cast<Kv8Cut*>(at);
+  p.starts = reinterpret_cast<int*>(at + kCutBytes);
+  Kv8Head* const head = reinterpret_cast<Kv8Head*>(at + 2 * kCutBytes);
+  Kv8Group *const groups = reinterpret_cast<Kv8Group*>(head + 1), *const rows = groups + a.T;
+  p.items = reinterpret_cast<Kv8Rows*>(rows + a.T);
   const bool drafts = most > 0 && most * G <= 128;   // runs of a tile of pairs at most: all of them to the rows kernel
   const int short_rows = drafts ? 0 : std::max(1, kShortPairs / G);
-  B200_CUDA(launch(kv8_plan_kernel, dim3(1), dim3(kPlanThreads), 0, s, p, short_rows, head, groups, items, reinterpret_cast<int*>(items + a.T + kNumSMs)));
+  uint8_t* const q_hi = reinterpret_cast<uint8_t*>(w + kCutBytes + kPartBytes + kPartRowsBytes + plan_bytes(a.T, a.hkv));
+  uint8_t* const q_lo = q_hi + query_bytes(a.T, a.hq);
+  float* const q_scale = reinterpret_cast<float*>(q_lo + query_bytes(a.T, a.hq));
+  Kv8QueryMaps qm;
+  for (int i = 0; i < 4; ++i)
+    if (const int rc = kv8_query_map(i & 1 ? q_lo : q_hi, a.T, a.hq, G, (i < 2 ? 128 : 32) / G, i < 2 ? (i ? &qm.lo : &qm.hi) : (i == 3 ? &qm.lo32 : &qm.hi32))) return rc;
+  const int64_t blocks = ((int64_t)a.T * a.hq + kPlanThreads / 16 - 1) / (kPlanThreads / 16);
+  B200_CUDA(launch(kv8_plan_kernel, dim3(1 + (int)std::min<int64_t>(blocks, 2 * kNumSMs)), dim3(kPlanThreads), 0, s, p, short_rows, head, groups, rows,
+                   reinterpret_cast<int*>(p.items + list_places(a.T, a.hkv)), q_hi, q_lo, q_scale));
   const PdlScope after;
-  p.head = head;
-  p.items = items;
+  p.q_scale = q_scale;
   if (!drafts) {
     p.groups = groups;
     if (const int rc = kv8_cols_launch(maps, p, short_rows * G, kNumSMs, s)) return rc;
   }
-  if (const int rc = kv8_rows_launch(maps, p, kNumSMs, s)) return rc;
+  if (const int rc = kv8_rows_launch(maps, qm, p, kNumSMs, s)) return rc;
   B200_CUDA(launch(kv8_join_kernel, dim3(drafts ? kNumSMs : 2 * kNumSMs, 4), dim3(256), 0, s, p, drafts ? kNumSMs : 0));
   return B200_OK;
 }

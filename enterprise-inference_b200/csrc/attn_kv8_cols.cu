@@ -329,11 +329,15 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           for (int u = 0; u < U; ++u) {
             const int c = c1 + 2 * u + (lane >> 4);
             uint2 hi, lo;
-            const float back = split_query<16>(v[u], hi, lo);
+            uint32_t m = query_max(v[u]);
+#pragma unroll
+            for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+            const uint32_t e = query_exponent(m);
+            split_query<16>(v[u], e, hi, lo);
             if (c < ncol) {
               *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = hi;
               *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = lo;
-              if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = back * p.scale2;
+              if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = query_back(e) * p.scale2;
             }
           }
         }
@@ -343,7 +347,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       }
     }
   } else if (warp == C::kSpare) {
-    // ===== factors: a token's 2^key exponent, and 256 * 2^(value exponent - the tile's largest); four tokens a lane.  The exponents are fetched four
+    // ===== factors: a token's 2^key exponent, and 256 * 2^(value exponent - the tile's largest) (in units of kE4m3Unit); four tokens a lane.  The exponents are fetched four
     // tiles ahead, their places in the cache eight (bulk copies of 128 bytes took the issuing warp 400 cycles each) =====
     constexpr int D = 4;
     const int stride = p.hkv * p.block_size;
@@ -409,7 +413,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           none = __any_sync(0xffffffffu, none);
           float vf[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vf[j] = ve[j] == 255u ? -0.f : __uint_as_float((uint32_t)max((int)(ve[j] - m) + 135, 0) << 23);
+          for (int j = 0; j < 4; ++j) vf[j] = ve[j] == 255u ? -0.f : __uint_as_float((uint32_t)max((int)(ve[j] - m) + 15, 0) << 23);
           // the slot is tile n - 2's until that one's weights are ready
           if (n >= kFacs) wait(w_ready + (n & 1), ((n - 2) >> 1) & 1);
           float* f = reinterpret_cast<float*>(facs + (n & (kFacs - 1)) * kFacBytes);
@@ -530,17 +534,10 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           }
           unsigned char* wb = ws + (n & 1) * C::kOperand;
 #pragma unroll
-          for (int j = 0; j < NCG; j += 2) {
-            const float a = wt[j], b = j + 1 < NCG ? wt[(j + 1) % NCG] : 0.f;
-            const uint32_t h = e4m3x2(a, b);
-            const float2 r = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)h, __NV_E4M3)));
-            const uint32_t g = e4m3x2((a - r.x) * 16.f, (b - r.y) * 16.f);
-            wb[operand_off(c0 + j, tau)] = (unsigned char)h;
-            wb[operand_off(NP + c0 + j, tau)] = (unsigned char)g;
-            if (j + 1 < NCG) {
-              wb[operand_off(c0 + j + 1, tau)] = (unsigned char)(h >> 8);
-              wb[operand_off(NP + c0 + j + 1, tau)] = (unsigned char)(g >> 8);
-            }
+          for (int j = 0; j < NCG; ++j) {   // (a weight that is not a number leaves its denominator so, whatever its codes)
+            const uint32_t two = e4m3_two<16>(wt[j]);
+            wb[operand_off(c0 + j, tau)] = (unsigned char)two;
+            wb[operand_off(NP + c0 + j, tau)] = (unsigned char)(two >> 8);
           }
           if (grp == 0 && __float_as_int(vr.y) != 0) {
             // value rows behind the context may hold anything, and 0 * NaN = NaN: zero them under their zero weights

@@ -9,6 +9,7 @@
 //
 // Bound by the exponentials (16 a cycle and SM) and by the shared-memory reads of the MMAs' operands.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_kv8.cuh"
 
@@ -22,46 +23,17 @@ constexpr int kOperand = 128 * 128;                  // a term of 128 queries; a
 constexpr int kKSlots = 3, kVSlots = 2, kWide = 3;   // tiles of codes, halves of widened values
 constexpr int kFacBytes = kHalf * 4 + 16;            // the keys' factors; the values' reference exponent
 constexpr int kStage = 8 * 2048;
-constexpr int kBars = 2 * kKSlots + 2 * kVSlots + 2 * kWide + 12 + 3 + 1;
-constexpr int kSmem = 1024 + 4 * kOperand + kWide * kOperand + (kKSlots + kVSlots) * kOperand + kStage + kWide * kFacBytes + 2 * 256 * 4 + kBars * 8 + 16;
+constexpr int kBars = 2 * kKSlots + 2 * kVSlots + 2 * kWide + 12 + 3 + 1;   // (and the two words behind them)
+constexpr int kSmem = 1024 + 4 * kOperand + kWide * kOperand + (kKSlots + kVSlots) * kOperand + kStage + kWide * kFacBytes + kBars * 8 + 16;
 static_assert(kSmem <= 232448, "shared memory");
 
 __device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | (1u << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
-struct Unit {
-  Kv8Rows w;
-  int kvh, slot;
-};
-
-// an item's queries -> the two terms of its one or two tiles, and their factors, by 128 threads: 16 lanes a pair
-__device__ __forceinline__ void stage_queries(const Kv8Params& p, unsigned char* qs, float* scale, const Unit& u, int R, int G, int thread) {
-  const int pieces = (u.w.nrows > R ? 2 : 1) * 128 * 16, chunk = thread & 15;
-  const __nv_bfloat16* q0 = p.q + (int64_t)u.w.row0 * p.ldq + (int64_t)u.kvh * G * kHeadDim + chunk * 8;
-  constexpr int U = 4;
-#pragma unroll 1
-  for (int e0 = thread; e0 < pieces; e0 += U * 128) {
-    uint4 v[U];
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int m = (e0 + i * 128) >> 4, r = (m & 127) / G, row = (m >> 7) * R + r;
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (r < R && row < u.w.nrows) v[i] = __ldg(reinterpret_cast<const uint4*>(q0 + (int64_t)row * p.ldq + ((m & 127) % G) * kHeadDim));
-    }
-#pragma unroll
-    for (int i = 0; i < U; ++i) {
-      const int m = (e0 + i * 128) >> 4;
-      uint2 hi, lo;
-      const float back = split_query<1>(v[i], hi, lo);
-      unsigned char* dst = qs + (m >> 7) * 2 * kOperand + operand_off(m & 127, chunk * 8);
-      *reinterpret_cast<uint2*>(dst) = hi;
-      *reinterpret_cast<uint2*>(dst + kOperand) = lo;
-      if (chunk == 0) scale[m] = fmaxf(back * fabsf(p.scale2), 1e-37f);   // (a scale of zero: keys behind the context are still -inf)
-    }
-  }
-}
+// an item of at most 32 pairs has them in each quarter of the MMA's rows: a quarter's warp takes a quarter of the keys
+__device__ __forceinline__ bool few_pairs(const Kv8Rows& w, int G) { return w.nrows * G <= 32; }
 
 __global__ void __launch_bounds__(kThreads, 1)
-kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
+kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv8QueryMaps qmaps, const Kv8Params p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* qs = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);   // [tile][term]
   unsigned char* wide = qs + 4 * kOperand;               // [kWide][2 x 64 dims][64 keys] f16
@@ -69,8 +41,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   unsigned char* vring = kring + kKSlots * kOperand;
   unsigned char* ostage = vring + kVSlots * kOperand;
   unsigned char* facs = ostage + kStage;
-  float* q_scale = reinterpret_cast<float*>(facs + kWide * kFacBytes);   // [2 items][256]
-  uint64_t* k_full = reinterpret_cast<uint64_t*>(q_scale + 2 * 256);
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(facs + kWide * kFacBytes);
   uint64_t* k_free = k_full + kKSlots;
   uint64_t* v_full = k_free + kKSlots;
   uint64_t* v_free = v_full + kVSlots;
@@ -90,7 +61,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     for (int s = 0; s < kVSlots; ++s) mbar_init(v_full + s, 1), mbar_init(v_free + s, 4);
     for (int s = 0; s < kWide; ++s) mbar_init(w_full + s, 4), mbar_init(w_free + s, 1);
     for (int s = 0; s < 4; ++s) mbar_init(s_full + s, 1), mbar_init(p_ready + s, 4), mbar_init(o_full + s, 1);
-    mbar_init(q_ready, 4);
+    mbar_init(q_ready, 1);
     mbar_init(q_free, 1);
     mbar_init(last, 1);
     tmem_slot[1] = 0;
@@ -98,9 +69,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   }
   pdl_wait();
   pdl_launch_dependents();
-  const Kv8Head head = *p.head;
-  const int n_units = head.items * p.hkv, grid = gridDim.x;
-  if ((int)blockIdx.x >= n_units) return;
+  if (p.starts[blockIdx.x] < 0) return;   // nothing for this CTA
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -110,14 +79,16 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   fence_after();
   const uint32_t tmem = *tmem_slot;   // per tile of pairs 256 columns: scores of even, odd halves, O
   const int G = p.hq / p.hkv, R = 128 / G;
-  // units in turn, the longest first, every other round backwards
-  auto unit = [&](int round, Unit& u) {
-    const int i = round * grid + ((round & 1) ? grid - 1 - (int)blockIdx.x : (int)blockIdx.x);
-    if (i >= n_units) return false;
-    u.slot = n_units - 1 - i;
-    u.kvh = u.slot % p.hkv;
-    u.w = p.items[u.slot / p.hkv];
-    return u.w.tile1 > u.w.tile0;   // (rows that see nothing: the plan wrote their zeros)
+  // the CTA's items, in the plan's order; the one behind the next is asked for
+  int at = p.starts[blockIdx.x];
+  Kv8Rows ahead = p.items[at];
+  auto next_unit = [&](Kv8Rows& u) {
+    for (;;) {
+      u = ahead;
+      if (u.cta != (int)blockIdx.x) return false;
+      ahead = p.items[++at];
+      if (u.tile1 > u.tile0) return true;   // (rows that see nothing: the plan wrote their zeros)
+    }
   };
 
   if (warp < 8) {
@@ -126,20 +97,142 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     const int x = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + x * 256;
     const int r = m / G, row = x * R + r;
-    int n = 0, half = 0, item = 0;   // halves of this tile of pairs, of the CTA; items
-    Unit u;
-    for (int round = 0; round * grid < n_units; ++round) {
-      if (!unit(round, u)) continue;
-      const Kv8Rows& w = u.w;
+    int n = 0, half = 0;   // halves of this tile of pairs, of the CTA
+    auto rescale = [&](int n, float fo) {   // O of the halves before n
+      wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
+      fence_after();
+#pragma unroll 1
+      for (int c = 0; c < kHeadDim; c += 16) {
+        uint32_t o[16];
+        ld16(base + 128 + c, o);
+        ld_wait<16>(o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
+        st16(base + 128 + c, o);
+      }
+    };
+    // an item of at most 32 pairs: lane = pair, this warp's 16 keys of each half; the four quarters' sums are joined at the end
+    auto few = [&](const Kv8Rows& w, int h0, int h1, int& n, int& half) {
+      const bool alive = lane < w.nrows * G;
+      const int fr = lane / G, t = w.row0 + fr, ctx = alive ? kv8_ctx(p, t) : 0;
+      const float qf = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + lane % G) : 1.f;
+      float mu = -INFINITY, l = 0.f;
+      int ref = 0;
+#pragma unroll 1
+      for (int h = h0; h < h1; ++h, ++n, ++half) {
+        const int b = half % kWide;
+        const float* f = reinterpret_cast<const float*>(facs + b * kFacBytes);
+        wait(s_full + (n & 1), (n >> 1) & 1);
+        wait(w_full + b, (half / kWide) & 1);
+        fence_after();
+        const uint32_t s_addr = base + (n & 1) * kHalf;
+        uint32_t s[16];
+        ld16(s_addr + 16 * quad, s);
+        const int ref_new = reinterpret_cast<const int*>(f)[kHalf], live = ctx - h * kHalf - 16 * quad;
+        float k[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(k + 4 * j) = reinterpret_cast<const float4*>(f)[4 * quad + j];
+        ld_wait<16>(s);
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const float v = j < live ? __uint_as_float(s[j]) * k[j] : -INFINITY;
+          s[j] = __float_as_uint(v);
+          mx = fmaxf(mx, v);
+        }
+        mx *= qf;
+        const bool jump = mx > mu + 8.f;
+        if (__any_sync(0xffffffffu, jump) || ref_new != ref) {
+          const float mn = jump ? mx : mu;
+          float fo = jump && mu != -INFINITY ? exp2_fast(mu - mn) : 1.f;
+          l *= fo;
+          mu = mn;
+          if (h > h0) {
+            fo *= __uint_as_float((uint32_t)max(127 - (ref_new - ref), 0) << 23);
+            if (__any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
+          }
+          ref = ref_new;
+        }
+        const float shift = 7.f - (mu > -INFINITY ? mu : 0.f);
+        uint32_t pk[8], none[8];
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float p0 = exp2_fast(fmaf(__uint_as_float(s[2 * j]), qf, shift)), p1 = exp2_fast(fmaf(__uint_as_float(s[2 * j + 1]), qf, shift));
+          sum += p0 + p1;
+          const __half2 h2 = __floats2half2_rn(p0, p1);
+          pk[j] = *reinterpret_cast<const uint32_t*>(&h2);
+          none[j] = 0u;
+        }
+        l += sum;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) st8(s_addr + 8 * c, c == quad ? pk : none);   // (other quarters' keys: nothing)
+        st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + (n & 1));
+      }
+      wait(o_full + ((n - 1) & 1), ((n - 1) >> 1) & 1);
+      fence_after();
+      // the quarters' maxima and denominators, then their sums, 32 columns at a time
+      float2* ml = reinterpret_cast<float2*>(ostage);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      ml[m] = make_float2(mu, l);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float top = -INFINITY, all = 0.f;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[32 * k + lane].x);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) all += ml[32 * k + lane].y * (top == -INFINITY ? 0.f : exp2_fast(ml[32 * k + lane].x - top));
+      const float back = __uint_as_float((uint32_t)max(ref - 7, 1) << 23), own = mu == -INFINITY ? 0.f : exp2_fast(mu - top);
+      const float mult = own * (w.parts > 1 ? back : all == 0.f ? 0.f : back / all);
+      const int head = w.kvh * G + lane % G;
+      float* part = p.part_rows + ((int64_t)w.slot * 128 + lane) * kKv8PartFloats;
+      if (w.parts > 1 && alive && quad == 0) part[128] = top, part[129] = all;
+#pragma unroll 1
+      for (int c = 0; c < kHeadDim; c += 32) {
+        uint32_t o[32];
+        ld32(base + 128 + c, o);
+        ld_wait<32>(o);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          *reinterpret_cast<float4*>(ostage + quad * 4096 + j * 512 + lane * 16) =
+              make_float4(__uint_as_float(o[4 * j]) * mult, __uint_as_float(o[4 * j + 1]) * mult, __uint_as_float(o[4 * j + 2]) * mult, __uint_as_float(o[4 * j + 3]) * mult);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        float y[8] = {};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const float4 v = *reinterpret_cast<const float4*>(ostage + k * 4096 + (2 * quad + j) * 512 + lane * 16);
+            y[4 * j] += v.x, y[4 * j + 1] += v.y, y[4 * j + 2] += v.z, y[4 * j + 3] += v.w;
+          }
+        if (alive && w.parts > 1) {
+          *reinterpret_cast<float4*>(part + c + 8 * quad) = make_float4(y[0], y[1], y[2], y[3]);
+          *reinterpret_cast<float4*>(part + c + 8 * quad + 4) = make_float4(y[4], y[5], y[6], y[7]);
+        } else if (alive) {
+          *reinterpret_cast<uint4*>(p.out + (int64_t)t * p.ldo + head * kHeadDim + c + 8 * quad) =
+              make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+        }
+      }
+      fence_before();
+    };
+    Kv8Rows w;
+    while (next_unit(w)) {
       const int h0 = 2 * w.tile0, h1 = min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf);
-      ++item;
       if (x == 1 && w.nrows <= R) {   // the item has one tile of pairs
         half += h1 - h0;
         continue;
       }
+      if (few_pairs(w, G)) {
+        few(w, h0, h1, n, half);
+        continue;
+      }
       const bool alive = r < R && row < w.nrows, any = __any_sync(0xffffffffu, alive);
       const int t = w.row0 + row, ctx = alive ? kv8_ctx(p, t) : 0;
-      float qf = 0.f, mu = -INFINITY, l = 0.f;
+      const float qf = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + m % G) : 1.f;
+      float mu = -INFINITY, l = 0.f;
       int ref = 0;
       for (int h = h0; h < h1; ++h, ++n, ++half) {
         const int b = half % kWide;
@@ -150,7 +243,6 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
           continue;
         }
-        if (h == h0) qf = q_scale[(item & 1) * 256 + x * 128 + m];
         fence_after();
         const uint32_t s_addr = base + (n & 1) * kHalf;
         uint32_t s[64];
@@ -180,19 +272,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           mu = mn;
           if (h > h0) {
             fo *= __uint_as_float((uint32_t)max(127 - (ref_new - ref), 0) << 23);
-            if (__any_sync(0xffffffffu, fo != 1.f)) {
-              wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
-              fence_after();
-#pragma unroll 1
-              for (int c = 0; c < kHeadDim; c += 16) {
-                uint32_t o[16];
-                ld16(base + 128 + c, o);
-                ld_wait<16>(o);
-#pragma unroll
-                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
-                st16(base + 128 + c, o);
-              }
-            }
+            if (__any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
           }
           ref = ref_new;
         }
@@ -225,7 +305,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       const float back = __uint_as_float((uint32_t)max(ref - 7, 1) << 23);   // 2^(ref - 134): values and weights as they are, but for the 2^7 that l has too
       const float mult = w.parts > 1 ? back : l == 0.f ? 0.f : back / l;
       if (w.parts > 1) {
-        float* dst = p.part_rows + ((int64_t)u.slot * 128 + m) * kKv8PartFloats;
+        float* dst = p.part_rows + ((int64_t)w.slot * 128 + m) * kKv8PartFloats;
         if (alive) dst[128] = mu, dst[129] = l;
 #pragma unroll 1
         for (int c = 0; c < kHeadDim; c += 16) {
@@ -260,7 +340,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
             const int rr = k * 8 + (lane >> 2), mm = quad * 32 + rr, row2 = x * R + mm / G, col = c + (lane & 3) * 8;
             const uint4 v = *reinterpret_cast<const uint4*>(st + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
             if (mm / G < R && row2 < w.nrows)
-              *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + row2) * p.ldo + (int64_t)(u.kvh * G + mm % G) * kHeadDim + col) = v;
+              *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + row2) * p.ldo + (int64_t)(w.kvh * G + mm % G) * kHeadDim + col) = v;
           }
           __syncwarp();
         }
@@ -271,7 +351,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   } else {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
     const int box = min(p.block_size, kKv8Tile), per_tile = kKv8Tile / box;   // boxes of a tile
-    Unit u;
+    Kv8Rows w;
     if (warp == 8 || warp == 10) {
       // ===== TMA: warp 8 keys, warp 10 values, a tile of 128 tokens at a time =====
       const bool issuer = elect_one(), values = warp == 10;
@@ -282,14 +362,13 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       int slot = 0;
       uint32_t ph = 1;
       bool stop = false;
-      for (int round = 0; round * grid < n_units && !stop; ++round) {
-        if (!unit(round, u)) continue;
-        const int32_t* bt = p.block_table + (int64_t)u.w.seq * p.bt_stride;
-        const int b0 = u.w.tile0 * per_tile, b1 = (min(u.w.ctx, u.w.tile1 * kKv8Tile) + box - 1) / box;
+      while (!stop && next_unit(w)) {
+        const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
+        const int b0 = w.tile0 * per_tile, b1 = (min(w.ctx, w.tile1 * kKv8Tile) + box - 1) / box;
         auto cell_of = [&](int b) {
           if (b >= b1) return 0;
           const int tok = b * box, blk = __ldg(bt + tok / p.block_size);
-          return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + u.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
+          return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
         };
         int have = cell_of(b0 + lane), next = b0 + 32 < b1 ? cell_of(b0 + 32 + lane) : 0;
         for (int b = b0; b < b1 && !(stop = wait.stop()); b += per_tile) {
@@ -307,6 +386,27 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       }
       if (wait.stop())   // the loads in flight: a slot's last one filled it in this round of the ring or in the one before
         for (int s = 0; s < slots; ++s) wait.drain(full + s, s < slot ? ph ^ 1 : ph);
+    } else if (warp == 11) {
+      // ===== TMA: an item's queries, in the two terms that the plan's launch left =====
+      const bool issuer = elect_one();
+      int done = 0;
+      while (!wait.stop() && next_unit(w)) {
+        const bool few = few_pairs(w, G);
+        const int copies = few ? 4 : w.nrows > R ? 2 : 1, bytes = (few ? 32 / G : R) * G * 128;
+        if (done > 0) wait(q_free, (done - 1) & 1);
+        ++done;
+        if (issuer) {
+          mbar_expect_tx(q_ready, 2 * copies * bytes);
+          for (int i = 0; i < copies; ++i) {
+            unsigned char* dst = few ? qs + i * 32 * 128 : qs + i * 2 * kOperand;
+            const int row = few ? w.row0 : w.row0 + i * R;
+            tma_load_3d(dst, few ? &qmaps.hi32 : &qmaps.hi, 0, w.kvh * G, row, q_ready);
+            tma_load_3d(dst + kOperand, few ? &qmaps.lo32 : &qmaps.lo, 0, w.kvh * G, row, q_ready);
+          }
+        }
+        __syncwarp();
+      }
+      if (wait.stop() && done > 0) wait.drain(q_ready, (done - 1) & 1);
     } else if (warp == 9) {
       // ===== MMA: per half, for either tile of pairs: the next half's scores, then this one's second product =====
       const uint32_t one = elect_one() ? 1u : 0u, tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -315,146 +415,169 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       const uint32_t id_o = idesc_f16(kHeadDim);
       int n[2] = {0, 0}, half = 0, slot = 0, done = 0;   // half: of the CTA; slot: of the keys
       uint32_t ph = 0;
-      for (int round = 0; round * grid < n_units; ++round) {
-        const bool have = unit(round, u);
-        if (!__shfl_sync(0xffffffffu, have, 0)) continue;
-        const int nh = __shfl_sync(0xffffffffu, min(2 * u.w.tile1, (u.w.ctx + kHalf - 1) / kHalf) - 2 * u.w.tile0, 0);
-        const int tiles = __shfl_sync(0xffffffffu, u.w.nrows > R ? 2 : 1, 0);
-        wait(q_ready, done++ & 1);
-        // step i: scores of half i (i < nh), the product of half i - 1 (i > 0)
-        for (int i = 0; i <= nh; ++i) {
-          if (i < nh && (i & 1) == 0) wait(k_full + slot, ph);
-          fence_after();
-#pragma unroll 1
-          for (int x = 0; x < tiles; ++x) {
-            if (i < nh) {
-              const uint64_t da = desc_q + (uint64_t)((x * 2 * kOperand) >> 4), db = desc_k + (uint64_t)((slot * kOperand + (i & 1) * kHalf * 128) >> 4);
-              const int nx = n[x] + (i > 0 ? 1 : 0);
-              const uint32_t d = tm + x * 256 + (nx & 1) * kHalf;
+      // an item of nh halves: straight code for either count of tiles (branches between the MMAs cost the issuing warp more than the MMAs take)
+      auto walk = [&](auto tiles_c, int nh) {
+        constexpr int TILES = decltype(tiles_c)::value;
+        auto scores = [&](int x, int nx, int i) {
+          const uint64_t da = desc_q + (uint64_t)((x * 2 * kOperand) >> 4), db = desc_k + (uint64_t)((slot * kOperand + (i & 1) * kHalf * 128) >> 4);
+          const uint32_t d = tm + x * 256 + (nx & 1) * kHalf;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) mma_f8_ss(one, d, da + ((j >> 2) * kOperand + (j & 3) * 32) / 16, db + ((j & 3) * 32) / 16, id_s, j ? 1u : 0u);
-              commit(one, s_full + 2 * x + (nx & 1));
-              if (x + 1 == tiles) {
-                commit(((i & 1) || i + 1 == nh) ? one : 0u, k_free + slot);
-                commit(i + 1 == nh ? one : 0u, q_free);   // the item's last scores are on their way
-              }
-            }
-            if (i > 0) {
-              const int b = half % kWide;
-              if (x == 0) wait(w_full + b, (half / kWide) & 1);
-              wait(p_ready + 2 * x + (n[x] & 1), (n[x] >> 1) & 1);
-              fence_after();
-              const uint32_t pa = tm + x * 256 + (n[x] & 1) * kHalf, d = tm + x * 256 + 128;
-              const uint64_t dv = desc_v + (uint64_t)((b * kOperand) >> 4);
+          for (int j = 0; j < 8; ++j) mma_f8_ss(one, d, da + ((j >> 2) * kOperand + (j & 3) * 32) / 16, db + ((j & 3) * 32) / 16, id_s, j ? 1u : 0u);
+          commit(one, s_full + 2 * x + (nx & 1));
+        };
+        auto scored = [&](int i) {   // half i's scores are on their way: the last of a tile, of the item
+          const bool end = i + 1 == nh;
+          commit((i & 1) || end ? one : 0u, k_free + slot);
+          commit(end ? one : 0u, q_free);
+          if (((i & 1) || end) && ++slot == kKSlots) slot = 0, ph ^= 1;
+        };
+        wait(k_full + slot, ph);
+        fence_after();
 #pragma unroll
-              for (int j = 0; j < 4; ++j) mma_ts(one, d, pa + j * 8, dv + (uint64_t)((j * 2048) >> 4), id_o, (i > 1 || j) ? 1u : 0u);
-              if (x + 1 == tiles) commit(one, w_free + b);
-              commit(one, o_full + 2 * x + (n[x] & 1));
-              ++n[x];
-            }
+        for (int x = 0; x < TILES; ++x) scores(x, n[x], 0);
+        scored(0);
+        int b = half % kWide;
+        uint32_t bph = (half / kWide) & 1;
+        auto step = [&](auto more_c, int i) {   // half i's product, behind the scores of half i + 1
+          constexpr bool MORE = decltype(more_c)::value;
+          if (MORE && (i & 1)) {
+            wait(k_full + slot, ph);
+            fence_after();
           }
-          if (i > 0) ++half;
-          if (i < nh && ((i & 1) || i + 1 == nh) && ++slot == kKSlots) slot = 0, ph ^= 1;
-        }
+          const uint64_t dv = desc_v + (uint64_t)((b * kOperand) >> 4);
+#pragma unroll
+          for (int x = 0; x < TILES; ++x) {
+            if constexpr (MORE) scores(x, n[x] + 1, i + 1);
+            if (MORE && x == TILES - 1) scored(i + 1);
+            if (x == 0) wait(w_full + b, bph);
+            wait(p_ready + 2 * x + (n[x] & 1), (n[x] >> 1) & 1);
+            fence_after();
+            const uint32_t pa = tm + x * 256 + (n[x] & 1) * kHalf, d = tm + x * 256 + 128;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) mma_ts(one, d, pa + j * 8, dv + (uint64_t)((j * 2048) >> 4), id_o, (i | j) ? 1u : 0u);
+            if (x == TILES - 1) commit(one, w_free + b);
+            commit(one, o_full + 2 * x + (n[x] & 1));
+            ++n[x];
+          }
+          if (++b == kWide) b = 0, bph ^= 1;
+        };
+        for (int i = 0; i + 1 < nh; ++i) step(std::true_type(), i);
+        step(std::false_type(), nh - 1);
+        half += nh;
+      };
+      for (;;) {
+        const bool more = next_unit(w);
+        if (!__shfl_sync(0xffffffffu, more, 0)) break;
+        const int nh = __shfl_sync(0xffffffffu, min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf) - 2 * w.tile0, 0);
+        const int tiles = __shfl_sync(0xffffffffu, w.nrows > R ? 2 : 1, 0);
+        wait(q_ready, done++ & 1);
+        if (tiles == 2) walk(std::integral_constant<int, 2>(), nh);
+        else walk(std::integral_constant<int, 1>(), nh);
       }
       if (wait.stop()) {
         commit(one, last);
         wait.drain(last, 0);
       }
     } else if (warp >= 12) {
-      // ===== queries of an item -> two terms; values of a half -> f16, factors of its keys =====
-      const int w4 = warp - 12, cl = lane & 7, stride = p.hkv * p.block_size;
+      // ===== values of a half -> f16, factors of its keys =====
+      const int w4 = warp - 12, stride = p.hkv * p.block_size;
+      const int r_own = 16 * w4 + 2 * (lane >> 3) + (lane >> 2 & 1), c_own = (lane & 3) + (lane & 4);
       const float sign = p.scale2 < 0.f ? -1.f : 1.f;
-      int half = 0, slot = 0, done = 0;
+      int half = 0, slot = 0;
       uint32_t ph = 0;
-      for (int round = 0; round * grid < n_units; ++round) {
-        if (!unit(round, u)) continue;
-        const Kv8Rows& w = u.w;
-        // exponents: lanes 0..15 four keys each, 16..31 four values; fetched a half ahead, their block two
+      while (next_unit(w)) {
+          // a lane's four tokens of a tile: their exponents are fetched a tile ahead, their block two
         const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
-        const uint8_t* src = lane < 16 ? p.ke : p.ve;
-        const int h0 = 2 * w.tile0, h1 = min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf);
-        int tok = h0 * kHalf + 4 * (lane & 15), at = tok / p.block_size, off = tok - at * p.block_size;
-        int blk = 0, cell = -1;
+        const int h1 = min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf);
+        int tok = w.tile0 * kKv8Tile + 4 * lane, at = tok / p.block_size, off = tok - at * p.block_size, blk = 0, cell = -1;
         auto place = [&]() {
-          cell = tok < w.ctx ? u.kvh * p.block_size + off : -1;
+          cell = tok < w.ctx ? w.kvh * p.block_size + off : -1;
           blk = __ldg(tok < w.ctx ? bt + at : p.block_table);
-          tok += kHalf, off += kHalf;
+          tok += kKv8Tile, off += kKv8Tile;
           while (off >= p.block_size) off -= p.block_size, ++at;
         };
+        uint32_t k_next = 0u, v_next = 0u;
         auto fetch = [&]() {
-          uint32_t v = 0u;
-          if (cell >= 0 && blk >= 0 && blk < p.n_blocks) v = __ldg(reinterpret_cast<const uint32_t*>(src + blk * stride + cell));   // (outside the cache: zeros)
-          return v;
+          k_next = v_next = 0u;
+          if (cell >= 0 && blk >= 0 && blk < p.n_blocks) {   // (outside the cache: zeros)
+            const int64_t c = (int64_t)blk * stride + cell;
+            k_next = __ldg(reinterpret_cast<const uint32_t*>(p.ke + c)), v_next = __ldg(reinterpret_cast<const uint32_t*>(p.ve + c));
+          }
         };
         place();
-        uint32_t e_next = fetch();
+        fetch();
         place();
-        if (done > 0) wait(q_free, (done - 1) & 1);
-        ++done;
-        stage_queries(p, qs, q_scale + (done & 1) * 256, u, R, G, threadIdx.x - 384);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_ready);
         int ref = 0;
 #pragma unroll 1
-        for (int h = h0; h < h1; ++h, ++half) {
-          const uint32_t e4 = e_next;
-          e_next = fetch();
+        for (int t = w.tile0; t < w.tile1; ++t) {
+          const uint32_t k4 = k_next, v4 = v_next;
+          fetch();
           place();
-          const int b = half % kWide, live = w.ctx - h * kHalf;   // tokens of the half
           // the reference: two bits above the largest exponent so far
+          const int left = w.ctx - t * kKv8Tile;
           uint32_t mx = 1u;
-          if (lane >= 16) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t v = (e4 >> (8 * j)) & 255u;
-              if (4 * (lane & 15) + j < live && v != 255u) mx = max(mx, v);
-            }
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t v = (v4 >> (8 * j)) & 255u;
+            if (4 * lane + j < left && v != 255u) mx = max(mx, v);
           }
           mx = __reduce_max_sync(0xffffffffu, mx);
-          if (h == h0 || (int)mx > ref) ref = (int)mx + 2;
-          if ((h & 1) == 0) wait(v_full + slot, ph);
-          if (half >= kWide) wait(w_free + b, (half / kWide - 1) & 1);
-          const unsigned char* raw = vring + slot * kOperand + (h & 1) * kHalf * 128;
-          unsigned char* dst = wide + b * kOperand;
+          if (t == w.tile0 || (int)mx > ref) ref = (int)mx + 2;
+          wait(v_full + slot, ph);
+          const int halves = min(2, h1 - 2 * t);
+#pragma unroll 1
+          for (int hh = 0; hh < halves; ++hh, ++half) {
+            const int b = half % kWide;
+            if (half >= kWide) wait(w_free + b, (half / kWide - 1) & 1);
+            const unsigned char* raw = vring + slot * kOperand + hh * kHalf * 128;
+            unsigned char* dst = wide + b * kOperand;
+            // pieces of 16 dims: eight lanes take four of a row and the other four of the next, so that neither the reads nor the writes (two pieces of f16 each)
+            // meet a bank twice; all are asked for before anything is stored
+            uint4 c[4];
+            uint32_t f[2];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int r = 16 * w4 + 4 * i + (lane >> 3);
-            const uint32_t ve = (__shfl_sync(0xffffffffu, e4, 16 + (r >> 2)) >> (8 * (r & 3))) & 255u;
-            const bool dead = r >= live || ve == 255u;
-            const int d = (int)ve - ref + 7;   // code * 2^d, exact while d >= -15
-            const uint32_t f1 = d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u, f = f1 | f1 << 16;
-            const uint4 c = *reinterpret_cast<const uint4*>(raw + r * 128 + ((cl ^ (r & 7)) << 4));
-            const uint32_t c4[4] = {c.x, c.y, c.z, c.w};
-            uint32_t o[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c4[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
-              const __half2 v = __hmul2(a, *reinterpret_cast<const __half2*>(&f));
-              o[j] = dead ? 0u : *reinterpret_cast<const uint32_t*>(&v);
+            for (int i = 0; i < 4; ++i) {
+              const int r = r_own + 8 * (i >> 1);
+              c[i] = *reinterpret_cast<const uint4*>(raw + r * 128 + (((c_own ^ 4 * (i & 1)) ^ (r & 7)) << 4));
             }
-            // 16 dims: two pieces of the first or the second 64; odd lanes' halves in another order, so that eight lanes meet no bank twice
-            unsigned char* row = dst + (cl >> 2) * (kOperand / 2) + r * 128;
-            const int i0 = (cl & 3) * 2, swap = cl >> 2;
-            *reinterpret_cast<uint4*>(row + (((i0 + swap) ^ (r & 7)) << 4)) = swap ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
-            *reinterpret_cast<uint4*>(row + (((i0 + 1 - swap) ^ (r & 7)) << 4)) = swap ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              const int rt = hh * kHalf + r_own + 8 * i;   // row of the tile
+              const uint32_t ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
+              const int d = (int)ve - ref + 7;   // code * 2^d, exact while d >= -15
+              const uint32_t f1 = rt >= left || ve == 255u ? 0x8000u : d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
+              f[i] = f1 | f1 << 16;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int r = r_own + 8 * (i >> 1), cc = c_own ^ 4 * (i & 1);
+              if (f[i >> 1] == 0x80008000u) c[i] = make_uint4(0u, 0u, 0u, 0u);   // behind the context, or not a number: zeros, whatever the codes
+              const uint32_t c4[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+              uint32_t o[8];
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c4[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
+                const __half2 v = __hmul2(a, *reinterpret_cast<const __half2*>(&f[i >> 1]));
+                o[j] = *reinterpret_cast<const uint32_t*>(&v);
+              }
+              unsigned char* row = dst + (cc >> 2) * (kOperand / 2) + r * 128;
+              *reinterpret_cast<uint4*>(row + ((((cc & 3) * 2) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+              *reinterpret_cast<uint4*>(row + ((((cc & 3) * 2 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+            }
+            {
+              // a value row that is not a number: the rows that see it are none either (its key's factor)
+              const int r = 16 * w4 + (lane & 15), rt = hh * kHalf + r;
+              const uint32_t ke = (__shfl_sync(0xffffffffu, k4, rt >> 2) >> (8 * (rt & 3))) & 255u, ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
+              float* fk = reinterpret_cast<float*>(facs + b * kFacBytes);
+              if (lane < 16) fk[r] = ve == 255u && rt < left ? __uint_as_float(0x7fffffffu) : sign * __uint_as_float(ke << 23);
+              if (warp == 12 && lane == 16) reinterpret_cast<int*>(fk)[kHalf] = ref;
+            }
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(w_full + b);
           }
-          {
-            // a value row that is not a number: the rows that see it are none either (its key's factor)
-            const int r = 16 * w4 + (lane & 15);
-            const uint32_t ke = (__shfl_sync(0xffffffffu, e4, r >> 2) >> (8 * (r & 3))) & 255u, ve = (__shfl_sync(0xffffffffu, e4, 16 + (r >> 2)) >> (8 * (r & 3))) & 255u;
-            float* fk = reinterpret_cast<float*>(facs + b * kFacBytes);
-            if (lane < 16) fk[r] = ve == 255u && r < live ? __uint_as_float(0x7fffffffu) : sign * __uint_as_float(ke << 23);
-            if (warp == 12 && lane == 16) reinterpret_cast<int*>(fk)[kHalf] = ref;
-          }
-          fence_async_smem();
-          __syncwarp();
-          if (lane == 0) {
-            mbar_arrive(w_full + b);
-            if ((h & 1) || h + 1 == h1) mbar_arrive(v_free + slot);
-          }
-          if (((h & 1) || h + 1 == h1) && ++slot == kVSlots) slot = 0, ph ^= 1;
+          if (lane == 0) mbar_arrive(v_free + slot);
+          if (++slot == kVSlots) slot = 0, ph ^= 1;
         }
       }
     }
@@ -469,11 +592,11 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
 
 }  // namespace
 
-int kv8_rows_launch(const Kv8Maps& m, const Kv8Params& p, int grid, cudaStream_t s) {
+int kv8_rows_launch(const Kv8Maps& m, const Kv8QueryMaps& q, const Kv8Params& p, int grid, cudaStream_t s) {
   if (const int e = wait_status()) return e;
   static bool done[64] = {};
   B200_CUDA(ensure_dynamic_smem(kv8_rows_kernel, kSmem, done));
-  B200_CUDA(launch(kv8_rows_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, s, m, p));
+  B200_CUDA(launch(kv8_rows_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, s, m, q, p));
   return B200_OK;
 }
 
