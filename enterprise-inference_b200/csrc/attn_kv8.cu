@@ -78,12 +78,12 @@ __device__ __forceinline__ int2 plan_scan(int& a, int& b, int2* sh) {
 }
 
 // block 0: the plan; the others: the rows kernel's queries, as two e4m3 terms and a factor each (16 lanes a query)
-__global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params p, int short_rows, Kv8Head* head, Kv8Group* groups, Kv8Group* rows, int* runs,
+__global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params p, int short_rows, int R, Kv8Head* head, Kv8Group* groups, Kv8Group* rows, int* runs,
                                                                 uint8_t* q_hi, uint8_t* q_lo, float* q_scale) {
   __shared__ int2 sh[32];
   pdl_wait();
   pdl_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, R = 128 / (p.hq / p.hkv);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (blockIdx.x > 0) {
     const int64_t pairs = (int64_t)p.T * p.hq, step = (int64_t)(gridDim.x - 1) * (kPlanThreads / 16);
     for (int64_t i0 = (int64_t)(blockIdx.x - 1) * (kPlanThreads / 16); i0 < pairs; i0 += step) {
@@ -125,7 +125,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
     if (n > short_rows) n1 += (n + R - 1) / R, n2 += (n + 2 * R - 1) / (2 * R);
   }
   const int2 both = plan_scan(n1, n2, sh);
-  const bool two = both.y * p.hkv >= kNumSMs && 2 * both.x >= 3 * both.y;
+  const bool two = R * (p.hq / p.hkv) > 32 && both.y * p.hkv >= kNumSMs && 2 * both.x >= 3 * both.y;
   const int per = two ? 2 * R : R;
   int n_groups = 0, n_items = 0;
   for (int i0 = 0; i0 < n_runs; i0 += kPlanThreads) {
@@ -192,7 +192,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
       }
     }
   }
-  if (tid == 0) *head = {n_groups, {0, 0, 0}};
+  if (tid == 0) *head = {n_groups, two, {0, 0}};
 }
 
 constexpr int kShortPairs = 8;    // (row, head) pairs of a group of the columns kernel in steps of longer runs
@@ -296,19 +296,22 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
   uint8_t* const q_hi = reinterpret_cast<uint8_t*>(w + kCutBytes + kPartBytes + kPartRowsBytes + plan_bytes(a.T, a.hkv));
   uint8_t* const q_lo = q_hi + query_bytes(a.T, a.hq);
   float* const q_scale = reinterpret_cast<float*>(q_lo + query_bytes(a.T, a.hq));
+  const bool few = most > 0 && most * G <= 32;
+  const int tile_rows = (few ? 32 : 128) / G;
   Kv8QueryMaps qm;
-  for (int i = 0; i < 4; ++i)
-    if (const int rc = kv8_query_map(i & 1 ? q_lo : q_hi, a.T, a.hq, G, (i < 2 ? 128 : 32) / G, i < 2 ? (i ? &qm.lo : &qm.hi) : (i == 3 ? &qm.lo32 : &qm.hi32))) return rc;
+  if (const int rc = kv8_query_map(q_hi, a.T, a.hq, G, tile_rows, &qm.hi)) return rc;
+  if (const int rc = kv8_query_map(q_lo, a.T, a.hq, G, tile_rows, &qm.lo)) return rc;
   const int64_t blocks = ((int64_t)a.T * a.hq + kPlanThreads / 16 - 1) / (kPlanThreads / 16);
-  B200_CUDA(launch(kv8_plan_kernel, dim3(1 + (int)std::min<int64_t>(blocks, 2 * kNumSMs)), dim3(kPlanThreads), 0, s, p, short_rows, head, groups, rows,
+  B200_CUDA(launch(kv8_plan_kernel, dim3(1 + (int)std::min<int64_t>(blocks, 2 * kNumSMs)), dim3(kPlanThreads), 0, s, p, short_rows, tile_rows, head, groups, rows,
                    reinterpret_cast<int*>(p.items + list_places(a.T, a.hkv)), q_hi, q_lo, q_scale));
   const PdlScope after;
   p.q_scale = q_scale;
+  p.groups_head = head;
   if (!drafts) {
     p.groups = groups;
     if (const int rc = kv8_cols_launch(maps, p, short_rows * G, kNumSMs, s)) return rc;
   }
-  if (const int rc = kv8_rows_launch(maps, qm, p, kNumSMs, s)) return rc;
+  if (const int rc = kv8_rows_launch(maps, qm, p, few, kNumSMs, s)) return rc;
   B200_CUDA(launch(kv8_join_kernel, dim3(drafts ? kNumSMs : 2 * kNumSMs, 4), dim3(256), 0, s, p, drafts ? kNumSMs : 0));
   return B200_OK;
 }

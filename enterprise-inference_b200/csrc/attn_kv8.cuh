@@ -22,7 +22,7 @@ struct alignas(16) Kv8Rows {
 };
 // what a plan found; its groups come right behind
 struct Kv8Head {
-  int groups, pad[3];
+  int groups, two, pad[2];   // two: items have up to two tiles of pairs
 };
 
 // CTA a's last item continues in `parts` - 1 further CTAs
@@ -40,7 +40,8 @@ struct Kv8Params {
   const Kv8Group* groups;      // a plan's groups (groups[-1].row0 of them), or null: found among the rows themselves
   float* part;                 // [CTA][2][pairs][kKv8PartFloats]: of an item that began in an earlier CTA, of one that goes on in the next
   Kv8Cut* cuts;                // [CTA]
-  Kv8Rows* items;              // of a plan
+  const Kv8Head* groups_head;  // of a plan
+  Kv8Rows* items;
   int* starts;                 // [CTA] its first item (-1: none)
   Kv8Cut* cuts_rows;           // [CTA]
   const float* q_scale;        // [row][head]: what the rows kernel's scores are multiplied by
@@ -52,17 +53,18 @@ struct Kv8Params {
 };
 
 // maps of the codes: [cells][128] bytes, boxes of so many rows, 128-byte swizzle; of the rows kernel's queries in two terms: [rows][heads][128] bytes, boxes of the
-// rows that fill a tile of 128 pairs, or of 32, by the heads of a kv head
+// rows that fill a tile of 128 pairs (or 32: few) by the heads of a kv head
 struct Kv8Maps {
   CUtensorMap k, v;
 };
 struct Kv8QueryMaps {
-  CUtensorMap hi, lo, hi32, lo32;
+  CUtensorMap hi, lo;
 };
 int kv8_maps(const Kv8Attn& a, int box_rows, Kv8Maps* m);
 
 int kv8_cols_launch(const Kv8Maps& m, const Kv8Params& p, int cols, int grid, cudaStream_t s);
-int kv8_rows_launch(const Kv8Maps& m, const Kv8QueryMaps& q, const Kv8Params& p, int grid, cudaStream_t s);
+// few: items of at most 32 pairs
+int kv8_rows_launch(const Kv8Maps& m, const Kv8QueryMaps& q, const Kv8Params& p, bool few, int grid, cudaStream_t s);
 
 __device__ __forceinline__ int kv8_ctx(const Kv8Params& p, int row) {
   return (int)min((int64_t)__ldg(p.ctx_lens + row), (int64_t)p.bt_stride * p.block_size);

@@ -29,9 +29,9 @@ static_assert(kSmem <= 232448, "shared memory");
 
 __device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | (1u << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
-// an item of at most 32 pairs has them in each quarter of the MMA's rows: a quarter's warp takes a quarter of the keys
-__device__ __forceinline__ bool few_pairs(const Kv8Rows& w, int G) { return w.nrows * G <= 32; }
-
+// FEW: items of at most 32 pairs, which are there in each quarter of the MMA's rows: a quarter's warp takes a quarter of the keys.  Softmax is half the work then, and
+// the second group of softmax warps widens every other half instead.
+template <bool FEW>
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv8QueryMaps qmaps, const Kv8Params p) {
   extern __shared__ unsigned char smem_raw[];
@@ -58,7 +58,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
   const Waits wait(tmem_slot + 1, p.status);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kKSlots; ++s) mbar_init(k_full + s, 1), mbar_init(k_free + s, 1);
-    for (int s = 0; s < kVSlots; ++s) mbar_init(v_full + s, 1), mbar_init(v_free + s, 4);
+    for (int s = 0; s < kVSlots; ++s) mbar_init(v_full + s, 1), mbar_init(v_free + s, FEW ? 8 : 4);
     for (int s = 0; s < kWide; ++s) mbar_init(w_full + s, 4), mbar_init(w_free + s, 1);
     for (int s = 0; s < 4; ++s) mbar_init(s_full + s, 1), mbar_init(p_ready + s, 4), mbar_init(o_full + s, 1);
     mbar_init(q_ready, 1);
@@ -70,6 +70,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
   pdl_wait();
   pdl_launch_dependents();
   if (p.starts[blockIdx.x] < 0) return;   // nothing for this CTA
+  const bool two = !FEW && p.groups_head->two != 0;   // items of two tiles of pairs; else of one, whose halves the two groups of softmax warps take in turn
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
@@ -78,7 +79,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;   // per tile of pairs 256 columns: scores of even, odd halves, O
-  const int G = p.hq / p.hkv, R = 128 / G;
+  const int G = p.hq / p.hkv, R = (FEW ? 32 : 128) / G;
   // the CTA's items, in the plan's order; the one behind the next is asked for
   int at = p.starts[blockIdx.x];
   Kv8Rows ahead = p.items[at];
@@ -91,13 +92,123 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
     }
   };
 
-  if (warp < 8) {
+  // ===== values of a half -> f16, factors of its keys: every half (group -1), or one of each tile's =====
+  auto widen = [&](int group) {
+    Kv8Rows w;
+    const int w4 = warp & 3, stride = p.hkv * p.block_size;
+    const int r_own = 16 * w4 + 2 * (lane >> 3) + (lane >> 2 & 1), c_own = (lane & 3) + (lane & 4);
+    const float sign = p.scale2 < 0.f ? -1.f : 1.f;
+    int half = 0, slot = 0;
+    uint32_t ph = 0;
+    while (next_unit(w)) {
+        // a lane's four tokens of a tile: their exponents are fetched a tile ahead, their block two
+      const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
+      const int h1 = min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf);
+      int tok = w.tile0 * kKv8Tile + 4 * lane, at = tok / p.block_size, off = tok - at * p.block_size, blk = 0, cell = -1;
+      auto place = [&]() {
+        cell = tok < w.ctx ? w.kvh * p.block_size + off : -1;
+        blk = __ldg(tok < w.ctx ? bt + at : p.block_table);
+        tok += kKv8Tile, off += kKv8Tile;
+        while (off >= p.block_size) off -= p.block_size, ++at;
+      };
+      uint32_t k_next = 0u, v_next = 0u;
+      auto fetch = [&]() {
+        k_next = v_next = 0u;
+        if (cell >= 0 && blk >= 0 && blk < p.n_blocks) {   // (outside the cache: zeros)
+          const int64_t c = (int64_t)blk * stride + cell;
+          k_next = __ldg(reinterpret_cast<const uint32_t*>(p.ke + c)), v_next = __ldg(reinterpret_cast<const uint32_t*>(p.ve + c));
+        }
+      };
+      place();
+      fetch();
+      place();
+      int ref = 0;
+#pragma unroll 1
+      for (int t = w.tile0; t < w.tile1; ++t) {
+        const uint32_t k4 = k_next, v4 = v_next;
+        fetch();
+        place();
+        // the reference: two bits above the largest exponent so far
+        const int left = w.ctx - t * kKv8Tile;
+        uint32_t mx = 1u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t v = (v4 >> (8 * j)) & 255u;
+          if (4 * lane + j < left && v != 255u) mx = max(mx, v);
+        }
+        mx = __reduce_max_sync(0xffffffffu, mx);
+        if (t == w.tile0 || (int)mx > ref) ref = (int)mx + 2;
+        wait(v_full + slot, ph);
+        const int halves = min(2, h1 - 2 * t);
+#pragma unroll 1
+        for (int hh = 0; hh < halves; ++hh, ++half) {
+          const int b = half % kWide;
+          if (FEW && hh != group) continue;   // the other warps'
+          if (half >= kWide) wait(w_free + b, (half / kWide - 1) & 1);
+          const unsigned char* raw = vring + slot * kOperand + hh * kHalf * 128;
+          unsigned char* dst = wide + b * kOperand;
+          // pieces of 16 dims: eight lanes take four of a row and the other four of the next, so that neither the reads nor the writes (two pieces of f16 each)
+          // meet a bank twice; all are asked for before anything is stored
+          uint4 c[4];
+          uint32_t f[2];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = r_own + 8 * (i >> 1);
+            c[i] = *reinterpret_cast<const uint4*>(raw + r * 128 + (((c_own ^ 4 * (i & 1)) ^ (r & 7)) << 4));
+          }
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const int rt = hh * kHalf + r_own + 8 * i;   // row of the tile
+            const uint32_t ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
+            const int d = (int)ve - ref + 7;   // code * 2^d, exact while d >= -15
+            const uint32_t f1 = rt >= left || ve == 255u ? 0x8000u : d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
+            f[i] = f1 | f1 << 16;
+          }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int r = r_own + 8 * (i >> 1), cc = c_own ^ 4 * (i & 1);
+            if (f[i >> 1] == 0x80008000u) c[i] = make_uint4(0u, 0u, 0u, 0u);   // behind the context, or not a number: zeros, whatever the codes
+            const uint32_t c4[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
+            uint32_t o[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c4[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
+              const __half2 v = __hmul2(a, *reinterpret_cast<const __half2*>(&f[i >> 1]));
+              o[j] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+            unsigned char* row = dst + (cc >> 2) * (kOperand / 2) + r * 128;
+            *reinterpret_cast<uint4*>(row + ((((cc & 3) * 2) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+            *reinterpret_cast<uint4*>(row + ((((cc & 3) * 2 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+          }
+          {
+            // a value row that is not a number: the rows that see it are none either (its key's factor)
+            const int r = 16 * w4 + (lane & 15), rt = hh * kHalf + r;
+            const uint32_t ke = (__shfl_sync(0xffffffffu, k4, rt >> 2) >> (8 * (rt & 3))) & 255u, ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
+            float* fk = reinterpret_cast<float*>(facs + b * kFacBytes);
+            if (lane < 16) fk[r] = ve == 255u && rt < left ? __uint_as_float(0x7fffffffu) : sign * __uint_as_float(ke << 23);
+            if (w4 == 0 && lane == 16) reinterpret_cast<int*>(fk)[kHalf] = ref;
+          }
+          fence_async_smem();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(w_full + b);
+        }
+        if (lane == 0) mbar_arrive(v_free + slot);
+        if (++slot == kVSlots) slot = 0, ph ^= 1;
+      }
+    }
+  };
+
+  if (FEW && warp >= 4 && warp < 8) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
+    widen(1);
+  } else if (warp < 8) {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     // ===== softmax and output: a thread owns a pair of tile x =====
     const int x = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + x * 256;
-    const int r = m / G, row = x * R + r;
-    int n = 0, half = 0;   // halves of this tile of pairs, of the CTA
+    const int r = m / G, row = (two ? x : 0) * R + r, step = two ? 1 : 2, first = two ? 0 : x;
+    unsigned char* const exchange = qs + 2 * kOperand;   // (items of one tile: the second one's queries are not there)
+    int n = 0, half = 0;   // halves of this group of warps', of the CTA
     auto rescale = [&](int n, float fo) {   // O of the halves before n
       wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
       fence_after();
@@ -111,19 +222,29 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         st16(base + 128 + c, o);
       }
     };
+    // 32 columns of the warp's pairs from shared memory to their rows: a row's 64 bytes leave from four neighbouring lanes
+    auto store_staged = [&](const unsigned char* st, const Kv8Rows& w, int c) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int rr = k * 8 + (lane >> 2), mm = quad * 32 + rr, row2 = (two ? x : 0) * R + mm / G, col = c + (lane & 3) * 8;
+        const uint4 v = *reinterpret_cast<const uint4*>(st + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
+        if (mm / G < R && row2 < w.nrows)
+          *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + row2) * p.ldo + (int64_t)(w.kvh * G + mm % G) * kHeadDim + col) = v;
+      }
+    };
     // an item of at most 32 pairs: lane = pair, this warp's 16 keys of each half; the four quarters' sums are joined at the end
-    auto few = [&](const Kv8Rows& w, int h0, int h1, int& n, int& half) {
+    auto few = [&](const Kv8Rows& w, int h0, int h1, int& n, int half) {
       const bool alive = lane < w.nrows * G;
       const int fr = lane / G, t = w.row0 + fr, ctx = alive ? kv8_ctx(p, t) : 0;
       const float qf = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + lane % G) : 1.f;
       float mu = -INFINITY, l = 0.f;
       int ref = 0;
 #pragma unroll 1
-      for (int h = h0; h < h1; ++h, ++n, ++half) {
-        const int b = half % kWide;
+      for (int h = h0; h < h1; ++h, ++n) {
+        const int at = half + h - h0, b = at % kWide;
         const float* f = reinterpret_cast<const float*>(facs + b * kFacBytes);
-        wait(s_full + (n & 1), (n >> 1) & 1);
-        wait(w_full + b, (half / kWide) & 1);
+        wait(s_full + 2 * x + (n & 1), (n >> 1) & 1);
+        wait(w_full + b, (at / kWide) & 1);
         fence_after();
         const uint32_t s_addr = base + (n & 1) * kHalf;
         uint32_t s[16];
@@ -147,7 +268,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
           float fo = jump && mu != -INFINITY ? exp2_fast(mu - mn) : 1.f;
           l *= fo;
           mu = mn;
-          if (h > h0) {
+          if (h > h0 + (FEW ? 0 : first)) {
             fo *= __uint_as_float((uint32_t)max(127 - (ref_new - ref), 0) << 23);
             if (__any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
           }
@@ -170,13 +291,12 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         st_wait();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + (n & 1));
+        if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
       }
       wait(o_full + ((n - 1) & 1), ((n - 1) >> 1) & 1);
       fence_after();
       // the quarters' maxima and denominators, then their sums, 32 columns at a time
-      float2* ml = reinterpret_cast<float2*>(ostage);
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      float2* ml = reinterpret_cast<float2*>(exchange);
       ml[m] = make_float2(mu, l);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       float top = -INFINITY, all = 0.f;
@@ -186,7 +306,6 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       for (int k = 0; k < 4; ++k) all += ml[32 * k + lane].y * (top == -INFINITY ? 0.f : exp2_fast(ml[32 * k + lane].x - top));
       const float back = __uint_as_float((uint32_t)max(ref - 7, 1) << 23), own = mu == -INFINITY ? 0.f : exp2_fast(mu - top);
       const float mult = own * (w.parts > 1 ? back : all == 0.f ? 0.f : back / all);
-      const int head = w.kvh * G + lane % G;
       float* part = p.part_rows + ((int64_t)w.slot * 128 + lane) * kKv8PartFloats;
       if (w.parts > 1 && alive && quad == 0) part[128] = top, part[129] = all;
 #pragma unroll 1
@@ -194,7 +313,6 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         uint32_t o[32];
         ld32(base + 128 + c, o);
         ld_wait<32>(o);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
 #pragma unroll
         for (int j = 0; j < 8; ++j)
           *reinterpret_cast<float4*>(ostage + quad * 4096 + j * 512 + lane * 16) =
@@ -212,21 +330,21 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
           *reinterpret_cast<float4*>(part + c + 8 * quad) = make_float4(y[0], y[1], y[2], y[3]);
           *reinterpret_cast<float4*>(part + c + 8 * quad + 4) = make_float4(y[4], y[5], y[6], y[7]);
         } else if (alive) {
-          *reinterpret_cast<uint4*>(p.out + (int64_t)t * p.ldo + head * kHeadDim + c + 8 * quad) =
+          *reinterpret_cast<uint4*>(p.out + (int64_t)t * p.ldo + (w.kvh * G + lane % G) * kHeadDim + c + 8 * quad) =
               make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
         }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
       }
       fence_before();
     };
     Kv8Rows w;
     while (next_unit(w)) {
       const int h0 = 2 * w.tile0, h1 = min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf);
-      if (x == 1 && w.nrows <= R) {   // the item has one tile of pairs
-        half += h1 - h0;
-        continue;
-      }
-      if (few_pairs(w, G)) {
-        few(w, h0, h1, n, half);
+      const int at0 = half;
+      half += h1 - h0;
+      if (two && x == 1 && w.nrows <= R) continue;   // the item has one tile of pairs
+      if constexpr (FEW) {
+        few(w, h0, h1, n, at0);
         continue;
       }
       const bool alive = r < R && row < w.nrows, any = __any_sync(0xffffffffu, alive);
@@ -234,11 +352,11 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       const float qf = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + m % G) : 1.f;
       float mu = -INFINITY, l = 0.f;
       int ref = 0;
-      for (int h = h0; h < h1; ++h, ++n, ++half) {
-        const int b = half % kWide;
+      for (int h = h0 + first; h < h1; h += step, ++n) {
+        const int at = at0 + h - h0, b = at % kWide;
         const float* f = reinterpret_cast<const float*>(facs + b * kFacBytes);
         wait(s_full + 2 * x + (n & 1), (n >> 1) & 1);
-        wait(w_full + b, (half / kWide) & 1);   // (after the scores: this tile's warps may have passed items over, and the phase three halves ago is complete now)
+        wait(w_full + b, (at / kWide) & 1);   // (after the scores: this tile's warps may have passed items over, and the phase three halves ago is complete now)
         if (!any) {   // no pair of this warp's: its weights may be anything
           if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
           continue;
@@ -270,7 +388,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
           float fo = jump && mu != -INFINITY ? exp2_fast(mu - mn) : 1.f;
           l *= fo;
           mu = mn;
-          if (h > h0) {
+          if (h > h0 + (FEW ? 0 : first)) {
             fo *= __uint_as_float((uint32_t)max(127 - (ref_new - ref), 0) << 23);
             if (__any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
           }
@@ -299,51 +417,79 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
       }
-      wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
-      fence_after();
-      if (!any) continue;
+      const bool some = h0 + first < h1;
+      if (some) {
+        wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
+        fence_after();
+      }
       const float back = __uint_as_float((uint32_t)max(ref - 7, 1) << 23);   // 2^(ref - 134): values and weights as they are, but for the 2^7 that l has too
-      const float mult = w.parts > 1 ? back : l == 0.f ? 0.f : back / l;
-      if (w.parts > 1) {
+      if (!two) {   // the other group's halves: its sums come over through shared memory, 32 columns at a time in two buffers
+        float2* ml = reinterpret_cast<float2*>(ostage + 8192);
+        ml[threadIdx.x] = make_float2(mu, l);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        const float2 other = ml[threadIdx.x ^ 128];
+        const float top = fmaxf(mu, other.x), own = mu == -INFINITY ? 0.f : exp2_fast(mu - top);
+        const float all = l * own + other.y * (other.x == -INFINITY ? 0.f : exp2_fast(other.x - top));
+        const float mult = own * (w.parts > 1 ? back : all == 0.f ? 0.f : back / all);
         float* dst = p.part_rows + ((int64_t)w.slot * 128 + m) * kKv8PartFloats;
-        if (alive) dst[128] = mu, dst[129] = l;
-#pragma unroll 1
-        for (int c = 0; c < kHeadDim; c += 16) {
-          uint32_t o[16];
-          ld16(base + 128 + c, o);
-          ld_wait<16>(o);
-          if (alive) {
-#pragma unroll
-            for (int j = 0; j < 16; j += 4)
-              *reinterpret_cast<float4*>(dst + c + j) = make_float4(__uint_as_float(o[j]) * mult, __uint_as_float(o[j + 1]) * mult, __uint_as_float(o[j + 2]) * mult,
-                                                                    __uint_as_float(o[j + 3]) * mult);
-          }
-        }
-      } else {
-        // 32 columns at a time through shared memory: a row's 64 bytes leave from four neighbouring lanes
+        if (w.parts > 1 && alive && x == 0) dst[128] = top, dst[129] = all;
         unsigned char* st = ostage + warp * 2048;
 #pragma unroll 1
         for (int c = 0; c < kHeadDim; c += 32) {
           uint32_t o[32];
-          ld32(base + 128 + c, o);
-          ld_wait<32>(o);
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            uint32_t v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = pack_bf16(__uint_as_float(o[8 * k + 2 * j]) * mult, __uint_as_float(o[8 * k + 2 * j + 1]) * mult);
-            *reinterpret_cast<uint4*>(st + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+          if (any && some) {
+            ld32(base + 128 + c, o);
+            ld_wait<32>(o);
           }
-          __syncwarp();
+          unsigned char* xb = exchange + (c & 32) * (kOperand / 32) + m * 16;
+          if (x == 1 && any) {
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int rr = k * 8 + (lane >> 2), mm = quad * 32 + rr, row2 = x * R + mm / G, col = c + (lane & 3) * 8;
-            const uint4 v = *reinterpret_cast<const uint4*>(st + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
-            if (mm / G < R && row2 < w.nrows)
-              *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + row2) * p.ldo + (int64_t)(w.kvh * G + mm % G) * kHeadDim + col) = v;
+            for (int j = 0; j < 8; ++j)
+              *reinterpret_cast<float4*>(xb + j * 2048) = some ? make_float4(__uint_as_float(o[4 * j]) * mult, __uint_as_float(o[4 * j + 1]) * mult,
+                                                                            __uint_as_float(o[4 * j + 2]) * mult, __uint_as_float(o[4 * j + 3]) * mult)
+                                                               : make_float4(0.f, 0.f, 0.f, 0.f);
           }
-          __syncwarp();
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (x == 0 && any) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              const float4 v = *reinterpret_cast<const float4*>(xb + j * 2048);
+              const float y0 = fmaf(__uint_as_float(o[4 * j]), mult, v.x), y1 = fmaf(__uint_as_float(o[4 * j + 1]), mult, v.y),
+                          y2 = fmaf(__uint_as_float(o[4 * j + 2]), mult, v.z), y3 = fmaf(__uint_as_float(o[4 * j + 3]), mult, v.w);
+              if (w.parts > 1) {
+                if (alive) *reinterpret_cast<float4*>(dst + c + 4 * j) = make_float4(y0, y1, y2, y3);
+              } else {
+                *reinterpret_cast<uint2*>(st + lane * 64 + (((j >> 1) ^ ((lane >> 1) & 3)) << 4) + (j & 1) * 8) = make_uint2(pack_bf16(y0, y1), pack_bf16(y2, y3));
+              }
+            }
+            if (w.parts == 1) {
+              __syncwarp();
+              store_staged(st, w, c);
+              __syncwarp();
+            }
+          }
         }
+        fence_before();
+        continue;
+      }
+      if (!any) continue;
+      const float mult = l == 0.f ? 0.f : back / l;
+      unsigned char* st = ostage + warp * 2048;
+#pragma unroll 1
+      for (int c = 0; c < kHeadDim; c += 32) {
+        uint32_t o[32];
+        ld32(base + 128 + c, o);
+        ld_wait<32>(o);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t v[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = pack_bf16(__uint_as_float(o[8 * k + 2 * j]) * mult, __uint_as_float(o[8 * k + 2 * j + 1]) * mult);
+          *reinterpret_cast<uint4*>(st + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+        }
+        __syncwarp();
+        store_staged(st, w, c);
+        __syncwarp();
       }
       fence_before();
       // all four warps of a tile have read its O before any of them hands over the next item's first weights (whose product restarts O)
@@ -391,17 +537,16 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       const bool issuer = elect_one();
       int done = 0;
       while (!wait.stop() && next_unit(w)) {
-        const bool few = few_pairs(w, G);
-        const int copies = few ? 4 : w.nrows > R ? 2 : 1, bytes = (few ? 32 / G : R) * G * 128;
+        const int copies = FEW ? 4 : w.nrows > R ? 2 : 1, bytes = R * G * 128;
         if (done > 0) wait(q_free, (done - 1) & 1);
         ++done;
         if (issuer) {
           mbar_expect_tx(q_ready, 2 * copies * bytes);
           for (int i = 0; i < copies; ++i) {
-            unsigned char* dst = few ? qs + i * 32 * 128 : qs + i * 2 * kOperand;
-            const int row = few ? w.row0 : w.row0 + i * R;
-            tma_load_3d(dst, few ? &qmaps.hi32 : &qmaps.hi, 0, w.kvh * G, row, q_ready);
-            tma_load_3d(dst + kOperand, few ? &qmaps.lo32 : &qmaps.lo, 0, w.kvh * G, row, q_ready);
+            unsigned char* dst = qs + i * (FEW ? 32 * 128 : 2 * kOperand);
+            const int row = w.row0 + (FEW ? 0 : i * R);
+            tma_load_3d(dst, &qmaps.hi, 0, w.kvh * G, row, q_ready);
+            tma_load_3d(dst + kOperand, &qmaps.lo, 0, w.kvh * G, row, q_ready);
           }
         }
         __syncwarp();
@@ -465,121 +610,68 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         step(std::false_type(), nh - 1);
         half += nh;
       };
+      // one tile of pairs, its even halves to the first group of softmax warps, its odd ones to the second: scores two halves ahead
+      auto walk_in_turn = [&](int nh) {
+        int s_slot = slot;
+        uint32_t s_ph = ph;
+        auto scores = [&](int i) {
+          if ((i & 1) == 0) {
+            wait(k_full + s_slot, s_ph);
+            fence_after();
+          }
+          const int x = i & 1, nx = (x ? n[1] : n[0]) + (i >> 1);
+          const uint64_t db = desc_k + (uint64_t)((s_slot * kOperand + (i & 1) * kHalf * 128) >> 4);
+          const uint32_t d = tm + x * 256 + (nx & 1) * kHalf;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mma_f8_ss(one, d, desc_q + ((j >> 2) * kOperand + (j & 3) * 32) / 16, db + ((j & 3) * 32) / 16, id_s, j ? 1u : 0u);
+          commit(one, s_full + 2 * x + (nx & 1));
+          const bool end = i + 1 == nh;
+          commit(x || end ? one : 0u, k_free + s_slot);
+          commit(end ? one : 0u, q_free);
+          if ((x || end) && ++s_slot == kKSlots) s_slot = 0, s_ph ^= 1;
+        };
+        int b = half % kWide;
+        uint32_t bph = (half / kWide) & 1;
+#pragma unroll 1
+        for (int i = -2; i < nh; ++i) {
+          if (i + 2 < nh) scores(i + 2);
+          if (i < 0) continue;
+          const int x = i & 1, nx = (x ? n[1] : n[0]) + (i >> 1);
+          wait(w_full + b, bph);
+          wait(p_ready + 2 * x + (nx & 1), (nx >> 1) & 1);
+          fence_after();
+          const uint32_t pa = tm + x * 256 + (nx & 1) * kHalf, d = tm + x * 256 + 128;
+          const uint64_t dv = desc_v + (uint64_t)((b * kOperand) >> 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_ts(one, d, pa + j * 8, dv + (uint64_t)((j * 2048) >> 4), id_o, (i > 1 || j) ? 1u : 0u);
+          commit(one, w_free + b);
+          commit(one, o_full + 2 * x + (nx & 1));
+          if (++b == kWide) b = 0, bph ^= 1;
+        }
+        n[0] += (nh + 1) >> 1, n[1] += nh >> 1;
+        half += nh;
+        slot = s_slot, ph = s_ph;
+      };
       for (;;) {
         const bool more = next_unit(w);
         if (!__shfl_sync(0xffffffffu, more, 0)) break;
         const int nh = __shfl_sync(0xffffffffu, min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf) - 2 * w.tile0, 0);
         const int tiles = __shfl_sync(0xffffffffu, w.nrows > R ? 2 : 1, 0);
         wait(q_ready, done++ & 1);
-        if (tiles == 2) walk(std::integral_constant<int, 2>(), nh);
+        if constexpr (FEW) {
+          walk(std::integral_constant<int, 1>(), nh);
+          continue;
+        }
+        if (!two) walk_in_turn(nh);
+        else if (tiles == 2) walk(std::integral_constant<int, 2>(), nh);
         else walk(std::integral_constant<int, 1>(), nh);
       }
       if (wait.stop()) {
         commit(one, last);
         wait.drain(last, 0);
       }
-    } else if (warp >= 12) {
-      // ===== values of a half -> f16, factors of its keys =====
-      const int w4 = warp - 12, stride = p.hkv * p.block_size;
-      const int r_own = 16 * w4 + 2 * (lane >> 3) + (lane >> 2 & 1), c_own = (lane & 3) + (lane & 4);
-      const float sign = p.scale2 < 0.f ? -1.f : 1.f;
-      int half = 0, slot = 0;
-      uint32_t ph = 0;
-      while (next_unit(w)) {
-          // a lane's four tokens of a tile: their exponents are fetched a tile ahead, their block two
-        const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
-        const int h1 = min(2 * w.tile1, (w.ctx + kHalf - 1) / kHalf);
-        int tok = w.tile0 * kKv8Tile + 4 * lane, at = tok / p.block_size, off = tok - at * p.block_size, blk = 0, cell = -1;
-        auto place = [&]() {
-          cell = tok < w.ctx ? w.kvh * p.block_size + off : -1;
-          blk = __ldg(tok < w.ctx ? bt + at : p.block_table);
-          tok += kKv8Tile, off += kKv8Tile;
-          while (off >= p.block_size) off -= p.block_size, ++at;
-        };
-        uint32_t k_next = 0u, v_next = 0u;
-        auto fetch = [&]() {
-          k_next = v_next = 0u;
-          if (cell >= 0 && blk >= 0 && blk < p.n_blocks) {   // (outside the cache: zeros)
-            const int64_t c = (int64_t)blk * stride + cell;
-            k_next = __ldg(reinterpret_cast<const uint32_t*>(p.ke + c)), v_next = __ldg(reinterpret_cast<const uint32_t*>(p.ve + c));
-          }
-        };
-        place();
-        fetch();
-        place();
-        int ref = 0;
-#pragma unroll 1
-        for (int t = w.tile0; t < w.tile1; ++t) {
-          const uint32_t k4 = k_next, v4 = v_next;
-          fetch();
-          place();
-          // the reference: two bits above the largest exponent so far
-          const int left = w.ctx - t * kKv8Tile;
-          uint32_t mx = 1u;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t v = (v4 >> (8 * j)) & 255u;
-            if (4 * lane + j < left && v != 255u) mx = max(mx, v);
-          }
-          mx = __reduce_max_sync(0xffffffffu, mx);
-          if (t == w.tile0 || (int)mx > ref) ref = (int)mx + 2;
-          wait(v_full + slot, ph);
-          const int halves = min(2, h1 - 2 * t);
-#pragma unroll 1
-          for (int hh = 0; hh < halves; ++hh, ++half) {
-            const int b = half % kWide;
-            if (half >= kWide) wait(w_free + b, (half / kWide - 1) & 1);
-            const unsigned char* raw = vring + slot * kOperand + hh * kHalf * 128;
-            unsigned char* dst = wide + b * kOperand;
-            // pieces of 16 dims: eight lanes take four of a row and the other four of the next, so that neither the reads nor the writes (two pieces of f16 each)
-            // meet a bank twice; all are asked for before anything is stored
-            uint4 c[4];
-            uint32_t f[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = r_own + 8 * (i >> 1);
-              c[i] = *reinterpret_cast<const uint4*>(raw + r * 128 + (((c_own ^ 4 * (i & 1)) ^ (r & 7)) << 4));
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              const int rt = hh * kHalf + r_own + 8 * i;   // row of the tile
-              const uint32_t ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
-              const int d = (int)ve - ref + 7;   // code * 2^d, exact while d >= -15
-              const uint32_t f1 = rt >= left || ve == 255u ? 0x8000u : d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
-              f[i] = f1 | f1 << 16;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int r = r_own + 8 * (i >> 1), cc = c_own ^ 4 * (i & 1);
-              if (f[i >> 1] == 0x80008000u) c[i] = make_uint4(0u, 0u, 0u, 0u);   // behind the context, or not a number: zeros, whatever the codes
-              const uint32_t c4[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
-              uint32_t o[8];
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c4[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
-                const __half2 v = __hmul2(a, *reinterpret_cast<const __half2*>(&f[i >> 1]));
-                o[j] = *reinterpret_cast<const uint32_t*>(&v);
-              }
-              unsigned char* row = dst + (cc >> 2) * (kOperand / 2) + r * 128;
-              *reinterpret_cast<uint4*>(row + ((((cc & 3) * 2) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-              *reinterpret_cast<uint4*>(row + ((((cc & 3) * 2 + 1) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
-            }
-            {
-              // a value row that is not a number: the rows that see it are none either (its key's factor)
-              const int r = 16 * w4 + (lane & 15), rt = hh * kHalf + r;
-              const uint32_t ke = (__shfl_sync(0xffffffffu, k4, rt >> 2) >> (8 * (rt & 3))) & 255u, ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
-              float* fk = reinterpret_cast<float*>(facs + b * kFacBytes);
-              if (lane < 16) fk[r] = ve == 255u && rt < left ? __uint_as_float(0x7fffffffu) : sign * __uint_as_float(ke << 23);
-              if (warp == 12 && lane == 16) reinterpret_cast<int*>(fk)[kHalf] = ref;
-            }
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(w_full + b);
-          }
-          if (lane == 0) mbar_arrive(v_free + slot);
-          if (++slot == kVSlots) slot = 0, ph ^= 1;
-        }
-      }
+    } else {
+      widen(FEW ? 0 : -1);
     }
   }
   fence_before();
@@ -592,11 +684,11 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
 
 }  // namespace
 
-int kv8_rows_launch(const Kv8Maps& m, const Kv8QueryMaps& q, const Kv8Params& p, int grid, cudaStream_t s) {
+int kv8_rows_launch(const Kv8Maps& m, const Kv8QueryMaps& q, const Kv8Params& p, bool few, int grid, cudaStream_t s) {
   if (const int e = wait_status()) return e;
-  static bool done[64] = {};
-  B200_CUDA(ensure_dynamic_smem(kv8_rows_kernel, kSmem, done));
-  B200_CUDA(launch(kv8_rows_kernel, dim3(grid), dim3(kThreads), (size_t)kSmem, s, m, q, p));
+  static bool done[2][64] = {};
+  B200_CUDA(few ? ensure_dynamic_smem(kv8_rows_kernel<true>, kSmem, done[1]) : ensure_dynamic_smem(kv8_rows_kernel<false>, kSmem, done[0]));
+  B200_CUDA(launch(few ? kv8_rows_kernel<true> : kv8_rows_kernel<false>, dim3(grid), dim3(kThreads), (size_t)kSmem, s, m, q, p));
   return B200_OK;
 }
 
