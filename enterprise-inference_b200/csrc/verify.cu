@@ -176,7 +176,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
                    const float* __restrict__ uniforms, int n_rows, int vocab, int n_slices, const Stat* __restrict__ stats, int32_t* __restrict__ out,
                    int32_t* __restrict__ accepted) {
   extern __shared__ __align__(16) unsigned char row_smem[];   // the CTA's part of the target row
-  __shared__ double table[16], chunk_sum[kMostChunks], warp_part[2][kDrawThreads / 32], mine[2], shared_w;
+  __shared__ double table[16], chunk_sum[kMostChunks], chunk_q[kMostChunks], warp_part[2][kDrawThreads / 32], mine[4], shared_w, known_ratio[kKnownRows], sh_ratio;
   __shared__ int sh_refused, sh_best, sh_chunk, known_at[kKnownRows];
   __shared__ float sh_m[2], known_m[kKnownRows][2];
   const cg::cluster_group cluster = cg::this_cluster();
@@ -214,6 +214,10 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     }
     if (m[0] == -INFINITY) at = 0;
   };
+  // the sums of a row's target over its draft, each relative to its largest logit, as near as fp32 has them
+  auto ratio = [&](const float (&m)[2], const float (&f)[2], const double (&z)[2]) {
+    return z[1] > 0.0 ? z[0] / z[1] * exp2(((double)f[0] - (double)m[0] * c) - ((double)f[1] - (double)m[1] * c)) : 0.0;
+  };
   // a warp a row: is the draft refused?
   for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
     double z[2];
@@ -226,7 +230,10 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     const uint32_t lx = ok ? __bfloat16_as_ushort(target[(int64_t)r * ldt + x]) : 0u, dx = ok && draft ? __bfloat16_as_ushort(draft[(int64_t)r * ldd + x]) : 0u;
     const double u = ok && !greedy ? (double)uniforms[2 * r] : 0.0;
     row_stats(r, m, f, z, at, !greedy);
-    if (lane == 0 && r - r0 < kKnownRows) known_m[r - r0][0] = m[0], known_m[r - r0][1] = m[1], known_at[r - r0] = at;
+    if (lane == 0 && r - r0 < kKnownRows) {
+      known_m[r - r0][0] = m[0], known_m[r - r0][1] = m[1], known_at[r - r0] = at;
+      known_ratio[r - r0] = ratio(m, f, z);
+    }
     ok = ok && m[0] > -INFINITY;
     if (ok && greedy) {
       ok = x == at;
@@ -242,13 +249,13 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   const bool any = r1 > r0, last = row == r1 - 1;
   // the row that draws: its largest logits
   if (any && taken < kKnownRows) {
-    if (tid == 0) sh_m[0] = known_m[taken][0], sh_m[1] = known_m[taken][1], sh_best = known_at[taken];
+    if (tid == 0) sh_m[0] = known_m[taken][0], sh_m[1] = known_m[taken][1], sh_best = known_at[taken], sh_ratio = known_ratio[taken];
   } else if (any && warp == 0) {
     double z[2];
     float m[2], f[2];
     int at;
-    row_stats(row, m, f, z, at, false);
-    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = at;
+    row_stats(row, m, f, z, at, !greedy);
+    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = at, sh_ratio = ratio(m, f, z);
   }
   __syncthreads();
   if (rank == 0) {
@@ -275,35 +282,85 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   f2::cp_wait_all();
   // entry j of eight, relative to 2^m
   auto weight = [&](const uint32_t* w, int j, double m) { return exp2_table(fma(float_double(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16), c, -m), table); };
-  // the CTA's two sums -> the cluster's, in rank order; before: what the ranks in front have
-  auto cluster_sum = [&](double a, double b, double* all, double* before) {
-    if (tid == 0) mine[0] = a, mine[1] = b;
+  // the CTA's N sums -> the cluster's, in rank order: use(rank, its sums)
+  auto cluster_sums = [&](auto use) {
     cluster.sync();
-    double t[2] = {0.0, 0.0};
-    for (int k = 0; k < kDrawCtas; ++k) {
-      const double* other = cluster.map_shared_rank(mine, k);
-      if (k == rank && before) *before = t[0];
-      t[0] += other[0], t[1] += other[1];
-    }
+    for (int k = 0; k < kDrawCtas; ++k) use(k, cluster.map_shared_rank(mine, k));
     cluster.sync();   // (nobody writes again, or leaves, while another reads)
-    all[0] = t[0], all[1] = t[1];
   };
+  // running sums of the chunks, by a warp: kMostChunks / 32 neighbours a lane, then over the lanes; returns their sum
+  auto running = [&](double* v) {
+    constexpr int N = kMostChunks / 32;
+    double t[N], sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int at = lane * N + i;
+      sum += at < ch1 - ch0 ? v[at] : 0.0;
+      t[i] = sum;
+    }
+    double front = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double w = __shfl_up_sync(0xffffffffu, front, o);
+      if (lane >= o) front += w;
+    }
+    const double prev = __shfl_up_sync(0xffffffffu, front, 1), base = lane ? prev : 0.0;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (lane * N + i < ch1 - ch0) v[lane * N + i] = base + t[i];
+    return __shfl_sync(0xffffffffu, front, 31);
+  };
+  double all = 0.0, before = 0.0;   // of all CTAs' weights, of those in front of this one's
+  bool found = false;               // are the sums there?
   if (probs) {
-    double a = 0.0, b = 0.0;
+    // One pass over both rows: sums of either, and of either over the entries of which p is the larger by far as fp32 knows the sums' ratio.  max(p - q, 0) sums to the
+    // difference of the latter two (an entry on the wrong side counts 1e-7 of itself, and only 1e-7 of them are).  Where less than 1e-4 is left that
+    // difference has lost digits: then entry by entry, below.
+    const double rho = sh_ratio;
+    double zp = 0.0, zq = 0.0;
     for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
       const uint4 v = part_p[(ch - ch0) * (kChunk / 8) + lane], w = load8(d, ch * kChunk + 8 * lane, vocab);
       const uint32_t p4[4] = {v.x, v.y, v.z, v.w}, q4[4] = {w.x, w.y, w.z, w.w};
+      double a = 0.0, b = 0.0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) a += weight(p4, j, mp), b += weight(q4, j, mq);
+      for (int j = 0; j < 8; ++j) {
+        const double ep = weight(p4, j, mp), eq = weight(q4, j, mq);
+        zp += ep, zq += eq;
+        if (ep > rho * eq) a += ep, b += eq;
+      }
+      a = warp_sum_double(a), b = warp_sum_double(b);
+      if (lane == 0) chunk_sum[ch - ch0] = a, chunk_q[ch - ch0] = b;
     }
-    a = warp_sum_double(a), b = warp_sum_double(b);
-    if (lane == 0) warp_part[0][warp] = a, warp_part[1][warp] = b;
+    zp = warp_sum_double(zp), zq = warp_sum_double(zq);
+    if (lane == 0) warp_part[0][warp] = zp, warp_part[1][warp] = zq;
     __syncthreads();
-    a = b = 0.0;
-    for (int w = 0; w < kDrawThreads / 32; ++w) a += warp_part[0][w], b += warp_part[1][w];
-    double z[2];
-    cluster_sum(a, b, z, nullptr);
-    mp += log2(z[0]), mq += log2(z[1]);   // from here on probabilities
+    if (warp < 2) {
+      const double t = running(warp ? chunk_q : chunk_sum);
+      if (lane == 0) {
+        double z = 0.0;
+        for (int w = 0; w < kDrawThreads / 32; ++w) z += warp_part[warp][w];
+        mine[warp] = t, mine[2 + warp] = z;
+      }
+    }
+    double za = 0.0, zb = 0.0, part[kDrawCtas][2];
+    cluster_sums([&](int k, const double* other) {
+      part[k][0] = other[0], part[k][1] = other[1];
+      za += other[2], zb += other[3];
+    });
+    mp += log2(za), mq += log2(zb);   // from here on probabilities
+    double own = 0.0;
+#pragma unroll
+    for (int k = 0; k < kDrawCtas; ++k) {
+      const double w = fmax(part[k][0] / za - part[k][1] / zb, 0.0);
+      if (k == rank) before = all, own = w;
+      all += w;
+    }
+    found = all > 1e-4;
+    if (found) {
+      for (int i = tid; i < ch1 - ch0; i += kDrawThreads) chunk_sum[i] = chunk_sum[i] / za - chunk_q[i] / zb;
+      if (tid == 0) shared_w = own;
+    }
+    __syncthreads();
   }
   for (int pass = residual ? 0 : 1; pass < 2; ++pass) {   // what the draft leaves of p; p itself behind the last draft, and where nothing is left
     auto weights8 = [&](int ch, double (&w)[8]) {
@@ -326,39 +383,26 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
       for (int j = 0; j < 8; ++j)
         if (i + j == x) w[j] = 0.0;
     };
-    for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
-      double w[8];
-      weights8(ch, w);
-      const double t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-      if (lane == 0) chunk_sum[ch - ch0] = t;
-    }
-    __syncthreads();
-    if (warp == 0) {   // running sums of the chunks: kMostChunks / 32 neighbours a lane, then over the lanes
-      constexpr int N = kMostChunks / 32;
-      double t[N], sum = 0.0;
-#pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int at = lane * N + i;
-        sum += at < ch1 - ch0 ? chunk_sum[at] : 0.0;
-        t[i] = sum;
+    if (!found) {
+      for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
+        double w[8];
+        weights8(ch, w);
+        const double t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
+        if (lane == 0) chunk_sum[ch - ch0] = t;
       }
-      double front = sum;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double v = __shfl_up_sync(0xffffffffu, front, o);
-        if (lane >= o) front += v;
+      __syncthreads();
+      if (warp == 0) {
+        const double t = running(chunk_sum);
+        if (lane == 0) mine[0] = shared_w = t;
       }
-      const double prev = __shfl_up_sync(0xffffffffu, front, 1), base = lane ? prev : 0.0;
-#pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (lane * N + i < ch1 - ch0) chunk_sum[lane * N + i] = base + t[i];
-      if (lane == 31) shared_w = front;
+      all = 0.0;
+      cluster_sums([&](int k, const double* other) {
+        if (k == rank) before = all;
+        all += other[0];
+      });
+      if (all == 0.0) continue;   // nothing left (pass 0): the cluster agrees
     }
-    __syncthreads();
-    double all[2], before = 0.0;
-    cluster_sum(shared_w, 0.0, all, &before);
-    if (all[0] == 0.0) continue;   // nothing left (pass 0): the cluster agrees
-    const double limit = (double)uniforms[2 * row + 1] * all[0];
+    const double limit = (double)uniforms[2 * row + 1] * all;
     if (tid == 0) sh_chunk = 0x7fffffff;
     __syncthreads();
     if (before + shared_w > limit && !(before > limit)) {   // the CTA that holds the border (each adds up the same numbers: there is one)
