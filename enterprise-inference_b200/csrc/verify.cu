@@ -22,6 +22,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kStatThreads = 256, kLeastSlice = 2048;
+constexpr float kMostScale = 1e30f;   // (temperatures below 1e-30 are taken as that)
 constexpr int kDrawThreads = 256, kDrawCtas = 8, kChunk = 256, kMostChunks = 192;
 constexpr int kMostVocab = kDrawCtas * kMostChunks * kChunk, kMostPart = kMostChunks * kChunk * 2;
 
@@ -76,7 +77,7 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
   const int i0 = slice * slice_len, i1 = min(vocab, i0 + slice_len), a0 = i0 - shift;
   float m = -INFINITY, f = 0.f, s = 0.f;
   int at = 0x7fffffff;
-  const float c = temp > 0.f ? 1.4426950408889634f / temp : 0.f;
+  const float c = temp > 0.f ? fminf(1.4426950408889634f / temp, kMostScale) : 0.f;
   constexpr int U = 4;
   for (int g0 = threadIdx.x * 8; a0 + g0 < i1; g0 += U * kStatThreads * 8) {
     uint4 v[U];
@@ -110,17 +111,20 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
         at = a0 + g0 + u * kStatThreads * 8;
       }
       if (temp > 0.f) {   // (-inf alone so far: 2^-inf)
-        float e[4];
+        uint64_t e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) e[j] = tc::exp2_fast(fmaf(bf16lo(w[j]), c, -f)) + tc::exp2_fast(fmaf(bf16hi(w[j]), c, -f));
-        s += (e[0] + e[1]) + (e[2] + e[3]);
+        for (int j = 0; j < 4; ++j) {
+          const uint64_t t = f2::fma(f2::pack(bf16lo(w[j]), bf16hi(w[j])), f2::both(c), f2::both(-f));
+          e[j] = f2::pack(tc::exp2_fast(f2::lo(t)), tc::exp2_fast(f2::hi(t)));
+        }
+        s += f2::sum(f2::add(f2::add(e[0], e[1]), f2::add(e[2], e[3])));
       }
     }
   }
   pdl_launch_dependents();   // (before the rows are read the next launch's CTAs would only take their places: 112 -> 141 us)
   // the first place of the thread's largest entry
   if (m > -INFINITY) {
-    for (int k = max(at, i0);; ++k)
+    for (int k = max(at, i0), end = min(at + 8, i1); k < end; ++k)
       if (__bfloat162float(l[k]) == m) {
         at = k;
         break;
@@ -146,24 +150,24 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
   }
 }
 
-// a bf16 as a double by its bits (zero and denormals come out as 2^-127 to 2^-126, -inf as -2^128: nothing beside any logit that counts)
-__device__ __forceinline__ double float_double(uint32_t f) {   // f: the value's fp32 bits
-  return __hiloint2double((int)(((f >> 3) & 0x0fffffffu) + 0x38000000u | (f & 0x80000000u)), 0);
-}
-__device__ __forceinline__ double bf16_double(uint32_t h) { return float_double(h << 16); }
-// 2^t for t <= 0 (or little more): t = n / 16 + r, 2^(n / 16) = 2^(n >> 4) table[n & 15], 2^r = 1 + r q(r), |r| <= 1 / 32, terms ln2^k / k! (the first left out: 1.5e-13)
+// a bf16 in its fp32 bits -> the double of 2^-896 times its value (the exponent's bits moved as they are; denormals stay what they are, -inf comes out as
+// -2^128 times that: nothing beside any logit that counts)
+__device__ __forceinline__ double scaled_double(uint32_t f) { return __hiloint2double((int)f >> 3 & (int)0x8fffffffu, 0); }
+constexpr double kScaledBack = 0x1p896;
+// 2^t for t <= 0 (or little more), 2^-1017 below: t = n / 32 + r, 2^(n / 32) = 2^(n >> 5) table[n & 31], 2^r = 1 + r q(r), |r| <= 1 / 64: the series of (2^r - 1) / r
+// with its terms above the third taken down to a cubic by Chebyshev polynomials, 1.6e-13 of 2^r
 __device__ __forceinline__ double exp2_table(double t, const double* table) {
-  const double u = t + 422212465065984.0;   // 1.5 * 2^48: n in the low bits
-  const double r = t - (u - 422212465065984.0);
+  t = __hiloint2double((int)min((uint32_t)__double2hiint(t), 0xc08fc800u), __double2loint(t));
+  const double u = t + 211106232532992.0;   // 1.5 * 2^47: n in the low bits
+  const double r = t - (u - 211106232532992.0);
   const int n = __double2loint(u);
-  double q = fma(r, 0.0013333558146428441, 0.009618129107628477);
-  q = fma(q, r, 0.05550410866482158);
-  q = fma(q, r, 0.24022650695910072);
-  q = fma(q, r, 0.6931471805599453);
-  const double b = table[n & 15], e = fma(b * r, q, b);
-  const bool none = (uint32_t)__double2hiint(t) > 0xc08f4000u;   // t < -1000
-  return __hiloint2double(none ? 0 : __double2hiint(e) + ((n >> 4) << 20), none ? 0 : __double2loint(e));
+  double q = fma(r, 0.00961817611557608, 0.05550443419199583);
+  q = fma(q, r, 0.24022650695623157);
+  q = fma(q, r, 0.693147180550011);
+  const double b = table[n & 31], e = fma(b * r, q, b);
+  return __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
 }
+constexpr double kNothing = 1e-300;   // what 2^t gives for a masked entry, and no weight that counts, is below
 __device__ __forceinline__ double warp_sum_double(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -176,18 +180,18 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
                    const float* __restrict__ uniforms, int n_rows, int vocab, int n_slices, const Stat* __restrict__ stats, int32_t* __restrict__ out,
                    int32_t* __restrict__ accepted) {
   extern __shared__ __align__(16) unsigned char row_smem[];   // the CTA's part of the target row
-  __shared__ double table[16], chunk_sum[kMostChunks], chunk_q[kMostChunks], warp_part[2][kDrawThreads / 32], mine[4], shared_w, known_ratio[kKnownRows], sh_ratio;
+  __shared__ double table[32], chunk_sum[kMostChunks], chunk_q[kMostChunks], warp_part[2][kDrawThreads / 32], mine[2], shared_w, known_ratio[kKnownRows], sh_ratio;
   __shared__ int sh_refused, sh_best, sh_chunk, known_at[kKnownRows];
   __shared__ float sh_m[2], known_m[kKnownRows][2];
   const cg::cluster_group cluster = cg::this_cluster();
   const int rank = (int)cluster.block_rank(), s = blockIdx.x / kDrawCtas, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid < 16) table[tid] = exp2(tid / 16.0);
+  if (tid < 32) table[tid] = exp2(tid / 32.0);
   pdl_wait();
   pdl_launch_dependents();
   const int r0 = min(max(starts[s], 0), n_rows), r1 = min(max(starts[s + 1], r0), n_rows);
   const float temp = temperature ? temperature[s] : 0.f;
   const bool greedy = !(temp > 0.f);
-  const double c = greedy ? 0.0 : 1.4426950408889634 / (double)temp, cf = greedy ? 0.0 : (double)(1.4426950408889634f / temp);   // cf: what the sums have
+  const double c = greedy ? 0.0 : fmin(1.4426950408889634 / (double)temp, (double)kMostScale), cf = greedy ? 0.0 : (double)fminf(1.4426950408889634f / temp, kMostScale);   // cf: what the sums have
   if (tid == 0) sh_refused = max(r1 - r0 - 1, 0);
   __syncthreads();
   // a row's largest logits and their first place, from the slices (by a warp)
@@ -216,7 +220,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   };
   // the sums of a row's target over its draft, each relative to its largest logit, as near as fp32 has them
   auto ratio = [&](const float (&m)[2], const float (&f)[2], const double (&z)[2]) {
-    return z[1] > 0.0 ? z[0] / z[1] * exp2(((double)f[0] - (double)m[0] * c) - ((double)f[1] - (double)m[1] * c)) : 0.0;
+    return z[1] > 0.0 ? z[0] / z[1] * exp2(((double)f[0] - (double)m[0] * cf) - ((double)f[1] - (double)m[1] * cf)) : 0.0;
   };
   // a warp a row: is the draft refused?
   for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
@@ -238,8 +242,8 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     if (ok && greedy) {
       ok = x == at;
     } else if (ok) {
-      const double p = exp2_table(fma(bf16_double(lx), cf, -(double)f[0]), table) / z[0];
-      const double q = !draft ? 1.0 : m[1] > -INFINITY ? exp2_table(fma(bf16_double(dx), cf, -(double)f[1]), table) / z[1] : 0.0;
+      const double p = lx == 0xff80u ? 0.0 : exp2_table(fma((double)__uint_as_float(lx << 16), cf, -(double)f[0]), table) / z[0];
+      const double q = !draft ? 1.0 : m[1] > -INFINITY && dx != 0xff80u ? exp2_table(fma((double)__uint_as_float(dx << 16), cf, -(double)f[1]), table) / z[1] : 0.0;
       ok = u * q < p;
     }
     if (!ok && lane == 0) atomicMin(&sh_refused, r - r0);
@@ -262,7 +266,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     if (tid == 0) accepted[s] = taken;
     for (int r = r0 + tid; r < r1; r += kDrawThreads)
       if (r != row) out[r] = r < row ? tokens[r] : -1;
-    if (any && tid == 0 && (greedy || sh_m[0] == -INFINITY)) out[row] = sh_best;
+    if (any && tid == 0) out[row] = sh_best;   // greedy, or nothing to draw from (or, with NaN among the logits, no border found); else a draw's CTA writes again
   }
   if (!any || greedy || sh_m[0] == -INFINITY) return;   // (the cluster's CTAs all leave here)
 
@@ -270,7 +274,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   const bool residual = !last, probs = residual && draft && sh_m[1] > -INFINITY;
   const __nv_bfloat16* d = probs ? draft + (int64_t)row * ldd : nullptr;
   const int x = residual && !draft ? tokens[row] : -1;   // a certain draft: what is left has nothing of it
-  double mp = (double)sh_m[0] * c, mq = probs ? (double)sh_m[1] * c : 0.0;
+  const double mp = (double)sh_m[0] * c, mq = probs ? (double)sh_m[1] * c : 0.0, scale = c * kScaledBack;
   const int n_chunks = (vocab + kChunk - 1) / kChunk, per = (n_chunks + kDrawCtas - 1) / kDrawCtas;
   const int ch0 = min(n_chunks, rank * per), ch1 = min(n_chunks, ch0 + per);
   // the CTA's entries, -inf behind the end (a thread reads back what it wrote: its eight of every 16th chunk)
@@ -281,13 +285,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   }
   f2::cp_wait_all();
   // entry j of eight, relative to 2^m
-  auto weight = [&](const uint32_t* w, int j, double m) { return exp2_table(fma(float_double(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16), c, -m), table); };
-  // the CTA's N sums -> the cluster's, in rank order: use(rank, its sums)
-  auto cluster_sums = [&](auto use) {
-    cluster.sync();
-    for (int k = 0; k < kDrawCtas; ++k) use(k, cluster.map_shared_rank(mine, k));
-    cluster.sync();   // (nobody writes again, or leaves, while another reads)
-  };
+  auto weight = [&](const uint32_t* w, int j, double m) { return exp2_table(fma(scaled_double(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16), scale, -m), table); };
   // running sums of the chunks, by a warp: kMostChunks / 32 neighbours a lane, then over the lanes; returns their sum
   auto running = [&](double* v) {
     constexpr int N = kMostChunks / 32;
@@ -310,57 +308,48 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
       if (lane * N + i < ch1 - ch0) v[lane * N + i] = base + t[i];
     return __shfl_sync(0xffffffffu, front, 31);
   };
-  double all = 0.0, before = 0.0;   // of all CTAs' weights, of those in front of this one's
-  bool found = false;               // are the sums there?
+  double to_p = 1.0, to_q = 1.0;   // one over the rows' sums
   if (probs) {
-    // One pass over both rows: sums of either, and of either over the entries of which p is the larger by far as fp32 knows the sums' ratio.  max(p - q, 0) sums to the
-    // difference of the latter two (an entry on the wrong side counts 1e-7 of itself, and only 1e-7 of them are).  Where less than 1e-4 is left that
-    // difference has lost digits: then entry by entry, below.
+    // One pass over both rows: their sums, and for each chunk the sums A of e^p and B of e^q over the entries of which p is the larger, going by the ratio of the rows' sums
+    // in fp32: max(p - q, 0) then sums to A / Zp - B / Zq.  A chunk with an entry of equal p and q to within 2^-17 (the ratio is good to 2^-19) is marked, and
+    // taken entry by entry below, as is one whose difference loses four digits.
     const double rho = sh_ratio;
     double zp = 0.0, zq = 0.0;
+    uint4 next = ch0 + warp < ch1 ? load8(d, (ch0 + warp) * kChunk + 8 * lane, vocab) : uint4{};
     for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
-      const uint4 v = part_p[(ch - ch0) * (kChunk / 8) + lane], w = load8(d, ch * kChunk + 8 * lane, vocab);
+      const uint4 v = part_p[(ch - ch0) * (kChunk / 8) + lane], w = next;
+      if (ch + kDrawThreads / 32 < ch1) next = load8(d, (ch + kDrawThreads / 32) * kChunk + 8 * lane, vocab);
       const uint32_t p4[4] = {v.x, v.y, v.z, v.w}, q4[4] = {w.x, w.y, w.z, w.w};
       double a = 0.0, b = 0.0;
+      bool near = false;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const double ep = weight(p4, j, mp), eq = weight(q4, j, mq);
+        const double ep = weight(p4, j, mp), eq = weight(q4, j, mq), more = fma(-rho, eq, ep);
         zp += ep, zq += eq;
-        if (ep > rho * eq) a += ep, b += eq;
+        near |= (__double2hiint(more) & 0x7fffffff) + (17 << 20) < __double2hiint(ep);
+        if (more > 0.0) a += ep, b += eq;
       }
       a = warp_sum_double(a), b = warp_sum_double(b);
-      if (lane == 0) chunk_sum[ch - ch0] = a, chunk_q[ch - ch0] = b;
+      near = __any_sync(0xffffffffu, near);
+      if (lane == 0) chunk_sum[ch - ch0] = near ? -1.0 : a, chunk_q[ch - ch0] = b;
     }
     zp = warp_sum_double(zp), zq = warp_sum_double(zq);
     if (lane == 0) warp_part[0][warp] = zp, warp_part[1][warp] = zq;
     __syncthreads();
-    if (warp < 2) {
-      const double t = running(warp ? chunk_q : chunk_sum);
-      if (lane == 0) {
-        double z = 0.0;
-        for (int w = 0; w < kDrawThreads / 32; ++w) z += warp_part[warp][w];
-        mine[warp] = t, mine[2 + warp] = z;
-      }
+    if (tid < 2) {
+      double z = 0.0;
+      for (int w = 0; w < kDrawThreads / 32; ++w) z += warp_part[tid][w];
+      mine[tid] = z;
     }
-    double za = 0.0, zb = 0.0, part[kDrawCtas][2];
-    cluster_sums([&](int k, const double* other) {
-      part[k][0] = other[0], part[k][1] = other[1];
-      za += other[2], zb += other[3];
-    });
-    mp += log2(za), mq += log2(zb);   // from here on probabilities
-    double own = 0.0;
+    cluster.sync();
+    zp = zq = 0.0;
 #pragma unroll
     for (int k = 0; k < kDrawCtas; ++k) {
-      const double w = fmax(part[k][0] / za - part[k][1] / zb, 0.0);
-      if (k == rank) before = all, own = w;
-      all += w;
+      const double* other = cluster.map_shared_rank(mine, k);
+      zp += other[0], zq += other[1];
     }
-    found = all > 1e-4;
-    if (found) {
-      for (int i = tid; i < ch1 - ch0; i += kDrawThreads) chunk_sum[i] = chunk_sum[i] / za - chunk_q[i] / zb;
-      if (tid == 0) shared_w = own;
-    }
-    __syncthreads();
+    cluster.sync();   // (nobody writes again while another reads)
+    to_p = 1.0 / zp, to_q = 1.0 / zq;
   }
   for (int pass = residual ? 0 : 1; pass < 2; ++pass) {   // what the draft leaves of p; p itself behind the last draft, and where nothing is left
     auto weights8 = [&](int ch, double (&w)[8]) {
@@ -375,7 +364,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
         const uint32_t q4[4] = {q.x, q.y, q.z, q.w};
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const double left = w[j] - weight(q4, j, mq);
+          const double left = __dsub_rn(__dmul_rn(w[j], to_p), __dmul_rn(weight(q4, j, mq), to_q));   // (equal rows leave zeros)
           w[j] = left > 0.0 ? left : 0.0;
         }
       }
@@ -383,25 +372,36 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
       for (int j = 0; j < 8; ++j)
         if (i + j == x) w[j] = 0.0;
     };
-    if (!found) {
-      for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
+    for (int ch = ch0 + warp; ch < ch1; ch += kDrawThreads / 32) {
+      double t = -1.0;
+      if (probs && !pass) {
+        const double a = chunk_sum[ch - ch0] * to_p;
+        t = a - chunk_q[ch - ch0] * to_q;
+        if (!(t > 1e-4 * a) && a != 0.0) t = -1.0;
+      }
+      if (t < 0.0) {
         double w[8];
         weights8(ch, w);
-        const double t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
-        if (lane == 0) chunk_sum[ch - ch0] = t;
+        t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
       }
-      __syncthreads();
-      if (warp == 0) {
-        const double t = running(chunk_sum);
-        if (lane == 0) mine[0] = shared_w = t;
-      }
-      all = 0.0;
-      cluster_sums([&](int k, const double* other) {
-        if (k == rank) before = all;
-        all += other[0];
-      });
-      if (all == 0.0) continue;   // nothing left (pass 0): the cluster agrees
+      __syncwarp();
+      if (lane == 0) chunk_sum[ch - ch0] = t;
     }
+    __syncthreads();
+    if (warp == 0) {
+      const double t = running(chunk_sum);
+      if (lane == 0) mine[0] = shared_w = t;
+    }
+    cluster.sync();
+    double all = 0.0, before = 0.0;   // of all CTAs' weights, of those in front of this one's
+#pragma unroll
+    for (int k = 0; k < kDrawCtas; ++k) {
+      const double w = *cluster.map_shared_rank(mine, k);
+      if (k == rank) before = all;
+      all += w;
+    }
+    cluster.sync();   // (nobody writes again, or leaves, while another reads)
+    if (!pass && !(all > kNothing)) continue;   // nothing left: the cluster agrees
     const double limit = (double)uniforms[2 * row + 1] * all;
     if (tid == 0) sh_chunk = 0x7fffffff;
     __syncthreads();
@@ -426,7 +426,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           front += w[j];
-          if (w[j] > 0.0) {
+          if (w[j] > kNothing) {
             some = i + j;
             if (front > limit && token == 0x7fffffff) token = i + j;
           }
