@@ -2,12 +2,14 @@
 //
 // stats: a CTA takes a slice of a logit row (target rows, and the rows that drafts were drawn from) and leaves its largest logit, the first place of it and the sum
 // of 2^(l c - f), c = log2e / T, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  f is the largest l c as a whole number,
-// so that l c - f is rounded once.  Bound by the rows' bytes, closely followed by the exponentials (12 entries a cycle and SM, of 16).
+// so that l c - f is rounded once.  A thread compares 32 entries with its maximum at once; the place is looked for at the end, by the threads that met the CTA's
+// largest (with a place kept by every thread the same took 23.5 million instructions for 64 x 5 drafts over 128256 entries, this 15.2).  35 us there, 4.2 TB/s;
+// bound by the exponentials (four a cycle and quarter of an SM: 16 us) and the latency of short loops.
 // draw: a cluster of eight CTAs takes a sequence: the kept drafts from the slices' sums, then the token from the one row that draws it.  A draw next to a border of
 // the cumulated weights has to come out as in exact arithmetic (128 k borders: sums that are off by 1e-9 pick another token once in 4000 draws), so weights and
-// sums are fp64 there: 2^t by a table of 16 powers and a polynomial of degree 5, relative error below 2e-13, twelve fp64 operations a weight (256 powers and a cubic
-// are ten, but 32 lanes that look up 256 doubles meet in the banks of shared memory; 16 fill them exactly).  Each CTA owns an eighth of the
-// row in chunks of 256 entries, the target's fetched once into shared memory; sums are taken in a fixed order, chunk by chunk.
+// sums are fp64 there: 2^t by a table of 32 powers and a cubic, relative error below 2e-13, nine fp64 operations a weight (16 powers and a degree of 5, with selects for
+// masked entries: 45 instructions a weight in all and 49 us, this 30 and 40).  Each CTA owns an eighth of the row in chunks of 256 entries, the target's fetched once
+// into shared memory; sums are taken in a fixed order, chunk by chunk.  Bound by the instructions of the weights: 26 thousand a quarter of an SM.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -21,7 +23,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kStatThreads = 256, kLeastSlice = 2048;
+constexpr int kStatThreads = 256, kStatGroups = 4, kLeastSlice = 2048, kWholeSlice = kStatThreads * 8 * kStatGroups;
 constexpr float kMostScale = 1e30f;   // (temperatures below 1e-30 are taken as that)
 constexpr int kDrawThreads = 256, kDrawCtas = 8, kChunk = 256, kMostChunks = 192;
 constexpr int kMostVocab = kDrawCtas * kMostChunks * kChunk, kMostPart = kMostChunks * kChunk * 2;
@@ -58,11 +60,11 @@ __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
 __global__ void __launch_bounds__(kStatThreads)
 verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const __nv_bfloat16* __restrict__ draft, int64_t ldd, const int32_t* __restrict__ starts,
                     const float* __restrict__ temperature, int n_seqs, int vocab, int slice_len, Stat* __restrict__ stats) {
-  __shared__ int found;
-  __shared__ Stat sh[kStatThreads / 32];
+  __shared__ int found, first;
+  __shared__ float sh_m[kStatThreads / 32], sh_s[kStatThreads / 32];
   pdl_wait();
   const int slice = blockIdx.x, row = blockIdx.y, which = blockIdx.z;
-  if (threadIdx.x == 0) found = -1;
+  if (threadIdx.x == 0) found = -1, first = 0x7fffffff;
   __syncthreads();
   for (int s = threadIdx.x; s < n_seqs; s += kStatThreads)
     if (starts[s] <= row && row < starts[s + 1]) found = s;
@@ -78,12 +80,12 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
   float m = -INFINITY, f = 0.f, s = 0.f;
   int at = 0x7fffffff;
   const float c = temp > 0.f ? fminf(1.4426950408889634f / temp, kMostScale) : 0.f;
-  constexpr int U = 4;
-  for (int g0 = threadIdx.x * 8; a0 + g0 < i1; g0 += U * kStatThreads * 8) {
+  constexpr int U = kStatGroups, S = kStatThreads * 8;
+  for (int g0 = a0 + threadIdx.x * 8; g0 < i1; g0 += U * S) {
     uint4 v[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const int i = a0 + g0 + u * kStatThreads * 8;
+      const int i = g0 + u * S;
       v[u] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
       if (i >= i0 && i + 8 <= i1) {
         v[u] = ld_stream(l + i);
@@ -98,55 +100,53 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
         v[u] = make_uint4(w[0], w[1], w[2], w[3]);
       }
     }
+    uint32_t h = 0xff80ff80u;
+#pragma unroll
+    for (int u = 0; u < U; ++u) h = max2(h, max2(max2(v[u].x, v[u].y), max2(v[u].z, v[u].w)));
+    const float top = fmaxf(bf16lo(h), bf16hi(h));
+    if (top > m) {
+      const float fn = rintf(top * c);
+      s *= tc::exp2_fast(f - fn);   // (nothing yet: s is 0, f too)
+      f = fn;
+      m = top;
+      at = g0;
+    }
+    if (!(temp > 0.f)) continue;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
+      if (g0 + u * S >= i1) break;
       const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
-      const uint32_t h = max2(max2(w[0], w[1]), max2(w[2], w[3]));
-      const float top = fmaxf(bf16lo(h), bf16hi(h));
-      if (top > m) {
-        const float fn = rintf(top * c);
-        s *= tc::exp2_fast(f - fn);   // (nothing yet: s is 0, f too)
-        f = fn;
-        m = top;
-        at = a0 + g0 + u * kStatThreads * 8;
-      }
-      if (temp > 0.f) {   // (-inf alone so far: 2^-inf)
-        uint64_t e[4];
+      uint64_t e[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const uint64_t t = f2::fma(f2::pack(bf16lo(w[j]), bf16hi(w[j])), f2::both(c), f2::both(-f));
-          e[j] = f2::pack(tc::exp2_fast(f2::lo(t)), tc::exp2_fast(f2::hi(t)));
-        }
-        s += f2::sum(f2::add(f2::add(e[0], e[1]), f2::add(e[2], e[3])));
+      for (int j = 0; j < 4; ++j) {   // (-inf alone so far: 2^-inf)
+        const uint64_t t = f2::fma(f2::pack(bf16lo(w[j]), bf16hi(w[j])), f2::both(c), f2::both(-f));
+        e[j] = f2::pack(tc::exp2_fast(f2::lo(t)), tc::exp2_fast(f2::hi(t)));
       }
+      s += f2::sum(f2::add(f2::add(e[0], e[1]), f2::add(e[2], e[3])));
     }
   }
   pdl_launch_dependents();   // (before the rows are read the next launch's CTAs would only take their places: 112 -> 141 us)
-  // the first place of the thread's largest entry
-  if (m > -INFINITY) {
-    for (int k = max(at, i0), end = min(at + 8, i1); k < end; ++k)
-      if (__bfloat162float(l[k]) == m) {
-        at = k;
-        break;
-      }
-  }
-  auto join = [](float& m1, float& f1, float& s1, int& at1, float m2, float f2, float s2, int at2) {
-    if (m2 > -INFINITY) {
-      const float fn = m1 > -INFINITY ? fmaxf(f1, f2) : f2;
-      s1 = s1 * tc::exp2_fast(m1 > -INFINITY ? f1 - fn : 0.f) + s2 * tc::exp2_fast(f2 - fn);
-      f1 = fn;
-      if (m2 > m1 || (m2 == m1 && at2 < at1)) m1 = m2, at1 = at2;
-    }
-  };
+  const float most = warp_max(m);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (lane == 0) sh_m[warp] = most;
+  __syncthreads();
+  float all = sh_m[0];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1)
-    join(m, f, s, at, __shfl_xor_sync(0xffffffffu, m, o), __shfl_xor_sync(0xffffffffu, f, o), __shfl_xor_sync(0xffffffffu, s, o),
-         __shfl_xor_sync(0xffffffffu, at, o));
-  if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = {m, f, s, at};
+  for (int w = 1; w < kStatThreads / 32; ++w) all = fmaxf(all, sh_m[w]);
+  const float fa = rintf(all * c);
+  // the first place of the largest entry: those look for it who met it
+  if (m == all && m > -INFINITY) {
+    bool there = false;
+    for (int u = 0; u < U && !there; ++u)
+      for (int k = max(at + u * S, i0), end = min(at + u * S + 8, i1); k < end && !there; ++k)
+        if (__bfloat162float(l[k]) == m) atomicMin(&first, k), there = true;
+  }
+  s = warp_sum(m > -INFINITY ? s * tc::exp2_fast(f - fa) : 0.f);
+  if (lane == 0) sh_s[warp] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
-    for (int w = 1; w < kStatThreads / 32; ++w) join(m, f, s, at, sh[w].m, sh[w].f, sh[w].s, sh[w].at);
-    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {m, f, s, at};
+    for (int w = 1; w < kStatThreads / 32; ++w) s += sh_s[w];
+    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {all, all > -INFINITY ? fa : 0.f, s, first};
   }
 }
 
@@ -440,10 +440,11 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   }
 }
 
-// slices of a row: 24 CTAs an SM, each of at least kLeastSlice entries
+// slices of a row: about 24 CTAs an SM (12 and 48: 64 x 5 drafts 67.5 and 68.9 us, with 24 67.0), each of whole turns of its loop (lengths between leave the last
+// turn's groups empty) or, where rows are few, of at least kLeastSlice entries
 int slice_length(int n_rows, int vocab) {
-  const int64_t want = std::max<int64_t>(1, kNumSMs * 24 / std::max(1, 2 * n_rows));
-  return (int)std::max<int64_t>(kLeastSlice, ((vocab + want - 1) / want + 7) / 8 * 8);
+  const int64_t want = std::max<int64_t>(1, kNumSMs * 24 / std::max(1, 2 * n_rows)), len = (vocab + want - 1) / want;
+  return (int)(len > kWholeSlice / 2 ? (len + kWholeSlice - 1) / kWholeSlice * kWholeSlice : std::max<int64_t>(kLeastSlice, (len + 7) / 8 * 8));
 }
 int slices(int n_rows, int vocab) {
   const int len = slice_length(n_rows, vocab);
