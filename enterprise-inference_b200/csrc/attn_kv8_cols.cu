@@ -1,5 +1,5 @@
 // Paged attention of few (row, head) pairs over the 8-bit cache, on tcgen05 in e4m3: the 128 tokens of a tile fill the MMA's M, the pairs of a
-// kv head are its columns (decode rows: the G heads; drafts: rows x G, up to 32).
+// kv head are its columns (decode rows: the G heads; drafts: rows x G), at most 16.
 //
 //   S^T[128 tokens][2 NP] = K_tile . Q^T        (A = K as the cache has it, K-major)
 //   O^T[128 dims][2 NP] = V_tile^T . W^T        (A = V as the cache has it, MN-major)
@@ -27,28 +27,26 @@ constexpr int kSlotBytes = kKv8Tile * 128;   // a tile of keys or of values: 16 
 constexpr int kTable = 96;                   // items of a CTA that are described at a time
 constexpr int kFacs = 2;                     // tiles whose factors are kept
 constexpr int kFacBytes = kKv8Tile * 8 + 16; // a token's (key factor, value factor); the tile's factor, whether a token is dead
+constexpr int kAhead = 8;                    // tiles ahead that the exponents are asked for (a power of two)
 constexpr int kStageWarps = 4;               // keys, MMA, queries, values
 
 struct Kv8Item {
   int row0, nrows, seq, kvh, tile0, tile1, ctx, ends;   // ends: 1 begins in an earlier CTA, 2 goes on in the next
 };
 
-#ifndef B200_CG
-#define B200_CG(NC) ((NC) >= 16 ? 4 : (NC) >= 4 ? 2 : (NC))
-#endif
 template <int NC>
 struct Cols {
   static constexpr int NP = NC < 8 ? 8 : NC;               // columns of either term: N = 2 NP is a multiple of 16
-  static constexpr int CG = B200_CG(NC);              // groups of four softmax warps that share the columns
+  static constexpr int CG = NC < 4 ? NC : 4;               // groups of four softmax warps that share the columns
   static constexpr int NCG = NC / CG;
   static constexpr int kSpare = kStageWarps + 4 * CG;      // the warp behind them makes the tokens' factors
   static constexpr int kThreads = (kSpare + 1) * 32;
   static constexpr int kOperand = 2 * NP * 128;            // queries, or weights, of an item or tile
-  static constexpr int kSlots = NP <= 16 ? 12 : 10;          // even: keys and values in turn
-  static constexpr int kBars = (2 * kSlots + 15 + kFacs + 1) & ~1;
+  static constexpr int kStages = 6;                        // tiles in flight, keys and values each
+  static constexpr int kBars = (3 * kStages + 15 + kFacs + 1) & ~1;
   static constexpr uint32_t kTmem = 8 * NP;                // S, S, O, O
-  static constexpr int kSmem = 1024 + kSlots * kSlotBytes + 4 * kOperand + kFacs * kFacBytes + kTable * (int)sizeof(Kv8Item) +
-                               kBars * 8 + (4 * 32 + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + 64;
+  static constexpr int kSmem = 1024 + 2 * kStages * kSlotBytes + 4 * kOperand + kFacs * kFacBytes + kTable * (int)sizeof(Kv8Item) +
+                               kBars * 8 + (4 * 32 + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + kAhead * 256 + 64;
   static_assert(kSmem + 8 * (kThreads + kThreads / 32) <= 232448, "shared memory");
 };
 
@@ -72,27 +70,28 @@ template <int NC>
 __global__ void __launch_bounds__(Cols<NC>::kThreads, 1)
 kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   using C = Cols<NC>;
-  constexpr int NP = C::NP, CG = C::CG, NCG = C::NCG, kSlots = C::kSlots, kThreads = C::kThreads;
+  constexpr int NP = C::NP, CG = C::CG, NCG = C::NCG, kStages = C::kStages, kThreads = C::kThreads;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* ring = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
-  unsigned char* qs = ring + kSlots * kSlotBytes;          // [2] queries of an item
+  unsigned char* qs = ring + 2 * kStages * kSlotBytes;          // [2] queries of an item
   unsigned char* ws = qs + 2 * C::kOperand;                // [2] weights of a tile
   unsigned char* facs = ws + 2 * C::kOperand;              // [kFacs]
   Kv8Item* table = reinterpret_cast<Kv8Item*>(facs + kFacs * kFacBytes);
-  uint64_t* full = reinterpret_cast<uint64_t*>(table + kTable);   // [kSlots]: K, V, K, V, ...
-  uint64_t* freed = full + kSlots;
-  uint64_t* s_full = freed + kSlots;                       // [2]
+  uint64_t* full = reinterpret_cast<uint64_t*>(table + kTable);   // [kStages]: a tile's keys and values are there
+  uint64_t* freed = full + kStages;                        // [2 kStages]: keys, values, keys, ...
+  uint64_t* s_full = freed + 2 * kStages;                  // [2]: the tile's scores, and its factors
   uint64_t* w_ready = s_full + 2;
   uint64_t* o_full = w_ready + 2;
   uint64_t* q_ready = o_full + 2;
   uint64_t* q_free = q_ready + 2;
   uint64_t* q_info = q_free + 2;                           // [4]: an item's scales, for the softmax warps (who may be three items behind)
-  uint64_t* f_full = q_info + 4;                           // [kFacs]
-  uint64_t* last = f_full + kFacs;
+  uint64_t* f_free = q_info + 4;                           // [kFacs]
+  uint64_t* last = f_free + kFacs;
   float* q_scale = reinterpret_cast<float*>(full + C::kBars);   // [4 items][32]; from here on in whole 16 bytes
   float* x_sum = q_scale + 4 * 32;                         // [CG][2][NCG][4 warps]
   float* x_max = x_sum + CG * 2 * NCG * 4;                 // [CG][2][NCG][4 warps]
-  int* shared_int = reinterpret_cast<int*>(x_max + CG * 2 * NCG * 4);        // 0: tensor memory, 1: a wait ran out, 2, 3: the share's first and last item
+  uint32_t* exps = reinterpret_cast<uint32_t*>(x_max + CG * 2 * NCG * 4);   // [kAhead][32 lanes][keys, values]
+  int* shared_int = reinterpret_cast<int*>(exps + kAhead * 64);            // 0: tensor memory, 1: a wait ran out, 2, 3: the share's first and last item
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const Waits wait(reinterpret_cast<uint32_t*>(shared_int + 1), p.status);
   if (p.groups) {
@@ -106,16 +105,16 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   __shared__ uint64_t scan_warp[kThreads / 32], scan_thread[kThreads];
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSlots; ++s) mbar_init(full + s, 1), mbar_init(freed + s, 1);
+    for (int s = 0; s < kStages; ++s) mbar_init(full + s, 2), mbar_init(freed + 2 * s, 1), mbar_init(freed + 2 * s + 1, 1);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(s_full + s, 1);
+      mbar_init(s_full + s, 2);
       mbar_init(w_ready + s, 4 * CG);
       mbar_init(o_full + s, 1);
       mbar_init(q_ready + s, 1);
       mbar_init(q_free + s, 1);
     }
     for (int s = 0; s < 4; ++s) mbar_init(q_info + s, 1);
-    for (int s = 0; s < kFacs; ++s) mbar_init(f_full + s, 1);
+    for (int s = 0; s < kFacs; ++s) mbar_init(f_free + s, CG);
     mbar_init(last, 1);
     shared_int[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -219,7 +218,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
     const int box = min(p.block_size, kKv8Tile), per_tile = kKv8Tile / box;   // boxes of a tile
     const int cells = (int)(p.n_blocks * p.hkv * p.block_size);
-    int slot = values ? 1 : 0;
+    int stage = 0;
     uint32_t ph = 1;
     bool stop = false;
     for (int count; (count = next_table()) > 0;) {
@@ -237,38 +236,35 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         for (int b = b0; b < b1 && !(stop = wait.stop()); b += per_tile) {
           if (b - b0 && ((b - b0) & 31) == 0) have = next, next = cell_of(b + 32 + lane);
           const int n = min(per_tile, b1 - b), first = (b - b0) & 31;
+          const int slot = 2 * stage + (values ? 1 : 0);
           wait(freed + slot, ph);
-          if (issuer) mbar_expect_tx(full + slot, n * box * 128);
+          if (issuer) mbar_expect_tx(full + stage, n * box * 128);
           __syncwarp();
           for (int i = 0; i < n; ++i) {
             const int cell = __shfl_sync(0xffffffffu, have, first + i);
-            if (issuer) tma_load_2d(ring + slot * kSlotBytes + i * box * 128, map, 0, cell, full + slot);
+            if (issuer) tma_load_2d(ring + slot * kSlotBytes + i * box * 128, map, 0, cell, full + stage);
           }
-          slot += 2;
-          if (slot >= kSlots) slot -= kSlots, ph ^= 1;
+          if (++stage == kStages) stage = 0, ph ^= 1;
         }
       }
     }
-    if (wait.stop())   // the loads in flight: a slot's last one filled it in this round of the ring or in the one before
-      for (int s = values ? 1 : 0; s < kSlots; s += 2) wait.drain(full + s, s < slot ? ph ^ 1 : ph);
+    if (wait.stop())   // the loads in flight: a stage's last ones filled it in this round of the ring or in the one before
+      for (int s = 0; s < kStages; ++s) wait.drain(full + s, s < stage ? ph ^ 1 : ph);
   } else if (warp == 1) {
     // ===== MMA: the scores of tile n + 1, of the next item if need be, then tile n's second product =====
     const uint32_t one = elect_one() ? 1u : 0u, tm = __shfl_sync(0xffffffffu, tmem, 0);
     const uint64_t desc_ring = make_desc(smem_u32(ring), 16, 1024), desc_q = make_desc(smem_u32(qs), 16, 1024), desc_w = make_desc(smem_u32(ws), 16, 1024);
     constexpr uint32_t id_s = idesc_e4m3(2 * NP, 0), id_o = idesc_e4m3(2 * NP, 1);
-    int slot = 0, n = 0, item = 0;   // slot: of the next tile's keys
+    int stage = 0, prev = 0, n = 0, item = 0;   // stages of the next tile and of the one before
     uint32_t ph = 0;
-    int prev_v = 0;                  // slot and phase of tile n's values
-    uint32_t prev_ph = 0;
     bool pending = false;
     auto product = [&](int m) {      // tile m's weights and values
-      wait(full + prev_v, prev_ph);
       wait(w_ready + (m & 1), (m >> 1) & 1);
       fence_after();
-      const uint64_t dv = desc_ring + (uint64_t)((prev_v * kSlotBytes) >> 4), dw = desc_w + (uint64_t)(((m & 1) * C::kOperand) >> 4);
+      const uint64_t dv = desc_ring + (uint64_t)(((2 * prev + 1) * kSlotBytes) >> 4), dw = desc_w + (uint64_t)(((m & 1) * C::kOperand) >> 4);
 #pragma unroll
       for (int j = 0; j < 4; ++j) mma_f8_ss(one, tm + 4 * NP + (m & 1) * 2 * NP, dv + (j * 4096) / 16, dw + (j * 32) / 16, id_o, j ? 1u : 0u);
-      commit(one, freed + prev_v);
+      commit(one, freed + 2 * prev + 1);
       commit(one, o_full + (m & 1));
     };
     for (int count; (count = __shfl_sync(0xffffffffu, next_table(), 0)) > 0;) {
@@ -279,20 +275,19 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         wait(q_ready + (item & 1), (item >> 1) & 1);
         const uint64_t dq = desc_q + (uint64_t)(((item & 1) * C::kOperand) >> 4);
         for (int i = 0; i < nt; ++i, ++n) {
-          if (pending && !mbar_test(full + slot, ph)) product(n - 1), pending = false;
-          wait(full + slot, ph);
+          if (pending && !mbar_test(full + stage, ph)) product(n - 1), pending = false;
+          wait(full + stage, ph);
           fence_after();
-          const uint64_t dk = desc_ring + (uint64_t)((slot * kSlotBytes) >> 4);
+          const uint64_t dk = desc_ring + (uint64_t)((2 * stage * kSlotBytes) >> 4);
 #pragma unroll
           for (int j = 0; j < 4; ++j) mma_f8_ss(one, tm + (n & 1) * 2 * NP, dk + (j * 32) / 16, dq + (j * 32) / 16, id_s, j ? 1u : 0u);
-          commit(one, freed + slot);
+          commit(one, freed + 2 * stage);
           commit(one, s_full + (n & 1));
           commit(i + 1 == nt ? one : 0u, q_free + (item & 1));
-          if (++slot == kSlots) slot = 0, ph ^= 1;
           if (pending) product(n - 1);
           pending = true;
-          prev_v = slot, prev_ph = ph;
-          if (++slot == kSlots) slot = 0, ph ^= 1;
+          prev = stage;
+          if (++stage == kStages) stage = 0, ph ^= 1;
         }
       }
       if (pending) product(n - 1);   // (the softmax warps finish a table's last item before they come to the next table)
@@ -347,75 +342,65 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
       }
     }
   } else if (warp == C::kSpare) {
-    // ===== factors: a token's 2^key exponent, and 256 * 2^(value exponent - the tile's largest) (in units of kE4m3Unit); four tokens a lane.  The exponents are fetched four
-    // tiles ahead, their places in the cache eight (bulk copies of 128 bytes took the issuing warp 400 cycles each) =====
-    constexpr int D = 4;
-    const int stride = p.hkv * p.block_size;
+    // ===== factors: a token's 2^key exponent, and 256 * 2^(value exponent - the tile's largest); four tokens a lane.  The exponents come by asynchronous copies kAhead tiles
+    // ahead, each lane's own (as loads into registers they are waited for together with those of the tiles behind: 1100 cycles a tile; as bulk copies of 128 bytes
+    // they took the issuing warp 400 each) =====
+    const int box = min(p.block_size, kKv8Tile), per_tile = kKv8Tile / box, my_box = 4 * lane / box, my_cell = 4 * lane % box;
     int n = 0;
     for (int count; (count = next_table()) > 0;) {
-      // the tiles in order: the block of this lane's tokens, asked for, and their cells in it (-1: behind the context, or the table)
-      int it_c = -1, i_c = 0, end_c = 0, ctx_c = 0, kvh_c = 0, blk_c = 0, off_c = 0;
+      // the tiles in order: the first cells of 32 boxes (-1: behind the context, or outside the cache), and of the 32 behind them
+      int it_c = -1, i_c = 0, first_c = 0, end_c = 0, ctx_c = 0, kvh_c = 0, have = 0, next = 0;
       const int32_t* bt_c = p.block_table;
-      auto place = [&](int& blk, int& cell) {
-        if (i_c == end_c && it_c < count) {
-          if (++it_c < count) {
-            const Kv8Item w = table[it_c];
-            const int tok = w.tile0 * kKv8Tile + 4 * lane;
-            i_c = w.tile0, end_c = w.tile1, ctx_c = w.ctx, kvh_c = w.kvh;
-            bt_c = p.block_table + (int64_t)w.seq * p.bt_stride;
-            blk_c = tok / p.block_size, off_c = tok - blk_c * p.block_size;
-          } else {
-            ctx_c = 0;
-          }
+      auto cell_of = [&](int b) {
+        const int tok = b * box;
+        if (tok >= ctx_c) return -1;
+        const int blk = __ldg(bt_c + tok / p.block_size);
+        return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + kvh_c) * p.block_size + tok % p.block_size : -1;
+      };
+      auto ask = [&](int m) {   // tile m's
+        if (i_c == end_c && it_c < count && ++it_c < count) {
+          const Kv8Item w = table[it_c];
+          i_c = w.tile0, end_c = w.tile1, ctx_c = min(w.ctx, w.tile1 * kKv8Tile), kvh_c = w.kvh, first_c = i_c * per_tile;
+          bt_c = p.block_table + (int64_t)w.seq * p.bt_stride;
+          have = cell_of(first_c + lane), next = cell_of(first_c + 32 + lane);
         }
-        const bool in = i_c * kKv8Tile + 4 * lane < ctx_c;
-        blk = __ldg(in ? bt_c + blk_c : p.block_table);
-        cell = in ? kvh_c * p.block_size + off_c : -1;
-        ++i_c;
-        off_c += kKv8Tile;
-        while (off_c >= p.block_size) off_c -= p.block_size, ++blk_c;
+        if (it_c < count) {
+          const int b = i_c * per_tile - first_c;
+          if (b && (b & 31) == 0) have = next, next = cell_of(first_c + b + 32 + lane);
+          const int cell = __shfl_sync(0xffffffffu, have, (b & 31) + my_box);
+          uint32_t* const at = exps + ((m & (kAhead - 1)) * 32 + lane) * 2;
+          if (cell >= 0 && i_c * kKv8Tile + 4 * lane < ctx_c) f2::cp4(at, p.ke + cell + my_cell), f2::cp4(at + 1, p.ve + cell + my_cell);
+          else at[0] = at[1] = 0u;
+          ++i_c;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
       };
-      auto fetch = [&](int blk, int cell, uint32_t& k4, uint32_t& v4) {
-        const bool in = cell >= 0 && blk >= 0 && blk < p.n_blocks;   // (outside the cache: zeros)
-        const int c = in ? blk * stride + cell : 0;
-        k4 = v4 = 0u;
-        if (in) k4 = __ldg(reinterpret_cast<const uint32_t*>(p.ke + c)), v4 = __ldg(reinterpret_cast<const uint32_t*>(p.ve + c));
-      };
-      int blk[D], cell[D];
-      uint32_t k4[D], v4[D];
-#pragma unroll
-      for (int d = 0; d < D; ++d) place(blk[d], cell[d]);
-#pragma unroll
-      for (int d = 0; d < D; ++d) fetch(blk[d], cell[d], k4[d], v4[d]);
-#pragma unroll
-      for (int d = 0; d < D; ++d) place(blk[d], cell[d]);
-      int it = 0, i = table[0].tile0;
-      while (it < count) {
-#pragma unroll
-        for (int d = 0; d < D; ++d) {
-          if (it >= count) break;
-          const int left = table[it].ctx - i * kKv8Tile - 4 * lane;   // tokens of this lane's four
+      for (int d = 0; d < kAhead; ++d) ask(n + d);
+      for (int it = 0; it < count; ++it) {
+        const int tile1 = table[it].tile1, ctx = table[it].ctx;
+        for (int i = table[it].tile0; i < tile1; ++i, ++n) {
+          const int left = ctx - i * kKv8Tile - 4 * lane;   // tokens of this lane's four
+          asm volatile("cp.async.wait_group %0;" ::"n"(kAhead - 1) : "memory");
+          const uint2 kv4 = *reinterpret_cast<const uint2*>(exps + ((n & (kAhead - 1)) * 32 + lane) * 2);
           // a value row that is not a number: the columns that see it are none either (its key's factor), the others must not meet it
           uint32_t ve[4], m = 1u;
           bool none = false;
           float kf[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            ve[j] = (v4[d] >> (8 * j)) & 255u;
-            kf[j] = __uint_as_float(j < left && ve[j] == 255u ? 0x7fffffffu : ((k4[d] >> (8 * j)) & 255u) << 23);   // (2^-127 counts as nothing)
+            ve[j] = (kv4.y >> (8 * j)) & 255u;
+            kf[j] = __uint_as_float(j < left && ve[j] == 255u ? 0x7fffffffu : ((kv4.x >> (8 * j)) & 255u) << 23);   // (2^-127 counts as nothing)
             if (j >= left) ve[j] = 255u;
             if (ve[j] == 255u) none = true;
             else m = max(m, ve[j]);
           }
-          fetch(blk[d], cell[d], k4[d], v4[d]);
-          place(blk[d], cell[d]);
+          ask(n + kAhead);
           m = __reduce_max_sync(0xffffffffu, m);
           none = __any_sync(0xffffffffu, none);
           float vf[4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) vf[j] = ve[j] == 255u ? -0.f : __uint_as_float((uint32_t)max((int)(ve[j] - m) + 15, 0) << 23);
-          // the slot is tile n - 2's until that one's weights are ready
-          if (n >= kFacs) wait(w_ready + (n & 1), ((n - 2) >> 1) & 1);
+          for (int j = 0; j < 4; ++j) vf[j] = ve[j] == 255u ? -0.f : __uint_as_float((uint32_t)max((int)(ve[j] - m) + 135, 0) << 23);
+          if (n >= kFacs) wait(f_free + (n & (kFacs - 1)), (n / kFacs - 1) & 1);   // (that tile's scores have been waited for, too: s_full is in tile n's phase)
           float* f = reinterpret_cast<float*>(facs + (n & (kFacs - 1)) * kFacBytes);
           reinterpret_cast<float4*>(f)[2 * lane] = make_float4(kf[0], vf[0], kf[1], vf[1]);
           reinterpret_cast<float4*>(f)[2 * lane + 1] = make_float4(kf[2], vf[2], kf[3], vf[3]);
@@ -424,9 +409,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
             reinterpret_cast<int*>(f)[2 * kKv8Tile + 1] = none;
           }
           __syncwarp();
-          if (lane == 0) mbar_arrive(f_full + (n & (kFacs - 1)));
-          ++n;
-          if (++i == table[it].tile1 && ++it < count) i = table[it].tile0;
+          if (lane == 0) mbar_arrive(s_full + (n & 1));
         }
       }
     }
@@ -436,20 +419,19 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + c0;
     float* xm = x_max + grp * 2 * NCG * 4;
     float* xs = x_sum + grp * 2 * NCG * 4;
-    int n = 0, item = 0, v_slot = 1;
+    int n = 0, item = 0, stage = 0;
     uint32_t ph = 0;
-    float mu[NCG], l[NCG], acc[NCG], keep[NCG], take[NCG];   // keep, take: what becomes of the sums, and of the previous tile's product
-    auto fold = [&](int m) {                                   // tile m's product
-      wait(o_full + (m & 1), (m >> 1) & 1);
-      fence_after();
-      uint32_t hi[NCG], lo[NCG];
-      ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP, hi);
-      ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP + NP, lo);
-      ld_wait<NCG>(hi);
+    float mu[NCG], l[NCG], acc[NCG], keep[NCG], take[NCG], keep0[NCG], take0[NCG];   // keep, take: what becomes of the sums, and of the previous tile's product; of that before it
+    uint32_t oh[NCG], ol[NCG];                                 // a product on its way from tensor memory
+    auto ask = [&](int m) {                                    // tile m's
+      ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP, oh);
+      ld_cols<NCG>(base + 4 * NP + (m & 1) * 2 * NP + NP, ol);
+    };
+    auto fold = [&](const float (&k)[NCG], const float (&t)[NCG]) {   // (it is there: ld_wait)
 #pragma unroll
       for (int j = 0; j < NCG; ++j) {
-        asm volatile("" : "+r"(lo[j]));
-        acc[j] = acc[j] * keep[j] + fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])) * take[j];
+        asm volatile("" : "+r"(oh[j]), "+r"(ol[j]));
+        acc[j] = acc[j] * k[j] + fmaf(__uint_as_float(ol[j]), 0.0625f, __uint_as_float(oh[j])) * t[j];
       }
     };
     // an item's results: its last product, then the denominators (every token's share)
@@ -460,7 +442,11 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         const float v = warp_sum(l0[j]);
         if (lane == 0) xt[j * 4 + quad] = v;
       }
-      fold(last_tile);
+      wait(o_full + (last_tile & 1), (last_tile >> 1) & 1);
+      fence_after();
+      ask(last_tile);
+      ld_wait<NCG>(oh);
+      fold(keep, take);
       asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
       const int ncol = w.nrows * G;
 #pragma unroll
@@ -483,6 +469,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
 #pragma unroll
     for (int j = 0; j < NCG; ++j) acc[j] = 0.f;
     for (int count; (count = next_table()) > 0;) {
+      bool two = false;   // the last two products are to be added, both of one item
       for (int it = 0; it < count; ++it, ++item) {
         const Kv8Item w = table[it];
         const int ncol = w.nrows * G;
@@ -500,16 +487,17 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         }
         for (int i = w.tile0; i < w.tile1; ++i, ++n) {
           const int tok = i * kKv8Tile + tau;
-          wait(f_full + (n & (kFacs - 1)), (n / kFacs) & 1);
-          const float* f = reinterpret_cast<const float*>(facs + (n & (kFacs - 1)) * kFacBytes);
-          const float2 kv = reinterpret_cast<const float2*>(f)[tau], vr = reinterpret_cast<const float2*>(f)[kKv8Tile];
           float* xt = xm + (n & 1) * NCG * 4;
           wait(s_full + (n & 1), (n >> 1) & 1);
           fence_after();
+          if (two) ask(n - 2);   // (scores of tile n are complete behind the product of tile n - 2)
           uint32_t hi[NCG], lo[NCG];
           ld_cols<NCG>(base + (n & 1) * 2 * NP, hi);
           ld_cols<NCG>(base + (n & 1) * 2 * NP + NP, lo);
+          const float* f = reinterpret_cast<const float*>(facs + (n & (kFacs - 1)) * kFacBytes);
+          const float2 kv = reinterpret_cast<const float2*>(f)[tau], vr = reinterpret_cast<const float2*>(f)[kKv8Tile];
           ld_wait<NCG>(hi);
+          if (two) fold(keep0, take0);
           float s[NCG];
 #pragma unroll
           for (int j = 0; j < NCG; ++j) {
@@ -519,6 +507,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
             if (lane == 0) xt[j * 4 + quad] = m;
           }
           asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory");
+          if (tau == 0) mbar_arrive(f_free + (n & (kFacs - 1)));
           float wt[NCG], keep1[NCG], take1[NCG];
 #pragma unroll
           for (int j = 0; j < NCG; ++j) {
@@ -534,16 +523,23 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           }
           unsigned char* wb = ws + (n & 1) * C::kOperand;
 #pragma unroll
-          for (int j = 0; j < NCG; ++j) {   // (a weight that is not a number leaves its denominator so, whatever its codes)
-            const uint32_t two = e4m3_two<16>(wt[j]);
-            wb[operand_off(c0 + j, tau)] = (unsigned char)two;
-            wb[operand_off(NP + c0 + j, tau)] = (unsigned char)(two >> 8);
+          for (int j = 0; j < NCG; j += 2) {   // (a weight that is not a number leaves its denominator so, whatever its codes)
+            const float2 x = make_float2(wt[j], NCG > 1 ? wt[j + (NCG > 1)] : 0.f);
+            const __nv_fp8x2_storage_t c = __nv_cvt_float2_to_fp8x2(x, __NV_SATFINITE, __NV_E4M3);
+            const float2 back = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3)));
+            const __nv_fp8x2_storage_t d = __nv_cvt_float2_to_fp8x2(make_float2((x.x - back.x) * 16.f, (x.y - back.y) * 16.f), __NV_SATFINITE, __NV_E4M3);
+            wb[operand_off(c0 + j, tau)] = (unsigned char)c;
+            wb[operand_off(NP + c0 + j, tau)] = (unsigned char)d;
+            if (NCG > 1) {
+              wb[operand_off(c0 + j + 1, tau)] = (unsigned char)(c >> 8);
+              wb[operand_off(NP + c0 + j + 1, tau)] = (unsigned char)(d >> 8);
+            }
           }
           if (grp == 0 && __float_as_int(vr.y) != 0) {
             // value rows behind the context may hold anything, and 0 * NaN = NaN: zero them under their zero weights
-            wait(full + v_slot, ph);
+            wait(full + stage, ph);
             if (__float_as_uint(kv.y) == 0x80000000u) {
-              unsigned char* vb = ring + v_slot * kSlotBytes + tau * 128;
+              unsigned char* vb = ring + (2 * stage + 1) * kSlotBytes + tau * 128;
 #pragma unroll
               for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(vb + c * 16) = make_uint4(0u, 0u, 0u, 0u);
             }
@@ -552,13 +548,19 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(w_ready + (n & 1));
-          if (i > w.tile0) fold(n - 1);
-          else if (it > 0) finish(table[it - 1], mu_before, l_before, n - 1);   // the item before, while this one's first product runs
+          if (i == w.tile0 && it > 0) finish(table[it - 1], mu_before, l_before, n - 1);   // the item before, while this one's first product runs
+          two = i > w.tile0;
 #pragma unroll
-          for (int j = 0; j < NCG; ++j) keep[j] = keep1[j], take[j] = take1[j];
-          v_slot += 2;
-          if (v_slot >= kSlots) v_slot -= kSlots, ph ^= 1;
+          for (int j = 0; j < NCG; ++j) keep0[j] = keep[j], take0[j] = take[j], keep[j] = keep1[j], take[j] = take1[j];
+          if (++stage == kStages) stage = 0, ph ^= 1;
         }
+      }
+      if (two) {
+        wait(o_full + (n & 1), ((n - 2) >> 1) & 1);
+        fence_after();
+        ask(n - 2);
+        ld_wait<NCG>(oh);
+        fold(keep0, take0);
       }
       finish(table[count - 1], mu, l, n - 1);
     }
@@ -586,8 +588,7 @@ int kv8_cols_launch(const Kv8Maps& m, const Kv8Params& p, int cols, int grid, cu
   if (cols <= 2) return launch_cols<2>(m, p, grid, s);
   if (cols <= 4) return launch_cols<4>(m, p, grid, s);
   if (cols <= 8) return launch_cols<8>(m, p, grid, s);
-  if (cols <= 16) return launch_cols<16>(m, p, grid, s);
-  return launch_cols<32>(m, p, grid, s);
+  return launch_cols<16>(m, p, grid, s);
 }
 
 }  // namespace b200
