@@ -28,6 +28,7 @@ constexpr int kTable = 96;                   // items of a CTA that are describe
 constexpr int kFacs = 2;                     // tiles whose factors are kept
 constexpr int kFacBytes = kKv8Tile * 8 + 16; // a token's (key factor, value factor); the tile's factor, whether a token is dead
 constexpr int kAhead = 8;                    // tiles ahead that the exponents are asked for (a power of two)
+constexpr float kLowest = -3.402823466e38f;
 constexpr int kStageWarps = 4;               // keys, MMA, queries, values
 
 struct Kv8Item {
@@ -482,7 +483,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           ctx[j] = !live ? 0 : w.nrows == 1 ? w.ctx : kv8_ctx(p, w.row0 + (c0 + j) / G);
           qf[j] = live ? q_scale[(item & 3) * 32 + c0 + j] : 0.f;
           mu_before[j] = mu[j], l_before[j] = l[j];
-          mu[j] = -INFINITY;
+          mu[j] = kLowest;
           l[j] = 0.f;
         }
         for (int i = w.tile0; i < w.tile1; ++i, ++n) {
@@ -512,10 +513,10 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
 #pragma unroll
           for (int j = 0; j < NCG; ++j) {
             const float4 x = reinterpret_cast<const float4*>(xt)[j];
-            const float mt = fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w));
-            const bool none = mt == -INFINITY;   // a column whose row does not see this tile
-            const float mn = fmaxf(mu[j], mt), e = none ? 0.f : exp2_fast(s[j] - mt), b = none ? 0.f : exp2_fast(mt - mn);
-            keep1[j] = mn == -INFINITY ? 1.f : exp2_fast(mu[j] - mn);
+            // (a column whose row does not see this tile: the lowest finite number stands for its maximum, and its scores are -inf)
+            const float mt = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), kLowest), mn = fmaxf(mu[j], mt);
+            const float e = exp2_fast(s[j] - mt), b = exp2_fast(mt - mn);
+            keep1[j] = exp2_fast(mu[j] - mn);
             take1[j] = b * vr.x;
             l[j] = l[j] * keep1[j] + e * b;
             mu[j] = mn;
