@@ -256,6 +256,7 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
   Kv8Maps maps;
   if (const int rc = kv8_maps(a, std::min(a.block_size, kKv8Tile), &maps)) return rc;
   const int G = a.hq / a.hkv;
+  const int64_t pairs = (int64_t)most * G;   // of a run of rows, where that is known
   char* const w = static_cast<char*>(ws);
   Kv8Params p = {};
   p.q = a.q;
@@ -278,7 +279,7 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
   p.hkv = a.hkv;
   p.block_size = a.block_size;
   p.scale2 = a.scale * 1.4426950408889634f;
-  if (most == 1 || (most > 0 && most * G <= kShortPairs)) {   // few pairs in every run: found by the kernel itself
+  if (most == 1 || (most > 0 && pairs <= kShortPairs)) {   // few pairs in every run: found by the kernel itself
     p.group_rows = most;
     if (const int rc = kv8_cols_launch(maps, p, most * G, kNumSMs, s)) return rc;
     const PdlScope join;
@@ -291,12 +292,12 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
   Kv8Head* const head = reinterpret_cast<Kv8Head*>(at + 2 * kCutBytes);
   Kv8Group *const groups = reinterpret_cast<Kv8Group*>(head + 1), *const rows = groups + a.T;
   p.items = reinterpret_cast<Kv8Rows*>(rows + a.T);
-  const bool drafts = most > 0 && most * G <= 128;   // runs of a tile of pairs at most: all of them to the rows kernel
+  const bool drafts = most > 0 && pairs <= 128;   // runs of a tile of pairs at most: all of them to the rows kernel
   const int short_rows = drafts ? 0 : std::max(1, kShortPairs / G);
   uint8_t* const q_hi = reinterpret_cast<uint8_t*>(w + kCutBytes + kPartBytes + kPartRowsBytes + plan_bytes(a.T, a.hkv));
   uint8_t* const q_lo = q_hi + query_bytes(a.T, a.hq);
   float* const q_scale = reinterpret_cast<float*>(q_lo + query_bytes(a.T, a.hq));
-  const bool few = most > 0 && most * G <= 32;
+  const bool few = most > 0 && pairs <= 32;
   const int tile_rows = (few ? 32 : 128) / G;
   Kv8QueryMaps qm;
   if (const int rc = kv8_query_map(q_hi, a.T, a.hq, G, tile_rows, &qm.hi)) return rc;

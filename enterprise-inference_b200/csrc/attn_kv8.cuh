@@ -7,7 +7,7 @@
 namespace b200 {
 
 constexpr int kKv8Tile = 128;          // tokens of a tile
-constexpr int kKv8Cols = 32;           // (row, head) pairs of a group at most
+constexpr int kKv8Cols = 16;           // (row, head) pairs of a group at most
 constexpr int kKv8PartFloats = 132;    // of a pair in a part: 128 sums, their maximum (log2 domain), the denominator
 
 // rows [row0, row0 + nrows) of one sequence that share its keys and values; nrows 0: none
@@ -84,12 +84,6 @@ __device__ __forceinline__ uint32_t e4m3_two(float scaled) {
   const float rest = (scaled - __uint_as_float(h)) * (float)LO;
   const uint32_t l = (__float_as_uint(rest) & 0x7fffffffu) + 0x80000u;   // (sign apart)
   return h >> 20 | (l >> 12 & 0x7f00u) | (__float_as_uint(rest) >> 16 & 0x8000u);
-}
-// four codes -> f16 pairs of their values times 2^-8
-__device__ __forceinline__ void e4m3_wide(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  const uint32_t h = ((w >> 1) & 0x3f3f3f3fu) | (w & 0x80808080u), l = (w << 7) & 0x80808080u;
-  lo = __byte_perm(l, h, 0x5140);
-  hi = __byte_perm(l, h, 0x7362);
 }
 
 // A query scaled by a power of two to [128, 256), as e4m3 and LO times what that rounding left.  With LO = 16 both terms are exact down to 2^-14 of the largest

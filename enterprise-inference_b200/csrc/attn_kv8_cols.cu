@@ -47,7 +47,7 @@ struct Cols {
   static constexpr int kBars = (3 * kStages + 15 + kFacs + 1) & ~1;
   static constexpr uint32_t kTmem = 8 * NP;                // S, S, O, O
   static constexpr int kSmem = 1024 + 2 * kStages * kSlotBytes + 4 * kOperand + kFacs * kFacBytes + kTable * (int)sizeof(Kv8Item) +
-                               kBars * 8 + (4 * 32 + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + kAhead * 256 + 64;
+                               kBars * 8 + (4 * kKv8Cols + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + kAhead * 256 + 64;
   static_assert(kSmem + 8 * (kThreads + kThreads / 32) <= 232448, "shared memory");
 };
 
@@ -88,8 +88,8 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   uint64_t* q_info = q_free + 2;                           // [4]: an item's scales, for the softmax warps (who may be three items behind)
   uint64_t* f_free = q_info + 4;                           // [kFacs]
   uint64_t* last = f_free + kFacs;
-  float* q_scale = reinterpret_cast<float*>(full + C::kBars);   // [4 items][32]; from here on in whole 16 bytes
-  float* x_sum = q_scale + 4 * 32;                         // [CG][2][NCG][4 warps]
+  float* q_scale = reinterpret_cast<float*>(full + C::kBars);   // [4 items][pairs]; from here on in whole 16 bytes
+  float* x_sum = q_scale + 4 * kKv8Cols;                         // [CG][2][NCG][4 warps]
   float* x_max = x_sum + CG * 2 * NCG * 4;                 // [CG][2][NCG][4 warps]
   uint32_t* exps = reinterpret_cast<uint32_t*>(x_max + CG * 2 * NCG * 4);   // [kAhead][32 lanes][keys, values]
   int* shared_int = reinterpret_cast<int*>(exps + kAhead * 64);            // 0: tensor memory, 1: a wait ran out, 2, 3: the share's first and last item
@@ -333,7 +333,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
             if (c < ncol) {
               *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = hi;
               *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = lo;
-              if ((lane & 15) == 0) q_scale[(item & 3) * 32 + c] = query_back(e) * p.scale2;
+              if ((lane & 15) == 0) q_scale[(item & 3) * kKv8Cols + c] = query_back(e) * p.scale2;
             }
           }
         }
@@ -481,7 +481,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         for (int j = 0; j < NCG; ++j) {
           const bool live = c0 + j < ncol;
           ctx[j] = !live ? 0 : w.nrows == 1 ? w.ctx : kv8_ctx(p, w.row0 + (c0 + j) / G);
-          qf[j] = live ? q_scale[(item & 3) * 32 + c0 + j] : 0.f;
+          qf[j] = live ? q_scale[(item & 3) * kKv8Cols + c0 + j] : 0.f;
           mu_before[j] = mu[j], l_before[j] = l[j];
           mu[j] = kLowest;
           l[j] = 0.f;

@@ -24,10 +24,6 @@ __device__ __forceinline__ uint32_t kv8_exp_byte(uint32_t amax_bits) {
   const int e = (int)(amax_bits >> 23) - 127 - 8 + ((amax_bits & 0x7fffffu) > 0x600000u ? 1 : 0);
   return (uint32_t)(max(e, kKv8MinExp) + 127);
 }
-// 2^(byte - 127); 255: NaN
-__device__ __forceinline__ float kv8_scale(uint32_t byte) {
-  return __uint_as_float(byte == 255u ? 0x7fffffffu : byte == 0u ? 0x00400000u : byte << 23);
-}
 // two codes, the first in the low byte; magnitudes above 448 do not occur (kv8_exp_byte)
 __device__ __forceinline__ uint32_t e4m3x2(float lo, float hi) {
   return (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);

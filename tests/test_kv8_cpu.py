@@ -112,3 +112,21 @@ def test_plain_check_keeps_what_the_drafter_had_right():
 def test_abi_integers_are_wide_enough():
     sig = pkg("_abi").SIGNATURES
     assert sig["b200_paged_attn_fp8_workspace_bytes"][0] is C.c_int64 and sig["b200_verify_drafts_workspace_bytes"][0] is C.c_int64
+
+
+def test_attention_counts_its_tiles_in_32_bits():
+    """Rows times kv heads times tiles of the block table stay below 2^31."""
+    assert _attend(True, T=70000, stride=1 << 20, hkv=32) == -3 and b"70000 rows" in _lib().b200_last_error()
+    assert _attend(False, T=1, stride=2 ** 31 - 1, block=1024, n_blocks=5) == -3
+    assert _attend(True, most=2 ** 31 - 1, ws=None) == -1   # (a bound above the rows is none)
+
+
+def test_plain_check_of_equal_probabilities():
+    """The plain form's leftovers where target and drafter agree but for a few entries."""
+    V, g = 400, torch.Generator().manual_seed(6)
+    target = torch.randn(2, V, generator=g).to(torch.bfloat16)
+    draft = target.clone()
+    draft[0, 7], draft[0, 9] = target[0, 9], target[0, 7]   # two entries trade places: all others are equally probable
+    lower, higher = (7, 9) if target[0, 7] < target[0, 9] else (9, 7)
+    out, kept, _ = K.verify(target, draft, torch.tensor([lower, 0]), [0, 2], torch.ones(1), torch.tensor([[0.999, 0.5], [0.5, 0.5]]))
+    assert int(kept[0]) == 0 and int(out[0]) == higher

@@ -552,3 +552,176 @@ def test_a_drafted_step():
         for s in range(S):
             history[s] = cache.rows[s]
         lens = lens + took + 1                   # refused rows are overwritten by the next step
+
+
+# ---- where the kernels' walks end ------------------------------------------------------------------------------------------
+
+def test_runs_of_two_tiles_of_pairs():
+    """Items of two tiles of pairs: runs that end inside the first and the second one, rows that see nothing, a context of its own for every row."""
+    hq, hkv = 64, 16
+    parts, before = [300, 333, 70, 64, 1], [0, 450, 129, 7, 60]
+    seq, ctx = _step(parts, before)
+    for t in (5, 64, 65, 299, 301):
+        ctx[t] = 0
+    for t in range(640, 690):
+        ctx[t] = 0 if t % 3 else 17
+    g = torch.Generator().manual_seed(77)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 32, g)
+    T = len(seq)
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, 333)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hq, 128), q, cache, seq, ctx)
+
+
+def test_more_items_than_a_cta_describes_at_a_time():
+    """2000 rows of their own contexts over 8 kv heads: over a hundred items a CTA, most of one tile."""
+    hkv, T = 8, 2000
+    g = torch.Generator().manual_seed(41)
+    ctxs = [int(x) for x in torch.randint(1, 40, (T,), generator=g)]
+    ctxs[3], ctxs[700], ctxs[1500] = 0, 300, 129
+    cache = K.Cache(ctxs, hkv, 16, g)
+    q = _rows(T, hkv, g)
+    qd, out = _on_device(q), torch.full((T, hkv * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, None, torch.tensor(ctxs, dtype=I32, device=DEV), out, hkv)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hkv, 128), q, cache, list(range(T)), ctxs)
+
+
+@pytest.mark.parametrize("hq,hkv", [(8, 4), (32, 8), (64, 4)])
+@pytest.mark.parametrize("most", [1, 2, 3, 7, 2 ** 31 - 1])
+def test_a_bound_on_runs_only_chooses_the_kernels(most, hq, hkv):
+    """Runs that are longer than the caller said, and a bound above all rows."""
+    parts, before = [6, 1, 19, 2, 40], [100, 0, 250, 127, 300]
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(hq)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 64, g)
+    T = len(seq)
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("most", [None, 40])
+def test_one_sequence_comes_up_again(most):
+    """Rows of a sequence that do not follow one another, rows in falling order, the same row twice."""
+    hq, hkv = 16, 2
+    g = torch.Generator().manual_seed(8)
+    cache = K.Cache([400, 200], hkv, 128, g)
+    seq = [0, 1, 0, 0, 1, 1, 0] * 5
+    ctx = [400, 200, 399, 399, 1, 200, 5] * 5
+    q = _rows(len(seq), hq, g)
+    q[7:14] = q[:7]
+    qd, out = _on_device(q), torch.full((len(seq), hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(len(seq), hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("V", [152064, 393216])
+def test_drafts_over_long_vocabularies(V):
+    g = torch.Generator().manual_seed(V)
+    parts = [3, 1, 2]
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    temperature, uniforms = torch.tensor([1.0, 0.6, 1.3]), torch.rand(6, 2, generator=g)
+    uniforms[0, 0] = 0.97   # (a refusal is likely: the leftovers of a whole row)
+    for d in (draft, None):
+        want, kept, margins = K.verify(target, d, tokens, starts, temperature, uniforms)
+        assert all(m > 1e-5 for m in margins)
+        got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
+        assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("temp", [1.0, 0.01, 40.0])
+def test_leftovers_of_nearly_equal_probabilities(temp):
+    """Drafters that agree with the target but for some entries: traded places (all others exactly as probable), one raised, one masked."""
+    V, g = 5000, torch.Generator().manual_seed(12)
+    parts = [2] * 6
+    target, _, tokens, starts = _drafts(parts, V, g)
+    draft = target.clone()
+    uniforms = torch.rand(12, 2, generator=g)
+    order = target.double().sort(1).indices
+    for s in range(6):
+        r, top, low = 2 * s, int(order[2 * s, -1]), int(order[2 * s, -2 - 300 * s])
+        draft[r, top], draft[r, low] = target[r, low], target[r, top]
+        if s % 3 == 1:
+            draft[r, int(order[r, -5])] = float("-inf")
+        if s % 3 == 2:
+            draft[r, int(order[r, -9])] = 6.5
+        tokens[r], uniforms[r, 0] = low, 0.999
+    temperature = torch.full((6,), temp)
+    want, kept, margins = K.verify(target, draft, tokens, starts, temperature, uniforms)
+    assert all(m > 1e-5 for m in margins)
+    assert int(kept.sum()) < 6
+    got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts, temperature, uniforms)
+    assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+def test_logits_that_are_not_numbers_still_yield_a_token():
+    V, g = 3000, torch.Generator().manual_seed(2)
+    parts = [3] * 6
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    target[0:3, 40:60] = float("nan")
+    draft[3:5, 100] = float("nan")
+    target[6:9] = float("nan")
+    target[9:12, 5] = float("inf")
+    draft[12:14, 7] = float("inf")
+    uniforms = torch.rand(18, 2, generator=g)
+    for temps in (torch.full((6,), 0.9), torch.zeros(6)):
+        got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts, temps, uniforms)
+        for s in range(6):
+            k = int(got[1][s])
+            assert 0 <= k <= 2 and 0 <= int(got[0][3 * s + k]) < V and bool((got[0][3 * s + k + 1:3 * s + 3] == -1).all())
+    want, kept, _ = K.verify(target[15:], draft[15:], tokens[15:], [0, 3], torch.zeros(1), uniforms[15:])
+    assert torch.equal(got[0][15:], want)   # (a sequence without any)
+
+
+def test_checks_of_drafts_in_graphs_and_on_other_streams():
+    """Captured once, replayed over new logits and draws; two streams at a time with a workspace each."""
+    V, g = 9001, torch.Generator().manual_seed(4)
+    parts = [5, 2, 4, 1]
+    lib, check = _lib()
+    sets = []
+    for _ in range(2):
+        target, draft, tokens, starts = _drafts(parts, V, g)
+        uniforms = torch.rand(len(tokens), 2, generator=g)
+        temperature = torch.tensor([1.0, 0.0, 0.6, 1.4])
+        want, kept, margins = K.verify(target, draft, tokens, starts, temperature, uniforms)
+        assert all(m > 1e-5 for m in margins)
+        sets.append(([t.to(DEV) for t in (target, draft, tokens.to(I32), uniforms)], want, kept))
+    fixed = [torch.tensor(starts, dtype=I32, device=DEV), temperature.to(DEV)]
+    n, size = len(tokens), int(lib.b200_verify_drafts_workspace_bytes(len(tokens), V))
+
+    def call(x, out, kept, ws, stream):
+        check(lib.b200_verify_drafts(x[0].data_ptr(), V, x[1].data_ptr(), V, x[2].data_ptr(), fixed[0].data_ptr(), fixed[1].data_ptr(), x[3].data_ptr(), len(parts), n, V,
+                                     out.data_ptr(), kept.data_ptr(), ws.data_ptr(), size, stream))
+
+    def results():
+        return torch.zeros(n, dtype=I32, device=DEV), torch.zeros(len(parts), dtype=I32, device=DEV), torch.zeros(size, dtype=torch.uint8, device=DEV)
+
+    static, (out, kept, ws) = [t.clone() for t in sets[0][0]], results()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        call(static, out, kept, ws, torch.cuda.current_stream().cuda_stream)
+    for x, w, k in sets + sets[:1]:
+        for a, b in zip(static, x):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out.long().cpu(), w) and torch.equal(kept.long().cpu(), k)
+    streams, both = [torch.cuda.Stream() for _ in range(2)], [results() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            call(sets[i][0], *both[i], st.cuda_stream)
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert torch.equal(both[i][0].long().cpu(), sets[i][1]) and torch.equal(both[i][1].long().cpu(), sets[i][2])
