@@ -7,36 +7,43 @@ namespace b200 {
 namespace {
 
 // sums `a`, their maximum (log2 domain) and denominator of `parts` parts, one after another `step` floats apart -> out = sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m),
-// by a warp, four entries a lane
+// by eight lanes, 16 entries each (a warp a pair, four entries a lane, waits four times for its parts where an item has 128 pairs: 2.5 us more behind 300 rows)
 __device__ __forceinline__ void join_parts(const float* first, const float* rest, int64_t step, int parts, __nv_bfloat16* out) {
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 7;
   auto part = [&](int i) { return i ? rest + (i - 1) * step : first; };
   float m = -INFINITY, l = 0.f;
-  for (int i = lane; i < parts; i += 32) m = fmaxf(m, part(i)[128]);
-  m = warp_max(m);
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
+  for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[128]);
+  float4 a[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
   for (int i = 0; i < parts; ++i) {
     const float* x = part(i);
     const float f = m == -INFINITY ? 1.f : tc::exp2_fast(x[128] - m);
-    const float4 v = reinterpret_cast<const float4*>(x)[lane];
     l += x[129] * f;
-    a.x += v.x * f, a.y += v.y * f, a.z += v.z * f, a.w += v.w * f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float4 v = reinterpret_cast<const float4*>(x)[lane + 8 * k];
+      a[k].x += v.x * f, a[k].y += v.y * f, a[k].z += v.z * f, a[k].w += v.w * f;
+    }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
-  *reinterpret_cast<uint2*>(out + 4 * lane) = make_uint2(pack_bf16(a.x * inv, a.y * inv), pack_bf16(a.z * inv, a.w * inv));
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint2*>(out + 4 * (lane + 8 * k)) = make_uint2(pack_bf16(a[k].x * inv, a[k].y * inv), pack_bf16(a[k].z * inv, a[k].w * inv));
 }
 
 // blocks [0, kNumSMs): items of the columns kernel that several CTAs share; [kNumSMs, 2 kNumSMs): items of the rows kernel in parts
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Params p, int base) {
   pdl_wait();
   pdl_launch_dependents();
-  const int G = p.hq / p.hkv, warp = threadIdx.x >> 5, block = blockIdx.x + base;
+  const int G = p.hq / p.hkv, pair = blockIdx.y * 32 + (threadIdx.x >> 3), step_pairs = 32 * gridDim.y, block = blockIdx.x + base;
   if (block < kNumSMs) {
     const Kv8Cut cut = p.cuts[block];
     if (cut.parts < 2) return;
     const int64_t step = 2ll * kKv8Cols * kKv8PartFloats;
-    for (int c = blockIdx.y * 8 + warp; c < cut.nrows * G; c += 8 * gridDim.y) {
+    for (int c = pair; c < cut.nrows * G; c += step_pairs) {
       const float* x = p.part + (2 * (int64_t)block * kKv8Cols + c) * kKv8PartFloats;
       join_parts(x + kKv8Cols * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
     }
@@ -45,14 +52,14 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Params p, int ba
   const Kv8Cut cut = p.cuts_rows[block - kNumSMs];
   if (cut.parts < 2) return;
   const int64_t step = 2ll * 128 * kKv8PartFloats;
-  for (int c = blockIdx.y * 8 + warp; c < cut.nrows * G; c += 8 * gridDim.y) {
+  for (int c = pair; c < cut.nrows * G; c += step_pairs) {
     const float* x = p.part_rows + (2 * (int64_t)(block - kNumSMs) * 128 + c) * kKv8PartFloats;
     join_parts(x + 128 * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
   }
 }
 
 // ---- plan: rows -> runs of one sequence -> groups of few pairs (columns kernel) and items of a tile of pairs or two (rows kernel).  One CTA. ----
-constexpr int kPlanThreads = 1024;
+constexpr int kPlanThreads = 1024, kPlanNear = 2048;   // (steps of at most so many rows: the lists in shared memory, 1 us of 300 rows' 69)
 
 // exclusive scan over the CTA of two counts; returns the totals
 __device__ __forceinline__ int2 plan_scan(int& a, int& b, int2* sh) {
@@ -81,9 +88,12 @@ __device__ __forceinline__ int2 plan_scan(int& a, int& b, int2* sh) {
 __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params p, int short_rows, int R, Kv8Head* head, Kv8Group* groups, Kv8Group* rows, int* runs,
                                                                 uint8_t* q_hi, uint8_t* q_lo, float* q_scale) {
   __shared__ int2 sh[32];
+  __shared__ int near_runs[kPlanNear];
+  __shared__ Kv8Group near_rows[kPlanNear];
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (p.T <= kPlanNear) runs = near_runs, rows = near_rows;   // every pass over the lists waits for the one before
   if (blockIdx.x > 0) {
     const int64_t pairs = (int64_t)p.T * p.hq, step = (int64_t)(gridDim.x - 1) * (kPlanThreads / 16);
     for (int64_t i0 = (int64_t)(blockIdx.x - 1) * (kPlanThreads / 16); i0 < pairs; i0 += step) {
@@ -195,6 +205,9 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
   if (tid == 0) *head = {n_groups, two, {0, 0}};
 }
 
+// rows beside the longest run, times the tokens that a block table has room for: up to here their groups are not worth the columns kernel's launch (64 rows of a chunk and 16
+// others over 500 or 2000 tokens: 34 and 53 us without it, 45 and 60 with; over 8000 140 and 99)
+constexpr int64_t kFewTokens = 32768;
 constexpr int kShortPairs = 8;    // (row, head) pairs of a group of the columns kernel in steps of longer runs
 constexpr int64_t kCutBytes = (kNumSMs * sizeof(Kv8Cut) + 255) / 256 * 256;
 constexpr int64_t kPartBytes = (int64_t)kNumSMs * 2 * kKv8Cols * kKv8PartFloats * 4, kPartRowsBytes = (int64_t)kNumSMs * 2 * 128 * kKv8PartFloats * 4;
@@ -283,7 +296,7 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
     p.group_rows = most;
     if (const int rc = kv8_cols_launch(maps, p, most * G, kNumSMs, s)) return rc;
     const PdlScope join;
-    B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs, (most * G + 7) / 8), dim3(256), 0, s, p, 0));
+    B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs), dim3(256), 0, s, p, 0));
     return B200_OK;
   }
   char* at = w + kCutBytes + kPartBytes + kPartRowsBytes;
@@ -292,7 +305,8 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
   Kv8Head* const head = reinterpret_cast<Kv8Head*>(at + 2 * kCutBytes);
   Kv8Group *const groups = reinterpret_cast<Kv8Group*>(head + 1), *const rows = groups + a.T;
   p.items = reinterpret_cast<Kv8Rows*>(rows + a.T);
-  const bool drafts = most > 0 && pairs <= 128;   // runs of a tile of pairs at most: all of them to the rows kernel
+  // runs of a tile of pairs at most, or little beside the longest run: all of them to the rows kernel
+  const bool drafts = most > 0 && (pairs <= 128 || std::max<int64_t>(a.T - most, 0) * a.bt_stride * a.block_size <= kFewTokens);
   const int short_rows = drafts ? 0 : std::max(1, kShortPairs / G);
   uint8_t* const q_hi = reinterpret_cast<uint8_t*>(w + kCutBytes + kPartBytes + kPartRowsBytes + plan_bytes(a.T, a.hkv));
   uint8_t* const q_lo = q_hi + query_bytes(a.T, a.hq);
