@@ -1,5 +1,6 @@
 // Host side of the attention over the 8-bit cache: maps, workspace, routes, and the joining of parts.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_kv8.cuh"
 
@@ -7,55 +8,66 @@ namespace b200 {
 namespace {
 
 // sums `a`, their maximum (log2 domain) and denominator of `parts` parts, one after another `step` floats apart -> out = sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m),
-// by eight lanes, 16 entries each (a warp a pair, four entries a lane, waits four times for its parts where an item has 128 pairs: 2.5 us more behind 300 rows)
+// by LANES neighbouring lanes.  Eight where an item of 128 pairs has few parts (a warp would wait for its parts four times: 2.5 us more behind 300 rows), a warp where
+// it has many (eight lanes: 1 row over 8000 tokens 21 us instead of 17, 5 rows over 3000 28 instead of 24)
+constexpr int kManyParts = 4;
+template <int LANES>
 __device__ __forceinline__ void join_parts(const float* first, const float* rest, int64_t step, int parts, __nv_bfloat16* out) {
-  const int lane = threadIdx.x & 7;
+  constexpr int K = 32 / LANES;   // four entries at a time
+  const int lane = threadIdx.x & (LANES - 1);
+  const unsigned group = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
   auto part = [&](int i) { return i ? rest + (i - 1) * step : first; };
   float m = -INFINITY, l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, part(i)[128]);
-  float4 a[4];
+  for (int i = lane; i < parts; i += LANES) m = fmaxf(m, part(i)[128]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
+  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
+  float4 a[K];
+#pragma unroll
+  for (int k = 0; k < K; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
   for (int i = 0; i < parts; ++i) {
     const float* x = part(i);
     const float f = m == -INFINITY ? 1.f : tc::exp2_fast(x[128] - m);
     l += x[129] * f;
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float4 v = reinterpret_cast<const float4*>(x)[lane + 8 * k];
+    for (int k = 0; k < K; ++k) {
+      const float4 v = reinterpret_cast<const float4*>(x)[lane + LANES * k];
       a[k].x += v.x * f, a[k].y += v.y * f, a[k].z += v.z * f, a[k].w += v.w * f;
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint2*>(out + 4 * (lane + 8 * k)) = make_uint2(pack_bf16(a[k].x * inv, a[k].y * inv), pack_bf16(a[k].z * inv, a[k].w * inv));
+  for (int k = 0; k < K; ++k)
+    *reinterpret_cast<uint2*>(out + 4 * (lane + LANES * k)) = make_uint2(pack_bf16(a[k].x * inv, a[k].y * inv), pack_bf16(a[k].z * inv, a[k].w * inv));
 }
 
 // blocks [0, kNumSMs): items of the columns kernel that several CTAs share; [kNumSMs, 2 kNumSMs): items of the rows kernel in parts
 __global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Params p, int base) {
   pdl_wait();
   pdl_launch_dependents();
-  const int G = p.hq / p.hkv, pair = blockIdx.y * 32 + (threadIdx.x >> 3), step_pairs = 32 * gridDim.y, block = blockIdx.x + base;
+  const int G = p.hq / p.hkv, block = blockIdx.x + base;
   if (block < kNumSMs) {
     const Kv8Cut cut = p.cuts[block];
     if (cut.parts < 2) return;
     const int64_t step = 2ll * kKv8Cols * kKv8PartFloats;
-    for (int c = pair; c < cut.nrows * G; c += step_pairs) {
+    for (int c = blockIdx.y * 8 + (threadIdx.x >> 5); c < cut.nrows * G; c += 8 * gridDim.y) {
       const float* x = p.part + (2 * (int64_t)block * kKv8Cols + c) * kKv8PartFloats;
-      join_parts(x + kKv8Cols * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
+      join_parts<32>(x + kKv8Cols * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
     }
     return;
   }
   const Kv8Cut cut = p.cuts_rows[block - kNumSMs];
   if (cut.parts < 2) return;
   const int64_t step = 2ll * 128 * kKv8PartFloats;
-  for (int c = pair; c < cut.nrows * G; c += step_pairs) {
-    const float* x = p.part_rows + (2 * (int64_t)(block - kNumSMs) * 128 + c) * kKv8PartFloats;
-    join_parts(x + 128 * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
-  }
+  auto join = [&](auto lanes_c) {
+    constexpr int LANES = decltype(lanes_c)::value, EACH = 256 / LANES;
+    for (int c = blockIdx.y * EACH + threadIdx.x / LANES; c < cut.nrows * G; c += EACH * gridDim.y) {
+      const float* x = p.part_rows + (2 * (int64_t)(block - kNumSMs) * 128 + c) * kKv8PartFloats;
+      join_parts<LANES>(x + 128 * kKv8PartFloats, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim);
+    }
+  };
+  if (cut.parts > kManyParts) join(std::integral_constant<int, 32>());
+  else join(std::integral_constant<int, 8>());
 }
 
 // ---- plan: rows -> runs of one sequence -> groups of few pairs (columns kernel) and items of a tile of pairs or two (rows kernel).  One CTA. ----
@@ -296,7 +308,7 @@ int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaS
     p.group_rows = most;
     if (const int rc = kv8_cols_launch(maps, p, most * G, kNumSMs, s)) return rc;
     const PdlScope join;
-    B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs), dim3(256), 0, s, p, 0));
+    B200_CUDA(launch(kv8_join_kernel, dim3(kNumSMs, (most * G + 7) / 8), dim3(256), 0, s, p, 0));
     return B200_OK;
   }
   char* at = w + kCutBytes + kPartBytes + kPartRowsBytes;

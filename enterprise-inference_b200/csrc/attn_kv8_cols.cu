@@ -29,7 +29,7 @@ constexpr int kFacs = 2;                     // tiles whose factors are kept
 constexpr int kFacBytes = kKv8Tile * 8 + 16; // a token's (key factor, value factor); the tile's factor, whether a token is dead
 constexpr int kAhead = 8;                    // tiles ahead that the exponents are asked for (a power of two)
 constexpr float kLowest = -3.402823466e38f;
-constexpr int kStageWarps = 4;               // keys, MMA, queries, values
+constexpr int kStageWarps = 4;               // keys and values, MMA, queries, factors
 
 struct Kv8Item {
   int row0, nrows, seq, kvh, tile0, tile1, ctx, ends;   // ends: 1 begins in an earlier CTA, 2 goes on in the next
@@ -40,14 +40,13 @@ struct Cols {
   static constexpr int NP = NC < 8 ? 8 : NC;               // columns of either term: N = 2 NP is a multiple of 16
   static constexpr int CG = NC < 4 ? NC : 4;               // groups of four softmax warps that share the columns
   static constexpr int NCG = NC / CG;
-  static constexpr int kSpare = kStageWarps + 4 * CG;      // the warp behind them makes the tokens' factors
-  static constexpr int kThreads = (kSpare + 1) * 32;
+  static constexpr int kThreads = (kStageWarps + 4 * CG) * 32;   // 640 at most: 96 registers a thread (a warp more would leave 80)
   static constexpr int kOperand = 2 * NP * 128;            // queries, or weights, of an item or tile
   static constexpr int kStages = 6;                        // tiles in flight, keys and values each
   static constexpr int kBars = (3 * kStages + 15 + kFacs + 1) & ~1;
   static constexpr uint32_t kTmem = 8 * NP;                // S, S, O, O
   static constexpr int kSmem = 1024 + 2 * kStages * kSlotBytes + 4 * kOperand + kFacs * kFacBytes + kTable * (int)sizeof(Kv8Item) +
-                               kBars * 8 + (4 * kKv8Cols + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + kAhead * 256 + 64;
+                               kBars * 8 + (8 * kKv8Cols + CG * 2 * 4 * NCG + CG * 2 * 4 * NCG) * 4 + kAhead * 256 + 64;
   static_assert(kSmem + 8 * (kThreads + kThreads / 32) <= 232448, "shared memory");
 };
 
@@ -88,8 +87,8 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   uint64_t* q_info = q_free + 2;                           // [4]: an item's scales, for the softmax warps (who may be three items behind)
   uint64_t* f_free = q_info + 4;                           // [kFacs]
   uint64_t* last = f_free + kFacs;
-  float* q_scale = reinterpret_cast<float*>(full + C::kBars);   // [4 items][pairs]; from here on in whole 16 bytes
-  float* x_sum = q_scale + 4 * kKv8Cols;                         // [CG][2][NCG][4 warps]
+  float2* info = reinterpret_cast<float2*>(full + C::kBars);   // [4 items][pairs]: what undoes a query's scaling, the tokens that its row sees; from here on in whole 16 bytes
+  float* x_sum = reinterpret_cast<float*>(info + 4 * kKv8Cols);                       // [CG][2][NCG][4 warps]
   float* x_max = x_sum + CG * 2 * NCG * 4;                 // [CG][2][NCG][4 warps]
   uint32_t* exps = reinterpret_cast<uint32_t*>(x_max + CG * 2 * NCG * 4);   // [kAhead][32 lanes][keys, values]
   int* shared_int = reinterpret_cast<int*>(exps + kAhead * 64);            // 0: tensor memory, 1: a wait ran out, 2, 3: the share's first and last item
@@ -106,7 +105,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   __shared__ uint64_t scan_warp[kThreads / 32], scan_thread[kThreads];
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kStages; ++s) mbar_init(full + s, 2), mbar_init(freed + 2 * s, 1), mbar_init(freed + 2 * s + 1, 1);
+    for (int s = 0; s < kStages; ++s) mbar_init(full + s, 1), mbar_init(freed + 2 * s, 1), mbar_init(freed + 2 * s + 1, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(s_full + s, 2);
       mbar_init(w_ready + s, 4 * CG);
@@ -212,39 +211,51 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
     return min(max(n_items - from, 0), kTable);
   };
 
-  if (warp == 0 || warp == 3) {
-    // ===== TMA: warp 0 keys, warp 3 values =====
-    const bool issuer = elect_one(), values = warp == 3;
-    const CUtensorMap* map = values ? &maps.v : &maps.k;
-    if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(map) : "memory");
+  if (warp == 0) {
+    // ===== TMA: keys and values =====
+    const bool issuer = elect_one();
+    if (issuer) {
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.k) : "memory");
+      asm volatile("prefetch.tensormap [%0];" ::"l"(&maps.v) : "memory");
+    }
     const int box = min(p.block_size, kKv8Tile), per_tile = kKv8Tile / box;   // boxes of a tile
     const int cells = (int)(p.n_blocks * p.hkv * p.block_size);
     int stage = 0;
     uint32_t ph = 1;
     bool stop = false;
+    // the first cell of an item's box number `at` (of those that hold something), a box to a lane
+    auto cell_of = [&](const Kv8Item& w, int at) {
+      const int tok = w.tile0 * kKv8Tile + at * box;
+      if (tok >= min(w.ctx, w.tile1 * kKv8Tile)) return 0;
+      const int blk = __ldg(p.block_table + (int64_t)w.seq * p.bt_stride + tok / p.block_size);
+      return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
+    };
     for (int count; (count = next_table()) > 0;) {
+      int lead = cell_of(table[0], lane);   // the next item's first 32 boxes (asked for when its turn comes, they take 1000 cycles and more)
       for (int it = 0; it < count && !stop; ++it) {
         const Kv8Item w = table[it];
-        const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
-        const int b0 = w.tile0 * per_tile, b1 = (min(w.ctx, w.tile1 * kKv8Tile) + box - 1) / box;   // boxes that hold something
-        // the first cells of the boxes, a box to a lane
-        auto cell_of = [&](int b) {
-          if (b >= b1) return 0;
-          const int tok = b * box, blk = __ldg(bt + tok / p.block_size);
-          return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
-        };
-        int have = cell_of(b0 + lane), next = b0 + 32 < b1 ? cell_of(b0 + 32 + lane) : 0;
-        for (int b = b0; b < b1 && !(stop = wait.stop()); b += per_tile) {
-          if (b - b0 && ((b - b0) & 31) == 0) have = next, next = cell_of(b + 32 + lane);
-          const int n = min(per_tile, b1 - b), first = (b - b0) & 31;
-          const int slot = 2 * stage + (values ? 1 : 0);
-          wait(freed + slot, ph);
-          if (issuer) mbar_expect_tx(full + stage, n * box * 128);
-          __syncwarp();
-          for (int i = 0; i < n; ++i) {
-            const int cell = __shfl_sync(0xffffffffu, have, first + i);
-            if (issuer) tma_load_2d(ring + slot * kSlotBytes + i * box * 128, map, 0, cell, full + stage);
+        const int boxes = (min(w.ctx, w.tile1 * kKv8Tile) - w.tile0 * kKv8Tile + box - 1) / box;
+        int have = lead, next = 32 < boxes ? cell_of(w, 32 + lane) : 0;
+        if (it + 1 < count) lead = cell_of(table[it + 1], lane);
+        for (int b = 0; b < boxes && !(stop = wait.stop()); b += per_tile) {
+          if (b && (b & 31) == 0) have = next, next = cell_of(w, b + 32 + lane);
+          const int n = min(per_tile, boxes - b);
+          unsigned char* const keys = ring + 2 * stage * kSlotBytes;
+          int cell[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) cell[i] = __shfl_sync(0xffffffffu, have, (b + i) & 31);
+          wait(freed + 2 * stage, ph);
+          wait(freed + 2 * stage + 1, ph);
+          if (issuer) {
+            mbar_expect_tx(full + stage, 2 * n * box * 128);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (i < n) {
+                tma_load_2d(keys + i * box * 128, &maps.k, 0, cell[i], full + stage);
+                tma_load_2d(keys + kSlotBytes + i * box * 128, &maps.v, 0, cell[i], full + stage);
+              }
           }
+          __syncwarp();
           if (++stage == kStages) stage = 0, ph ^= 1;
         }
       }
@@ -315,10 +326,12 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         constexpr int U = NC < 8 ? (NC + 1) / 2 : 4;   // pairs of columns that are asked for at a time
         for (int c1 = 0; c1 < ncol; c1 += 2 * U) {
           uint4 v[U];
+          int ctx[U];
 #pragma unroll
           for (int u = 0; u < U; ++u) {
             const int c = c1 + 2 * u + (lane >> 4);
             v[u] = make_uint4(0u, 0u, 0u, 0u);
+            ctx[u] = c < ncol && w.nrows > 1 ? kv8_ctx(p, w.row0 + c / G) : w.ctx;
             if (c < ncol) v[u] = __ldg(reinterpret_cast<const uint4*>(p.q + (int64_t)(w.row0 + c / G) * p.ldq + (w.kvh * G + c % G) * kHeadDim + d));
           }
 #pragma unroll
@@ -333,7 +346,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
             if (c < ncol) {
               *reinterpret_cast<uint2*>(qb + operand_off(c, d)) = hi;
               *reinterpret_cast<uint2*>(qb + operand_off(NP + c, d)) = lo;
-              if ((lane & 15) == 0) q_scale[(item & 3) * kKv8Cols + c] = query_back(e) * p.scale2;
+              if ((lane & 15) == 0) info[(item & 3) * kKv8Cols + c] = make_float2(query_back(e) * p.scale2, __int_as_float(ctx[u]));
             }
           }
         }
@@ -342,32 +355,32 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         if (lane == 0) mbar_arrive(q_ready + (item & 1)), mbar_arrive(q_info + (item & 3));
       }
     }
-  } else if (warp == C::kSpare) {
+  } else if (warp == 3) {
     // ===== factors: a token's 2^key exponent, and 256 * 2^(value exponent - the tile's largest); four tokens a lane.  The exponents come by asynchronous copies kAhead tiles
     // ahead, each lane's own (as loads into registers they are waited for together with those of the tiles behind: 1100 cycles a tile; as bulk copies of 128 bytes
     // they took the issuing warp 400 each) =====
     const int box = min(p.block_size, kKv8Tile), per_tile = kKv8Tile / box, my_box = 4 * lane / box, my_cell = 4 * lane % box;
     int n = 0;
     for (int count; (count = next_table()) > 0;) {
-      // the tiles in order: the first cells of 32 boxes (-1: behind the context, or outside the cache), and of the 32 behind them
-      int it_c = -1, i_c = 0, first_c = 0, end_c = 0, ctx_c = 0, kvh_c = 0, have = 0, next = 0;
-      const int32_t* bt_c = p.block_table;
-      auto cell_of = [&](int b) {
-        const int tok = b * box;
-        if (tok >= ctx_c) return -1;
-        const int blk = __ldg(bt_c + tok / p.block_size);
-        return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + kvh_c) * p.block_size + tok % p.block_size : -1;
+      // the tiles in order: the first cells of 32 boxes (-1: behind the context, or outside the cache), of the 32 behind them, of the next item's first 32
+      int it_c = -1, i_c = 0, first_c = 0, end_c = 0, ctx_c = 0, have = 0, next = 0;
+      auto cell_of = [&](const Kv8Item& w, int at) {
+        const int tok = w.tile0 * kKv8Tile + at * box;
+        if (tok >= min(w.ctx, w.tile1 * kKv8Tile)) return -1;
+        const int blk = __ldg(p.block_table + (int64_t)w.seq * p.bt_stride + tok / p.block_size);
+        return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : -1;
       };
+      int lead = cell_of(table[0], lane);
       auto ask = [&](int m) {   // tile m's
         if (i_c == end_c && it_c < count && ++it_c < count) {
           const Kv8Item w = table[it_c];
-          i_c = w.tile0, end_c = w.tile1, ctx_c = min(w.ctx, w.tile1 * kKv8Tile), kvh_c = w.kvh, first_c = i_c * per_tile;
-          bt_c = p.block_table + (int64_t)w.seq * p.bt_stride;
-          have = cell_of(first_c + lane), next = cell_of(first_c + 32 + lane);
+          i_c = w.tile0, end_c = w.tile1, ctx_c = min(w.ctx, w.tile1 * kKv8Tile), first_c = i_c * per_tile;
+          have = lead, next = (w.tile1 - w.tile0) * per_tile > 32 ? cell_of(w, 32 + lane) : -1;
+          if (it_c + 1 < count) lead = cell_of(table[it_c + 1], lane);
         }
         if (it_c < count) {
           const int b = i_c * per_tile - first_c;
-          if (b && (b & 31) == 0) have = next, next = cell_of(first_c + b + 32 + lane);
+          if (b && (b & 31) == 0) have = next, next = cell_of(table[it_c], b + 32 + lane);
           const int cell = __shfl_sync(0xffffffffu, have, (b & 31) + my_box);
           uint32_t* const at = exps + ((m & (kAhead - 1)) * 32 + lane) * 2;
           if (cell >= 0 && i_c * kKv8Tile + 4 * lane < ctx_c) f2::cp4(at, p.ke + cell + my_cell), f2::cp4(at + 1, p.ve + cell + my_cell);
@@ -479,9 +492,8 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
         wait(q_info + (item & 3), (item >> 2) & 1);
 #pragma unroll
         for (int j = 0; j < NCG; ++j) {
-          const bool live = c0 + j < ncol;
-          ctx[j] = !live ? 0 : w.nrows == 1 ? w.ctx : kv8_ctx(p, w.row0 + (c0 + j) / G);
-          qf[j] = live ? q_scale[(item & 3) * kKv8Cols + c0 + j] : 0.f;
+          const float2 x = c0 + j < ncol ? info[(item & 3) * kKv8Cols + c0 + j] : make_float2(0.f, 0.f);
+          qf[j] = x.x, ctx[j] = __float_as_int(x.y);
           mu_before[j] = mu[j], l_before[j] = l[j];
           mu[j] = kLowest;
           l[j] = 0.f;
