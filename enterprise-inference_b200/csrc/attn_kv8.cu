@@ -140,14 +140,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
   }
   __syncthreads();
   auto run_rows = [&](int i) { return i < n_runs ? (i + 1 < n_runs ? runs[i + 1] : p.T) - runs[i] : 0; };
-  // items of two tiles of pairs where that leaves every SM one, and most of them are full
+  // Items of two tiles of pairs, which share what is widened (2048 rows over 1000 tokens: 103 us, of one tile 159), where most of them are full and whole items keep
+  // four of seven SMs busy in every round (of 8 kv heads, 1024 rows, 128 items: 55 and 72 us; 700 rows, 88: 50 and 54; of 16, 640 rows, 160: 182 and 163)
   int n1 = 0, n2 = 0;
   for (int i = tid; i < n_runs; i += kPlanThreads) {
     const int n = run_rows(i);
     if (n > short_rows) n1 += (n + R - 1) / R, n2 += (n + 2 * R - 1) / (2 * R);
   }
   const int2 both = plan_scan(n1, n2, sh);
-  const bool two = R * (p.hq / p.hkv) > 32 && both.y * p.hkv >= kNumSMs && 2 * both.x >= 3 * both.y;
+  const int pairs2 = both.y * p.hkv, rounds2 = (pairs2 + kNumSMs - 1) / kNumSMs;
+  const bool two = R * (p.hq / p.hkv) > 32 && 7 * (int64_t)pairs2 >= 4ll * kNumSMs * rounds2 && 2 * both.x >= 3 * both.y && both.y > 0;
   const int per = two ? 2 * R : R;
   int n_groups = 0, n_items = 0;
   for (int i0 = 0; i0 < n_runs; i0 += kPlanThreads) {
@@ -220,7 +222,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
 // rows beside the longest run, times the tokens that a block table has room for: up to here their groups are not worth the columns kernel's launch (64 rows of a chunk and 16
 // others over 500 or 2000 tokens: 34 and 53 us without it, 45 and 60 with; over 8000 140 and 99)
 constexpr int64_t kFewTokens = 32768;
-constexpr int kShortPairs = 8;    // (row, head) pairs of a group of the columns kernel in steps of longer runs
+// (row, head) pairs of a run, or group, for the columns kernel (48 runs of 8 pairs over 2000 tokens: 47 us, by the rows kernel 77; of 12: 83 and 77, of 16: 88 and 77)
+constexpr int kShortPairs = 8;
 constexpr int64_t kCutBytes = (kNumSMs * sizeof(Kv8Cut) + 255) / 256 * 256;
 constexpr int64_t kPartBytes = (int64_t)kNumSMs * 2 * kKv8Cols * kKv8PartFloats * 4, kPartRowsBytes = (int64_t)kNumSMs * 2 * 128 * kKv8PartFloats * 4;
 // places of the list of items: one for each and one for each CTA, or (whole items) a round's for every CTA and one behind them

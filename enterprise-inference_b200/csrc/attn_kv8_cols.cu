@@ -408,8 +408,8 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
             if (ve[j] == 255u) none = true;
             else m = max(m, ve[j]);
           }
-          ask(n + kAhead);
           m = __reduce_max_sync(0xffffffffu, m);
+          ask(n + kAhead);   // (its place has been read)
           none = __any_sync(0xffffffffu, none);
           float vf[4];
 #pragma unroll

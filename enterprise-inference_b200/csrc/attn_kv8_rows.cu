@@ -91,6 +91,8 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       if (u.tile1 > u.tile0) return true;   // (rows that see nothing: the plan wrote their zeros)
     }
   };
+  // does the item that was asked for come next? (its block numbers, contexts and factors may be asked for)
+  auto comes_next = [&]() { return ahead.cta == (int)blockIdx.x && ahead.tile1 > ahead.tile0; };
 
   // ===== values of a half -> f16, factors of its keys: every half (group -1), or one of each tile's =====
   auto widen = [&](int group) {
@@ -232,11 +234,23 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
           *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + row2) * p.ldo + (int64_t)(w.kvh * G + mm % G) * kHeadDim + col) = v;
       }
     };
+    // (few) what a lane's pair sees, and its scores' factor: the next item's are asked for before this one's results are written
+    int ctx_next = 0;
+    float qf_next = 1.f;
+    bool led = false;
+    auto ask = [&](const Kv8Rows& w) {
+      const int t = w.row0 + lane / G;
+      const bool alive = lane < w.nrows * G;
+      ctx_next = alive ? kv8_ctx(p, t) : 0;
+      qf_next = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + lane % G) : 1.f;
+    };
     // an item of at most 32 pairs: lane = pair, this warp's 16 keys of each half; the four quarters' sums are joined at the end
     auto few = [&](const Kv8Rows& w, int h0, int h1, int& n, int half) {
       const bool alive = lane < w.nrows * G;
-      const int fr = lane / G, t = w.row0 + fr, ctx = alive ? kv8_ctx(p, t) : 0;
-      const float qf = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + lane % G) : 1.f;
+      const int t = w.row0 + lane / G;
+      if (!led) ask(w);
+      const int ctx = ctx_next;
+      const float qf = qf_next;
       float mu = -INFINITY, l = 0.f;
       int ref = 0;
 #pragma unroll 1
@@ -293,6 +307,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         __syncwarp();
         if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
       }
+      if ((led = comes_next())) ask(ahead);
       wait(o_full + ((n - 1) & 1), ((n - 1) >> 1) & 1);
       fence_after();
       // the quarters' maxima and denominators, then their sums, 32 columns at a time
@@ -508,25 +523,29 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       int slot = 0;
       uint32_t ph = 1;
       bool stop = false;
+      // the first cell of an item's box number `at` (of those that hold something), a box to a lane
+      auto cell_of = [&](const Kv8Rows& w, int at) {
+        const int tok = w.tile0 * kKv8Tile + at * box;
+        if (tok >= min(w.ctx, w.tile1 * kKv8Tile)) return 0;
+        const int blk = __ldg(p.block_table + (int64_t)w.seq * p.bt_stride + tok / p.block_size);
+        return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
+      };
+      int lead = 0;   // (few) the next item's first 32 boxes, asked for behind this one's first tile (longer items gain nothing)
+      bool led = false;
       while (!stop && next_unit(w)) {
-        const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
-        const int b0 = w.tile0 * per_tile, b1 = (min(w.ctx, w.tile1 * kKv8Tile) + box - 1) / box;
-        auto cell_of = [&](int b) {
-          if (b >= b1) return 0;
-          const int tok = b * box, blk = __ldg(bt + tok / p.block_size);
-          return blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + tok % p.block_size : cells;   // behind the cache: zeros
-        };
-        int have = cell_of(b0 + lane), next = b0 + 32 < b1 ? cell_of(b0 + 32 + lane) : 0;
-        for (int b = b0; b < b1 && !(stop = wait.stop()); b += per_tile) {
-          if (b - b0 && ((b - b0) & 31) == 0) have = next, next = cell_of(b + 32 + lane);
-          const int k = min(per_tile, b1 - b);
+        const int boxes = (min(w.ctx, w.tile1 * kKv8Tile) - w.tile0 * kKv8Tile + box - 1) / box;
+        int have = led ? lead : cell_of(w, lane), next = 32 < boxes ? cell_of(w, 32 + lane) : 0;
+        for (int b = 0; b < boxes && !(stop = wait.stop()); b += per_tile) {
+          if (b && (b & 31) == 0) have = next, next = cell_of(w, b + 32 + lane);
+          const int k = min(per_tile, boxes - b);
           wait(freed + slot, ph);
           if (issuer) mbar_expect_tx(full + slot, k * box * 128);
           __syncwarp();
           for (int i = 0; i < k; ++i) {
-            const int cell = __shfl_sync(0xffffffffu, have, ((b - b0) & 31) + i);
+            const int cell = __shfl_sync(0xffffffffu, have, (b & 31) + i);
             if (issuer) tma_load_2d(ring + slot * kOperand + i * box * 128, map, 0, cell, full + slot);
           }
+          if (FEW && b == 0 && (led = comes_next())) lead = cell_of(ahead, lane);
           if (++slot == slots) slot = 0, ph ^= 1;
         }
       }
