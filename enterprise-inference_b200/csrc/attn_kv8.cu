@@ -24,7 +24,7 @@ __device__ __forceinline__ void join_parts(const float* first, const float* rest
   float4 a[K];
 #pragma unroll
   for (int k = 0; k < K; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
+#pragma unroll (LANES == 32 ? 4 : 2)
   for (int i = 0; i < parts; ++i) {
     const float* x = part(i);
     const float f = m == -INFINITY ? 1.f : tc::exp2_fast(x[128] - m);
@@ -42,7 +42,7 @@ __device__ __forceinline__ void join_parts(const float* first, const float* rest
 }
 
 // blocks [0, kNumSMs): items of the columns kernel that several CTAs share; [kNumSMs, 2 kNumSMs): items of the rows kernel in parts
-__global__ void __launch_bounds__(256) kv8_join_kernel(const Kv8Params p, int base) {
+__global__ void __launch_bounds__(256, 4) kv8_join_kernel(const Kv8Params p, int base) {
   pdl_wait();
   pdl_launch_dependents();
   const int G = p.hq / p.hkv, block = blockIdx.x + base;
