@@ -4,7 +4,8 @@
 // fp32 and once to what it is stored as (bf16 for q, e4m3 for k): closer to the formula than rope_kv_kernel's bf16 arithmetic, which follows the
 // reference's image.
 // Eight lanes take a head of a row: lane j the entries 8 j .. 8 j + 7 and their partners, 16 bytes each, so that the pairs are rotated and the head's largest
-// magnitude found (three shuffles) without shared memory.
+// magnitude found (three shuffles) without shared memory.  A group of lanes for every head: with two or four heads each the loads of a group overlap, but rows of few
+// heads take longer (1024 rows, 48 heads: 5.1, 6.0, 8.9 us; 2047 rows, 80 heads: 16.4, 16.8, 23.9).  Bound by the rows' bytes, 4.9 TB/s at 2047.
 #include "kv8.cuh"
 
 namespace b200 {
@@ -33,14 +34,21 @@ rope_kv_append_fp8_kernel(const __nv_bfloat16* qkv, int64_t ld, const int32_t* _
   const unsigned group = 0xffu << (threadIdx.x & 24);   // the head's lanes
   if (t >= T) return;
   const __nv_bfloat16* x = qkv + (int64_t)t * ld + head * kHeadDim + 8 * j;
-  float a[8], b[8];
-  unpack8(*reinterpret_cast<const uint4*>(x), a);
-  unpack8(*reinterpret_cast<const uint4*>(x + 64), b);
+  // all that is read, asked for at once
+  const uint4 x0 = *reinterpret_cast<const uint4*>(x), x1 = *reinterpret_cast<const uint4*>(x + 64);
+  const int slot = slots[t];
+  uint4 cs0 = {}, cs1 = {};
   if (head < hq + hkv) {
     const __nv_bfloat16* cs = cos_sin + (int64_t)positions[t] * kHeadDim + 8 * j;
+    cs0 = ld_ro(cs), cs1 = ld_ro(cs + 64);
+  }
+  float a[8], b[8];
+  unpack8(x0, a);
+  unpack8(x1, b);
+  if (head < hq + hkv) {
     float c[8], s[8];
-    unpack8(ld_ro(cs), c);
-    unpack8(ld_ro(cs + 64), s);
+    unpack8(cs0, c);
+    unpack8(cs1, s);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float u = a[i] * c[i] - b[i] * s[i], w = b[i] * c[i] + a[i] * s[i];
@@ -53,7 +61,6 @@ rope_kv_append_fp8_kernel(const __nv_bfloat16* qkv, int64_t ld, const int32_t* _
     *reinterpret_cast<uint4*>(y + 64) = pack8(b);
     return;
   }
-  const int slot = slots[t];
   if (slot < 0 || slot >= n_slots) return;
   // magnitudes as integers: inf and NaN are the largest
   uint32_t m = 0;
