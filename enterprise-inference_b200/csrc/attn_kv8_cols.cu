@@ -13,7 +13,10 @@
 // The flattened list of (group, kv head, tile) is cut into equal shares, one per SM: contexts may differ as they like.  An item that a cut goes through
 // leaves its sums as parts, joined by the next launch.
 //
-// Bound by the cache's bytes: 258 a token and kv head.
+// Bound by the cache's bytes, 258 a token and kv head, where contexts are long: 8 rows of 32 k tokens, 64 heads over 8, 76 us, 5.1 TB/s.  A tile takes 1050 to 1300
+// cycles there (the bytes alone 1020): the softmax warps' chain of scores, maximum, weights, and 950 for the warp that issues the MMAs.  In front of it 9000 cycles until the
+// first load is asked for (groups, shares, table; much of it instructions fetched for the first time), and 2000 for every item that ends: 64 rows of 500 to
+// 1000 tokens 32 us, 3.1 TB/s.
 #include <algorithm>
 
 #include "attn_kv8.cuh"
@@ -38,9 +41,11 @@ struct Kv8Item {
 template <int NC>
 struct Cols {
   static constexpr int NP = NC < 8 ? 8 : NC;               // columns of either term: N = 2 NP is a multiple of 16
-  static constexpr int CG = NC < 4 ? NC : 4;               // groups of four softmax warps that share the columns
+  // groups of four softmax warps that share the columns (two for eight columns: 8 rows of 32 k tokens 90 us instead of 81, 200 rows of 500 60 instead of 53; two sets
+  // of two that take the tiles in turn: 108)
+  static constexpr int CG = NC < 4 ? NC : 4;
   static constexpr int NCG = NC / CG;
-  static constexpr int kThreads = (kStageWarps + 4 * CG) * 32;   // 640 at most: 96 registers a thread (a warp more would leave 80)
+  static constexpr int kThreads = (kStageWarps + 4 * CG) * 32;   // 640 at most: 96 registers a thread (a warp more would leave 80: 79 us instead of 74 for 8 rows of 32 k)
   static constexpr int kOperand = 2 * NP * 128;            // queries, or weights, of an item or tile
   static constexpr int kStages = 6;                        // tiles in flight, keys and values each
   static constexpr int kBars = (3 * kStages + 15 + kFacs + 1) & ~1;

@@ -273,7 +273,8 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * The cache of a layer, caller-owned: k_codes, v_codes [n_blocks][n_kv_heads][block_size][128] e4m3, k_exps, v_exps
  * [n_blocks][n_kv_heads][block_size] uint8.  A value is code * 2^(byte - 127): one exponent per token and kv head, the
  * smallest e >= -100 with max |x| <= 448 * 2^e (every value is an exact bf16; relative error of a normal code at most
- * 2^-4).  Byte 255: the row held an inf or a NaN; its codes are NaN.  129 bytes a row where bf16 takes 256.
+ * 2^-4).  Byte 255: the row held an inf or a NaN; its codes are NaN, and of such rows alone.  Byte 0 stands for nothing (a
+ * caller that writes a cache of its own).  129 bytes a row where bf16 takes 256.
  * block_size is 16, 32, 64 or a multiple of 128; n_blocks * n_kv_heads * block_size < 2^31.  Codes are 16-byte aligned.
  *
  * (a4+a5) b200_rope_kv_append_fp8: NeoX RoPE of the q and k heads of qkv [T][ld] in fp32 with one rounding (where
@@ -287,7 +288,9 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * fp32, weights of at least eight significant bits, one rounding of the result.  A row sees ctx_lens[t] tokens of its
  * sequence (no more than bt_stride blocks of them): none gives zeros.  What lies behind them in a block is never looked at.  A block id outside
  * [0, n_blocks) stands for keys and values of zero.  max_rows: a HOST bound on the rows of one sequence that follow one
- * another in this step (0: not known): it only chooses the kernels.  The workspace has no state between calls.
+ * another in this step (0: not known): it only chooses the kernels (a longer run than it says is attended as well).  The
+ * workspace has no state between calls; calls that may run at the same time, two captured graphs among them, need one each.
+ * Rows times kv heads times 128-token tiles of the block table stay below 2^31 (B200_ERR_UNSUPPORTED).
  *
  * b200_verify_drafts: which drafted tokens the target keeps, and the token that follows them (speculative sampling: what comes
  * out is distributed as the target's own draws).  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1 of target_logits
@@ -301,8 +304,8 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * temperature[s] <= 0 (or temperature NULL, uniforms then unused): a draft is kept if it is the row's argmax (ties: the lowest
  * index), and the token is the argmax.  A draft outside [0, vocab) is refused; a row of nothing but -inf refuses and yields token 0.
  * uniforms [n_rows][2] in [0, 1).  out_tokens[n_rows]: per sequence the kept drafts, the drawn token, then -1; out_accepted[s]:
- * drafts kept.  A sequence without rows gets out_accepted 0; rows of no sequence stay as they are.  At most 65535 rows of
- * 393216 entries. */
+ * drafts kept.  A sequence without rows gets out_accepted 0; rows of no sequence stay as they are.  Temperatures below 1e-30
+ * count as that.  At most 65535 rows of 393216 entries (B200_ERR_UNSUPPORTED). */
 B200_API int b200_rope_kv_append_fp8(const void* qkv, int64_t ld, const int32_t* positions, const int32_t* slot_mapping,
                             const void* cos_sin, void* q_out, int64_t ldq, void* k_codes, void* v_codes, void* k_exps,
                             void* v_exps, int64_t n_blocks, int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,
