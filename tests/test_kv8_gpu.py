@@ -725,3 +725,55 @@ def test_checks_of_drafts_in_graphs_and_on_other_streams():
     torch.cuda.synchronize()
     for i in range(2):
         assert torch.equal(both[i][0].long().cpu(), sets[i][1]) and torch.equal(both[i][1].long().cpu(), sets[i][2])
+
+
+@pytest.mark.parametrize("most,hq,hkv", [(500, 2, 2), (0, 4, 1), (3, 4, 1), (3, 8, 2)])
+def test_steps_of_many_runs(most, hq, hkv):
+    """2600 rows: 700 runs of three and, but for the last two, one of 500."""
+    parts = [3] * 350 + ([500] if most != 3 else []) + [3] * 350
+    g = torch.Generator().manual_seed(hq + most)
+    before = [int(x) for x in torch.randint(0, 30, (len(parts),), generator=g)]
+    before[5], before[600], before[-1] = 400, 129, 127
+    seq, ctx = _step(parts, before)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 32, g)
+    T = len(seq)
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("most", [0, 1, 5, 64, 300])
+def test_rows_that_are_their_own_sequences_in_any_step(most):
+    """No row_to_seq: row t is sequence t, whatever the bound says."""
+    hq, hkv = 16, 2
+    g = torch.Generator().manual_seed(most)
+    ctxs = [7, 0, 200, 128, 1, 500, 33]
+    cache = K.Cache(ctxs, hkv, 1024, g)
+    q = _rows(len(ctxs), hq, g)
+    qd, out = _on_device(q), torch.full((len(ctxs), hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, None, torch.tensor(ctxs, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(len(ctxs), hq, 128), q, cache, list(range(len(ctxs))), ctxs)
+
+
+def test_checks_of_many_sequences():
+    """300 sequences, one of 90 rows (more than a CTA keeps the maxima of), some without any; rows in front of the first one."""
+    V, g = 700, torch.Generator().manual_seed(21)
+    parts = [int(x) for x in torch.randint(0, 5, (300,), generator=g)]
+    parts[17] = 90
+    target, draft, tokens, starts = _drafts(parts, V, g, noise=0.05)
+    temperature = torch.rand(300, generator=g) * 1.5 + 0.2
+    temperature[::7] = 0
+    uniforms = torch.rand(len(tokens), 2, generator=g)
+    r = starts[17]
+    uniforms[r:r + 80, 0] = 1e-4   # (most of the long one's drafts are kept: its draw comes from a row that is not among the first 64)
+    want, kept, margins = K.verify(target, draft, tokens, starts, temperature, uniforms)
+    assert all(m > 1e-5 for m in margins)
+    lead = 3
+    front = [torch.cat([x[:lead], x]) for x in (target, draft, tokens, uniforms)]
+    got = check_drafts(front[0].to(DEV), front[1].to(DEV), front[2], [s + lead for s in starts], temperature, front[3])
+    assert bool((got[0][:lead] == -9).all()) and torch.equal(got[1], kept) and torch.equal(got[0][lead:], want)
