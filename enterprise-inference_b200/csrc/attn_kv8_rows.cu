@@ -80,7 +80,8 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = *tmem_slot;   // per tile of pairs 256 columns: scores of even, odd halves, O
+  const uint32_t tmem = *tmem_slot;   // per tile of pairs 256 columns: scores of even, odd halves, O; few: scores of even, odd tiles, O
+  constexpr int kO = FEW ? 256 : 128;
   const int G = p.hq / p.hkv, R = (FEW ? 32 : 128) / G;
   // the CTA's items, in the plan's order; the one behind the next is asked for
   int at = p.starts[blockIdx.x];
@@ -212,18 +213,19 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16) + x * 256;
     const int r = m / G, row = (two ? x : 0) * R + r, step = two ? 1 : 2, first = two ? 0 : x;
     unsigned char* const exchange = qs + 2 * kOperand;   // (items of one tile: the second one's queries are not there)
-    int n = 0, half = 0;   // halves of this group of warps', of the CTA
+    int n = 0, half = 0, tiles = 0;   // halves of this group of warps', of the CTA; (few) tiles of the items before this one
     auto rescale = [&](int n, float fo) {   // O of the halves before n
-      wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
+      if (FEW) wait(o_full + ((n - 1) & 3), ((n - 1) >> 2) & 1);
+      else wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
       fence_after();
 #pragma unroll 1
       for (int c = 0; c < kHeadDim; c += 16) {
         uint32_t o[16];
-        ld16(base + 128 + c, o);
+        ld16(base + kO + c, o);
         ld_wait<16>(o);
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * fo);
-        st16(base + 128 + c, o);
+        st16(base + kO + c, o);
       }
     };
     // 32 columns of the warp's pairs from shared memory to their rows: a row's 64 bytes leave from four neighbouring lanes
@@ -259,10 +261,11 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       for (int h = h0; h < h1; ++h, ++n) {
         const int at = half + h - h0, b = at % kWide;
         const float* f = reinterpret_cast<const float*>(facs + b * kFacBytes);
-        wait(s_full + 2 * x + (n & 1), (n >> 1) & 1);
+        const int tile = tiles + (h >> 1) - w.tile0;
+        if ((h & 1) == 0) wait(s_full + (tile & 1), (tile >> 1) & 1);
         wait(w_full + b, (at / kWide) & 1);
         fence_after();
-        const uint32_t s_addr = base + (n & 1) * kHalf;
+        const uint32_t s_addr = base + (tile & 1) * 128 + (h & 1) * kHalf;
         uint32_t s[16];
         ld16(s_addr + 16 * quad, s);
         const int ref_new = reinterpret_cast<const int*>(f)[kHalf], live = ctx - h * kHalf - 16 * quad;
@@ -307,10 +310,10 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         st_wait();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
+        if (lane == 0) mbar_arrive(p_ready + (n & 3));
       }
       if ((led = comes_next())) ask(ahead);
-      wait(o_full + ((n - 1) & 1), ((n - 1) >> 1) & 1);
+      wait(o_full + ((n - 1) & 3), ((n - 1) >> 2) & 1);
       fence_after();
       // the quarters' maxima and denominators, then their sums, 32 columns at a time
       float2* ml = reinterpret_cast<float2*>(exchange);
@@ -328,7 +331,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
 #pragma unroll 1
       for (int c = 0; c < kHeadDim; c += 32) {
         uint32_t o[32];
-        ld32(base + 128 + c, o);
+        ld32(base + kO + c, o);
         ld_wait<32>(o);
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -362,6 +365,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       if (two && x == 1 && w.nrows <= R) continue;   // the item has one tile of pairs
       if constexpr (FEW) {
         few(w, h0, h1, n, at0);
+        tiles += w.tile1 - w.tile0;
         continue;
       }
       const bool alive = r < R && row < w.nrows, any = __any_sync(0xffffffffu, alive);
@@ -455,7 +459,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         for (int c = 0; c < kHeadDim; c += 32) {
           uint32_t o[32];
           if (any && some) {
-            ld32(base + 128 + c, o);
+            ld32(base + kO + c, o);
             ld_wait<32>(o);
           }
           unsigned char* xb = exchange + (c & 32) * (kOperand / 32) + m * 16;
@@ -495,7 +499,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
 #pragma unroll 1
       for (int c = 0; c < kHeadDim; c += 32) {
         uint32_t o[32];
-        ld32(base + 128 + c, o);
+        ld32(base + kO + c, o);
         ld_wait<32>(o);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
@@ -579,7 +583,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       const uint64_t desc_q = make_desc(smem_u32(qs), 16, 1024), desc_k = make_desc(smem_u32(kring), 16, 1024), desc_v = make_desc(smem_u32(wide), kOperand / 2, 1024);
       constexpr uint32_t id_s = idesc_e4m3(kHalf, 0);
       const uint32_t id_o = idesc_f16(kHeadDim);
-      int n[2] = {0, 0}, half = 0, slot = 0, done = 0;   // half: of the CTA; slot: of the keys
+      int n[2] = {0, 0}, half = 0, tile = 0, slot = 0, done = 0;   // half, tile: of the CTA; slot: of the keys
       uint32_t ph = 0;
       // an item of nh halves: straight code for either count of tiles (branches between the MMAs cost the issuing warp more than the MMAs take)
       auto walk = [&](auto tiles_c, int nh) {
@@ -631,6 +635,42 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         step(std::false_type(), nh - 1);
         half += nh;
       };
+      // few pairs: the scores of whole tiles (the queries' operands are read once for 128 keys: 200 x 5 rows over 300 tokens 120 -> 109 us, 48 x 5 over 2500 81 -> 79.5), a tile ahead.  Four barriers for the halves in turn: at half n all products of
+      // the tile before the last are known to be complete, n - 4 among them, and a wait for the one before n - 1 in its place must not be one for n - 1
+      auto walk_few = [&](int nh) {
+        const int nt = (nh + 1) >> 1;
+        auto scores = [&](int t) {
+          wait(k_full + slot, ph);
+          fence_after();
+          const uint64_t db = desc_k + (uint64_t)((slot * kOperand) >> 4);
+          const uint32_t d = tm + ((tile + t) & 1) * 128;
+#pragma unroll
+          for (int j = 0; j < 8; ++j) mma_f8_ss(one, d, desc_q + ((j >> 2) * kOperand + (j & 3) * 32) / 16, db + ((j & 3) * 32) / 16, idesc_e4m3(128, 0), j ? 1u : 0u);
+          commit(one, s_full + ((tile + t) & 1));
+          commit(one, k_free + slot);
+          commit(t + 1 == nt ? one : 0u, q_free);
+          if (++slot == kKSlots) slot = 0, ph ^= 1;
+        };
+        scores(0);
+        int b = half % kWide;
+        uint32_t bph = (half / kWide) & 1;
+#pragma unroll 1
+        for (int i = 0; i < nh; ++i) {
+          if ((i & 1) == 0 && (i >> 1) + 1 < nt) scores((i >> 1) + 1);
+          wait(w_full + b, bph);
+          wait(p_ready + (n[0] & 3), (n[0] >> 2) & 1);
+          fence_after();
+          const uint32_t pa = tm + ((tile + (i >> 1)) & 1) * 128 + (i & 1) * kHalf, d = tm + kO;
+          const uint64_t dv = desc_v + (uint64_t)((b * kOperand) >> 4);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma_ts(one, d, pa + j * 8, dv + (uint64_t)((j * 2048) >> 4), id_o, (i | j) ? 1u : 0u);
+          commit(one, w_free + b);
+          commit(one, o_full + (n[0] & 3));
+          ++n[0];
+          if (++b == kWide) b = 0, bph ^= 1;
+        }
+        half += nh, tile += nt;
+      };
       // one tile of pairs, its even halves to the first group of softmax warps, its odd ones to the second: scores two halves ahead
       auto walk_in_turn = [&](int nh) {
         int s_slot = slot;
@@ -680,7 +720,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         const int tiles = __shfl_sync(0xffffffffu, w.nrows > R ? 2 : 1, 0);
         wait(q_ready, done++ & 1);
         if constexpr (FEW) {
-          walk(std::integral_constant<int, 1>(), nh);
+          walk_few(nh);
           continue;
         }
         if (!two) walk_in_turn(nh);

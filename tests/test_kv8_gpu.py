@@ -777,3 +777,21 @@ def test_checks_of_many_sequences():
     front = [torch.cat([x[:lead], x]) for x in (target, draft, tokens, uniforms)]
     got = check_drafts(front[0].to(DEV), front[1].to(DEV), front[2], [s + lead for s in starts], temperature, front[3])
     assert bool((got[0][:lead] == -9).all()) and torch.equal(got[1], kept) and torch.equal(got[0][lead:], want)
+
+
+def test_many_short_items_one_after_another():
+    """200 sequences of five rows over 150 to 300 tokens: a dozen items a CTA, of one to three tiles, cut anywhere; twice the same bits."""
+    hq, hkv, n = 32, 8, 200
+    g = torch.Generator().manual_seed(200)
+    before = [int(x) for x in torch.randint(145, 296, (n,), generator=g)]
+    parts = [5] * n
+    seq, ctx = _step(parts, before)
+    cache = K.Cache([a + b for a, b in zip(parts, before)], hkv, 128, g)
+    q = _rows(5 * n, hq, g)
+    qd, outs = _on_device(q), [torch.full((5 * n, hq * 128), float("nan"), dtype=BF, device=DEV) for _ in range(6)]
+    cache.to(DEV)
+    for out in outs:
+        attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, 5)
+    torch.cuda.synchronize()
+    check_attention(outs[0].reshape(5 * n, hq, 128), q, cache, seq, ctx)
+    assert all(torch.equal(out.view(torch.int16), outs[0].view(torch.int16)) for out in outs)
