@@ -159,7 +159,14 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
     const bool group = ga;
     const int2 all = plan_scan(ga, it, sh);
     if (group) groups[n_groups + ga] = {runs[i], n, seq_of(runs[i]), 0};
-    for (int k = 0; k < mine; ++k) rows[n_items + it + k] = {runs[i] + k * per, min(per, n - k * per), seq_of(runs[i]), 0};
+    if (mine <= 2) {
+      for (int k = 0; k < mine; ++k) rows[n_items + it + k] = {runs[i] + k * per, min(per, n - k * per), seq_of(runs[i]), 0};
+    }
+    for (unsigned many = __ballot_sync(0xffffffffu, mine > 2); many; many &= many - 1) {   // a run of many items: by its warp
+      const int from = __ffs(many) - 1, row0 = __shfl_sync(0xffffffffu, i < n_runs ? runs[i] : 0, from), rn = __shfl_sync(0xffffffffu, n, from),
+                to = n_items + __shfl_sync(0xffffffffu, it, from), count = __shfl_sync(0xffffffffu, mine, from), seq = seq_of(row0);
+      for (int k = lane; k < count; k += 32) rows[to + k] = {row0 + k * per, min(per, rn - k * per), seq, 0};
+    }
     n_groups += all.x, n_items += all.y;
   }
   __syncthreads();
@@ -194,25 +201,28 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
     int tiles = 0, none = 0;
     for (int i = tid; i < n_items; i += kPlanThreads) tiles += (max(rows[i].ctx, 0) + kKv8Tile - 1) / kKv8Tile;
     const int total = plan_scan(tiles, none, sh).x * p.hkv, share = max(1, (total + kNumSMs - 1) / kNumSMs);
+    // tiles in front of an item (of one kv head), in the place of the runs' first rows, which nobody needs any more
     int front = 0;
     for (int i0 = 0; i0 < n_items; i0 += kPlanThreads) {
       const int i = i0 + tid;
-      Kv8Group g = {0, 0, 0, 0};
-      if (i < n_items) g = rows[i];
-      const int nt = (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile;
-      int base = nt;
+      int base = i < n_items ? (max(rows[i].ctx, 0) + kKv8Tile - 1) / kKv8Tile : 0;
       none = 0;
       const int all = plan_scan(base, none, sh).x;
-      base = (front + base) * p.hkv;
+      if (i < n_items) runs[i] = front + base;
       front += all;
-      for (int h = 0; h < p.hkv && nt > 0; ++h, base += nt) {
-        const int k0 = base / share, k1 = (base + nt - 1) / share;
-        for (int k = k0; k <= k1; ++k) {
-          const int from = max(base, k * share), to = min(base + nt, (k + 1) * share), place = i * p.hkv + h + k;
-          p.items[place] = {g.row0, g.nrows, g.seq, g.ctx, from - base, to - base, h, k, k1 - k0 + 1, 2 * k + (k == k0 ? 1 : 0), {0, 0}};
-          if (from == k * share) p.starts[k] = place;
-          if (k == k0 && k1 > k0) p.cuts_rows[k] = {g.row0, g.nrows, h, k1 - k0 + 1};
-        }
+    }
+    __syncthreads();
+    for (int u = tid; u < n_items * p.hkv; u += kPlanThreads) {
+      const int i = u / p.hkv, h = u % p.hkv;
+      const Kv8Group g = rows[i];
+      const int nt = (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile, base = runs[i] * p.hkv + h * nt;
+      if (nt == 0) continue;
+      const int k0 = base / share, k1 = (base + nt - 1) / share;
+      for (int k = k0; k <= k1; ++k) {
+        const int from = max(base, k * share), to = min(base + nt, (k + 1) * share), place = u + k;
+        p.items[place] = {g.row0, g.nrows, g.seq, g.ctx, from - base, to - base, h, k, k1 - k0 + 1, 2 * k + (k == k0 ? 1 : 0), {0, 0}};
+        if (from == k * share) p.starts[k] = place;
+        if (k == k0 && k1 > k0) p.cuts_rows[k] = {g.row0, g.nrows, h, k1 - k0 + 1};
       }
     }
   }
