@@ -8,8 +8,8 @@
 // exponent of the values follows the largest one seen (two bits ahead of it); where it rises O is rescaled, as it is where a row's maximum rises by more than 2^8.
 //
 // Bound by the warp that issues the MMAs (1000 to 1250 cycles for a half of 64 keys and 128 pairs: 12 MMAs, whose operands take 640 cycles of shared memory's reads, commits and
-// three waits) and, beside it, by the softmax of the half (900) and the widening (1900 for both halves of a tile).  2048 rows behind 1000 tokens, 32 heads over 8, 103 us, 660
-// TFLOP/s; 300 rows of three sequences behind 6000 tokens 69 us.  An item's end costs 7000 cycles: its last product, results by way of shared memory, the next one's first scores.
+// three waits) and, beside it, by the softmax of the half (900) and the widening (1900 for both halves of a tile).  2048 rows behind 1000 tokens, 32 heads over 8, 104 us, 650
+// TFLOP/s; 300 rows of three sequences behind 6000 tokens 68 us.  An item's end costs 7000 cycles: its last product, results by way of shared memory, the next one's first scores.
 #include <algorithm>
 #include <type_traits>
 
@@ -32,7 +32,7 @@ static_assert(kSmem <= 232448, "shared memory");
 __device__ __forceinline__ uint32_t idesc_f16(int n) { return (1u << 4) | (1u << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24); }
 
 // FEW: items of at most 32 pairs, which are there in each quarter of the MMA's rows: a quarter's warp takes a quarter of the keys.  Softmax is half the work then, and
-// the second group of softmax warps widens every other half instead (48 x 5 rows of 4 heads over 2500 tokens 80 us; as items of 128 pairs 90).
+// the second group of softmax warps widens every other half instead (48 x 5 rows of 4 heads over 2500 tokens 79 us; as items of 128 pairs 90).
 template <bool FEW>
 __global__ void __launch_bounds__(kThreads, 1)
 kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv8QueryMaps qmaps, const Kv8Params p) {
