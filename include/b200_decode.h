@@ -282,7 +282,7 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * rotated in place), k and v rows are quantised into the cache at slot_mapping[t].  qkv's k and v columns keep what they
  * hold.  A row whose slot is negative or behind the cache is not stored (its q is rotated).  Slots of one call differ.
  *
- * (a6) b200_paged_attn_decode_fp8: attention of rows by themselves; b200_paged_attn_prefill_fp8: the same results for steps in
+ * (a6) b200_paged_attn_decode_fp8: attention of rows by themselves; b200_paged_attn_prefill_fp8: the same attention for steps in
  * which neighbouring rows belong to one sequence (drafts under verification, chunks of prompts): they share its keys and
  * values.  Arguments as b200_paged_attn_decode / _prefill; up to 16 query heads to a kv head; scores, sums and softmax in
  * fp32, weights of at least eight significant bits, one rounding of the result.  A row sees ctx_lens[t] tokens of its
