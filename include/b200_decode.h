@@ -298,7 +298,8 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * its last draft (its draft_tokens entry is not read).  draft_logits (bf16 [n_rows][ldd], last rows not read): what the drafts
  * were drawn from; NULL: a drafter without probabilities (each draft taken as certain).  With p, q the softmax of target and
  * draft row over the sequence's temperature (filtered logits are -inf in both; NaN and +inf are not expected):
- *   draft x is kept while uniforms[r][0] * q(x) < p(x); the first row r that is not, or the last one, draws the token
+ *   draft x is kept while uniforms[r][0] * q(x) < p(x) (sums of fp32 exponentials, good to about 1e-6); the first row r that
+ *   is not, or the last one, draws the token
  *   min { i : sum over j <= i of w_j > uniforms[r][1] * sum of w },  w = max(p - q, 0) for a refused draft (p where that
  *   leaves nothing), p behind the last one; sums in 64 bits.
  * temperature[s] <= 0 (or temperature NULL, uniforms then unused): a draft is kept if it is the row's argmax (ties: the lowest
