@@ -182,6 +182,20 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
       for (int r = 0; r < n; ++r)
         for (int c = lane; c < p.hq * kHeadDim / 8; c += 32) *reinterpret_cast<uint4*>(p.out + (int64_t)(row0 + r) * p.ldo + 8 * c) = make_uint4(0u, 0u, 0u, 0u);
   }
+  __syncthreads();
+  // Items that see nothing leave the list: a CTA takes the first place that is not its own for the end of its items, and the shares are of tiles.  `runs` holds the
+  // tiles in front of an item (of one kv head) from here on; nobody needs the runs' first rows any more
+  int kept = 0, tiles = 0;
+  for (int i0 = 0; i0 < n_items; i0 += kPlanThreads) {
+    const int i = i0 + tid;
+    const Kv8Group g = i < n_items ? rows[i] : Kv8Group{0, 0, 0, 0};
+    int front = (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile, at = front > 0;
+    const bool sees = front > 0;
+    const int2 all = plan_scan(front, at, sh);   // (all have read theirs: places in front are written)
+    if (sees) rows[kept + at] = g, runs[kept + at] = tiles + front;
+    tiles += all.x, kept += all.y;
+  }
+  n_items = kept;
   const int n_list = n_items * p.hkv + 2 * kNumSMs + 1;   // places that the list may use, and the one behind them
   for (int i = tid; i < n_list; i += kPlanThreads) p.items[i].cta = -1;
   if (tid < kNumSMs) p.starts[tid] = -1, p.cuts_rows[tid].parts = 0;
@@ -193,30 +207,16 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
       const int round = i / kNumSMs, k = i % kNumSMs, cta = round & 1 ? kNumSMs - 1 - k : k, u = n - 1 - i;
       const Kv8Group g = rows[u / p.hkv];
       // a CTA's items have places of their own: one a round, and one behind them (the last round may have nothing for it)
-      p.items[cta * (rounds + 1) + round] = {g.row0, g.nrows, g.seq, g.ctx, 0, (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile, u % p.hkv, cta, 1, 0, {0, 0}};
+      p.items[cta * (rounds + 1) + round] = {g.row0, g.nrows, g.seq, g.ctx, 0, (g.ctx + kKv8Tile - 1) / kKv8Tile, u % p.hkv, cta, 1, 0, {0, 0}};
       if (round == 0) p.starts[cta] = cta * (rounds + 1);
     }
   } else {
     // one tile of pairs: the flattened list of (item, kv head, tile) in equal shares
-    int tiles = 0, none = 0;
-    for (int i = tid; i < n_items; i += kPlanThreads) tiles += (max(rows[i].ctx, 0) + kKv8Tile - 1) / kKv8Tile;
-    const int total = plan_scan(tiles, none, sh).x * p.hkv, share = max(1, (total + kNumSMs - 1) / kNumSMs);
-    // tiles in front of an item (of one kv head), in the place of the runs' first rows, which nobody needs any more
-    int front = 0;
-    for (int i0 = 0; i0 < n_items; i0 += kPlanThreads) {
-      const int i = i0 + tid;
-      int base = i < n_items ? (max(rows[i].ctx, 0) + kKv8Tile - 1) / kKv8Tile : 0;
-      none = 0;
-      const int all = plan_scan(base, none, sh).x;
-      if (i < n_items) runs[i] = front + base;
-      front += all;
-    }
-    __syncthreads();
+    const int share = max(1, (tiles * p.hkv + kNumSMs - 1) / kNumSMs);
     for (int u = tid; u < n_items * p.hkv; u += kPlanThreads) {
       const int i = u / p.hkv, h = u % p.hkv;
       const Kv8Group g = rows[i];
-      const int nt = (max(g.ctx, 0) + kKv8Tile - 1) / kKv8Tile, base = runs[i] * p.hkv + h * nt;
-      if (nt == 0) continue;
+      const int nt = (g.ctx + kKv8Tile - 1) / kKv8Tile, base = runs[i] * p.hkv + h * nt;
       const int k0 = base / share, k1 = (base + nt - 1) / share;
       for (int k = k0; k <= k1; ++k) {
         const int from = max(base, k * share), to = min(base + nt, (k + 1) * share), place = u + k;

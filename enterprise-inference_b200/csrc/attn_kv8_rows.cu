@@ -87,15 +87,13 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
   int at = p.starts[blockIdx.x];
   Kv8Rows ahead = p.items[at];
   auto next_unit = [&](Kv8Rows& u) {
-    for (;;) {
-      u = ahead;
-      if (u.cta != (int)blockIdx.x) return false;
-      ahead = p.items[++at];
-      if (u.tile1 > u.tile0) return true;   // (rows that see nothing: the plan wrote their zeros)
-    }
+    u = ahead;
+    if (u.cta != (int)blockIdx.x) return false;
+    ahead = p.items[++at];
+    return true;
   };
   // does the item that was asked for come next? (its block numbers, contexts and factors may be asked for)
-  auto comes_next = [&]() { return ahead.cta == (int)blockIdx.x && ahead.tile1 > ahead.tile0; };
+  auto comes_next = [&]() { return ahead.cta == (int)blockIdx.x; };
 
   // ===== values of a half -> f16, factors of its keys: every half (group -1), or one of each tile's =====
   auto widen = [&](int group) {

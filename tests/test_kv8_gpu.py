@@ -795,3 +795,99 @@ def test_many_short_items_one_after_another():
     torch.cuda.synchronize()
     check_attention(outs[0].reshape(5 * n, hq, 128), q, cache, seq, ctx)
     assert all(torch.equal(out.view(torch.int16), outs[0].view(torch.int16)) for out in outs)
+
+
+# ---- sequences without anything to attend, between others ------------------------------------------------------------------
+
+def _idle(parts, before, idle):
+    seq, ctx = _step(parts, before)
+    return seq, [0 if s in idle else c for s, c in zip(seq, ctx)]
+
+
+@pytest.mark.parametrize("most", [5, 0])
+@pytest.mark.parametrize("idle", [(0,), (4,), (7,), (13,), (19,), (1, 2, 3, 11), (0, 1, 17, 18, 19), tuple(range(0, 20, 2)), tuple(range(20))])
+def test_idle_sequences_between_drafts(idle, most):
+    """20 sequences of five rows over 300 to 1000 tokens and 7 kv heads: shares of up to six tiles, cut anywhere; idle ones first, last, in a row, alternating.
+    Bound 0: the items of 128 pairs."""
+    hq, hkv = 28, 7
+    g = torch.Generator().manual_seed(61)
+    before = [int(x) for x in torch.randint(300, 1000, (20,), generator=g)]
+    parts = [5] * 20
+    seq, ctx = _idle(parts, before, idle)
+    cache = K.Cache([a + b for a, b in zip(parts, before)], hkv, 128, g)
+    q = _rows(100, hq, g)
+    qd, out = _on_device(q), torch.full((100, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(100, hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("idle", [(1,), (0, 2), (2,), (0, 1), (3,)])
+@pytest.mark.parametrize("hq,hkv,block", [(28, 7, 128), (7, 7, 64)])
+def test_idle_sequences_between_chunks(idle, hq, hkv, block):
+    """Chunks of several items of 128 pairs (fewer than fill two tiles), parts of them in several CTAs."""
+    parts, before = [45, 150, 33, 70, 5], [1000, 700, 1700, 200, 1100]
+    seq, ctx = _idle(parts, before, idle)
+    g = torch.Generator().manual_seed(62)
+    cache = K.Cache([a + b for a, b in zip(parts, before)], hkv, block, g)
+    T = len(seq)
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    for most in (150, 0):
+        out.fill_(float("nan"))
+        attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+        torch.cuda.synchronize()
+        check_attention(out.reshape(T, hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("hq,hkv,most", [(28, 7, 230), (64, 16, 460), (16, 2, 4)])
+def test_padding_inside_a_run(hq, hkv, most):
+    """Whole items of a run whose rows see nothing, between items that do; most 4: the same run in items of four rows; 460 rows over 16 kv heads: items of two tiles."""
+    T = 460 if hkv == 16 else 230
+    ctx = [500 + i for i in range(T)]
+    for lo, hi in ((0, 3), (32, 70), (96, 130), (T - 40, T)):
+        ctx[lo:hi] = [0 if i % 5 else -3 for i in range(hi - lo)]
+    g = torch.Generator().manual_seed(63)
+    cache = K.Cache([500 + T], hkv, 128, g)
+    q = _rows(T, hq, g)
+    qd, out = _on_device(q), torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.zeros(T, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_attention(out.reshape(T, hq, 128), q, cache, [0] * T, ctx)
+
+
+@pytest.mark.parametrize("hq", [16, 32])
+def test_many_idle_sequences(hq):
+    """600 drafting slots of which 20, here and there, are in use: captured once, replayed with other slots in use."""
+    hkv, n = 8, 600
+    g = torch.Generator().manual_seed(64)
+    cache = K.Cache([450] * 3, hkv, 128, g)
+    seq, T = [s for s in range(n) for _ in range(4)], 4 * n
+    q = _rows(T, hq, g)
+    cache.bt = cache.bt[torch.arange(n) % 3]           # slots share three sequences' blocks
+    cache.rows = [cache.rows[s % 3] for s in range(n)]
+    cache.to(DEV)
+    sd, cd, qd, out = torch.tensor(seq, dtype=I32, device=DEV), torch.zeros(T, dtype=I32, device=DEV), _on_device(q), torch.zeros(T, hq * 128, dtype=BF, device=DEV)
+    ws = attend(qd, cache, sd, cd, out, hq, 4)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        attend(qd, cache, sd, cd, out, hq, 4, ws=ws, stream=torch.cuda.current_stream().cuda_stream)
+    for _ in range(3):
+        ctx = [0] * T
+        for s in torch.randperm(n, generator=g)[:20].tolist():
+            b = int(torch.randint(0, 446, (1,), generator=g))
+            ctx[4 * s:4 * s + 4] = [b + 1, b + 2, b + 3, b + 4]
+        cd.copy_(torch.tensor(ctx, dtype=I32))
+        out.fill_(float("nan"))
+        ws.fill_(0xff)
+        graph.replay()
+        torch.cuda.synchronize()
+        busy = [t for t in range(T) if ctx[t]]
+        got = out.reshape(T, hq, 128)
+        rest = torch.tensor([c == 0 for c in ctx])
+        assert not bool(got[rest.to(DEV)].any())
+        check_attention(got[busy], q[busy], cache, [seq[t] for t in busy], [ctx[t] for t in busy])
