@@ -106,7 +106,7 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
     const float top = fmaxf(bf16lo(h), bf16hi(h));
     if (top > m) {
       const float fn = rintf(top * c);
-      s *= tc::exp2_fast(f - fn);   // (nothing yet: s is 0, f too)
+      s = s > 0.f ? s * tc::exp2_fast(f - fn) : 0.f;   // (nothing yet: f is 0, and fn may be far below it)
       f = fn;
       m = top;
       at = g0;

@@ -891,3 +891,43 @@ def test_many_idle_sequences(hq):
         rest = torch.tensor([c == 0 for c in ctx])
         assert not bool(got[rest.to(DEV)].any())
         check_attention(got[busy], q[busy], cache, [seq[t] for t in busy], [ctx[t] for t in busy])
+
+
+# ---- rows of probabilities at the ends of their ranges ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("shift,temp", [(-100.0, 1.0), (-1000.0, 0.7), (500.0, 0.9), (-10.0, 0.05), (-60.0, 0.3), (-3e4, 40.0)])
+def test_rows_far_from_zero(shift, temp, probs):
+    """All logits of a row far below zero, or above: probabilities do not depend on it."""
+    V, g = 5003, torch.Generator().manual_seed(int(abs(shift)) + probs)
+    parts = [4] * 8
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    target, draft = ((x.float() * max(1.0, temp) + shift).to(BF) for x in (target, draft))
+    uniforms, temperature = torch.rand(32, 2, generator=g), torch.full((8,), temp)
+    d = draft if probs else None
+    want, kept, margins = K.verify(target, d, tokens, starts, temperature, uniforms)
+    assert all(m > 1e-5 for m in margins)
+    got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
+    assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("low", [-20.0, -95.0, -1e4])
+@pytest.mark.parametrize("temp", [1.0, 0.1])
+def test_long_stretches_of_low_logits(low, temp):
+    """Most of a row at a low, finite value (reserved entries, masks), in front of, between and behind the others; a row of nothing else."""
+    V, g = 40003, torch.Generator().manual_seed(5)
+    parts = [4] * 8
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    for x in (target, draft):
+        x[:, :9000] = low
+        x[:, 12000:33000] = low
+        x[:, 39000:] = low
+    target[9, :], draft[9, :] = low, low
+    gumbel = -torch.log(-torch.log(torch.rand(32, V, generator=g).clamp(1e-9, 1 - 1e-7)))
+    tokens = (draft.float() / temp + gumbel).argmax(1)
+    uniforms, temperature = torch.rand(32, 2, generator=g), torch.full((8,), temp)
+    for d in (draft, None):
+        want, kept, margins = K.verify(target, d, tokens, starts, temperature, uniforms)
+        assert all(m > 1e-5 for m in margins)
+        got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
+        assert torch.equal(got[1], kept) and torch.equal(got[0], want)
