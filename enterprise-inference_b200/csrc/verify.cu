@@ -1,8 +1,8 @@
 // Check of drafted tokens against the target's probabilities (b200_verify_drafts), two launches.
 //
-// stats: a CTA takes a slice of a logit row (target rows, and the rows that drafts were drawn from) and leaves its largest logit, the first place of it and the sum
-// of 2^(l c - f), c = log2e / T, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  f is the largest l c as a whole number,
-// so that l c - f is rounded once.  A thread compares 32 entries with its maximum at once; the place is looked for at the end, by the threads that met the CTA's
+// stats: a CTA takes a slice of a logit row (target rows, and the rows that drafts were drawn from) and leaves its largest logit m, the first place of it and the sum
+// of 2^((l - m) c), c = log2e / T, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  The difference of two logits is exact, or
+// rounded once, and never above zero, whatever the temperature: l c by itself has no bits left for its fraction where T is small.  A thread compares 32 entries with its maximum at once; the place is looked for at the end, by the threads that met the CTA's
 // largest (with a place kept by every thread the same took 23.5 million instructions for 64 x 5 drafts over 128256 entries, this 15.2).  35 us there, 4.2 TB/s;
 // bound by the exponentials (four a cycle and quarter of an SM: 16 us) and the latency of short loops.
 // draw: a cluster of eight CTAs takes a sequence: the kept drafts from the slices' sums, then the token from the one row that draws it.  A draw next to a border of
@@ -24,12 +24,12 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kStatThreads = 256, kStatGroups = 4, kLeastSlice = 2048, kWholeSlice = kStatThreads * 8 * kStatGroups;
-constexpr float kMostScale = 1e30f;   // (temperatures below 1e-30 are taken as that)
+constexpr float kLeastScale = 1.4426950408889634e-30f, kMostScale = 1.4426950408889634e30f;   // log2e / T of temperatures between 1e30 (masked entries weigh nothing) and 1e-30
 constexpr int kDrawThreads = 256, kDrawCtas = 8, kChunk = 256, kMostChunks = 192;
 constexpr int kMostVocab = kDrawCtas * kMostChunks * kChunk, kMostPart = kMostChunks * kChunk * 2;
 
-struct Stat {
-  float m, f, s;
+struct alignas(16) Stat {
+  float m, s;
   int at;
 };
 constexpr int kKnownRows = 64;   // rows of a sequence whose largest logits are kept
@@ -77,9 +77,9 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
   // entries from i0 on in groups of eight that start at 16-byte addresses (the slice's ends may lie inside a group)
   const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7);
   const int i0 = slice * slice_len, i1 = min(vocab, i0 + slice_len), a0 = i0 - shift;
-  float m = -INFINITY, f = 0.f, s = 0.f;
+  float m = -INFINITY, s = 0.f;
   int at = 0x7fffffff;
-  const float c = temp > 0.f ? fminf(1.4426950408889634f / temp, kMostScale) : 0.f;
+  const float c = temp > 0.f ? fmaxf(fminf(1.4426950408889634f / temp, kMostScale), kLeastScale) : 0.f;
   constexpr int U = kStatGroups, S = kStatThreads * 8;
   for (int g0 = a0 + threadIdx.x * 8; g0 < i1; g0 += U * S) {
     uint4 v[U];
@@ -105,21 +105,20 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
     for (int u = 0; u < U; ++u) h = max2(h, max2(max2(v[u].x, v[u].y), max2(v[u].z, v[u].w)));
     const float top = fmaxf(bf16lo(h), bf16hi(h));
     if (top > m) {
-      const float fn = rintf(top * c);
-      s = s > 0.f ? s * tc::exp2_fast(f - fn) : 0.f;   // (nothing yet: f is 0, and fn may be far below it)
-      f = fn;
+      s *= tc::exp2_fast((m - top) * c);   // (nothing yet: 2^-inf)
       m = top;
       at = g0;
     }
     if (!(temp > 0.f)) continue;
+    const float from = m > -INFINITY ? -m : 0.f;
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       if (g0 + u * S >= i1) break;
       const uint32_t w[4] = {v[u].x, v[u].y, v[u].z, v[u].w};
       uint64_t e[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {   // (-inf alone so far: 2^-inf)
-        const uint64_t t = f2::fma(f2::pack(bf16lo(w[j]), bf16hi(w[j])), f2::both(c), f2::both(-f));
+      for (int j = 0; j < 4; ++j) {
+        const uint64_t t = f2::mul(f2::add(f2::pack(bf16lo(w[j]), bf16hi(w[j])), f2::both(from)), f2::both(c));
         e[j] = f2::pack(tc::exp2_fast(f2::lo(t)), tc::exp2_fast(f2::hi(t)));
       }
       s += f2::sum(f2::add(f2::add(e[0], e[1]), f2::add(e[2], e[3])));
@@ -133,7 +132,6 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
   float all = sh_m[0];
 #pragma unroll
   for (int w = 1; w < kStatThreads / 32; ++w) all = fmaxf(all, sh_m[w]);
-  const float fa = rintf(all * c);
   // the first place of the largest entry: those look for it who met it
   if (m == all && m > -INFINITY) {
     bool there = false;
@@ -141,20 +139,21 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
       for (int k = max(at + u * S, i0), end = min(at + u * S + 8, i1); k < end && !there; ++k)
         if (__bfloat162float(l[k]) == m) atomicMin(&first, k), there = true;
   }
-  s = warp_sum(m > -INFINITY ? s * tc::exp2_fast(f - fa) : 0.f);
+  s = warp_sum(m > -INFINITY ? s * tc::exp2_fast((m - all) * c) : 0.f);
   if (lane == 0) sh_s[warp] = s;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < kStatThreads / 32; ++w) s += sh_s[w];
-    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {all, all > -INFINITY ? fa : 0.f, s, first};
+    stats[((int64_t)row * 2 + which) * gridDim.x + slice] = {all, s, first};
   }
 }
 
 // a bf16 in its fp32 bits -> the double of 2^-896 times its value (the exponent's bits moved as they are; denormals stay what they are, -inf comes out as
 // -2^128 times that: nothing beside any logit that counts)
 __device__ __forceinline__ double scaled_double(uint32_t f) { return __hiloint2double((int)f >> 3 & (int)0x8fffffffu, 0); }
-constexpr double kScaledBack = 0x1p896;
-// 2^t for t <= 0 (or little more), 2^-1017 below: t = n / 32 + r, 2^(n / 32) = 2^(n >> 5) table[n & 31], 2^r = 1 + r q(r), |r| <= 1 / 64: the series of (2^r - 1) / r
+__device__ __forceinline__ double scaled_double(float x) { return scaled_double(__float_as_uint(x)); }
+constexpr double kScaledBack = 0x1p896, kLeastPower = -1017.0;
+// 2^t for t <= 0, 2^kLeastPower below that: t = n / 32 + r, 2^(n / 32) = 2^(n >> 5) table[n & 31], 2^r = 1 + r q(r), |r| <= 1 / 64: the series of (2^r - 1) / r
 // with its terms above the third taken down to a cubic by Chebyshev polynomials, 1.6e-13 of 2^r
 __device__ __forceinline__ double exp2_table(double t, const double* table) {
   t = __hiloint2double((int)min((uint32_t)__double2hiint(t), 0xc08fc800u), __double2loint(t));
@@ -191,41 +190,44 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   const int r0 = min(max(starts[s], 0), n_rows), r1 = min(max(starts[s + 1], r0), n_rows);
   const float temp = temperature ? temperature[s] : 0.f;
   const bool greedy = !(temp > 0.f);
-  const double c = greedy ? 0.0 : fmin(1.4426950408889634 / (double)temp, (double)kMostScale), cf = greedy ? 0.0 : (double)fminf(1.4426950408889634f / temp, kMostScale);   // cf: what the sums have
+  const double c = greedy ? 0.0 : fmax(fmin(1.4426950408889634 / (double)temp, (double)kMostScale), (double)kLeastScale);
+  const double cf = greedy ? 0.0 : (double)fmaxf(fminf(1.4426950408889634f / temp, kMostScale), kLeastScale);   // what the sums have
   if (tid == 0) sh_refused = max(r1 - r0 - 1, 0);
   __syncthreads();
-  // a row's largest logits and their first place, from the slices (by a warp)
-  auto row_stats = [&](int r, float (&m)[2], float (&f)[2], double (&z)[2], int& at, bool sums) {
+  // a row's largest logits, their first place and (relative to them) the sums, from the slices (by a warp)
+  auto row_stats = [&](int r, float (&m)[2], double (&z)[2], int& at, bool sums) {
     at = 0x7fffffff;
 #pragma unroll
     for (int k = 0; k < 2; ++k) {
-      m[k] = -INFINITY, f[k] = -INFINITY, z[k] = 0.0;
+      m[k] = -INFINITY, z[k] = 0.0;
       if (k && (greedy || r == r1 - 1 || !draft)) continue;
       const Stat* st = stats + ((int64_t)r * 2 + k) * n_slices;
       for (int i = lane; i < n_slices; i += 32) {
         const Stat x = st[i];
-        if (x.m > -INFINITY) f[k] = fmaxf(f[k], x.f);
         if (!k && (x.m > m[0] || (x.m == m[0] && x.at < at))) at = x.at;
         m[k] = fmaxf(m[k], x.m);
       }
       const float own = m[k];
-      m[k] = warp_max(own), f[k] = warp_max(f[k]);
+      m[k] = warp_max(own);
       if (!k) at = __reduce_min_sync(0xffffffffu, own == m[0] ? at : 0x7fffffff);
       if (!sums || !(m[k] > -INFINITY)) continue;
       for (int i = lane; i < n_slices; i += 32)
-        if (st[i].m > -INFINITY) z[k] += (double)st[i].s * exp2_table((double)st[i].f - (double)f[k], table);
+        if (st[i].m > -INFINITY) z[k] += (double)st[i].s * exp2_table(((double)st[i].m - (double)m[k]) * cf, table);
       z[k] = warp_sum_double(z[k]);
     }
     if (m[0] == -INFINITY) at = 0;
   };
   // the sums of a row's target over its draft, each relative to its largest logit, as near as fp32 has them
-  auto ratio = [&](const float (&m)[2], const float (&f)[2], const double (&z)[2]) {
-    return z[1] > 0.0 ? z[0] / z[1] * exp2(((double)f[0] - (double)m[0] * cf) - ((double)f[1] - (double)m[1] * cf)) : 0.0;
+  auto ratio = [&](const double (&z)[2]) { return z[1] > 0.0 ? z[0] / z[1] : 0.0; };
+  // the probability of an entry (its bits) of a row; what 2^t has no number for is none
+  auto probability = [&](uint32_t bits, float m, double z) {
+    const double t = ((double)__uint_as_float(bits << 16) - (double)m) * cf;
+    return t > kLeastPower ? exp2_table(t, table) / z : 0.0;
   };
   // a warp a row: is the draft refused?
   for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
     double z[2];
-    float m[2], f[2];
+    float m[2];
     int at;
     const bool last = r == r1 - 1;
     const int x = last ? -1 : tokens[r];
@@ -233,17 +235,16 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     // (asked for before the sums are there)
     const uint32_t lx = ok ? __bfloat16_as_ushort(target[(int64_t)r * ldt + x]) : 0u, dx = ok && draft ? __bfloat16_as_ushort(draft[(int64_t)r * ldd + x]) : 0u;
     const double u = ok && !greedy ? (double)uniforms[2 * r] : 0.0;
-    row_stats(r, m, f, z, at, !greedy);
+    row_stats(r, m, z, at, !greedy);
     if (lane == 0 && r - r0 < kKnownRows) {
       known_m[r - r0][0] = m[0], known_m[r - r0][1] = m[1], known_at[r - r0] = at;
-      known_ratio[r - r0] = ratio(m, f, z);
+      known_ratio[r - r0] = ratio(z);
     }
     ok = ok && m[0] > -INFINITY;
     if (ok && greedy) {
       ok = x == at;
     } else if (ok) {
-      const double p = lx == 0xff80u ? 0.0 : exp2_table(fma((double)__uint_as_float(lx << 16), cf, -(double)f[0]), table) / z[0];
-      const double q = !draft ? 1.0 : m[1] > -INFINITY && dx != 0xff80u ? exp2_table(fma((double)__uint_as_float(dx << 16), cf, -(double)f[1]), table) / z[1] : 0.0;
+      const double p = probability(lx, m[0], z[0]), q = !draft ? 1.0 : m[1] > -INFINITY ? probability(dx, m[1], z[1]) : 0.0;
       ok = u * q < p;
     }
     if (!ok && lane == 0) atomicMin(&sh_refused, r - r0);
@@ -256,10 +257,10 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     if (tid == 0) sh_m[0] = known_m[taken][0], sh_m[1] = known_m[taken][1], sh_best = known_at[taken], sh_ratio = known_ratio[taken];
   } else if (any && warp == 0) {
     double z[2];
-    float m[2], f[2];
+    float m[2];
     int at;
-    row_stats(row, m, f, z, at, !greedy);
-    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = at, sh_ratio = ratio(m, f, z);
+    row_stats(row, m, z, at, !greedy);
+    if (lane == 0) sh_m[0] = m[0], sh_m[1] = m[1], sh_best = at, sh_ratio = ratio(z);
   }
   __syncthreads();
   if (rank == 0) {
@@ -274,7 +275,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   const bool residual = !last, probs = residual && draft && sh_m[1] > -INFINITY;
   const __nv_bfloat16* d = probs ? draft + (int64_t)row * ldd : nullptr;
   const int x = residual && !draft ? tokens[row] : -1;   // a certain draft: what is left has nothing of it
-  const double mp = (double)sh_m[0] * c, mq = probs ? (double)sh_m[1] * c : 0.0, scale = c * kScaledBack;
+  const double mp = scaled_double(sh_m[0]), mq = probs ? scaled_double(sh_m[1]) : 0.0, scale = c * kScaledBack;
   const int n_chunks = (vocab + kChunk - 1) / kChunk, per = (n_chunks + kDrawCtas - 1) / kDrawCtas;
   const int ch0 = min(n_chunks, rank * per), ch1 = min(n_chunks, ch0 + per);
   // the CTA's entries, -inf behind the end (a thread reads back what it wrote: its eight of every 16th chunk)
@@ -284,8 +285,8 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
     fetch8(part_p + at, l, i, vocab);
   }
   f2::cp_wait_all();
-  // entry j of eight, relative to 2^m
-  auto weight = [&](const uint32_t* w, int j, double m) { return exp2_table(fma(scaled_double(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16), scale, -m), table); };
+  // entry j of eight, relative to the row's largest logit (m: scaled as they are)
+  auto weight = [&](const uint32_t* w, int j, double m) { return exp2_table((scaled_double(j & 1 ? w[j >> 1] & 0xffff0000u : w[j >> 1] << 16) - m) * scale, table); };
   // running sums of the chunks, by a warp: kMostChunks / 32 neighbours a lane, then over the lanes; returns their sum
   auto running = [&](double* v) {
     constexpr int N = kMostChunks / 32;

@@ -931,3 +931,49 @@ def test_long_stretches_of_low_logits(low, temp):
         assert all(m > 1e-5 for m in margins)
         got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
         assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("temp", [1.0, 0.1, 40.0])
+def test_masks_of_the_lowest_value(temp):
+    """Logits of the type's lowest number in most places, in rows with others, with one other, and without any (all entries equally probable)."""
+    V, g = 20011, torch.Generator().manual_seed(6)
+    parts = [3] * 10
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    low = torch.finfo(BF).min
+    for x in (target, draft):
+        x[:, :9000], x[:, 9500:19000] = low, low
+        x[3:6], x[6:12] = low, low
+        x[6:12, 17] = -2.0
+    tokens[0:12] = torch.tensor([9100, 9200, 0, 4, 19500, 0, 17, 18, 0, 17, 17, 0])
+    uniforms, temperature = torch.rand(30, 2, generator=g), torch.full((10,), temp)
+    for d in (draft, None):
+        want, kept, margins = K.verify(target, d, tokens, starts, temperature, uniforms)
+        assert all(m > 1e-5 for m in margins if m > 0)
+        got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
+        assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("probs", [True, False])
+@pytest.mark.parametrize("temp,size", [(1e-4, 1.0), (1e-6, 1.0), (1e-8, 1.0), (1e-9, 1.0), (1e-10, 1.0), (1e-12, 1.0), (1e-16, 1.0), (1e-20, 1.0), (1e-30, 1.0),
+                                       (1e-8, 1e-8), (1e-20, 1e-20), (1e-30, 1e-30), (1e4, 1e4), (1e30, 1e30), (1e38, 1.0), (3.4e38, 1e-3)])
+def test_temperatures_of_every_size(temp, size, probs):
+    """Logits of ordinary size at the smallest temperatures (the largest entry has all of the probability, drafts that are it, and others), logits and temperatures that
+    are both small or large, and one temperature above all logits (every entry that is not masked equally probable)."""
+    V, g = 6007, torch.Generator().manual_seed(40 + probs)
+    parts = [5] * 12
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    target, draft = ((x.float() * size).to(BF) for x in (target, draft))
+    for x in (target, draft):
+        x[:, 100:200] = float("-inf")
+        x[::7, 5], x[::7, 4000] = 11 * size, 11 * size   # two largest entries
+    best, drafted = target.double().argmax(1), draft.double().argmax(1)
+    if size == 1.0 and temp < 1:   # (elsewhere the drafts as they were drawn)
+        kind = torch.arange(60) % 5
+        tokens = torch.where(kind < 2, best, torch.where(kind == 2, drafted, tokens))
+        tokens[56], tokens[57] = 150, V
+    uniforms, temperature = torch.rand(60, 2, generator=g), torch.full((12,), temp)
+    d = draft if probs else None
+    want, kept, margins = K.verify(target, d, tokens, starts, temperature, uniforms)
+    assert all(m > 1e-5 for m in margins if m > 0)   # (0: a draft that neither row gives anything)
+    got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
+    assert torch.equal(got[1], kept) and torch.equal(got[0], want)
