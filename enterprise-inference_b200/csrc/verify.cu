@@ -455,7 +455,11 @@ int slices(int n_rows, int vocab) {
 
 }  // namespace
 
-int64_t verify_drafts_workspace_bytes(int n_rows, int vocab) { return (int64_t)n_rows * 2 * slices(n_rows, vocab) * (int64_t)sizeof(Stat); }
+// enough for this many rows and for any smaller number (rows times slices falls where slices get longer): a row has at most want slices, and so many of kLeastSlice
+int64_t verify_drafts_workspace_bytes(int n_rows, int vocab) {
+  const int64_t most = ((int64_t)vocab + kLeastSlice - 1) / kLeastSlice;
+  return std::min(n_rows * most, std::max<int64_t>(n_rows, kNumSMs * 24 / 2)) * 2 * (int64_t)sizeof(Stat);
+}
 
 int verify_drafts(const __nv_bfloat16* target, int64_t ldt, const __nv_bfloat16* draft, int64_t ldd, const int32_t* tokens, const int32_t* starts,
                   const float* temperature, const float* uniforms, int n_seqs, int n_rows, int vocab, int32_t* out, int32_t* accepted, void* ws,

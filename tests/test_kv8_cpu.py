@@ -130,3 +130,25 @@ def test_plain_check_of_equal_probabilities():
     lower, higher = (7, 9) if target[0, 7] < target[0, 9] else (9, 7)
     out, kept, _ = K.verify(target, draft, torch.tensor([lower, 0]), [0, 2], torch.ones(1), torch.tensor([[0.999, 0.5], [0.5, 0.5]]))
     assert int(kept[0]) == 0 and int(out[0]) == higher
+
+
+@pytest.mark.parametrize("V", [1, 300, 2048, 2049, 16032, 32000, 65537, 128256, 152064, 393216])
+def test_workspaces_for_many_rows_do_for_fewer(V):
+    """A caller asks once, for its largest step: the size of drafts' checks never falls as rows or entries rise, and a step of that size has what it needs."""
+    lib = _lib()
+    sizes = [lib.b200_verify_drafts_workspace_bytes(n, V) for n in range(5000)]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:])) and sizes[1] > 0
+    assert all(lib.b200_verify_drafts_workspace_bytes(n, V) <= lib.b200_verify_drafts_workspace_bytes(n, V + 1000) for n in (1, 7, 48, 320, 65535))
+    # what a step of n rows writes, restated: 16 bytes a row, slice and kind of row
+    for n in list(range(1, 400)) + [999, 1776, 1777, 5000, 65535]:
+        want = max(1, 148 * 24 // max(1, 2 * n))
+        length = -(-V // want)
+        length = -(-length // 8192) * 8192 if length > 4096 else max(2048, -(-length // 8) * 8)
+        assert lib.b200_verify_drafts_workspace_bytes(n, V) >= n * 2 * 16 * -(-V // length)
+
+
+def test_attention_workspaces_for_many_rows_do_for_fewer():
+    lib = _lib()
+    for hq, hkv in ((1, 1), (32, 8), (40, 8), (64, 4), (128, 128)):
+        sizes = [lib.b200_paged_attn_fp8_workspace_bytes(n, hq, hkv) for n in range(3000)]
+        assert all(a <= b for a, b in zip(sizes, sizes[1:]))

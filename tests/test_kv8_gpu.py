@@ -977,3 +977,26 @@ def test_temperatures_of_every_size(temp, size, probs):
     assert all(m > 1e-5 for m in margins if m > 0)   # (0: a draft that neither row gives anything)
     got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, temperature, uniforms)
     assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("probs", [True, False])
+def test_checks_of_smaller_steps_in_the_largest_ones_workspace(probs):
+    """One workspace of the size asked for 64 x 5 rows, with nothing behind it that a call may touch, for every smaller step."""
+    V, g = 128256, torch.Generator().manual_seed(9)
+    lib, check = _lib()
+    size = int(lib.b200_verify_drafts_workspace_bytes(320, V))
+    ws = torch.full((size + 4096,), 0xff, dtype=torch.uint8, device=DEV)
+    target, draft, tokens, starts = _drafts([5] * 64, V, g)
+    best = target.double().argmax(1)
+    td, dd, kd = target.to(DEV), draft.to(DEV), best.to(I32).to(DEV)
+    temp, uni = torch.full((64,), 1e-6, device=DEV), torch.full((320, 2), 0.5, device=DEV)   # (the largest entries have all of the probability, in equal parts)
+    want, took, _ = K.verify(target, draft if probs else None, best, starts, temp.cpu(), uni.cpu())
+    for n in (1, 2, 5, 10, 12, 20, 48, 60, 64):
+        out, kept = torch.full((320,), -9, dtype=I32, device=DEV), torch.full((64,), -9, dtype=I32, device=DEV)
+        begin = torch.arange(0, 5 * n + 1, 5).to(I32).to(DEV)
+        check(lib.b200_verify_drafts(td.data_ptr(), V, dd.data_ptr() if probs else None, V, kd.data_ptr(), begin.data_ptr(), temp.data_ptr(), uni.data_ptr(), n, 5 * n, V,
+                                     out.data_ptr(), kept.data_ptr(), ws.data_ptr(), size, None))
+        torch.cuda.synchronize()
+        assert torch.equal(kept[:n].cpu().long(), took[:n]) and bool((kept[n:] == -9).all())
+        assert torch.equal(out[:5 * n].cpu().long(), want[:5 * n]) and bool((out[5 * n:] == -9).all())
+        assert bool((ws[size:] == 0xff).all())
