@@ -6,8 +6,9 @@
 //
 // The codes go to the tensor core as they are: nothing is widened.  Each column is there twice, as e4m3 and as 16 times what that rounding left: for a
 // bf16 query scaled by a power of two both terms together are exact (4 + 4 significant bits), for a weight they have eight.  A token's exponents are
-// applied in fp32: the key's to its scores, the value's to its weights, relative to the largest one of the tile.  The weights of a tile are taken
-// relative to the tile's own maximum and its product is added to the running sums in registers, so that the 22 bits between the largest and the
+// applied in fp32: the key's to its scores, the value's to its weights.  What a column's codes hold is 2^(score + value exponent), relative to the tile's
+// largest such one among the tokens that the column sees: a large value that a row does not see, or hardly weighs, takes no bits from the others, nor do small ones
+// that take most of the weight.  The product of a tile is added to the running sums in registers, so that the 22 bits between the largest and the
 // smallest code pair only have to span one tile (weights relative to a running maximum would lose a long context's small ones).
 //
 // The flattened list of (group, kv head, tile) is cut into equal shares, one per SM: contexts may differ as they like.  An item that a cut goes through
@@ -32,6 +33,7 @@ constexpr int kFacs = 2;                     // tiles whose factors are kept
 constexpr int kFacBytes = kKv8Tile * 8 + 16; // a token's (key factor, value factor); the tile's factor, whether a token is dead
 constexpr int kAhead = 8;                    // tiles ahead that the exponents are asked for (a power of two)
 constexpr float kLowest = -3.402823466e38f;
+constexpr float kMostSpan = 100.f;           // bits between a tile's value exponents that are told apart: 2^that times a tile's tokens is an fp32 number
 constexpr int kStageWarps = 4;               // keys and values, MMA, queries, factors
 
 struct Kv8Item {
@@ -514,13 +516,14 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           ld_cols<NCG>(base + (n & 1) * 2 * NP + NP, lo);
           const float* f = reinterpret_cast<const float*>(facs + (n & (kFacs - 1)) * kFacBytes);
           const float2 kv = reinterpret_cast<const float2*>(f)[tau], vr = reinterpret_cast<const float2*>(f)[kKv8Tile];
+          const float lv = fmaxf((float)(int)(__float_as_uint(kv.y) >> 23 & 255u) - 135.f, -kMostSpan);   // the value's exponent below the tile's largest
           ld_wait<NCG>(hi);
           if (two) fold(keep0, take0);
-          float s[NCG];
+          float s[NCG];   // score + lv
 #pragma unroll
           for (int j = 0; j < NCG; ++j) {
             asm volatile("" : "+r"(lo[j]));
-            s[j] = tok < ctx[j] ? fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])) * (kv.x * qf[j]) : -INFINITY;
+            s[j] = tok < ctx[j] ? fmaf(fmaf(__uint_as_float(lo[j]), 0.0625f, __uint_as_float(hi[j])), kv.x * qf[j], lv) : -INFINITY;
             const float m = warp_max_f32(s[j]);
             if (lane == 0) xt[j * 4 + quad] = m;
           }
@@ -531,8 +534,9 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           for (int j = 0; j < NCG; ++j) {
             const float4 x = reinterpret_cast<const float4*>(xt)[j];
             // (a column whose row does not see this tile: the lowest finite number stands for its maximum, and its scores are -inf)
+            // the denominators are relative to this maximum too: e may be above 1 for tokens of smaller values, by 2^kMostSpan at most
             const float mt = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), kLowest), mn = fmaxf(mu[j], mt);
-            const float e = exp2_fast(s[j] - mt), b = exp2_fast(mt - mn);
+            const float e = exp2_fast(s[j] - mt - lv), b = exp2_fast(mt - mn);
             keep1[j] = exp2_fast(mu[j] - mn);
             take1[j] = b * vr.x;
             l[j] = l[j] * keep1[j] + e * b;

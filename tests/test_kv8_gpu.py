@@ -1000,3 +1000,106 @@ def test_checks_of_smaller_steps_in_the_largest_ones_workspace(probs):
         assert torch.equal(kept[:n].cpu().long(), took[:n]) and bool((kept[n:] == -9).all())
         assert torch.equal(out[:5 * n].cpu().long(), want[:5 * n]) and bool((out[5 * n:] == -9).all())
         assert bool((ws[size:] == 0xff).all())
+
+
+# ---- values of very different sizes ----------------------------------------------------------------------------------------
+
+def check_shares(out, q, cache, seq, ctx, scale=128 ** -0.5):
+    """As check_attention, but what is lost of a small weight is held against the row's own largest share (weight times largest entry of a value row) and not against
+    the largest value: a code of eight bits relative to it is off by 2^-22 of it where small, times 2 (a value row's entries are below twice 2^its exponent's
+    range of largest codes) and 127 tokens of a tile: 2^-14."""
+    out, q = out.double().cpu(), q.cpu()
+    for t in range(len(ctx)):
+        want, share, _ = K.attention(q[t], cache.rows[seq[t]], ctx[t], scale)
+        k, v = (x[:ctx[t]].repeat_interleave(q.shape[1] // x.shape[1], 1) for x in cache.rows[seq[t]])
+        p = torch.softmax(torch.einsum("hd,chd->hc", q[t].double(), k) * scale, -1)
+        top = (p * v.abs().amax(-1).T).amax(-1, keepdim=True)
+        bound = 2.0 ** -8 * want.abs() + (2.0 ** -8 + 2.0 ** -12) * share + 2.0 ** -14 * top
+        off = (out[t] - want).abs() - bound
+        assert (off <= 0).all(), (t, ctx[t], float(off.max()), int(off.argmax()))
+
+
+def _scale_values(cache, s, at, power):
+    """Value rows of a sequence (before cache.to) times 2^power, in the cache and in the oracle's copy."""
+    blk = cache.bt[s, at // cache.block]
+    cache.ve[blk, :, at % cache.block] += power
+    cache.rows[s][1][at] *= 2.0 ** power
+
+
+def _set_key(cache, s, at, key):
+    """A key row of a sequence for all kv heads."""
+    codes, exps = K.quantise(key[None])
+    blk = cache.bt[s, at // cache.block]
+    cache.k[blk, :, at % cache.block], cache.ke[blk, :, at % cache.block] = codes, exps
+    cache.rows[s][0][at] = K.values(codes, exps)[0]
+
+
+WIDE_STEPS = {   # heads, kv heads, bound, rows and cached tokens of each sequence
+    "decode": (8, 1, None, [1] * 5, [40, 127, 130, 600, 2900]),
+    "columns": (4, 4, 4, [4] * 6, [0, 3, 124, 126, 300, 1100]),
+}
+
+
+@pytest.mark.parametrize("power", [9, 15, 19, 24, 40, 90])
+@pytest.mark.parametrize("name", sorted(WIDE_STEPS))
+def test_rows_do_not_meet_values_that_they_do_not_see(name, power):
+    """Values of a step's own tokens grow by a power of two at two places: the rows in front of them are what they would be without."""
+    hq, hkv, most, parts, before = WIDE_STEPS[name]
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(71)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 64, g, spread=0.5)
+    for s, (n, b) in enumerate(zip(parts, before)):
+        _scale_values(cache, s, b + n - 1, power)
+        if n > 20:
+            _scale_values(cache, s, b + n // 2, power // 2)
+    q = _rows(len(seq), hq, g)
+    qd, out = _on_device(q), torch.full((len(seq), hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_shares(out.reshape(len(seq), hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("power,lean", [(12, -0.2), (18, -0.3), (25, -0.3), (40, -0.6), (60, -0.6), (-12, 0.3), (-30, 0.5), (-70, 0.9)])
+@pytest.mark.parametrize("name", sorted(WIDE_STEPS))
+def test_large_values_of_little_weight(name, power, lean):
+    """Three tokens a sequence whose values are far larger (smaller) than the others' and whose keys turn every query away (attract it), so that either kind
+    may make up a row's result."""
+    hq, hkv, most, parts, before = WIDE_STEPS[name]
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(72)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 64, g, spread=0.5)
+    base = torch.randn(128, generator=g) * 2
+    for s, (n, b) in enumerate(zip(parts, before)):
+        for at in {0, (n + b) // 2, n + b - 1}:
+            _scale_values(cache, s, at, power)
+            _set_key(cache, s, at, base * lean * (1 + 0.1 * at / (n + b)))
+    q = (base + torch.randn(len(seq), hq, 128, generator=g) * 0.2).to(BF)
+    qd, out = _on_device(q), torch.full((len(seq), hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_shares(out.reshape(len(seq), hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("name", sorted(WIDE_STEPS))
+def test_value_rows_of_zeros_among_others(name):
+    """Rows of zeros have the least exponent; a row whose every other token is one, a sequence of nothing else, zeros that take most of the weight."""
+    hq, hkv, most, parts, before = WIDE_STEPS[name]
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(73)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 64, g)
+    base = torch.randn(128, generator=g) * 2
+    for s, (n, b) in enumerate(zip(parts, before)):
+        for at in range(0, n + b, 1 if s == 1 else 2):
+            blk = cache.bt[s, at // 64]
+            cache.v[blk, :, at % 64], cache.ve[blk, :, at % 64] = 0, 27
+            cache.rows[s][1][at] = 0
+        if n + b > 100:
+            _set_key(cache, s, 64, base * 0.6)
+    q = (base + torch.randn(len(seq), hq, 128, generator=g) * 0.2).to(BF)
+    qd, out = _on_device(q), torch.full((len(seq), hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    check_shares(out.reshape(len(seq), hq, 128), q, cache, seq, ctx)
