@@ -8,6 +8,7 @@ namespace b200 {
 
 constexpr int kKv8Tile = 128;          // tokens of a tile
 constexpr int kKv8Cols = 16;           // (row, head) pairs of a group at most
+constexpr int kKv8Span = 100;          // bits between value exponents that are told apart: 2^that times a long context's weights is an fp32 number
 constexpr int kKv8PartFloats = 132;    // of a pair in a part: 128 sums, their maximum (log2 domain), the denominator
 
 // rows [row0, row0 + nrows) of one sequence that share its keys and values; nrows 0: none

@@ -33,7 +33,6 @@ constexpr int kFacs = 2;                     // tiles whose factors are kept
 constexpr int kFacBytes = kKv8Tile * 8 + 16; // a token's (key factor, value factor); the tile's factor, whether a token is dead
 constexpr int kAhead = 8;                    // tiles ahead that the exponents are asked for (a power of two)
 constexpr float kLowest = -3.402823466e38f;
-constexpr float kMostSpan = 100.f;           // bits between a tile's value exponents that are told apart: 2^that times a tile's tokens is an fp32 number
 constexpr int kStageWarps = 4;               // keys and values, MMA, queries, factors
 
 struct Kv8Item {
@@ -516,7 +515,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           ld_cols<NCG>(base + (n & 1) * 2 * NP + NP, lo);
           const float* f = reinterpret_cast<const float*>(facs + (n & (kFacs - 1)) * kFacBytes);
           const float2 kv = reinterpret_cast<const float2*>(f)[tau], vr = reinterpret_cast<const float2*>(f)[kKv8Tile];
-          const float lv = fmaxf((float)(int)(__float_as_uint(kv.y) >> 23 & 255u) - 135.f, -kMostSpan);   // the value's exponent below the tile's largest
+          const float lv = fmaxf((float)(int)(__float_as_uint(kv.y) >> 23 & 255u) - 135.f, -(float)kKv8Span);   // the value's exponent below the tile's largest
           ld_wait<NCG>(hi);
           if (two) fold(keep0, take0);
           float s[NCG];   // score + lv
@@ -534,7 +533,7 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
           for (int j = 0; j < NCG; ++j) {
             const float4 x = reinterpret_cast<const float4*>(xt)[j];
             // (a column whose row does not see this tile: the lowest finite number stands for its maximum, and its scores are -inf)
-            // the denominators are relative to this maximum too: e may be above 1 for tokens of smaller values, by 2^kMostSpan at most
+            // the denominators are relative to this maximum too: e may be above 1 for tokens of smaller values, by 2^kKv8Span at most
             const float mt = fmaxf(fmaxf(fmaxf(x.x, x.y), fmaxf(x.z, x.w)), kLowest), mn = fmaxf(mu[j], mt);
             const float e = exp2_fast(s[j] - mt - lv), b = exp2_fast(mt - mn);
             keep1[j] = exp2_fast(mu[j] - mn);

@@ -6,6 +6,10 @@
 // Here one column of scores belongs to one thread's pair, so nothing is reduced across lanes, and a weight is one f16: 11 bits, and 2^-31 of the largest before
 // it is lost (e4m3 in two terms would lose it at 2^-22, and cost twice the conversions).  Widening the values is shared by 256 pairs.  The reference
 // exponent of the values follows the largest one seen (two bits ahead of it); where it rises O is rescaled, as it is where a row's maximum rises by more than 2^8.
+// The reference is shared by rows that see different tokens, and values far below it would lose bits to ones that a row does not see or hardly weighs: from the tile
+// on where they are more than 2^kSpan apart, an item's weights carry the value exponents themselves, relative to the row's own largest share (always: 2048 rows 120 us
+// instead of 104; where they do from the start 203).  Items of few pairs always do: their softmax is short, and the widening, which bounds them, has nothing to scale (200 x 5 rows over
+// 300 tokens 108 -> 102.5 us).
 //
 // Bound by the warp that issues the MMAs (1000 to 1250 cycles for a half of 64 keys and 128 pairs: 12 MMAs, whose operands take 640 cycles of shared memory's reads, commits and
 // three waits) and, beside it, by the softmax of the half (900) and the widening (1900 for both halves of a tile).  2048 rows behind 1000 tokens, 32 heads over 8, 104 us, 650
@@ -23,7 +27,9 @@ using namespace tc;
 constexpr int kThreads = 512, kHalf = 64;            // keys of a score tile: half of a tile of the cache
 constexpr int kOperand = 128 * 128;                  // a term of 128 queries; a tile of keys or values in codes: 16 KiB
 constexpr int kKSlots = 3, kVSlots = 2, kWide = 3;   // tiles of codes, halves of widened values
-constexpr int kFacBytes = kHalf * 4 + 16;            // the keys' factors; the values' reference exponent
+constexpr int kFacBytes = 3 * kHalf * 4 + 16;        // the keys' factors; the values' reference exponent (-1: in the weights); their own exponents; (few) 2^-those
+constexpr int kSpan = 14;   // bits between an item's value exponents up to which they have one reference (a weight is good to 2^-32 of the largest, a share then to
+                            // 2^-17 of the row's largest share)
 constexpr int kStage = 8 * 2048;
 constexpr int kBars = 2 * kKSlots + 2 * kVSlots + 2 * kWide + 12 + 3 + 1;   // (and the two words behind them)
 constexpr int kSmem = 1024 + 4 * kOperand + kWide * kOperand + (kKSlots + kVSlots) * kOperand + kStage + kWide * kFacBytes + kBars * 8 + 16;
@@ -126,6 +132,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       fetch();
       place();
       int ref = 0;
+      bool apart = false;
 #pragma unroll 1
       for (int t = w.tile0; t < w.tile1; ++t) {
         const uint32_t k4 = k_next, v4 = v_next;
@@ -133,14 +140,17 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         place();
         // the reference: two bits above the largest exponent so far
         const int left = w.ctx - t * kKv8Tile;
-        uint32_t mx = 1u;
+        uint32_t mx = 1u, mn = 255u;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const uint32_t v = (v4 >> (8 * j)) & 255u;
-          if (4 * lane + j < left && v != 255u) mx = max(mx, v);
+          if (4 * lane + j < left && v != 255u) mx = max(mx, v), mn = min(mn, v - 1u);   // (0 stands for nothing)
         }
         mx = __reduce_max_sync(0xffffffffu, mx);
+        mn = __reduce_min_sync(0xffffffffu, mn);
         if (t == w.tile0 || (int)mx > ref) ref = (int)mx + 2;
+        apart |= (int)mn + 1 < ref - 2 - kSpan;
+        const int least = max(ref - 2 - kKv8Span, kKv8MinExp + 127);   // (few) values below are nothing beside the largest so far
         wait(v_full + slot, ph);
         const int halves = min(2, h1 - 2 * t);
 #pragma unroll 1
@@ -163,20 +173,24 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
           for (int i = 0; i < 2; ++i) {
             const int rt = hh * kHalf + r_own + 8 * i;   // row of the tile
             const uint32_t ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
-            const int d = (int)ve - ref + 7;   // code * 2^d, exact while d >= -15
-            const uint32_t f1 = rt >= left || ve == 255u ? 0x8000u : d >= -14 ? (uint32_t)(d + 15) << 10 : d >= -24 ? 1u << (d + 24) : 0u;
-            f[i] = f1 | f1 << 16;
+            if constexpr (FEW) {   // codes as they are
+              f[i] = rt >= left || ve == 255u || (int)ve < least ? 0x80008000u : 0u;
+            } else {
+              const int d = apart ? 5 : (int)ve - ref + 7;   // code * 2^d: exact, 5 - kSpan or more, but for bytes of 0
+              const uint32_t f1 = rt >= left || ve == 255u ? 0x8000u : (uint32_t)max(d + 15, 0) << 10;
+              f[i] = f1 | f1 << 16;
+            }
           }
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int r = r_own + 8 * (i >> 1), cc = c_own ^ 4 * (i & 1);
-            if (f[i >> 1] == 0x80008000u) c[i] = make_uint4(0u, 0u, 0u, 0u);   // behind the context, or not a number: zeros, whatever the codes
+            if (f[i >> 1] == 0x80008000u) c[i] = make_uint4(0u, 0u, 0u, 0u);   // behind the context, not a number, or (few) nothing: zeros, whatever the codes
             const uint32_t c4[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
             uint32_t o[8];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               const __half2 a = __half2(__nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(c4[j >> 1] >> (16 * (j & 1))), __NV_E4M3));
-              const __half2 v = __hmul2(a, *reinterpret_cast<const __half2*>(&f[i >> 1]));
+              const __half2 v = FEW ? a : __hmul2(a, *reinterpret_cast<const __half2*>(&f[i >> 1]));
               o[j] = *reinterpret_cast<const uint32_t*>(&v);
             }
             unsigned char* row = dst + (cc >> 2) * (kOperand / 2) + r * 128;
@@ -189,7 +203,13 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
             const uint32_t ke = (__shfl_sync(0xffffffffu, k4, rt >> 2) >> (8 * (rt & 3))) & 255u, ve = (__shfl_sync(0xffffffffu, v4, rt >> 2) >> (8 * (rt & 3))) & 255u;
             float* fk = reinterpret_cast<float*>(facs + b * kFacBytes);
             if (lane < 16) fk[r] = ve == 255u && rt < left ? __uint_as_float(0x7fffffffu) : sign * __uint_as_float(ke << 23);
-            if (w4 == 0 && lane == 16) reinterpret_cast<int*>(fk)[kHalf] = ref;
+            if constexpr (FEW) {
+              const int e = rt >= left || ve == 255u ? 0 : max((int)ve, least) - 127;
+              if (lane < 16) fk[kHalf + 4 + r] = (float)e, fk[2 * kHalf + 4 + r] = __uint_as_float((uint32_t)(127 - e) << 23);
+            } else {
+              if (lane < 16 && apart) fk[kHalf + 4 + r] = ve == 255u ? 0.f : (float)(int)ve;
+              if (w4 == 0 && lane == 16) reinterpret_cast<int*>(fk)[kHalf] = apart ? -1 : ref;
+            }
           }
           fence_async_smem();
           __syncwarp();
@@ -226,6 +246,50 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         st16(base + kO + c, o);
       }
     };
+    // The weights of a half whose values' exponents they carry: 2^(score + exponent) relative to the largest one that the row has met, `share` (followed to within 2^8, as
+    // mu is), which O is relative to then; the denominators stay relative to mu.  Scores are read twice: registers are for the halves that have a reference
+    auto carry = [&](uint32_t s_addr, const float* f, int live, float qf, int n, bool rescales, float& mu, float& l, float& share) {
+      uint32_t s[16];
+      auto read = [&](int c) {
+        ld16(s_addr + 16 * c, s);
+        ld_wait<16>(s);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = 16 * c + j < live ? __float_as_uint(__uint_as_float(s[j]) * f[16 * c + j] * qf) : 0xff800000u;
+      };
+      float ms = -INFINITY, mt = -INFINITY;
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        read(c);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) ms = fmaxf(ms, __uint_as_float(s[j])), mt = fmaxf(mt, __uint_as_float(s[j]) + f[kHalf + 4 + 16 * c + j]);
+      }
+      if (ms > mu + 8.f) l *= exp2_fast(mu - ms), mu = ms;   // (nothing yet: l is 0)
+      float fo = 1.f;
+      if (mt > share + 8.f) {
+        if (share > -INFINITY) fo = exp2_fast(share - mt);
+        share = mt;
+      }
+      if (rescales && __any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
+      const float less = 7.f - (share > -INFINITY ? share : 0.f), shift = 7.f - (mu > -INFINITY ? mu : 0.f);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        read(c);
+        uint32_t pk[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float s0 = __uint_as_float(s[2 * j]), s1 = __uint_as_float(s[2 * j + 1]);
+          const float* g = f + kHalf + 4 + 16 * c + 2 * j;
+          l += exp2_fast(s0 + shift) + exp2_fast(s1 + shift);
+          const __half2 h2 = __floats2half2_rn(exp2_fast(s0 + g[0] + less), exp2_fast(s1 + g[1] + less));
+          pk[j] = *reinterpret_cast<const uint32_t*>(&h2);
+        }
+        st8(s_addr + 8 * c, pk);   // (below what is still to be read)
+      }
+    };
+    // what a row's O is times its result's denominator: values and weights as they are, but for the 2^7 that l has too
+    auto undone = [&](int ref, float mu, float share, bool carried) {
+      return carried && mu > -INFINITY ? exp2_fast(share - mu - 132.f) : __uint_as_float((uint32_t)max(ref - 7, 1) << 23);
+    };
     // 32 columns of the warp's pairs from shared memory to their rows: a row's 64 bytes leave from four neighbouring lanes
     auto store_staged = [&](const unsigned char* st, const Kv8Rows& w, int c) {
 #pragma unroll
@@ -253,8 +317,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       if (!led) ask(w);
       const int ctx = ctx_next;
       const float qf = qf_next;
-      float mu = -INFINITY, l = 0.f;
-      int ref = 0;
+      float share = -INFINITY, l = 0.f;   // the largest 2^(score + exponent) so far (followed to within 2^8), which O and the denominator are relative to
 #pragma unroll 1
       for (int h = h0; h < h1; ++h, ++n) {
         const int at = half + h - h0, b = at % kWide;
@@ -266,38 +329,36 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         const uint32_t s_addr = base + (tile & 1) * 128 + (h & 1) * kHalf;
         uint32_t s[16];
         ld16(s_addr + 16 * quad, s);
-        const int ref_new = reinterpret_cast<const int*>(f)[kHalf], live = ctx - h * kHalf - 16 * quad;
-        float k[16];
+        const int live = ctx - h * kHalf - 16 * quad;
+        float k[16], e[16], back[16];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<float4*>(k + 4 * j) = reinterpret_cast<const float4*>(f)[4 * quad + j];
+        for (int j = 0; j < 4; ++j) {
+          *reinterpret_cast<float4*>(k + 4 * j) = reinterpret_cast<const float4*>(f)[4 * quad + j];
+          *reinterpret_cast<float4*>(e + 4 * j) = reinterpret_cast<const float4*>(f + kHalf + 4)[4 * quad + j];
+          *reinterpret_cast<float4*>(back + 4 * j) = reinterpret_cast<const float4*>(f + 2 * kHalf + 4)[4 * quad + j];
+        }
         ld_wait<16>(s);
         float mx = -INFINITY;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
-          const float v = j < live ? __uint_as_float(s[j]) * k[j] : -INFINITY;
+          const float v = j < live ? fmaf(__uint_as_float(s[j]) * k[j], qf, e[j]) : -INFINITY;
           s[j] = __float_as_uint(v);
           mx = fmaxf(mx, v);
         }
-        mx *= qf;
-        const bool jump = mx > mu + 8.f;
-        if (__any_sync(0xffffffffu, jump) || ref_new != ref) {
-          const float mn = jump ? mx : mu;
-          float fo = jump && mu != -INFINITY ? exp2_fast(mu - mn) : 1.f;
+        const bool jump = mx > share + 8.f;
+        if (__any_sync(0xffffffffu, jump)) {
+          const float mn = jump ? mx : share, fo = jump && share != -INFINITY ? exp2_fast(share - mn) : 1.f;
           l *= fo;
-          mu = mn;
-          if (h > h0 + (FEW ? 0 : first)) {
-            fo *= __uint_as_float((uint32_t)max(127 - (ref_new - ref), 0) << 23);
-            if (__any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
-          }
-          ref = ref_new;
+          share = mn;
+          if (h > h0 && __any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
         }
-        const float shift = 7.f - (mu > -INFINITY ? mu : 0.f);
+        const float shift = 7.f - (share > -INFINITY ? share : 0.f);
         uint32_t pk[8], none[8];
         float sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float p0 = exp2_fast(fmaf(__uint_as_float(s[2 * j]), qf, shift)), p1 = exp2_fast(fmaf(__uint_as_float(s[2 * j + 1]), qf, shift));
-          sum += p0 + p1;
+          const float p0 = exp2_fast(__uint_as_float(s[2 * j]) + shift), p1 = exp2_fast(__uint_as_float(s[2 * j + 1]) + shift);
+          sum = fmaf(p0, back[2 * j], fmaf(p1, back[2 * j + 1], sum));
           const __half2 h2 = __floats2half2_rn(p0, p1);
           pk[j] = *reinterpret_cast<const uint32_t*>(&h2);
           none[j] = 0u;
@@ -315,15 +376,14 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       fence_after();
       // the quarters' maxima and denominators, then their sums, 32 columns at a time
       float2* ml = reinterpret_cast<float2*>(exchange);
-      ml[m] = make_float2(mu, l);
+      ml[m] = make_float2(share, l > 3e38f ? 3e38f : l);   // (not infinite: times nothing it would not be a number)
       asm volatile("bar.sync 1, 128;" ::: "memory");
       float top = -INFINITY, all = 0.f;
 #pragma unroll
       for (int k = 0; k < 4; ++k) top = fmaxf(top, ml[32 * k + lane].x);
 #pragma unroll
       for (int k = 0; k < 4; ++k) all += ml[32 * k + lane].y * (top == -INFINITY ? 0.f : exp2_fast(ml[32 * k + lane].x - top));
-      const float back = __uint_as_float((uint32_t)max(ref - 7, 1) << 23), own = mu == -INFINITY ? 0.f : exp2_fast(mu - top);
-      const float mult = own * (w.parts > 1 ? back : all == 0.f ? 0.f : back / all);
+      const float own = share == -INFINITY ? 0.f : exp2_fast(share - top), mult = w.parts > 1 ? own : all == 0.f ? 0.f : own / all;
       float* part = p.part_rows + ((int64_t)w.slot * 128 + lane) * kKv8PartFloats;
       if (w.parts > 1 && alive && quad == 0) part[128] = top, part[129] = all;
 #pragma unroll 1
@@ -369,9 +429,15 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
       const bool alive = r < R && row < w.nrows, any = __any_sync(0xffffffffu, alive);
       const int t = w.row0 + row, ctx = alive ? kv8_ctx(p, t) : 0;
       const float qf = alive ? __ldg(p.q_scale + (int64_t)t * p.hq + w.kvh * G + m % G) : 1.f;
-      float mu = -INFINITY, l = 0.f;
-      int ref = 0;
-      for (int h = h0 + first; h < h1; h += step, ++n) {
+      float mu = -INFINITY, l = 0.f, share = -INFINITY;
+      int ref = 0, h = h0 + first;
+      auto handed = [&]() {
+        st_wait();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
+      };
+      for (; h < h1; h += step, ++n) {
         const int at = at0 + h - h0, b = at % kWide;
         const float* f = reinterpret_cast<const float*>(facs + b * kFacBytes);
         wait(s_full + 2 * x + (n & 1), (n >> 1) & 1);
@@ -385,7 +451,7 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         uint32_t s[64];
         ld32(s_addr, s);
         ld32(s_addr + 32, s + 32);
-        const int ref_new = reinterpret_cast<const int*>(f)[kHalf];
+        const int ref_new = reinterpret_cast<const int*>(f)[kHalf], live = ctx - h * kHalf;
         ld_wait<64>(s);
 #pragma unroll
         for (int j = 0; j < 64; j += 4) {
@@ -394,7 +460,6 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
                          c = f2::mul(f2::pack(__uint_as_float(s[j + 2]), __uint_as_float(s[j + 3])), f2::pack(k.z, k.w));
           s[j] = (uint32_t)a, s[j + 1] = (uint32_t)(a >> 32), s[j + 2] = (uint32_t)c, s[j + 3] = (uint32_t)(c >> 32);
         }
-        const int live = ctx - h * kHalf;
         if (__any_sync(0xffffffffu, live < kHalf)) {
 #pragma unroll
           for (int j = 0; j < 64; ++j)
@@ -403,11 +468,12 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
         const float mx = max64(s) * qf;
         const bool jump = mx > mu + 8.f;   // also the first live key (mu = -inf)
         if (__any_sync(0xffffffffu, jump) || ref_new != ref) {
+          if (ref_new < 0) break;   // from here on the weights carry the exponents
           const float mn = jump ? mx : mu;
           float fo = jump && mu != -INFINITY ? exp2_fast(mu - mn) : 1.f;
           l *= fo;
           mu = mn;
-          if (h > h0 + (FEW ? 0 : first)) {
+          if (h > h0 + first) {
             fo *= __uint_as_float((uint32_t)max(127 - (ref_new - ref), 0) << 23);
             if (__any_sync(0xffffffffu, fo != 1.f)) rescale(n, fo);
           }
@@ -431,17 +497,25 @@ kv8_rows_kernel(const __grid_constant__ Kv8Maps maps, const __grid_constant__ Kv
           st16(s_addr + c * 16, pk);
         }
         l += f2::sum(sum[0]) + f2::sum(sum[1]);
-        st_wait();
-        fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(p_ready + 2 * x + (n & 1));
+        handed();
+      }
+      const bool carried = h < h1;
+      if (carried) share = mu + (float)(ref - 2);
+#pragma unroll 1
+      for (; h < h1; h += step, ++n) {
+        const int at = at0 + h - h0, b = at % kWide;
+        wait(s_full + 2 * x + (n & 1), (n >> 1) & 1);
+        wait(w_full + b, (at / kWide) & 1);
+        fence_after();
+        carry(base + (n & 1) * kHalf, reinterpret_cast<const float*>(facs + b * kFacBytes), ctx - h * kHalf, qf, n, h > h0 + first, mu, l, share);
+        handed();
       }
       const bool some = h0 + first < h1;
       if (some) {
         wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
         fence_after();
       }
-      const float back = __uint_as_float((uint32_t)max(ref - 7, 1) << 23);   // 2^(ref - 134): values and weights as they are, but for the 2^7 that l has too
+      const float back = undone(ref, mu, share, carried);
       if (!two) {   // the other group's halves: its sums come over through shared memory, 32 columns at a time in two buffers
         float2* ml = reinterpret_cast<float2*>(ostage + 8192);
         ml[threadIdx.x] = make_float2(mu, l);

@@ -274,7 +274,7 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * [n_blocks][n_kv_heads][block_size] uint8.  A value is code * 2^(byte - 127): one exponent per token and kv head, the
  * smallest e >= -100 with max |x| <= 448 * 2^e (every value is an exact bf16; relative error of a normal code at most
  * 2^-4).  Byte 255: the row held an inf or a NaN; its codes are NaN, and of such rows alone.  Byte 0 stands for nothing (a
- * caller that writes a cache of its own).  129 bytes a row where bf16 takes 256.
+ * caller that writes a cache of its own), bytes from 1 to 26 may count as nothing.  129 bytes a row where bf16 takes 256.
  * block_size is 16, 32, 64 or a multiple of 128; n_blocks * n_kv_heads * block_size < 2^31.  Codes are 16-byte aligned.
  *
  * (a4+a5) b200_rope_kv_append_fp8: NeoX RoPE of the q and k heads of qkv [T][ld] in fp32 with one rounding (where
@@ -285,7 +285,9 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * (a6) b200_paged_attn_decode_fp8: attention of rows by themselves; b200_paged_attn_prefill_fp8: the same attention for steps in
  * which neighbouring rows belong to one sequence (drafts under verification, chunks of prompts): they share its keys and
  * values.  Arguments as b200_paged_attn_decode / _prefill; up to 16 query heads to a kv head; scores, sums and softmax in
- * fp32, weights of at least eight significant bits, one rounding of the result.  A row sees ctx_lens[t] tokens of its
+ * fp32, weights of at least eight significant bits, one rounding of the result.  A weight that is small is held, together with its
+ * value's exponent, to 2^-17 of the row's own largest such product: tokens that a row does not see take no bits from those that
+ * it does (values up to 2^100 apart).  In runs of rows a query's entries below 2^-10 of its largest are held to 2^-19 of it.  A row sees ctx_lens[t] tokens of its
  * sequence (no more than bt_stride blocks of them): none gives zeros.  What lies behind them in a block is never looked at.  A block id outside
  * [0, n_blocks) stands for keys and values of zero.  max_rows: a HOST bound on the rows of one sequence that follow one
  * another in this step (0: not known): it only chooses the kernels (a longer run than it says is attended as well).  The

@@ -1020,8 +1020,8 @@ def check_shares(out, q, cache, seq, ctx, scale=128 ** -0.5):
 
 
 def _scale_values(cache, s, at, power):
-    """Value rows of a sequence (before cache.to) times 2^power, in the cache and in the oracle's copy."""
-    blk = cache.bt[s, at // cache.block]
+    """A value row of a sequence times 2^power, in the cache and in the oracle's copy."""
+    blk = int(cache.bt[s, at // cache.block])
     cache.ve[blk, :, at % cache.block] += power
     cache.rows[s][1][at] *= 2.0 ** power
 
@@ -1037,6 +1037,9 @@ def _set_key(cache, s, at, key):
 WIDE_STEPS = {   # heads, kv heads, bound, rows and cached tokens of each sequence
     "decode": (8, 1, None, [1] * 5, [40, 127, 130, 600, 2900]),
     "columns": (4, 4, 4, [4] * 6, [0, 3, 124, 126, 300, 1100]),
+    "few": (8, 2, 5, [5] * 6, [0, 3, 122, 126, 300, 1100]),
+    "items of one tile": (16, 2, 0, [40, 150, 9], [90, 30, 600]),
+    "items of two tiles": (64, 16, 333, [333, 64], [20, 100]),
 }
 
 
@@ -1103,3 +1106,35 @@ def test_value_rows_of_zeros_among_others(name):
     attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
     torch.cuda.synchronize()
     check_shares(out.reshape(len(seq), hq, 128), q, cache, seq, ctx)
+
+
+@pytest.mark.parametrize("at", [3, 130, 190, 700])
+@pytest.mark.parametrize("hq,hkv,most,parts,before", [(8, 8, 0, [120] * 6, [700] * 6), (64, 16, 0, [330, 64, 128], [800, 700, 760]), (16, 8, 8, [8] * 30, [800] * 30)],
+                         ids=["one tile", "two tiles", "few"])
+def test_an_item_whose_values_drift_apart(hq, hkv, most, parts, before, at):
+    """Whole items, and parts of several tiles, in which the exponents stay together up to a token in either half of a tile, and are 2^30 apart from there on; then
+    the same with the large one behind all rows but the last (some of the rows are looked at)."""
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(at)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 128, g, spread=0.5)
+    q = _rows(len(seq), hq, g)
+    qd, out = _on_device(q), torch.full((len(seq), hq * 128), float("nan"), dtype=BF, device=DEV)
+    sd, cd = torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV)
+    cache.to(DEV)
+    some = [t for t in range(len(seq)) if ctx[t] < parts[seq[t]] + before[seq[t]]][::17]
+
+    def scale(places, power):
+        for s in range(len(parts)):
+            _scale_values(cache, s, places[s], power)
+
+    def check():
+        attend(qd, cache, sd, cd, out, hq, most)
+        torch.cuda.synchronize()
+        check_shares(out.reshape(len(seq), hq, 128)[some], q[some], cache, [seq[t] for t in some], [ctx[t] for t in some])
+
+    scale([at] * len(parts), 30)
+    scale([at + 5] * len(parts), -20)
+    check()
+    scale([at] * len(parts), -30)
+    scale([n + b - 1 for n, b in zip(parts, before)], 30)
+    check()
