@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(kPlanThreads) kv8_plan_kernel(const Kv8Params 
   if (tid == 0) *head = {n_groups, two, {0, 0}};
 }
 
+constexpr int64_t kMostTokens = 0x7fffffff - 2 * kKv8Tile;   // of a block table: the kernels count tokens, up to two tiles past a context's end, in 32 bits
 // rows beside the longest run, times the tokens that a block table has room for: up to here their groups are not worth the columns kernel's launch (64 rows of a chunk and 16
 // others over 500 or 2000 tokens: 34 and 53 us without it, 45 and 60 with; over 8000 140 and 99)
 constexpr int64_t kFewTokens = 32768;
@@ -291,6 +292,8 @@ int64_t paged_attn_fp8_workspace_bytes(int T, int hq, int hkv) { return kCutByte
 int paged_attn_fp8(const Kv8Attn& a, int most, void* ws, int64_t ws_bytes, cudaStream_t s) {
   B200_REQUIRE((int64_t)a.T * a.hkv * (((int64_t)a.bt_stride * a.block_size + kKv8Tile - 1) / kKv8Tile) < 0x7fffffffll, B200_ERR_UNSUPPORTED,
                "paged_attn_fp8: %d rows of up to %lld tokens", a.T, (long long)a.bt_stride * a.block_size);
+  B200_REQUIRE((int64_t)a.bt_stride * a.block_size <= kMostTokens, B200_ERR_UNSUPPORTED, "paged_attn_fp8: block tables of %lld tokens (at most %lld)",
+               (long long)a.bt_stride * a.block_size, (long long)kMostTokens);
   Kv8Maps maps;
   if (const int rc = kv8_maps(a, std::min(a.block_size, kKv8Tile), &maps)) return rc;
   const int G = a.hq / a.hkv;

@@ -292,7 +292,7 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * [0, n_blocks) stands for keys and values of zero.  max_rows: a HOST bound on the rows of one sequence that follow one
  * another in this step (0: not known): it only chooses the kernels (a longer run than it says is attended as well).  The
  * workspace has no state between calls; calls that may run at the same time, two captured graphs among them, need one each.
- * Rows times kv heads times 128-token tiles of the block table stay below 2^31 (B200_ERR_UNSUPPORTED).
+ * Rows times kv heads times 128-token tiles of the block table stay below 2^31, its tokens below 2^31 - 256 (B200_ERR_UNSUPPORTED).
  *
  * b200_verify_drafts: which drafted tokens the target keeps, and the token that follows them (speculative sampling: what comes
  * out is distributed as the target's own draws).  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1 of target_logits

@@ -152,3 +152,11 @@ def test_attention_workspaces_for_many_rows_do_for_fewer():
     for hq, hkv in ((1, 1), (32, 8), (40, 8), (64, 4), (128, 128)):
         sizes = [lib.b200_paged_attn_fp8_workspace_bytes(n, hq, hkv) for n in range(3000)]
         assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
+@pytest.mark.parametrize("prefill", [False, True])
+@pytest.mark.parametrize("stride,block", [(2 ** 24, 128), (2 ** 27, 16), (2 ** 24 - 1, 128), (2 ** 21, 1024), (2 ** 31 - 1, 128)])
+def test_attention_counts_tokens_in_32_bits(prefill, stride, block):
+    """One row and one kv head: few enough tiles, but a table of more tokens than the kernels can count to the end of the last tile."""
+    assert _attend(prefill, T=1, hq=1, hkv=1, stride=stride, block=block) == -3
+    assert b"tokens" in _lib().b200_last_error()
