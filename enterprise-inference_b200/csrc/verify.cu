@@ -466,6 +466,7 @@ int verify_drafts(const __nv_bfloat16* target, int64_t ldt, const __nv_bfloat16*
                   int64_t ws_bytes, cudaStream_t s) {
   B200_REQUIRE(vocab <= kMostVocab, B200_ERR_UNSUPPORTED, "verify_drafts: vocab=%d (at most %d)", vocab, kMostVocab);
   B200_REQUIRE(n_rows <= 65535, B200_ERR_UNSUPPORTED, "verify_drafts: %d rows (at most 65535)", n_rows);
+  B200_REQUIRE(n_seqs <= 0x7fffffff / kDrawCtas, B200_ERR_UNSUPPORTED, "verify_drafts: %d sequences (at most %d)", n_seqs, 0x7fffffff / kDrawCtas);
   Stat* stats = static_cast<Stat*>(ws);
   const int n = slices(n_rows, vocab), per = ((vocab + kChunk - 1) / kChunk + kDrawCtas - 1) / kDrawCtas, smem = per * kChunk * 2;
   static bool done[64] = {};

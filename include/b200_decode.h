@@ -308,7 +308,7 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * index), and the token is the argmax.  A draft outside [0, vocab) is refused; a row of nothing but -inf refuses and yields token 0.
  * uniforms [n_rows][2] in [0, 1).  out_tokens[n_rows]: per sequence the kept drafts, the drawn token, then -1; out_accepted[s]:
  * drafts kept.  A sequence without rows gets out_accepted 0; rows of no sequence stay as they are.  Temperatures below 1e-30
- * and above 1e30 count as those.  At most 65535 rows of 393216 entries (B200_ERR_UNSUPPORTED). */
+ * and above 1e30 count as those.  At most 65535 rows of 393216 entries, 2^28 - 1 sequences (B200_ERR_UNSUPPORTED). */
 B200_API int b200_rope_kv_append_fp8(const void* qkv, int64_t ld, const int32_t* positions, const int32_t* slot_mapping,
                             const void* cos_sin, void* q_out, int64_t ldq, void* k_codes, void* v_codes, void* k_exps,
                             void* v_exps, int64_t n_blocks, int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads,

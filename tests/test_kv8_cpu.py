@@ -160,3 +160,9 @@ def test_attention_counts_tokens_in_32_bits(prefill, stride, block):
     """One row and one kv head: few enough tiles, but a table of more tokens than the kernels can count to the end of the last tile."""
     assert _attend(prefill, T=1, hq=1, hkv=1, stride=stride, block=block) == -3
     assert b"tokens" in _lib().b200_last_error()
+
+
+@pytest.mark.parametrize("S", [2 ** 28, 2 ** 29 + 1, 2 ** 31 - 1])
+def test_verify_counts_its_clusters_in_32_bits(S):
+    """Eight CTAs a sequence: of more sequences only some would be looked at (2^29 + 1: one)."""
+    assert _verify(S=S) == -3 and b"sequences" in _lib().b200_last_error()
