@@ -152,8 +152,8 @@ verify_stats_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const
 // -2^128 times that: nothing beside any logit that counts)
 __device__ __forceinline__ double scaled_double(uint32_t f) { return __hiloint2double((int)f >> 3 & (int)0x8fffffffu, 0); }
 __device__ __forceinline__ double scaled_double(float x) { return scaled_double(__float_as_uint(x)); }
-constexpr double kScaledBack = 0x1p896, kLeastPower = -1017.0;
-// 2^t for t <= 0, 2^kLeastPower below that: t = n / 32 + r, 2^(n / 32) = 2^(n >> 5) table[n & 31], 2^r = 1 + r q(r), |r| <= 1 / 64: the series of (2^r - 1) / r
+constexpr double kScaledBack = 0x1p896;
+// 2^t for t <= 0, 2^-1017 below that: t = n / 32 + r, 2^(n / 32) = 2^(n >> 5) table[n & 31], 2^r = 1 + r q(r), |r| <= 1 / 64: the series of (2^r - 1) / r
 // with its terms above the third taken down to a cubic by Chebyshev polynomials, 1.6e-13 of 2^r
 __device__ __forceinline__ double exp2_table(double t, const double* table) {
   t = __hiloint2double((int)min((uint32_t)__double2hiint(t), 0xc08fc800u), __double2loint(t));
@@ -219,11 +219,8 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
   };
   // the sums of a row's target over its draft, each relative to its largest logit, as near as fp32 has them
   auto ratio = [&](const double (&z)[2]) { return z[1] > 0.0 ? z[0] / z[1] : 0.0; };
-  // the probability of an entry (its bits) of a row; what 2^t has no number for is none
-  auto probability = [&](uint32_t bits, float m, double z) {
-    const double t = ((double)__uint_as_float(bits << 16) - (double)m) * cf;
-    return t > kLeastPower ? exp2_table(t, table) / z : 0.0;
-  };
+  // the probability of an entry (its bits) of a row, down to the least number there is (the table's powers end before)
+  auto probability = [&](uint32_t bits, float m, double z) { return exp2(((double)__uint_as_float(bits << 16) - (double)m) * cf) / z; };
   // a warp a row: is the draft refused?
   for (int r = r0 + warp; r < r1; r += kDrawThreads / 32) {
     double z[2];

@@ -1138,3 +1138,21 @@ def test_an_item_whose_values_drift_apart(hq, hkv, most, parts, before, at):
     scale([at] * len(parts), -30)
     scale([n + b - 1 for n, b in zip(parts, before)], 30)
     check()
+
+
+def test_drafts_of_the_least_probabilities():
+    """Probabilities below the powers of the draw's table, and below any number: kept where the drafter gives the draft still less, refused where it gives more."""
+    V = 50
+    target, draft = torch.full((2 * 6, V), -3000.0).to(BF), torch.full((2 * 6, V), -3000.0).to(BF)
+    for x in (target, draft):
+        x[:, 0] = 0.0
+        x[1::2, 3] = 1.0
+    sizes = [(-720.0, -900.0), (-900.0, -720.0), (-720.0, -732.0), (-732.0, -720.0), (-704.0, -710.0), (-2000.0, -1500.0)]
+    for s, (p, q) in enumerate(sizes):
+        target[2 * s, 7], draft[2 * s, 7] = p, q
+    tokens, starts, temperature = torch.full((12,), 7), list(range(0, 13, 2)), torch.ones(6)
+    uniforms = torch.full((12, 2), 0.5)
+    want, kept, _ = K.verify(target, draft, tokens, starts, temperature, uniforms)
+    assert kept.tolist() == [1, 0, 1, 0, 1, 0]
+    got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts, temperature, uniforms)
+    assert torch.equal(got[1], kept) and torch.equal(got[0], want)
