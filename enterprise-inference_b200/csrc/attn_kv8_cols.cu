@@ -56,14 +56,26 @@ struct Cols {
   static_assert(kSmem + 8 * (kThreads + kThreads / 32) <= 232448, "shared memory");
 };
 
-// group i: of the plan, or the one that starts at row i
-__device__ __forceinline__ Kv8Group find_group(const Kv8Params& p, int i) {
-  if (p.groups) return p.groups[i];
+// the first row of row i's run: few loads where runs are as short as the caller said, eight at a time where they are longer
+__device__ __forceinline__ int run_start(const Kv8Params& p, int i) {
+  const int seq = __ldg(p.row_to_seq + i);
+  while (i > 0 && __ldg(p.row_to_seq + i - 1) == seq) {
+    --i;
+    if (i < 8) continue;
+    bool same = true;
+#pragma unroll
+    for (int j = 1; j <= 8; ++j) same &= __ldg(p.row_to_seq + i - j) == seq;
+    if (same) i -= 8;
+  }
+  return i;
+}
+// group i: of the plan, or (RUNS) the one that starts at row i (start: the first row of its run), or row i
+template <bool RUNS>
+__device__ __forceinline__ Kv8Group find_group(const Kv8Params& p, int i, int start) {
+  if (!RUNS && p.groups) return p.groups[i];
   Kv8Group g = {i, 1, p.row_to_seq ? __ldg(p.row_to_seq + i) : i, kv8_ctx(p, i)};
-  if (p.group_rows == 1 || !p.row_to_seq) return g;
-  int before = 0;   // rows of the sequence in front of this one
-  while (i - before > 0 && __ldg(p.row_to_seq + i - before - 1) == g.seq) ++before;
-  if (before % p.group_rows) {
+  if constexpr (!RUNS) return g;
+  if ((i - start) % p.group_rows) {
     g.nrows = g.ctx = 0;
     return g;
   }
@@ -72,7 +84,8 @@ __device__ __forceinline__ Kv8Group find_group(const Kv8Params& p, int i) {
 }
 __device__ __forceinline__ int group_tiles(const Kv8Group& g) { return g.nrows > 0 && g.ctx > 0 ? (g.ctx + kKv8Tile - 1) / kKv8Tile : 0; }
 
-template <int NC>
+// RUNS: runs of rows are found among the rows (at most group_rows to a group)
+template <int NC, bool RUNS>
 __global__ void __launch_bounds__(Cols<NC>::kThreads, 1)
 kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   using C = Cols<NC>;
@@ -137,10 +150,14 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   // ---- the CTA's share of the tiles: a thread counts its groups' (32 bits hold them: the host's check) ----
   const int n_groups = p.groups ? p.groups[-1].row0 : p.T, each = (n_groups + kThreads - 1) / kThreads;
   const int g0 = min((int)threadIdx.x * each, n_groups), g1 = min(g0 + each, n_groups);
+  const int start0 = RUNS && g0 < g1 ? run_start(p, g0) : g0;
+  auto next_start = [&](int start, int i) { return RUNS && i > g0 && __ldg(p.row_to_seq + i) != __ldg(p.row_to_seq + i - 1) ? i : start; };
   Kv8Group own = {0, 0, 0, 0};
   uint64_t sum = 0;   // groups that see something << 32 | their tiles
-  for (int i = g0; i < g1; ++i) {
-    own = find_group(p, i);
+#pragma unroll 1
+  for (int i = g0, start = start0; i < g1; ++i) {
+    start = next_start(start, i);
+    own = find_group<RUNS>(p, i, start);
     const uint32_t nt = group_tiles(own);
     sum += (uint64_t)(nt > 0) << 32 | nt;
   }
@@ -168,8 +185,10 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   // the groups of this thread that the share touches: f(group, its first tile, tiles of a head, items in front of it)
   auto own_groups = [&](auto f) {
     uint64_t at = scan_thread[threadIdx.x];
-    for (int i = g0; i < g1; ++i) {
-      const Kv8Group g = each == 1 ? own : find_group(p, i);
+#pragma unroll 1
+    for (int i = g0, start = start0; i < g1; ++i) {
+      start = next_start(start, i);
+      const Kv8Group g = each == 1 ? own : find_group<RUNS>(p, i, start);
       const uint32_t nt = group_tiles(g), base = (uint32_t)at * p.hkv;
       if (nt > 0 && base < end && base + nt * p.hkv > begin) f(g, base, nt, (int)(at >> 32) * p.hkv);
       at += (uint64_t)(nt > 0) << 32 | nt;
@@ -594,11 +613,11 @@ kv8_cols_kernel(const __grid_constant__ Kv8Maps maps, const Kv8Params p) {
   }
 }
 
-template <int NC>
+template <int NC, bool RUNS>
 int launch_cols(const Kv8Maps& m, const Kv8Params& p, int grid, cudaStream_t s) {
   static bool done[64] = {};
-  B200_CUDA(ensure_dynamic_smem(kv8_cols_kernel<NC>, Cols<NC>::kSmem, done));
-  B200_CUDA(launch(kv8_cols_kernel<NC>, dim3(grid), dim3(Cols<NC>::kThreads), (size_t)Cols<NC>::kSmem, s, m, p));
+  B200_CUDA(ensure_dynamic_smem(kv8_cols_kernel<NC, RUNS>, Cols<NC>::kSmem, done));
+  B200_CUDA(launch(kv8_cols_kernel<NC, RUNS>, dim3(grid), dim3(Cols<NC>::kThreads), (size_t)Cols<NC>::kSmem, s, m, p));
   return B200_OK;
 }
 
@@ -606,10 +625,15 @@ int launch_cols(const Kv8Maps& m, const Kv8Params& p, int grid, cudaStream_t s) 
 
 int kv8_cols_launch(const Kv8Maps& m, const Kv8Params& p, int cols, int grid, cudaStream_t s) {
   if (const int e = wait_status()) return e;
-  if (cols <= 2) return launch_cols<2>(m, p, grid, s);
-  if (cols <= 4) return launch_cols<4>(m, p, grid, s);
-  if (cols <= 8) return launch_cols<8>(m, p, grid, s);
-  return launch_cols<16>(m, p, grid, s);
+  if (!p.groups && p.group_rows > 1 && p.row_to_seq) {   // (of at most eight pairs)
+    if (cols <= 2) return launch_cols<2, true>(m, p, grid, s);
+    if (cols <= 4) return launch_cols<4, true>(m, p, grid, s);
+    return launch_cols<8, true>(m, p, grid, s);
+  }
+  if (cols <= 2) return launch_cols<2, false>(m, p, grid, s);
+  if (cols <= 4) return launch_cols<4, false>(m, p, grid, s);
+  if (cols <= 8) return launch_cols<8, false>(m, p, grid, s);
+  return launch_cols<16, false>(m, p, grid, s);
 }
 
 }  // namespace b200

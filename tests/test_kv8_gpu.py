@@ -1156,3 +1156,27 @@ def test_drafts_of_the_least_probabilities():
     assert kept.tolist() == [1, 0, 1, 0, 1, 0]
     got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts, temperature, uniforms)
     assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("most", [2, 3])
+def test_runs_far_longer_than_their_bound(most):
+    """16384 rows of two sequences whose caller said two or three: attended in groups of so many, in milliseconds (a sample of the rows is looked at)."""
+    hq, hkv = 4, 2
+    g = torch.Generator().manual_seed(83)
+    seq = [0] * 16000 + [1] * 384
+    ctx = [1 + (i * 7) % 300 for i in range(16384)]
+    cache = K.Cache([300, 300], hkv, 128, g)
+    q = _rows(16384, hq, g)
+    qd, out = _on_device(q), torch.full((16384, hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    sd, cd = torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV)
+    ws = attend(qd, cache, sd, cd, out, hq, most)
+    begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+    torch.cuda.synchronize()
+    begin.record()
+    attend(qd, cache, sd, cd, out, hq, most, ws=ws, stream=torch.cuda.current_stream().cuda_stream)
+    end.record()
+    torch.cuda.synchronize()
+    assert begin.elapsed_time(end) < 100   # (with a walk to the start of the run from every row: seconds)
+    some = list(range(0, 16384, 331)) + [15998, 15999, 16000, 16001, 16382, 16383]
+    check_attention(out.reshape(16384, hq, 128)[some], q[some], cache, [seq[t] for t in some], [ctx[t] for t in some])
