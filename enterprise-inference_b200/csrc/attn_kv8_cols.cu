@@ -14,10 +14,10 @@
 // The flattened list of (group, kv head, tile) is cut into equal shares, one per SM: contexts may differ as they like.  An item that a cut goes through
 // leaves its sums as parts, joined by the next launch.
 //
-// Bound by the cache's bytes, 258 a token and kv head, where contexts are long: 8 rows of 32 k tokens, 64 heads over 8, 76 us, 5.1 TB/s.  A tile takes 1050 to 1300
+// Bound by the cache's bytes, 258 a token and kv head, where contexts are long: 8 rows of 32 k tokens, 64 heads over 8, 77 us, 5.0 TB/s.  A tile takes 1050 to 1300
 // cycles there (the bytes alone 1020): the softmax warps' chain of scores, maximum, weights, and 950 for the warp that issues the MMAs.  In front of it 9000 cycles until the
 // first load is asked for (groups, shares, table; much of it instructions fetched for the first time), and 2000 for every item that ends: 64 rows of 500 to
-// 1000 tokens 32 us, 3.1 TB/s.
+// 1000 tokens 34.5 us, 2.9 TB/s.
 #include <algorithm>
 
 #include "attn_kv8.cuh"

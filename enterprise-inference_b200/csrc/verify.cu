@@ -3,13 +3,14 @@
 // stats: a CTA takes a slice of a logit row (target rows, and the rows that drafts were drawn from) and leaves its largest logit m, the first place of it and the sum
 // of 2^((l - m) c), c = log2e / T, in fp32 on the hardware's exponential: enough for a draft's limit u q(x) < p(x).  The difference of two logits is exact, or
 // rounded once, and never above zero, whatever the temperature: l c by itself has no bits left for its fraction where T is small.  A thread compares 32 entries with its maximum at once; the place is looked for at the end, by the threads that met the CTA's
-// largest (with a place kept by every thread the same took 23.5 million instructions for 64 x 5 drafts over 128256 entries, this 15.2).  35 us there, 4.2 TB/s;
+// largest (with a place kept by every thread the same took 23.5 million instructions for 64 x 5 drafts over 128256 entries, this 15.2; differences and products in place of one
+// fused operation made them 16.1, in the same time).  35 us there, 4.2 TB/s;
 // bound by the exponentials (four a cycle and quarter of an SM: 16 us) and the latency of short loops.
 // draw: a cluster of eight CTAs takes a sequence: the kept drafts from the slices' sums, then the token from the one row that draws it.  A draw next to a border of
 // the cumulated weights has to come out as in exact arithmetic (128 k borders: sums that are off by 1e-9 pick another token once in 4000 draws), so weights and
-// sums are fp64 there: 2^t by a table of 32 powers and a cubic, relative error below 2e-13, nine fp64 operations a weight (16 powers and a degree of 5, with selects for
+// sums are fp64 there: 2^t by a table of 32 powers and a cubic, relative error below 2e-13, ten fp64 operations a weight (16 powers and a degree of 5, with selects for
 // masked entries: 45 instructions a weight in all and 49 us, this 30 and 40).  Each CTA owns an eighth of the row in chunks of 256 entries, the target's fetched once
-// into shared memory; sums are taken in a fixed order, chunk by chunk.  Bound by the instructions of the weights: 26 thousand a quarter of an SM.
+// into shared memory; sums are taken in a fixed order, chunk by chunk.  Bound by the instructions of the weights: 27 thousand a quarter of an SM.
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -275,7 +275,7 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  * smallest e >= -100 with max |x| <= 448 * 2^e (every value is an exact bf16; relative error of a normal code at most
  * 2^-4).  Byte 255: the row held an inf or a NaN; its codes are NaN, and of such rows alone.  Byte 0 stands for nothing (a
  * caller that writes a cache of its own), bytes from 1 to 26 may count as nothing.  129 bytes a row where bf16 takes 256.
- * block_size is 16, 32, 64 or a multiple of 128; n_blocks * n_kv_heads * block_size < 2^31.  Codes are 16-byte aligned.
+ * block_size is 16, 32, 64 or a multiple of 128; n_blocks * n_kv_heads * block_size < 2^31.  Codes, and for attention exponents, are 16-byte aligned.
  *
  * (a4+a5) b200_rope_kv_append_fp8: NeoX RoPE of the q and k heads of qkv [T][ld] in fp32 with one rounding (where
  * b200_rope_kv_append follows the image's bf16 arithmetic); q rows go to q_out [T][ldq] (which may be qkv itself: q is then
