@@ -1180,3 +1180,35 @@ def test_runs_far_longer_than_their_bound(most):
     assert begin.elapsed_time(end) < 100   # (with a walk to the start of the run from every row: seconds)
     some = list(range(0, 16384, 331)) + [15998, 15999, 16000, 16001, 16382, 16383]
     check_attention(out.reshape(16384, hq, 128)[some], q[some], cache, [seq[t] for t in some], [ctx[t] for t in some])
+
+
+def test_idle_sequences_cost_little():
+    """Ten sequences of nine rows by themselves, and among 500 idle ones: zeros for rows that see nothing come from many CTAs (from one: ten times as long)."""
+    hq, hkv, each, g = 32, 8, 9, torch.Generator().manual_seed(90)
+    cache = K.Cache([1000], hkv, 128, g)
+    times = []
+    for n in (10, 510):
+        T = n * each
+        cache.bt = cache.bt.cpu()[:1].repeat(n, 1).contiguous()
+        cache.to(DEV)
+        seq, place = torch.arange(n).repeat_interleave(each), torch.arange(T) % each
+        ctx = torch.where(seq < 10, 900 + place, 0)
+        sd, cd, qd = seq.to(I32).to(DEV), ctx.to(I32).to(DEV), _on_device(_rows(T, hq, g))
+        out = torch.full((T, hq * 128), float("nan"), dtype=BF, device=DEV)
+        ws = attend(qd, cache, sd, cd, out, hq, each)
+        torch.cuda.synchronize()
+        assert not bool(out[10 * each:].any())
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            for _ in range(20):
+                attend(qd, cache, sd, cd, out, hq, each, ws=ws, stream=torch.cuda.current_stream().cuda_stream)
+        took = []
+        for _ in range(7):
+            begin, end = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            begin.record()
+            graph.replay()
+            end.record()
+            torch.cuda.synchronize()
+            took.append(begin.elapsed_time(end))
+        times.append(sorted(took)[3])
+    assert times[1] < 5 * times[0], times
