@@ -167,7 +167,9 @@ __device__ __forceinline__ double exp2_table(double t, const double* table) {
   const double b = table[n & 31], e = fma(b * r, q, b);
   return __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
 }
-constexpr double kNothing = 1e-300;   // what 2^t gives for a masked entry, and no weight that counts, is below
+// what 2^t gives for a masked entry, 7.2e-307, is no weight, nor is a row's sum of them; a sum that is one (of kMostVocab entries at most) has an entry that is
+constexpr double kLeastWeight = 1e-306, kNothing = 1e-300;
+static_assert(kMostVocab * 7.2e-307 < kNothing && kMostVocab * kLeastWeight < kNothing, "weights");
 __device__ __forceinline__ double warp_sum_double(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -425,7 +427,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           front += w[j];
-          if (w[j] > kNothing) {
+          if (w[j] > kLeastWeight) {
             some = i + j;
             if (front > limit && token == 0x7fffffff) token = i + j;
           }

@@ -1212,3 +1212,24 @@ def test_idle_sequences_cost_little():
             took.append(begin.elapsed_time(end))
         times.append(sorted(took)[3])
     assert times[1] < 5 * times[0], times
+
+
+def test_leftovers_of_the_least_weights():
+    """What a refused draft leaves is more than nothing (1e-300) as a sum, and each of its entries is less: one of them is drawn.  Where the sum is less, too, the draw
+    is the target's own (bf16 has -696 for -694: 100 entries of 5.3e-303)."""
+    V = 400
+    target, draft = torch.full((6, V), -3000.0).to(BF), torch.full((6, V), -3000.0).to(BF)
+    target[:, 0], draft[:, 0] = 0.0, 0.0
+    target[0, 100:200] = -694.0
+    target[2, 10:400:2] = -696.0                 # 195 entries: 1.04e-300
+    target[4, 100:200] = -692.0                  # 100 of 2.9e-301
+    draft[::2, 7] = -600.0                       # the drafts: the target gives them less
+    tokens, temperature, starts = torch.full((6,), 7), torch.ones(3), [0, 2, 4, 6]
+    for u in (0.0, 0.505, 0.9999):
+        uniforms = torch.full((6, 2), u)
+        uniforms[:, 0] = 0.5
+        want, kept, _ = K.verify(target, draft, tokens, starts, temperature, uniforms)
+        assert kept.tolist() == [0, 0, 0] and 100 <= int(want[4]) < 200
+        want[0] = 0                              # (the plain form's nothing is 0)
+        got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts, temperature, uniforms)
+        assert torch.equal(got[1], kept) and torch.equal(got[0], want)
