@@ -167,9 +167,9 @@ __device__ __forceinline__ double exp2_table(double t, const double* table) {
   const double b = table[n & 31], e = fma(b * r, q, b);
   return __hiloint2double(__double2hiint(e) + ((n & ~31) << 15), __double2loint(e));
 }
-// what 2^t gives for a masked entry, 7.2e-307, is no weight, nor is a row's sum of them; a sum that is one (of kMostVocab entries at most) has an entry that is
-constexpr double kLeastWeight = 1e-306, kNothing = 1e-300;
-static_assert(kMostVocab * 7.2e-307 < kNothing && kMostVocab * kLeastWeight < kNothing, "weights");
+// what 2^t gives for a masked entry, 7.2e-307, is no weight, nor is a chunk's sum of them: a chunk whose sum is one has an entry that is, a row whose sum is one a chunk
+constexpr double kLeastWeight = 1e-306, kLeastChunk = kChunk * kLeastWeight, kNothing = 1e-300;
+static_assert(kDrawCtas * kMostChunks * kLeastChunk < kNothing, "weights");
 __device__ __forceinline__ double warp_sum_double(double v) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -386,7 +386,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
         t = warp_sum_double(((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])));
       }
       __syncwarp();
-      if (lane == 0) chunk_sum[ch - ch0] = t;
+      if (lane == 0) chunk_sum[ch - ch0] = t > kLeastChunk ? t : 0.0;   // (a draw of 0 takes the first chunk that is not 0)
     }
     __syncthreads();
     if (warp == 0) {
@@ -434,7 +434,7 @@ verify_draw_kernel(const __nv_bfloat16* __restrict__ target, int64_t ldt, const 
         }
         token = __reduce_min_sync(0xffffffffu, token);
         some = __reduce_max_sync(0xffffffffu, some);
-        if (lane == 0) out[row] = token == 0x7fffffff ? some : token;
+        if (lane == 0 && some >= 0) out[row] = token == 0x7fffffff ? some : token;   // (a chunk that only rounding let through: the largest entry stays)
       }
     }
     break;

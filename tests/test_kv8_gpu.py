@@ -1233,3 +1233,27 @@ def test_leftovers_of_the_least_weights():
         want[0] = 0                              # (the plain form's nothing is 0)
         got = check_drafts(target.to(DEV), draft.to(DEV), tokens, starts, temperature, uniforms)
         assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("V", [700, 5000, 128256])
+@pytest.mark.parametrize("probs", [True, False])
+def test_draws_of_zero_over_masked_entries(V, probs):
+    """The least uniform number picks the first entry of any probability, however many masked ones lie in front of it: behind a last draft and for refused ones, few
+    entries left or many."""
+    g = torch.Generator().manual_seed(V)
+    parts = [1, 2, 3, 1, 2, 4]
+    target, draft, tokens, starts = _drafts(parts, V, g)
+    for x in (target, draft):
+        for r, lead in enumerate((256, 300, 699, 257, 640, 1, 255, 256, 512, 698, 300, 256, 690)):
+            x[r, :lead] = float("-inf") if r % 3 else -1e5
+    for r, keep in ((2, 3), (4, 5), (8, 2), (12, 4)):   # filtered down to a few
+        rest = torch.ones(V, dtype=torch.bool)
+        rest[torch.randperm(V - 690, generator=g)[:keep] + 690] = False
+        target[r, rest], draft[r, rest] = float("-inf"), float("-inf")
+    uniforms = torch.zeros(13, 2)
+    uniforms[:, 0] = torch.tensor([0.0, 0.999, 0.999, 0.0, 0.0, 0.999, 0.0, 0.999, 0.0, 0.0, 0.0, 0.999, 0.0])
+    d = draft if probs else None
+    for temp in (1.0, 0.3, 50.0):
+        want, kept, margins = K.verify(target, d, tokens, starts, torch.full((6,), temp), uniforms)
+        got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, torch.full((6,), temp), uniforms)
+        assert torch.equal(got[1], kept) and torch.equal(got[0], want)
