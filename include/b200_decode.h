@@ -303,7 +303,7 @@ B200_API int b200_paged_attn_decode_static(const void* q, int64_t ldq, const voi
  *   draft x is kept while uniforms[r][0] * q(x) < p(x) (sums of fp32 exponentials, good to about 1e-6); the first row r that
  *   is not, or the last one, draws the token
  *   min { i : sum over j <= i of w_j > uniforms[r][1] * sum of w },  w = max(p - q, 0) for a refused draft (p where that
- *   leaves less than 1e-300), p behind the last one; sums in 64 bits.
+ *   leaves less than 1e-300), p behind the last one; sums in 64 bits, entries below 1e-300 count as none.
  * temperature[s] <= 0 (or temperature NULL, uniforms then unused): a draft is kept if it is the row's argmax (ties: the lowest
  * index), and the token is the argmax.  A draft outside [0, vocab) is refused; a row of nothing but -inf refuses and yields token 0.
  * uniforms [n_rows][2] in [0, 1).  out_tokens[n_rows]: per sequence the kept drafts, the drawn token, then -1; out_accepted[s]:

@@ -1257,3 +1257,40 @@ def test_draws_of_zero_over_masked_entries(V, probs):
         want, kept, margins = K.verify(target, d, tokens, starts, torch.full((6,), temp), uniforms)
         got = check_drafts(target.to(DEV), None if d is None else d.to(DEV), tokens, starts, torch.full((6,), temp), uniforms)
         assert torch.equal(got[1], kept) and torch.equal(got[0], want)
+
+
+@pytest.mark.parametrize("power", [0, 40])
+@pytest.mark.parametrize("name", sorted(WIDE_STEPS))
+def test_what_is_not_a_number_stays_with_its_rows(name, power):
+    """Queries with NaN or inf, keys and values that are not numbers, with values of one size and far apart: rows and heads that do not meet them are what they are."""
+    hq, hkv, most, parts, before = WIDE_STEPS[name]
+    seq, ctx = _step(parts, before)
+    g = torch.Generator().manual_seed(74)
+    cache = K.Cache([n + b for n, b in zip(parts, before)], hkv, 64, g, spread=0.5)
+    q = _rows(len(seq), hq, g)
+    bad_q = {1: float("nan"), len(seq) - 2: float("inf"), len(seq) // 2: float("-inf")}
+    for t, v in bad_q.items():
+        q[t, t % hq, 5] = v
+    s = len(parts) - 1                                     # of the last sequence: a key row, in front of the last two rows, and a value row behind it
+    n = parts[s] + before[s]
+    for at, (c, e) in ((n - 3, (cache.k, cache.ke)), (n - 1, (cache.v, cache.ve))):
+        blk = int(cache.bt[s, at // 64])
+        c[blk, :, at % 64], e[blk, :, at % 64] = 0x7f, 255
+    if power:
+        for s2, (a, b) in enumerate(zip(parts, before)):
+            _scale_values(cache, s2, (a + b) // 2, power)
+    qd, out = _on_device(q), torch.full((len(seq), hq * 128), float("nan"), dtype=BF, device=DEV)
+    cache.to(DEV)
+    attend(qd, cache, torch.tensor(seq, dtype=I32, device=DEV), torch.tensor(ctx, dtype=I32, device=DEV), out, hq, most)
+    torch.cuda.synchronize()
+    got = out.reshape(len(seq), hq, 128)
+    sees = [seq[t] == s and ctx[t] > n - 3 for t in range(len(seq))]
+    bad = torch.isnan(got).any(-1).cpu()
+    want = torch.zeros_like(bad)
+    for t in range(len(seq)):
+        want[t] = sees[t]
+    for t in bad_q:
+        want[t, t % hq] = True
+    assert torch.equal(bad, want) and bool(torch.isnan(got.cpu()[want]).all())
+    fine = [t for t in range(len(seq)) if not sees[t] and t not in bad_q][::3]
+    check_shares(got[fine], q[fine], cache, [seq[t] for t in fine], [ctx[t] for t in fine])
