@@ -123,6 +123,12 @@ SIGNATURES = {
                                               _vp, _i64, _vp]),
     "b200_verify_drafts_workspace_bytes": (_i64, [_i32, _i32]),
     "b200_verify_drafts": (C.c_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _i64, _vp]),
+    "b200_paged_attn_tree_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "b200_paged_attn_tree": (C.c_int, [_vp, _i64, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _vp, _i64, _vp]),
+    "b200_beam_select_workspace_bytes": (_i64, [_i32, _i32, _i32]),
+    "b200_beam_select": (C.c_int, [_vp, _i64, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _i64, _vp]),
+    "b200_accept_tree": (C.c_int, [_vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "b200_cache_move": (C.c_int, [_vp, _vp, _i32, _i64, _i64, _i32, _i32, _i64, _vp, _vp, _vp, _i32, _i32, _vp]),
     "b200_silu_mul": (C.c_int, [_vp, _vp, _i32, _i32, _vp]),
     "b200_argmax": (C.c_int, [_vp, _i64, _i32, _i32, _i32, _vp, _vp, _vp]),
     "b200_sample": (C.c_int, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

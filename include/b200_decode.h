@@ -330,6 +330,55 @@ B200_API int b200_verify_drafts(const void* target_logits, int64_t ldt, const vo
                        const float* uniforms, int32_t n_seqs, int32_t n_rows, int32_t vocab, int32_t* out_tokens,
                        int32_t* out_accepted, void* workspace, int64_t workspace_bytes, void* stream);
 
+/* ---- several continuations of a sequence: trees of drafted tokens, beams ---------------------------------------------
+ * A sequence's continuations lie in its cache behind the tokens that they share, in any order, and every row says by a mask which of them it sees.
+ *
+ * (a6) b200_paged_attn_tree: attention of rows t over the paged bf16 cache of a layer, [n_blocks][n_kv_heads][block_size][128] each for keys and values.  Row t sees
+ * the tokens of its sequence in front of ctx_lens[t], and token ctx_lens[t] + 32 w + b for each bit b of tree_masks[t][w] (uint32 [n_tokens][mask_words], up to 32 words; with
+ * none, or NULL and 0, this is attention over contexts): a drafted node its way up to the root, itself included; a beam the tokens that it chose.  Tokens
+ * behind the bt_stride blocks of a block table do not exist; a row that sees none gives zeros; contexts below 0 count as 0.  What stands in a token that a row does not see is
+ * never part of its result (an inf or a NaN there included); a block id outside [0, n_blocks) stands for keys and values of zero.  Rows of one sequence that follow one another
+ * (row_to_seq; NULL: row t is sequence t) share its keys and values, whatever their contexts.  Up to 16 query heads to a kv head; block_size 16, 32, 64 or a multiple
+ * of 128; n_blocks * n_kv_heads * block_size and a block table's tokens below 2^31 - 256; scale > 0.  Scores, softmax and sums in fp32, weights of 16 bits, one rounding.  The workspace has
+ * no state between calls; calls that may run at the same time, two captured graphs among them, need one each.
+ *
+ * b200_beam_select: the n_select best continuations of a sequence's beams.  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1 of logits (bf16
+ * [n_rows][ld]); with scores[r] a beam's sum of log-probabilities (NULL: zeros),
+ *   score(r, i) = scores[r] + logits[r][i] - log sum over j of exp logits[r][j],
+ * in 64 bits where two candidates are near each other; out_rows, out_tokens, out_scores [n_seqs][n_select] (int32, int32, fp32) hold the rows (0 .. n_rows-1), entries and scores of
+ * the best, the best first; alike scores: the lower row, then the larger logit, then the lower entry.  Logits of -inf are no candidates, nor is any entry of a row whose score or log-sum is not finite (a
+ * beam that has ended: -inf; a NaN or +inf among its logits).  Where candidates run out, row and token are -1 and the score is -inf.  At most 128 to select, 65535 rows of 393216
+ * entries, 2^28 - 1 sequences (B200_ERR_UNSUPPORTED).  The workspace has no state between calls; one for many rows does for fewer.
+ *
+ * b200_accept_tree: the way through a checked tree.  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1: first its root (the last token that is certain), then drafted
+ * nodes; parents[r] is the place of a node's parent in its sequence's rows (0: the root), in front of its own; the root's is not read.  target_tokens[r] is what the target chose behind
+ * row r (b200_argmax or b200_sample of its logits: what is kept is distributed as the target's own draws).  From the root on, the first child whose draft is
+ * the target's choice is taken.  out_tokens[n_rows]: per sequence the tokens chosen on that way (the kept drafts, then the token behind the last of them), then -1; out_rows[n_rows]:
+ * the rows on it, the root's first, then -1; out_accepted[s]: drafts kept (0 for a sequence without rows).  With slot_mapping (the cache slots of the rows; else NULL, as
+ * move_src and move_dst): move_src, move_dst [n_rows] are the moves that bring the kept rows' keys and values to the slots of their sequence's first rows, -1 where there is nothing
+ * to move.  Rows of no sequence stay as they are.
+ *
+ * b200_cache_move: rows of caches, whole blocks or states to new places.  cache_a and cache_b (or NULL) each are n_layers times, layer_stride bytes apart,
+ * [n_blocks][heads][block_size][row_bytes]; slot = block * block_size + place, as in slot_mapping.  The moves of group g, src_slots[i] -> dst_slots[i] for group_starts[g] <= i <
+ * group_starts[g+1], happen at once in all layers, heads and both caches: what is read is what stood there before the call, so beams may change places.  A move with a slot outside the
+ * cache is none.  Destinations of one call differ, and no group reads what another one writes.  Groups have at most max_group moves (a HOST bound up to 1024; those behind
+ * it are not made).  States, or blocks as a whole: heads = block_size = 1 and row_bytes their size.  Fastest where addresses, strides and row_bytes are multiples of 16. */
+B200_API int64_t b200_paged_attn_tree_workspace_bytes(int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads);
+B200_API int b200_paged_attn_tree(const void* q, int64_t ldq, const void* k_cache_layer, const void* v_cache_layer, int64_t n_blocks,
+                         const int32_t* block_table, int32_t bt_stride, const int32_t* row_to_seq, const int32_t* ctx_lens,
+                         const uint32_t* tree_masks, int32_t mask_words, void* out, int64_t ldo, int32_t n_tokens, int32_t n_q_heads,
+                         int32_t n_kv_heads, int32_t block_size, float scale, void* workspace, int64_t workspace_bytes, void* stream);
+B200_API int64_t b200_beam_select_workspace_bytes(int32_t n_rows, int32_t vocab, int32_t n_select);
+B200_API int b200_beam_select(const void* logits, int64_t ld, const float* scores, const int32_t* row_starts, int32_t n_seqs, int32_t n_rows,
+                     int32_t vocab, int32_t n_select, int32_t* out_rows, int32_t* out_tokens, float* out_scores, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+B200_API int b200_accept_tree(const int32_t* target_tokens, const int32_t* draft_tokens, const int32_t* parents, const int32_t* row_starts,
+                     const int32_t* slot_mapping, int32_t n_seqs, int32_t n_rows, int32_t* out_tokens, int32_t* out_rows,
+                     int32_t* out_accepted, int32_t* move_src, int32_t* move_dst, void* stream);
+B200_API int b200_cache_move(void* cache_a, void* cache_b, int32_t n_layers, int64_t layer_stride, int64_t n_blocks, int32_t heads,
+                    int32_t block_size, int64_t row_bytes, const int32_t* src_slots, const int32_t* dst_slots,
+                    const int32_t* group_starts, int32_t n_groups, int32_t max_group, void* stream);
+
 /* (a8) out[T][I] = bf16(bf16(silu(g))*u), gu = [T][2I] gate|up ([V22] activation.py:137-141). */
 B200_API int b200_silu_mul(const void* gu, void* out, int32_t n_tokens, int32_t intermediate, void* stream);
 
