@@ -62,6 +62,7 @@ struct Kv8QueryMaps {
   CUtensorMap hi, lo;
 };
 int kv8_maps(const Kv8Attn& a, int box_rows, Kv8Maps* m);
+int query_map_bf16(const __nv_bfloat16* q, int T, int hq, int64_t ld, int G, int n, CUtensorMap* m);
 int rows_map_bf16(const __nv_bfloat16* base, int64_t rows, int box_rows, CUtensorMap* m);
 
 int kv8_cols_launch(const Kv8Maps& m, const Kv8Params& p, int cols, int grid, cudaStream_t s);
@@ -122,39 +123,6 @@ __device__ __forceinline__ float warp_max_f32(float v) {
   float m;
   asm volatile("redux.sync.max.NaN.f32 %0, %1, 0xffffffff;" : "=f"(m) : "f"(v));
   return m;
-}
-
-// sums `a`, their maximum (of exponents, which are of base 2 in units of `unit`) and denominator of `parts` parts, one after another `step` floats apart -> out = sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m),
-// by LANES neighbouring lanes.  Eight where an item of 128 pairs has few parts (a warp would wait for its parts four times: 2.5 us more behind 300 rows), a warp where
-// it has many (eight lanes: 1 row over 8000 tokens 21 us instead of 17, 5 rows over 3000 28 instead of 24)
-template <int LANES>
-__device__ __forceinline__ void join_parts(const float* first, const float* rest, int64_t step, int parts, __nv_bfloat16* out, float unit = 1.f) {
-  constexpr int K = 32 / LANES;   // four entries at a time
-  const int lane = threadIdx.x & (LANES - 1);
-  const unsigned group = LANES == 32 ? 0xffffffffu : ((1u << (LANES & 31)) - 1u) << (threadIdx.x & 31 & ~(LANES - 1));
-  auto part = [&](int i) { return i ? rest + (i - 1) * step : first; };
-  float m = -INFINITY, l = 0.f;
-  for (int i = lane; i < parts; i += LANES) m = fmaxf(m, part(i)[128]);
-#pragma unroll
-  for (int o = LANES / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(group, m, o));
-  float4 a[K];
-#pragma unroll
-  for (int k = 0; k < K; ++k) a[k] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll (LANES == 32 ? 4 : 2)
-  for (int i = 0; i < parts; ++i) {
-    const float* x = part(i);
-    const float f = m == -INFINITY ? 1.f : tc::exp2_fast((x[128] - m) * unit);
-    l += x[129] * f;
-#pragma unroll
-    for (int k = 0; k < K; ++k) {
-      const float4 v = reinterpret_cast<const float4*>(x)[lane + LANES * k];
-      a[k].x += v.x * f, a[k].y += v.y * f, a[k].z += v.z * f, a[k].w += v.w * f;
-    }
-  }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll
-  for (int k = 0; k < K; ++k)
-    *reinterpret_cast<uint2*>(out + 4 * (lane + LANES * k)) = make_uint2(pack_bf16(a[k].x * inv, a[k].y * inv), pack_bf16(a[k].z * inv, a[k].w * inv));
 }
 
 namespace tc {

@@ -27,17 +27,18 @@ constexpr int kTrChunk = kTreeKeys * 128;       // [64 keys][64 columns] bf16
 constexpr int kTrTile = 2 * kTrChunk;
 constexpr int kTrStage = 8 * 2048;              // output staging: 2 KiB per softmax warp
 constexpr int kTrBad = 64;                      // tiles of an item for which it is known which keys' values are no numbers
-constexpr int kTrPart = 136;                    // floats of a pair in a part: 128 sums, their maximum (of the products q . k), the denominator; whole sectors
-constexpr int kTrSmem = 1024 + 4 * kTrQChunk + kTreeSlots * kTrTile + kTrStage + 2 * 128 * 8 + 2 * kTrBad * 16 + (2 * kTreeSlots + 16) * 8 + 16;
-static_assert(kTrSmem <= 232448, "shared memory");
-constexpr int kPlanThreads = 1024, kPlanNear = 1024;   // rows of a step whose lists are in shared memory
+constexpr int kTrPart = kHeadDim + 2;           // floats of a pair in a part: sums, their maximum (of the products q . k), the denominator
+constexpr int kTreeTable = 48;                  // units of a CTA in shared memory
+constexpr int kMostRows = 4096;                 // of a step: the plan's lists fit where the tiles come to lie
 
-// what an item's walk over the tiles [tile0, tile1) needs; parts > 1: further CTAs have the rest, each leaves its sums in a slot.  A CTA's items follow one another; cta -1: none
-struct alignas(16) TreeWork {
-  int row0, nrows, seq, clear, end, tile0, tile1, kvh, cta, parts, slot, pad;   // clear, end: tokens that all rows see, up to the last one that any sees
-};
+// rows [row0, row0 + nrows) of one sequence; clear, end: tokens that all of them see, up to the last one that any sees
 struct TreeItem {
   int row0, nrows, seq, clear, end;
+};
+// a CTA's walk over an item's tiles [tile0, tile1) of a kv head; parts > 1: other CTAs have the rest, each leaves its sums in a slot
+struct alignas(16) TreeWork {
+  TreeItem rows;
+  int kvh, tile0, tile1, parts, slot, pad[2];
 };
 
 struct TreeParams {
@@ -50,149 +51,186 @@ struct TreeParams {
   int bt_stride, words, T, hq, hkv, block_size;
   float scale;
   // workspace
-  TreeWork* list;
-  int* starts;           // [CTA] its first place of the list (-1: none)
+  TreeWork* list;        // [item x kv head + CTA] the units of CTAs that have more than kTreeTable
   Kv8Cut* cuts;          // [CTA] its last item, where further CTAs have parts of it
-  float* part;           // [CTA][2][pairs][kTrPart]: of an item that began in an earlier CTA, of one that goes on in the next
-  int pairs;
+  // [CTA][2]: of an item that began in an earlier CTA, of one that goes on in the next.  [32 x 4 columns][pairs][4], then [pairs][maximum, denominator]: neighbouring lanes own
+  // neighbouring pairs (a row to a lane touches 32 lines with every store)
+  float* part;
+  int pairs;             // a multiple of 32
   uint32_t* status;
 };
 
 __host__ __device__ __forceinline__ int64_t tree_tokens(const TreeParams& p) { return (int64_t)p.bt_stride * p.block_size; }
 __device__ __forceinline__ int tree_ctx(const TreeParams& p, int row) { return (int)min((int64_t)max(__ldg(p.ctx_lens + row), 0), tree_tokens(p)); }
 
-// ---- plan -----------------------------------------------------------------------------------------------------------------------------
-// Costs, in units of a key tile with one tile of pairs: with two of them, and of an item's start and end
-constexpr int kCostOne = 2, kCostTwo = 4, kCostItem = 2;
+constexpr int kTrSmem = 1024 + 4 * kTrQChunk + kTreeSlots * kTrTile + kTrStage + 2 * 128 * 8 + 2 * kTrBad * 16 + (2 * kTreeSlots + 16) * 8 + 32 + kTreeTable * (int)sizeof(TreeWork) + 320;
+static_assert(3 * kMostRows * 4 <= kTreeSlots * kTrTile, "the plan's lists");
+static_assert(kTrSmem <= 232448, "shared memory");
 
-__device__ __forceinline__ int64_t scan64(int64_t& x, int64_t* sh) {   // exclusive over the CTA; returns the total
+// ---- plan -----------------------------------------------------------------------------------------------------------------------------
+// Every CTA makes the step's items and finds its own share of them: 1 to 2 us, where a launch before this one took 6 and lists in global memory two more.
+//
+// Units, an item's walk for a kv head, lie one after another on a line of costs, a unit's first tile at its front, tile t at gap + t x its cost behind that; CTA k has the
+// tiles in [k share, (k + 1) share).  A share is no less than the widest distance of neighbouring tiles, so that every CTA between a unit's first and last tile has one of its tiles.
+// Costs in halves of a key tile with one tile of pairs: with one, with two, and of an item's start and end (one tile of pairs 1300 cycles, two 2000).  Where units are few, they
+// start at a CTA's share each (which costs a CTA a unit at most): a CTA with the end of one and the start of another would be 5 000 cycles later than the others.
+constexpr int kCostOne = 2, kCostTwo = 3, kCostItem = 3, kFewUnits = kNumSMs / 4;
+
+struct PlanShared {
+  int64_t sums[2][kTreeThreads / 32];
+  int starts[kTreeThreads / 32], first, units;
+  Kv8Cut cut;
+};
+static_assert(sizeof(PlanShared) <= 320, "shared memory");
+
+// exclusive scan over the CTA (one barrier; `sh` is used once); all: of everything
+template <typename T, typename F>
+__device__ __forceinline__ T plan_scan(T x, T none, F op, T* sh, T& all) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t own = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += u;
+    const T u = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x = op(x, u);
   }
-  __syncthreads();
   if (lane == 31) sh[warp] = x;
+  const T left = __shfl_up_sync(0xffffffffu, x, 1);
   __syncthreads();
-  int64_t w = sh[lane];
+  T before = none;
+  all = none;
 #pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int64_t u = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += u;
+  for (int w = 0; w < kTreeThreads / 32; ++w) {
+    const T t = sh[w];
+    if (w < warp) before = op(before, t);
+    all = op(all, t);
   }
-  const int64_t before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-  x += (warp ? before : 0) - own;
-  return __shfl_sync(0xffffffffu, w, 31);
+  return lane ? op(before, left) : before;
+}
+// x / y for quotients up to a few hundred
+__device__ __forceinline__ int small_quotient(int64_t x, int64_t y) {
+  int q = (int)__fdividef((float)x, (float)y);
+  while (q * y > x) --q;
+  while ((q + 1) * y <= x) ++q;
+  return q;
 }
 
-struct PlanLists {   // of T entries each
-  int *ctx, *end, *runs;
-  TreeItem* items;
-  int64_t* front;
-};
-
-__global__ void __launch_bounds__(kPlanThreads) tree_plan_kernel(const TreeParams p, int R, PlanLists far) {
-  __shared__ int64_t sh[32];
-  __shared__ int near_ctx[kPlanNear], near_end[kPlanNear], near_runs[kPlanNear];
-  __shared__ TreeItem near_items[kPlanNear];
-  __shared__ int64_t near_front[kPlanNear];
-  pdl_wait();
-  pdl_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const bool near = p.T <= kPlanNear;
-  int *const ctx = near ? near_ctx : far.ctx, *const end = near ? near_end : far.end, *const runs = near ? near_runs : far.runs;
-  TreeItem* const items = near ? near_items : far.items;
-  int64_t* const front = near ? near_front : far.front;
-  const int64_t tokens = tree_tokens(p);
+// the CTA's units -> table or, where there are more than it holds, p.list; returns their number, and the place of the first in p.list (-1: in the table)
+__device__ __forceinline__ int2 tree_plan(const TreeParams& p, int R, int cta, int* scratch, PlanShared* sh, TreeWork* table) {
+  int *const clear = scratch, *const end = scratch + kMostRows, *const count = scratch + 2 * kMostRows;   // of the item that starts with a row (count 0: none does)
+  const int tid = threadIdx.x, lane = tid & 31, each_rows = (p.T + kTreeThreads - 1) / kTreeThreads, ra = min(p.T, tid * each_rows), rb = min(p.T, ra + each_rows);
+  const int tokens = (int)tree_tokens(p);
+  for (int r = ra; r < rb; ++r) {   // what is read below
+    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.ctx_lens + r));
+    for (int w = 0; w < p.words; w += 8) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.masks + (int64_t)r * p.words + w));
+  }
   auto seq_of = [&](int r) { return p.row_to_seq ? __ldg(p.row_to_seq + r) : r; };
-  // rows: their context, and the end of what they see; the runs' first rows
-  int n_runs = 0;
-  for (int r0 = 0; r0 < p.T; r0 += kPlanThreads) {
-    const int r = r0 + tid;
-    int64_t at = 0;
-    bool flag = false;
-    if (r < p.T) {
-      const int c = tree_ctx(p, r);
-      int64_t e = c;
+  if (tid == 0) sh->first = 0x7fffffff, sh->units = 0, sh->cut = {0, 0, 0, 0};
+  int start = -1;   // the last row here that starts a run of one sequence
+  for (int r = ra; r < rb; ++r) {
+    clear[r] = 0x7fffffff, end[r] = 0, count[r] = 0;
+    if (r == 0 || seq_of(r) != seq_of(r - 1)) start = r;
+  }
+  int any;
+  int run = plan_scan(start, -1, [](int a, int b) { return max(a, b); }, sh->starts, any);
+  const int each_max = __reduce_max_sync(0xffffffffu, rb - ra);
+  for (int k = 0; k < each_max; ++k) {
+    const int r = ra + k;
+    const bool in = r < rb;
+    int r0 = -1, c = 0x7fffffff, e = 0;
+    if (in) {
+      if (r == 0 || seq_of(r) != seq_of(r - 1)) run = r;
+      r0 = run + (r - run) / (2 * R) * (2 * R);   // its item's first row
+      c = (int)min((int64_t)max(__ldg(p.ctx_lens + r), 0), (int64_t)tokens);
+      e = c;
       const uint32_t* m = p.masks + (int64_t)r * p.words;
-#pragma unroll 8
-      for (int w = 0; w < p.words; ++w) {
-        const uint32_t x = __ldg(m + w);
-        if (x) e = (int64_t)c + 32 * w + 32 - __clz(x);
+      for (int w = 0; w < p.words; w += 8) {
+        uint32_t x[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[j] = w + j < p.words ? __ldg(m + w + j) : 0u;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (x[j]) e = (int)min((int64_t)c + 32 * (w + j) + 32 - __clz(x[j]), (int64_t)tokens);
       }
-      ctx[r] = c;
-      end[r] = (int)min(e, tokens);
-      flag = r == 0 || seq_of(r) != seq_of(r - 1);
     }
-    at = flag;
-    const int n = (int)scan64(at, sh);
-    if (flag) runs[n_runs + at] = r;
-    n_runs += n;
+    const int same = __shfl_sync(0xffffffffu, r0, 0);
+    if (__all_sync(0xffffffffu, r0 == same || !in)) {   // a warp's rows are one item's
+      c = __reduce_min_sync(0xffffffffu, c);
+      e = __reduce_max_sync(0xffffffffu, e);
+      const int n = __reduce_max_sync(0xffffffffu, in ? r - r0 + 1 : 0);
+      if (lane == 0 && in) atomicMin(clear + r0, c), atomicMax(end + r0, e), atomicMax(count + r0, n);
+    } else if (in) {
+      atomicMin(clear + r0, c), atomicMax(end + r0, e), atomicMax(count + r0, r - r0 + 1);
+    }
   }
   __syncthreads();
-  // items: up to two tiles of pairs
-  int n_items = 0;
-  for (int i0 = 0; i0 < n_runs; i0 += kPlanThreads) {
-    const int i = i0 + tid, first = i < n_runs ? runs[i] : 0, n = i < n_runs ? (i + 1 < n_runs ? runs[i + 1] : p.T) - first : 0, mine = (n + 2 * R - 1) / (2 * R);
-    int64_t at = mine;
-    const int all = (int)scan64(at, sh);
-    for (int k = 0; k < mine; ++k) items[n_items + at + k] = {first + 2 * R * k, min(2 * R, n - 2 * R * k), seq_of(first), 0, 0};
-    n_items += all;
-  }
-  __syncthreads();
-  for (int i = warp; i < n_items; i += kPlanThreads / 32) {
-    const int row0 = items[i].row0, n = items[i].nrows;
-    int c = 0x7fffffff, e = 0;
-    for (int r = lane; r < n; r += 32) c = min(c, ctx[row0 + r]), e = max(e, end[row0 + r]);
-    c = __reduce_min_sync(0xffffffffu, c);
-    e = __reduce_max_sync(0xffffffffu, e);
-    if (lane == 0) items[i].clear = c, items[i].end = e;
-  }
-  const int n_units = n_items * p.hkv;
-  for (int i = tid; i < n_units + kNumSMs + 1; i += kPlanThreads) p.list[i].cta = -1;
-  if (tid < kNumSMs) p.starts[tid] = -1, p.cuts[tid].parts = 0;
-  __syncthreads();
-  // costs in front of an item (of one kv head)
-  auto tiles_of = [&](const TreeItem& t) { return (t.end + kTreeKeys - 1) / kTreeKeys; };
-  auto each_of = [&](const TreeItem& t) { return t.nrows > R ? kCostTwo : kCostOne; };
-  int64_t total = 0;
-  for (int i0 = 0; i0 < n_items; i0 += kPlanThreads) {
-    const int i = i0 + tid;
-    int64_t c = i < n_items ? kCostItem + (int64_t)max(tiles_of(items[i]), 1) * each_of(items[i]) : 0;
-    const int64_t all = scan64(c, sh);
-    if (i < n_items) front[i] = total + c;
-    total += all;
-  }
-  __syncthreads();
-  // Tile t of an item lies at its front + (t ? kCostItem : 0) + t x its cost on the line of all costs; CTA k has what lies in [k share, (k + 1) share).  A share is no less than the
-  // widest gap, so none between the first and the last of an item is without a tile
-  const int64_t share = max((int64_t)(kCostItem + kCostTwo), (total * p.hkv + kNumSMs - 1) / kNumSMs);
-  auto at_line = [&](int u, int64_t& base, int64_t& last) {   // of an item's first and last tile
-    const TreeItem& g = items[u / p.hkv];
-    const int nt = tiles_of(g), each = each_of(g);
-    base = front[u / p.hkv] * p.hkv + (int64_t)(u % p.hkv) * (kCostItem + (int64_t)max(nt, 1) * each);
-    last = base + (nt > 1 ? kCostItem + (int64_t)(nt - 1) * each : 0);
+  // costs in front (the upper 40 bits) and items (the lower 24)
+  auto tiles_of = [&](int r) { return (end[r] + kTreeKeys - 1) / kTreeKeys; };
+  auto each_of = [&](int r) { return count[r] > R ? kCostTwo : kCostOne; };
+  auto plus = [](int64_t a, int64_t b) { return a + b; };
+  int64_t sum = 0, all;
+  for (int r = ra; r < rb; ++r)
+    if (count[r] > 0) sum += ((int64_t)(kCostItem + max(tiles_of(r), 1) * each_of(r)) << 24) + 1;
+  const int64_t before = plan_scan(sum, (int64_t)0, plus, sh->sums[0], all);
+  const int n_items = (int)(all & 0xffffff), n_units = n_items * p.hkv;
+  int64_t total = (all >> 24) * p.hkv, mine = (before >> 24) * p.hkv, share;
+  const bool few = n_units <= kFewUnits;
+  const int gap = few ? 0 : kCostItem, widest = p.T > R ? kCostTwo : kCostOne;
+  auto whole_of = [&](int r) {
+    const int64_t c = gap + (int64_t)max(tiles_of(r), 1) * each_of(r);
+    return few ? small_quotient(c + share - 1, share) * share : c;
   };
-  for (int u = tid; u < n_units; u += kPlanThreads) {
-    const TreeItem g = items[u / p.hkv];
-    const int nt = tiles_of(g), each = each_of(g), h = u % p.hkv;
-    int64_t base, last, base_before = 0, last_before = -share;
-    at_line(u, base, last);
-    if (u > 0) at_line(u - 1, base_before, last_before);
-    const int k0 = (int)(base / share), k1 = (int)(last / share);
-    auto first_tile = [&](int k) {   // the first one, but for the item's first, at or behind the start of share k
-      const int64_t behind = k * share - base - kCostItem;
-      return behind <= each ? 1 : (int)min((int64_t)nt, (behind + each - 1) / each);
-    };
-    for (int k = k0; k <= k1; ++k) {
-      const int place = u + k;
-      p.list[place] = {g.row0, g.nrows, g.seq, g.clear, g.end, k == k0 ? 0 : first_tile(k), k == k1 ? nt : first_tile(k + 1), h, k, k1 - k0 + 1, 2 * k + (k == k0 ? 1 : 0), 0};
-      if (k > k0 || u == 0 || last_before / share < k) p.starts[k] = place;
-    }
-    if (k1 > k0) p.cuts[k0] = {g.row0, g.nrows, h, k1 - k0 + 1};
+  if (few) {
+    total -= (int64_t)n_units * kCostItem;
+    share = max((int64_t)2 * kCostOne, (total + kNumSMs - n_units - 1) / (kNumSMs - n_units));   // (two groups of softmax warps: two key tiles at least)
+    sum = 0;
+    for (int r = ra; r < rb; ++r)
+      if (count[r] > 0) sum += whole_of(r) * p.hkv;
+    mine = plan_scan(sum, (int64_t)0, plus, sh->sums[1], total);
+  } else {
+    share = max((int64_t)(gap + widest), (total + kNumSMs - 1) / kNumSMs);
   }
+  const int64_t lo = cta * share, hi = lo + share;
+  auto emit = [&](auto put) {   // the CTA's units
+    int64_t front = mine;
+    int item = (int)(before & 0xffffff);
+    for (int r = ra; r < rb && front < hi; ++r) {
+      if (count[r] == 0) continue;
+      const int nt = tiles_of(r), each = each_of(r), behind = nt > 1 ? gap + (nt - 1) * each : 0;   // behind: of the last tile
+      const int64_t whole = whole_of(r);
+      auto first_tile = [&](int64_t x) {   // the first one, but for tile 0, at or behind this place of the unit's line
+        const uint32_t y = (uint32_t)(x - gap);
+        return x <= gap + each ? 1 : min(nt, (int)(each == kCostTwo ? (y + kCostTwo - 1) / kCostTwo : (y + kCostOne - 1) / kCostOne));
+      };
+      for (int h = 0; h < p.hkv; ++h, front += whole) {
+        const int64_t last = front + behind;
+        if (front >= hi || last < lo) continue;
+        TreeWork w;
+        w.rows = {r, count[r], seq_of(r), clear[r], end[r]};
+        w.kvh = h;
+        w.tile0 = front < lo ? first_tile(lo - front) : 0;
+        w.tile1 = last < hi ? nt : first_tile(hi - front);
+        w.parts = 1, w.slot = 0;
+        if (front < lo || last >= hi) {
+          const int back = front < lo ? small_quotient(lo - front + share - 1, share) : 0, ahead = last >= hi ? small_quotient(last - lo, share) : 0;   // CTAs before, behind
+          w.parts = back + 1 + ahead;
+          w.slot = 2 * cta + (back == 0);
+          if (back == 0) sh->cut = {r, count[r], h, w.parts};
+        }
+        put(item * p.hkv + h, w);
+      }
+      ++item;
+    }
+  };
+  emit([&](int u, const TreeWork& w) {
+    const int place = atomicAdd(&sh->units, 1);
+    if (place < kTreeTable) table[place] = w;
+    atomicMin(&sh->first, u);
+  });
+  __syncthreads();
+  const int units = sh->units;
+  if (units <= kTreeTable) return make_int2(units, -1);
+  emit([&](int u, const TreeWork& w) { p.list[u + cta] = w; });
+  __syncthreads();
+  return make_int2(units, sh->first + cta);
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------------------------------------------
@@ -221,9 +259,9 @@ __device__ __forceinline__ void tree_bits(const TreeRow& r, int k0, uint32_t (&b
 // Values that are no numbers, back into 32 sums of a pair (columns c..): those that were taken out of a tile, and in front of it infinities, whose products with weights' low
 // terms of zero are not what the formula has (weights are above zero: the sum of such values is the result)
 __device__ __noinline__ void tree_repair(const TreeParams& p, const TreeWork& w, const TreeRow& r, const uint32_t (*bad)[4], bool taken_out, float* o, int c) {
-  const int first = max(w.tile0, w.clear / kTreeKeys);   // the first tile that not all rows see
+  const int first = max(w.tile0, w.rows.clear / kTreeKeys);   // the first tile that not all rows see
   auto add = [&](int key, float* to) {
-    const int64_t blk = __ldg(p.block_table + (int64_t)w.seq * p.bt_stride + key / p.block_size);
+    const int64_t blk = __ldg(p.block_table + (int64_t)w.rows.seq * p.bt_stride + key / p.block_size);
     if (blk < 0 || blk >= p.n_blocks) return;
     const __nv_bfloat16* v = p.v + ((blk * p.hkv + w.kvh) * p.block_size + key % p.block_size) * kHeadDim + c;
     for (int d = 0; d < 32; ++d) {
@@ -253,7 +291,7 @@ __device__ __noinline__ void tree_repair(const TreeParams& p, const TreeWork& w,
 }
 
 __global__ void __launch_bounds__(kTreeThreads, 1)
-attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeParams p) {
+attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const __grid_constant__ TreeParams p) {
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, cta = blockIdx.x;
@@ -268,73 +306,50 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
   uint64_t* p_ready = s_full + 4;                  // [group][2] their weights are
   uint64_t* o_full = p_ready + 4;                  // [group][2] their second product has finished
   uint64_t* q_ready = o_full + 4;
-  uint64_t* q_first = q_ready + 1;                 // the CTA's first queries, staged by the softmax warps as well
-  uint64_t* q_free = q_first + 1;
-  uint64_t* last = q_free + 1;                     // the MMAs in flight when a wait ran out
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 1);   // and, behind it, the mark of a wait that ran out
+  uint64_t* q_free = q_ready + 1;
+  uint64_t* last = q_free + 1;                     // [group] the MMAs in flight when a wait ran out
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 2);   // and, behind it, the mark of a wait that ran out
   int* taken_item = reinterpret_cast<int*>(tmem_slot + 2);       // [item's parity] the last one (counted from 1) with values that were taken out of a tile
+  TreeWork* table = reinterpret_cast<TreeWork*>((reinterpret_cast<uintptr_t>(taken_item + 2) + 15) & ~(uintptr_t)15);
+  PlanShared* plan = reinterpret_cast<PlanShared*>(table + kTreeTable);
   const Waits mbar_wait(tmem_slot + 1, p.status);
   if (threadIdx.x == 0) {
     for (int s = 0; s < kTreeSlots; ++s) {
       mbar_init(kv_full + s, 1);
-      mbar_init(kv_free + s, 1);
+      mbar_init(kv_free + s, 2);
     }
     for (int s = 0; s < 4; ++s) {
       mbar_init(s_full + s, 1);
       mbar_init(p_ready + s, 4);
       mbar_init(o_full + s, 1);
     }
-    mbar_init(q_ready, 2);
-    mbar_init(q_first, 10);
-    mbar_init(q_free, 1);
+    mbar_init(q_ready, 1);
+    mbar_init(q_free, 2);
     mbar_init(last, 1);
+    mbar_init(last + 1, 1);
     tmem_slot[1] = 0;
     taken_item[0] = taken_item[1] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  pdl_wait();
-  pdl_launch_dependents();
-  const int start = __ldcg(p.starts + cta);
-  if (start < 0) return;
   if (warp == 9) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
   }
   const int G = p.hq / p.hkv, R = 128 / G;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int2 units = tree_plan(p, R, cta, reinterpret_cast<int*>(ring), plan, table);
+  fence_async_smem();   // (the plan's lists lie where tiles come)
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = *tmem_slot;   // per group 256 columns: scores of even, odd key tiles, O
-  auto next_work = [&](int& at, TreeWork& w) {
-    const int4* src = reinterpret_cast<const int4*>(p.list + at);
-    const int4 a = __ldcg(src), b = __ldcg(src + 1), c = __ldcg(src + 2);
-    w = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, c.x, c.y, c.z, c.w};
-    ++at;
-    return w.cta == cta;
-  };
-  // the A operands of an item, thread i of `threads`: 16-byte pieces of rows
-  auto stage_q = [&](const TreeWork& w, int i, int threads) {
-    const __nv_bfloat16* q0 = p.q + (int64_t)w.row0 * p.ldq + (int64_t)w.kvh * G * kHeadDim;
-    const int pieces = (w.nrows > R ? 2 : 1) * 128 * 16;
-    constexpr int U = 8;
-#pragma unroll 1
-    for (int e0 = i; e0 < pieces; e0 += U * threads) {
-      uint4 v[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int e = e0 + u * threads, m = e >> 4, chunk = e & 15, r = (m & 127) / G, g = (m & 127) % G, row = (m >> 7) * R + r;
-        v[u] = make_uint4(0u, 0u, 0u, 0u);
-        if (e < pieces && r < R && row < w.nrows) v[u] = __ldg(reinterpret_cast<const uint4*>(q0 + (int64_t)row * p.ldq + g * kHeadDim + chunk * 8));
-      }
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int e = e0 + u * threads, m = e >> 4, chunk = e & 15, mm = m & 127;
-        if (e < pieces)
-          *reinterpret_cast<uint4*>(qs + (2 * (m >> 7) + (chunk >> 3)) * kTrQChunk + (mm >> 3) * 1024 + (mm & 7) * 128 + (((chunk & 7) ^ (mm & 7)) << 4)) = v[u];
-      }
-    }
-    fence_async_smem();
-    __syncwarp();
+  int unit = 0;
+  auto next_work = [&](TreeWork& w) {
+    if (unit >= units.x) return false;
+    w = units.y < 0 ? table[unit] : p.list[units.y + unit];   // (written by this CTA)
+    ++unit;
+    return true;
   };
 
   if (warp == 8) {
@@ -346,32 +361,27 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     const int box = min(p.block_size, kTreeKeys), boxes = kTreeKeys / box, ahead = 32 / boxes;   // rows of a box; boxes of a tile; tiles whose rows are looked up at once
     const int none = (int)(p.n_blocks * p.hkv * p.block_size);   // behind the cache: zeros
-    const int64_t tokens = tree_tokens(p);
     int slot = 0, row = 0;
     uint32_t ph = 1;
     bool stop = false;
     TreeWork w;
-    for (int at = start; !stop && next_work(at, w);) {
-      const int32_t* bt = p.block_table + (int64_t)w.seq * p.bt_stride;
+    while (!stop && next_work(w)) {
+      const int32_t* bt = p.block_table + (int64_t)w.rows.seq * p.bt_stride;
       for (int i = w.tile0; i < w.tile1 && !(stop = mbar_wait.stop()); ++i) {
         const int k = (i - w.tile0) % ahead;
         if (k == 0) {   // lane: the row of box lane % boxes of tile i + lane / boxes
-          const int64_t tok = (int64_t)(i + lane / boxes) * kTreeKeys + lane % boxes * box;
-          const int blk = tok < tokens && i + lane / boxes < w.tile1 ? __ldg(bt + tok / p.block_size) : -1;
-          row = blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + (int)(tok % p.block_size) : none;
+          const int tok = (i + lane / boxes) * kTreeKeys + lane % boxes * box, b = tok / p.block_size;
+          const int blk = b < p.bt_stride && i + lane / boxes < w.tile1 ? __ldg(bt + b) : -1;
+          row = blk >= 0 && blk < p.n_blocks ? (blk * p.hkv + w.kvh) * p.block_size + (tok - b * p.block_size) : none;
         }
 #pragma unroll
         for (int kv = 0; kv < 2; ++kv) {
           mbar_wait(kv_free + slot, ph);
           if (issuer) mbar_expect_tx(kv_full + slot, kTrTile);
-          for (int b = 0; b < boxes; ++b) {
-            const int from = __shfl_sync(0xffffffffu, row, k * boxes + b);
-            if (issuer) {
-              unsigned char* dst = ring + slot * kTrTile + b * box * 128;
-              tma_load_2d(dst, kv ? &map_v : &map_k, 0, from, kv_full + slot);
-              tma_load_2d(dst + kTrChunk, kv ? &map_v : &map_k, 64, from, kv_full + slot);
-            }
-          }
+          __syncwarp();
+          const int from = __shfl_sync(0xffffffffu, row, k * boxes + (lane >> 1) % boxes);
+          if (lane < 2 * boxes)   // a lane a box and half of its columns
+            tma_load_2d(ring + slot * kTrTile + (lane & 1) * kTrChunk + (lane >> 1) * box * 128, kv ? &map_v : &map_k, (lane & 1) * 64, from, kv_full + slot);
           __syncwarp();
           if (++slot == kTreeSlots) slot = 0, ph ^= 1;
         }
@@ -379,157 +389,106 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
     }
     if (mbar_wait.stop())   // the loads in flight: a slot's last one filled it in this round of the ring or in the one before
       for (int s = 0; s < kTreeSlots; ++s) mbar_wait.drain(kv_full + s, s < slot ? ph ^ 1 : ph);
-  } else if (warp == 9) {
-    // ===== MMA: per key tile the next one's scores, then this one's second product.  The whole warp walks the loop; bounds and addresses that come from memory are broadcast, so
-    // that they are uniform to the compiler =====
-    const uint32_t one = elect_one() ? 1u : 0u, tm = __shfl_sync(0xffffffffu, tmem, 0);
-    const uint64_t desc_q = make_desc(smem_u32(qs), 16, 1024), desc_k = make_desc(smem_u32(ring), 16, 1024), desc_v = make_desc(smem_u32(ring), kTrChunk, 1024);
+  } else if (warp == 9 || warp == 11) {
+    // ===== MMA, a warp for each group of softmax warps: its next key tile's scores, then this one's second product (one warp for both has its hands full: waits, commits and
+    // the issue of 32 MMAs are as long as what it issues).  The whole warp walks the loop; bounds and addresses that come from memory are broadcast, so that they are uniform to the
+    // compiler =====
+    const int x = __shfl_sync(0xffffffffu, warp == 11 ? 1 : 0, 0);
+    const uint32_t one = elect_one() ? 1u : 0u, tm = __shfl_sync(0xffffffffu, tmem, 0) + x * 256;
+    const uint64_t desc_k = make_desc(smem_u32(ring), 16, 1024), desc_v = make_desc(smem_u32(ring), kTrChunk, 1024);
     const uint32_t id_s = idesc_bf16(kTreeKeys, 0), id_o = idesc_bf16(kHeadDim, 1);
-    int slot = 0, active = 0, n[2] = {0, 0};   // n: key tiles of either group so far
-    uint32_t ph = 0;
-    auto next_slot = [&]() {
-      if (++slot == kTreeSlots) slot = 0, ph ^= 1;
-    };
-    auto scores = [&](int x, int tile, int nx, int k_slot) {   // group x, its tile of pairs
-      const uint64_t da = desc_q + (uint64_t)((tile * 2 * kTrQChunk) >> 4), db = desc_k + (uint64_t)((k_slot * kTrTile) >> 4);
-      const uint32_t d = tm + x * 256 + (nx & 1) * kTreeKeys;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        mma_ss(one, d, da + ((j >> 2) * kTrQChunk + (j & 3) * 32) / 16, db + ((j >> 2) * kTrChunk + (j & 3) * 32) / 16, id_s, j ? 1u : 0u);
-      commit(one, s_full + 2 * x + (nx & 1));
-    };
-    auto product = [&](int x, int nx, int v_slot, uint32_t more) {
-      const uint64_t dv = desc_v + (uint64_t)((v_slot * kTrTile) >> 4);
-      mbar_wait(p_ready + 2 * x + (nx & 1), (nx >> 1) & 1);
-      fence_after();
-      const uint32_t pa = tm + x * 256 + (nx & 1) * kTreeKeys, d = tm + x * 256 + 128;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {   // 16 keys per step: 8 columns of weights, 16 further those of the second term
-        mma_ts(one, d, pa + (j >> 1) * 32 + (j & 1) * 8, dv + (uint64_t)((j * 2048) >> 4), id_o, j ? 1u : more);
-        mma_ts(one, d, pa + (j >> 1) * 32 + (j & 1) * 8 + 16, dv + (uint64_t)((j * 2048) >> 4), id_o, 1u);
-      }
-    };
-    // an item of nt key tiles with both tiles of pairs, or its key tiles by the groups in turn
-    auto walk = [&](auto two_c, int nt) {
-      constexpr bool TWO = decltype(two_c)::value;
-      mbar_wait(kv_full + slot, ph);
-      fence_after();
-      int k_slot = slot;
-      next_slot();
-      scores(0, 0, n[0], k_slot);
-      if (TWO) scores(1, 1, n[1], k_slot);
-      commit(one, kv_free + k_slot);
-      commit(nt == 1 ? one : 0u, q_free);
-      auto step = [&](auto more_c, auto x_c, int i) {
-        constexpr bool MORE = decltype(more_c)::value;
-        [[maybe_unused]] constexpr int X = decltype(x_c)::value;   // (not TWO) the group of key tile i
-        const int v_slot = slot;
-        const uint32_t v_ph = ph;
-        next_slot();
-        if constexpr (MORE) {
-          mbar_wait(kv_full + slot, ph);
-          fence_after();
-          k_slot = slot;
-          next_slot();
-        }
-        if constexpr (TWO) {
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if constexpr (MORE) scores(x, x, n[x] + 1, k_slot);
-            if (MORE && x == 1) {
-              commit(one, kv_free + k_slot);
-              commit(i + 2 == nt ? one : 0u, q_free);   // the item's last scores are on their way
-            }
-            if (x == 0) mbar_wait(kv_full + v_slot, v_ph);
-            product(x, n[x], v_slot, i ? 1u : 0u);
-            if (x == 1) commit(one, kv_free + v_slot);
-            commit(one, o_full + 2 * x + (n[x] & 1));
-            ++n[x];
-          }
-        } else {
-          if constexpr (MORE) {
-            scores(X ^ 1, 0, n[X ^ 1], k_slot);
-            commit(one, kv_free + k_slot);
-            commit(i + 2 == nt ? one : 0u, q_free);
-          }
-          mbar_wait(kv_full + v_slot, v_ph);
-          product(X, n[X], v_slot, i > 1 ? 1u : 0u);
-          commit(one, kv_free + v_slot);
-          commit(one, o_full + 2 * X + (n[X] & 1));
-          ++n[X];
-        }
-      };
-      const std::integral_constant<int, 0> even;
-      const std::integral_constant<int, 1> odd;
-      if constexpr (TWO) {
-        for (int i = 0; i + 1 < nt; ++i) step(std::true_type(), even, i);
-        step(std::false_type(), even, nt - 1);
-      } else {
-        int i = 0;
-        for (; i + 2 < nt; i += 2) {
-          step(std::true_type(), even, i);
-          step(std::true_type(), odd, i + 1);
-        }
-        if (i + 1 < nt) {
-          step(std::true_type(), even, i);
-          step(std::false_type(), odd, i + 1);
-        } else {
-          step(std::false_type(), even, i);
-        }
-      }
-    };
+    uint64_t *const s_done = s_full + 2 * x, *const weights = p_ready + 2 * x, *const o_done = o_full + 2 * x;
+    uint32_t at_ring = 0, n = 0;   // places of the ring used up by the items before; key tiles of the group so far
+    int active = 0;
     TreeWork w;
-    for (int at = start; __shfl_sync(0xffffffffu, next_work(at, w), 0);) {
-      const int nt = __shfl_sync(0xffffffffu, w.tile1 - w.tile0, 0), two = __shfl_sync(0xffffffffu, w.nrows > R ? 1 : 0, 0);
+    while (__shfl_sync(0xffffffffu, next_work(w), 0)) {
+      const int nt = __shfl_sync(0xffffffffu, w.tile1 - w.tile0, 0), two = __shfl_sync(0xffffffffu, w.rows.nrows > R ? 1 : 0, 0);
       if (nt <= 0) continue;
-      if (active == 0) mbar_wait(q_first, 0);
-      else mbar_wait(q_ready, (active - 1) & 1);
-      if (two) walk(std::true_type(), nt);
-      else walk(std::false_type(), nt);
+      // both tiles of pairs: every key tile, by either warp; one: every other one
+      const int step = two ? 1 : 2, first = two ? 0 : x;
+      const uint64_t desc_q = make_desc(smem_u32(qs + (two ? x : 0) * 2 * kTrQChunk), 16, 1024);
+      auto arrived = [&](uint32_t place) {
+        mbar_wait(kv_full + (place & (kTreeSlots - 1)), (place / kTreeSlots) & 1);
+        fence_after();
+        return place & (kTreeSlots - 1);
+      };
+      auto done_with = [&](uint32_t slot) {   // (two arrivals)
+        if (!two && one) mbar_arrive(kv_free + slot);
+        __syncwarp();
+        commit(one, kv_free + slot);
+      };
+      auto scores = [&](int i, uint32_t nx) {   // of key tile i: places 2 i and 2 i + 1 of the item's part of the ring
+        const uint32_t slot = arrived(at_ring + 2 * i);
+        const uint64_t db = desc_k + (uint64_t)((slot * kTrTile) >> 4);
+        const uint32_t d = tm + (nx & 1) * kTreeKeys;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          mma_ss(one, d, desc_q + ((j >> 2) * kTrQChunk + (j & 3) * 32) / 16, db + ((j >> 2) * kTrChunk + (j & 3) * 32) / 16, id_s, j ? 1u : 0u);
+        commit(one, s_done + (nx & 1));
+        done_with(slot);
+        if (i + step >= nt) commit(one, q_free);   // the group's last scores are on their way
+      };
+      mbar_wait(q_ready, active & 1);
+      if (first < nt) scores(first, n);
+      else if (one) mbar_arrive(q_free);
+      __syncwarp();
+      for (int i = first; i < nt; i += step, ++n) {
+        if (i + step < nt) scores(i + step, n + 1);
+        const uint32_t slot = arrived(at_ring + 2 * i + 1);
+        const uint64_t dv = desc_v + (uint64_t)((slot * kTrTile) >> 4);
+        mbar_wait(weights + (n & 1), (n >> 1) & 1);
+        fence_after();
+        const uint32_t pa = tm + (n & 1) * kTreeKeys, d = tm + 128, more = i > first ? 1u : 0u;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {   // 16 keys per step: 8 columns of weights, 16 further those of the second term
+          mma_ts(one, d, pa + (j >> 1) * 32 + (j & 1) * 8, dv + (uint64_t)((j * 2048) >> 4), id_o, j ? 1u : more);
+          mma_ts(one, d, pa + (j >> 1) * 32 + (j & 1) * 8 + 16, dv + (uint64_t)((j * 2048) >> 4), id_o, 1u);
+        }
+        commit(one, o_done + (n & 1));
+        done_with(slot);
+      }
+      at_ring += 2 * nt;
       ++active;
     }
     if (mbar_wait.stop()) {
-      commit(one, last);
-      mbar_wait.drain(last, 0);
+      commit(one, last + x);
+      mbar_wait.drain(last + x, 0);
     }
-  } else if (warp >= 10) {
-    // ===== queries of the next item -> the A operands =====
+  } else if (warp == 10) {
+    // ===== queries -> the A operands: R rows of a kv head's G heads are R G rows of an operand (those behind them are never looked at) =====
+    const bool issuer = elect_one();
     int active = 0;
     TreeWork w;
-    for (int at = start; next_work(at, w);) {
+    if (lane == 0) p.cuts[cta] = plan->cut;
+    while (next_work(w)) {
       if (w.tile1 <= w.tile0) continue;
-      if (active == 0) {
-        stage_q(w, threadIdx.x - 64, 320);   // (beside the softmax warps' threads 0..255)
-        if (lane == 0) mbar_arrive(q_first);
-      } else {
-        mbar_wait(q_free, (active - 1) & 1);
-        stage_q(w, threadIdx.x - 320, 64);
-        if (lane == 0) mbar_arrive(q_ready);
+      const int tiles = w.rows.nrows > R ? 2 : 1;
+      if (active > 0) mbar_wait(q_free, (active - 1) & 1);
+      if (mbar_wait.stop()) break;
+      if (issuer) {
+        mbar_expect_tx(q_ready, tiles * 2 * R * G * 128);
+        for (int e = 0; e < 2 * tiles; ++e) tma_load_3d(qs + e * kTrQChunk, &map_q, (e & 1) * 64, w.kvh * G, w.rows.row0 + (e >> 1) * R, q_ready);
       }
+      __syncwarp();
       ++active;
     }
-  } else {
+    if (mbar_wait.stop() && active > 0) mbar_wait.drain(q_ready, (active - 1) & 1);
+  } else if (warp < 8) {
     // ===== softmax and output: a thread owns a pair, of tile x of the item's, or with its fellow in the other group of the only one =====
     const int x = warp >> 2, quad = warp & 3, m = quad * 32 + lane;
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16), own = base + x * 256;
     const int r = m / G, g = m % G;
     const float sc2 = p.scale * 1.4426950408889634f;   // scores in the log2 domain
-    bool first = true;
-    int n = 0, done = 0, item = 0;   // key tiles of this group so far; of all items before; items
+    int n = 0, done = 0, item = 0, cleaned = 0;   // key tiles of this group so far; of all items before; items; tiles cleaned by group 0 for both
     TreeWork w;
-    for (int at = start; next_work(at, w);) {
+    while (next_work(w)) {
       ++item;   // (a group is at most one item ahead of the other)
       uint32_t(*const bad)[4] = bad_keys + (item & 1) * kTrBad;
-      if (first && w.tile1 > w.tile0) {
-        stage_q(w, threadIdx.x, 320);   // (the stagers are threads 256..319 of this)
-        if (lane == 0) mbar_arrive(q_first);
-        first = false;
-      }
-      const bool two = w.nrows > R;
-      const int row = (two ? x * R : 0) + r, t = w.row0 + row;
-      const bool alive = r < R && row < w.nrows;
-      const TreeRow see = {p.masks + (int64_t)t * p.words, alive ? tree_ctx(p, t) : 0, alive ? p.words : 0, w.end, alive};
-      const int masked = max(w.tile0, w.clear / kTreeKeys);   // the first tile that not all rows see
+      const bool two = w.rows.nrows > R;
+      const int row = (two ? x * R : 0) + r, t = w.rows.row0 + row;
+      const bool alive = r < R && row < w.rows.nrows;
+      const TreeRow see = {p.masks + (int64_t)t * p.words, alive ? tree_ctx(p, t) : 0, alive ? p.words : 0, w.rows.end, alive};
+      const int masked = max(w.tile0, w.rows.clear / kTreeKeys);   // the first tile that not all rows see
       float mu = -INFINITY, l = 0.f;
       const int n0 = n;
       for (int i = w.tile0 + (two ? 0 : x); i < w.tile1; i += two ? 1 : 2, ++n) {
@@ -569,7 +528,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         }
         // exponents as (score - maximum) x scale: a product less a rounded one would be off by 2^-24 of either, which is more than the exponent itself where scores are large
         const uint64_t minus = f2::both(mu > -INFINITY ? -mu : 0.f), unit = f2::both(sc2);
-        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        uint64_t sum2[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           uint32_t pk[32];
@@ -578,20 +537,21 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             const uint64_t e = f2::mul(f2::add(f2::pack(__uint_as_float(s[c * 32 + 2 * j]), __uint_as_float(s[c * 32 + 2 * j + 1])), minus), unit);
             const float p0 = exp2_fast(f2::lo(e)), p1 = exp2_fast(f2::hi(e));
             // the high term truncated, the rest rounded
-            sum[j & 3] += p0 + p1;
-            const uint32_t h0 = __float_as_uint(p0) & 0xffff0000u, h1 = __float_as_uint(p1) & 0xffff0000u;
-            pk[j] = __byte_perm(h0, h1, 0x7632);
-            pk[16 + j] = pack_bf16(p0 - __uint_as_float(h0), p1 - __uint_as_float(h1));
+            sum2[j & 1] = f2::add(sum2[j & 1], f2::pack(p0, p1));
+            pk[j] = pack_bf16(p0, p1);
+            const uint32_t h0 = pk[j] << 16, h1 = pk[j] & 0xffff0000u;
+            const uint64_t rest = f2::add(f2::pack(p0, p1), f2::pack(-__uint_as_float(h0), -__uint_as_float(h1)));
+            pk[16 + j] = pack_bf16(f2::lo(rest), f2::hi(rest));
           }
           st32(s_addr + c * 32, pk);
         }
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        l += f2::sum(sum2[0]) + f2::sum(sum2[1]);
         if (i >= masked && !(two && x)) {
           // 0 x NaN = NaN: what is no number leaves the value tile (two threads a key), everything behind the end does
           const int v_at = 2 * (done + i - w.tile0) + 1, vs = v_at % kTreeSlots, key = m >> 1;
           mbar_wait(kv_full + vs, (v_at / kTreeSlots) & 1);
           uint4* const vb = reinterpret_cast<uint4*>(ring + vs * kTrTile + (m & 1) * kTrChunk + key * 128);
-          const bool behind = i * kTreeKeys + key >= w.end;
+          const bool behind = i * kTreeKeys + key >= w.rows.end;
           uint32_t found = 0;
 #pragma unroll
           for (int k = 0; k < 8; ++k) {
@@ -615,6 +575,11 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
             if (keys) reinterpret_cast<volatile int*>(taken_item)[item & 1] = item;
           }
           fence_async_smem();
+        }
+        if (two && i >= masked) {   // group 1's product waits for the clean values too (group 0 is at most three key tiles ahead: the ring)
+          if (x) asm volatile("bar.sync %0, 256;" ::"r"(3 + (cleaned & 3)) : "memory");
+          else asm volatile("bar.arrive %0, 256;" ::"r"(3 + (cleaned & 3)) : "memory");
+          ++cleaned;
         }
         st_wait();
         fence_before();
@@ -645,8 +610,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
       const bool taken = reinterpret_cast<volatile int*>(taken_item)[item & 1] == item;
       const int c0 = two ? 0 : x * 64, c1 = two ? kHeadDim : c0 + 64;
       const float inv = w.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
-      float* const part = p.part + ((int64_t)w.slot * p.pairs + row * G + g) * kTrPart;
-      if (w.parts > 1 && alive && c0 == 0) *reinterpret_cast<float2*>(part + kHeadDim) = make_float2(mu, l);
+      float4* const part = reinterpret_cast<float4*>(p.part + (int64_t)w.slot * p.pairs * kTrPart) + row * G + g;
+      if (w.parts > 1 && alive && c0 == 0) reinterpret_cast<float2*>(p.part + (int64_t)w.slot * p.pairs * kTrPart + (int64_t)p.pairs * kHeadDim)[row * G + g] = make_float2(mu, l);
       unsigned char* const st = ostage + warp * 2048;
 #pragma unroll 1
       for (int c = c0; c < c1; c += 32) {
@@ -679,7 +644,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
         if (w.parts > 1) {
           if (alive) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) store_sector(part + c + 8 * k, o + 8 * k);
+            for (int k = 0; k < 8; ++k) part[(c / 4 + k) * p.pairs] = *reinterpret_cast<const float4*>(o + 4 * k);
           }
         } else {
           // 32 columns at a time through shared memory: a row's 64 bytes leave from four neighbouring lanes
@@ -695,7 +660,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
           for (int k = 0; k < 4; ++k) {
             const int rr = k * 8 + (lane >> 2), mm = quad * 32 + rr, row2 = (two ? x * R : 0) + mm / G, col = c + (lane & 3) * 8;
             const uint4 v = *reinterpret_cast<const uint4*>(st + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4));
-            if (mm / G < R && row2 < w.nrows) *reinterpret_cast<uint4*>(p.out + (int64_t)(w.row0 + row2) * p.ldo + (int64_t)(w.kvh * G + mm % G) * kHeadDim + col) = v;
+            if (mm / G < R && row2 < w.rows.nrows) *reinterpret_cast<uint4*>(p.out + (int64_t)(w.rows.row0 + row2) * p.ldo + (int64_t)(w.kvh * G + mm % G) * kHeadDim + col) = v;
           }
           __syncwarp();
         }
@@ -714,79 +679,97 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constan
 }
 
 // ---- parts -> out -----------------------------------------------------------------------------------------------------------------------
-constexpr int kTreeManyParts = 4;
+// A warp takes 32 pairs of an item and eight columns: sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m) over its parts, in their order
+constexpr int kJoinThreads = 256, kJoinColumns = 8;
 
-__global__ void __launch_bounds__(256) tree_join_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p) {
+  __shared__ int front[kJoinThreads + 1], sh[kJoinThreads / 32];
   pdl_wait();
   pdl_launch_dependents();
-  const Kv8Cut cut = p.cuts[blockIdx.x];
-  if (cut.parts < 2) return;
-  const int G = p.hq / p.hkv;
-  const int64_t step = 2ll * p.pairs * kTrPart;
-  auto join = [&](auto lanes_c) {
-    constexpr int LANES = decltype(lanes_c)::value, EACH = 256 / LANES;
-    for (int c = blockIdx.y * EACH + threadIdx.x / LANES; c < cut.nrows * G; c += EACH * gridDim.y) {
-      const float* x = p.part + (2 * (int64_t)blockIdx.x * p.pairs + c) * kTrPart;
-      join_parts<LANES>(x + p.pairs * kTrPart, x + step, step, cut.parts, p.out + (int64_t)(cut.row0 + c / G) * p.ldo + (cut.kvh * G + c % G) * kHeadDim, p.scale * 1.4426950408889634f);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.hq / p.hkv;
+  const Kv8Cut mine = tid < kNumSMs ? p.cuts[tid] : Kv8Cut{0, 0, 0, 0};
+  int n = mine.parts < 2 ? 0 : (mine.nrows * G + 31) / 32 * (kHeadDim / kJoinColumns);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, n, o);
+    if (lane >= o) n += u;
+  }
+  if (lane == 31) sh[warp] = n;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) n += sh[w];
+  front[tid + 1] = n;
+  if (tid == 0) front[0] = 0;
+  __syncthreads();
+  const float unit = p.scale * 1.4426950408889634f;
+  const int64_t slot = (int64_t)p.pairs * kTrPart;
+  for (int job = blockIdx.x * (kJoinThreads / 32) + warp; job < front[kJoinThreads]; job += gridDim.x * (kJoinThreads / 32)) {
+    int k = 0;   // the last with front[k] <= job
+#pragma unroll
+    for (int b = kJoinThreads / 2; b > 0; b >>= 1)
+      if (front[k + b] <= job) k += b;
+    const Kv8Cut cut = p.cuts[k];
+    const int at = job - front[k], c = at % (kHeadDim / kJoinColumns), pair = at / (kHeadDim / kJoinColumns) * 32 + lane;
+    const bool alive = pair < cut.nrows * G;
+    const float* part = p.part + (2 * k + 1) * slot;   // the first: behind it every other one
+    auto part_of = [&](int i) { return part + (i ? 2 * i - 1 : 0) * slot; };
+    auto ml = [&](int i) { return __ldcg(reinterpret_cast<const float2*>(part_of(i) + (int64_t)p.pairs * kHeadDim) + pair); };
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < cut.parts; ++i) m = fmaxf(m, ml(i).x);
+    float a[8] = {};
+#pragma unroll 4
+    for (int i = 0; i < cut.parts; ++i) {
+      const float2 t = ml(i);
+      const float4 *v = reinterpret_cast<const float4*>(part_of(i)) + (int64_t)(2 * c) * p.pairs + pair, x = __ldcg(v), y = __ldcg(v + p.pairs);
+      const float f = t.x == m ? 1.f : exp2_fast((t.x - m) * unit);
+      l += t.y * f;
+      a[0] += x.x * f, a[1] += x.y * f, a[2] += x.z * f, a[3] += x.w * f, a[4] += y.x * f, a[5] += y.y * f, a[6] += y.z * f, a[7] += y.w * f;
     }
-  };
-  if (cut.parts > kTreeManyParts) join(std::integral_constant<int, 32>());
-  else join(std::integral_constant<int, 8>());
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    if (alive)
+      *reinterpret_cast<uint4*>(p.out + (int64_t)(cut.row0 + pair / G) * p.ldo + (cut.kvh * G + pair % G) * kHeadDim + c * kJoinColumns) =
+          make_uint4(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv), pack_bf16(a[4] * inv, a[5] * inv), pack_bf16(a[6] * inv, a[7] * inv));
+  }
 }
 
 // ---- workspace ----------------------------------------------------------------------------------------------------------------------------
 int64_t up256(int64_t n) { return (n + 255) / 256 * 256; }
 int64_t tree_pairs(int T, int hq, int hkv) {   // of an item at most
   const int G = hq / hkv;
-  return std::min<int64_t>((int64_t)T * G, 2 * (128 / G) * G);
+  return (std::min<int64_t>((int64_t)T * G, 2 * (128 / G) * G) + 31) / 32 * 32;
 }
 struct TreeSizes {
-  int64_t list, starts, cuts, part, rows, items, front, all;
+  int64_t cuts, part, list, all;
 };
 TreeSizes tree_sizes(int T, int hq, int hkv) {
   TreeSizes s = {};
-  s.list = up256(((int64_t)T * hkv + kNumSMs + 1) * (int64_t)sizeof(TreeWork));
-  s.starts = up256(kNumSMs * 4);
   s.cuts = up256(kNumSMs * (int64_t)sizeof(Kv8Cut));
   s.part = up256(2 * kNumSMs * tree_pairs(T, hq, hkv) * kTrPart * 4);
-  s.rows = up256((int64_t)T * 4);
-  s.items = up256((int64_t)T * (int64_t)sizeof(TreeItem));
-  s.front = up256((int64_t)T * 8);
-  s.all = s.list + s.starts + s.cuts + s.part + 3 * s.rows + s.items + s.front;
+  s.list = up256(((int64_t)T * hkv + kNumSMs) * (int64_t)sizeof(TreeWork));
+  s.all = s.cuts + s.part + s.list;
   return s;
 }
 
 int tree_launch(TreeParams p, void* ws, cudaStream_t s) {
   if (const int e = wait_status()) return e;
-  CUtensorMap mk, mv;
+  CUtensorMap mq, mk, mv;
   const int64_t rows = p.n_blocks * p.hkv * p.block_size;
+  const int G = p.hq / p.hkv;
+  if (const int rc = query_map_bf16(p.q, p.T, p.hq, p.ldq, G, 128 / G, &mq)) return rc;
   if (const int rc = rows_map_bf16(p.k, rows, std::min(p.block_size, kTreeKeys), &mk)) return rc;
   if (const int rc = rows_map_bf16(p.v, rows, std::min(p.block_size, kTreeKeys), &mv)) return rc;
   const TreeSizes z = tree_sizes(p.T, p.hq, p.hkv);
-  char* w = static_cast<char*>(ws);
-  auto take = [&](int64_t n) {
-    char* const at = w;
-    w += n;
-    return at;
-  };
-  p.list = reinterpret_cast<TreeWork*>(take(z.list));
-  p.starts = reinterpret_cast<int*>(take(z.starts));
-  p.cuts = reinterpret_cast<Kv8Cut*>(take(z.cuts));
-  p.part = reinterpret_cast<float*>(take(z.part));
+  char* const w = static_cast<char*>(ws);
+  p.cuts = reinterpret_cast<Kv8Cut*>(w);
+  p.part = reinterpret_cast<float*>(w + z.cuts);
+  p.list = reinterpret_cast<TreeWork*>(w + z.cuts + z.part);
   p.pairs = (int)tree_pairs(p.T, p.hq, p.hkv);
   p.status = wait_status_word();
-  PlanLists far;
-  far.ctx = reinterpret_cast<int*>(take(z.rows));
-  far.end = reinterpret_cast<int*>(take(z.rows));
-  far.runs = reinterpret_cast<int*>(take(z.rows));
-  far.items = reinterpret_cast<TreeItem*>(take(z.items));
-  far.front = reinterpret_cast<int64_t*>(take(z.front));
   static bool done[64] = {};
   B200_CUDA(ensure_dynamic_smem(attn_tree_kernel, kTrSmem, done));
-  B200_CUDA(launch(tree_plan_kernel, dim3(1), dim3(kPlanThreads), (size_t)0, s, p, 128 / (p.hq / p.hkv), far));
+  B200_CUDA(launch(attn_tree_kernel, dim3(kNumSMs), dim3(kTreeThreads), (size_t)kTrSmem, s, mq, mk, mv, p));
   const PdlScope after;
-  B200_CUDA(launch(attn_tree_kernel, dim3(kNumSMs), dim3(kTreeThreads), (size_t)kTrSmem, s, mk, mv, p));
-  B200_CUDA(launch(tree_join_kernel, dim3(kNumSMs, 4), dim3(256), (size_t)0, s, p));
+  B200_CUDA(launch(tree_join_kernel, dim3(kNumSMs), dim3(kJoinThreads), (size_t)0, s, p));
   return B200_OK;
 }
 
@@ -823,7 +806,7 @@ extern "C" int b200_paged_attn_tree(const void* q, int64_t ldq, const void* k_ca
   B200_REQUIRE(ws && aligned16(ws) && ws_bytes >= need, B200_ERR_INVALID, "paged_attn_tree: the workspace is 16-byte aligned and has at least %lld bytes (%lld)",
                (long long)need, (long long)ws_bytes);
   B200_REQUIRE(n_blocks * hkv * block_size <= 0x7fffffff - 256, B200_ERR_UNSUPPORTED, "paged_attn_tree: a cache of %lld rows", (long long)(n_blocks * hkv * block_size));
-  B200_REQUIRE((int64_t)T * hkv <= 0x7fffffff - 2 * kNumSMs, B200_ERR_UNSUPPORTED, "paged_attn_tree: %d rows of %d kv heads", T, hkv);
+  B200_REQUIRE(T <= kMostRows && (int64_t)T * hkv <= 0x7fffffff - 2 * kNumSMs, B200_ERR_UNSUPPORTED, "paged_attn_tree: %d rows of %d kv heads (at most %d rows)", T, hkv, kMostRows);
   TreeParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.k = static_cast<const __nv_bfloat16*>(k_cache_layer);

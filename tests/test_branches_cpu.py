@@ -24,7 +24,7 @@ def _attend(**kw):
     ({"words": 33}, -3), ({"T": -2}, -1), ({"hq": 31}, -1), ({"hkv": 0}, -1), ({"hq": 34, "hkv": 2, "ldq": 34 * 128, "ldo": 34 * 128}, -3), ({"stride": 0}, -1),
     ({"block": 100}, -3), ({"block": 8}, -3), ({"block": 192}, -3), ({"n_blocks": 0}, -1), ({"n_blocks": 1 << 40}, -1), ({"ldq": 32 * 128 - 8}, -1), ({"ldo": 32 * 128 + 2}, -1),
     ({"q": BUF + 2}, -1), ({"out": BUF + 8}, -1), ({"k": BUF + 8}, -1), ({"v": BUF + 4}, -1), ({"masks": BUF + 2}, -1), ({"scale": float("inf")}, -1), ({"scale": float("nan")}, -1),
-    ({"scale": 0.0}, -1), ({"scale": -1.0}, -1), ({"ws": None}, -1), ({"size": 0}, -1), ({"ws": BUF + 8}, -1), ({"stride": 2 ** 24, "block": 128}, -3)])
+    ({"scale": 0.0}, -1), ({"scale": -1.0}, -1), ({"ws": None}, -1), ({"size": 0}, -1), ({"ws": BUF + 8}, -1), ({"stride": 2 ** 24, "block": 128}, -3), ({"T": 4097}, -3)])
 def test_attention_refuses(kw, code):
     assert _attend(**kw) == code
     assert b"paged_attn_tree" in _lib().b200_last_error()
