@@ -64,7 +64,7 @@ __host__ __device__ __forceinline__ int64_t tree_tokens(const TreeParams& p) { r
 __device__ __forceinline__ int tree_ctx(const TreeParams& p, int row) { return (int)min((int64_t)max(__ldg(p.ctx_lens + row), 0), tree_tokens(p)); }
 
 constexpr int kTrSmem = 1024 + 4 * kTrQChunk + kTreeSlots * kTrTile + kTrStage + 2 * 128 * 8 + 2 * kTrBad * 16 + (2 * kTreeSlots + 16) * 8 + 32 + kTreeTable * (int)sizeof(TreeWork) + 320;
-static_assert(3 * kMostRows * 4 <= kTreeSlots * kTrTile, "the plan's lists");
+static_assert(5 * kMostRows * 4 <= kTreeSlots * kTrTile, "the plan's lists");
 static_assert(kTrSmem <= 232448, "shared memory");
 
 // ---- plan -----------------------------------------------------------------------------------------------------------------------------
@@ -74,163 +74,172 @@ static_assert(kTrSmem <= 232448, "shared memory");
 // tiles in [k share, (k + 1) share).  A share is no less than the widest distance of neighbouring tiles, so that every CTA between a unit's first and last tile has one of its tiles.
 // Costs in halves of a key tile with one tile of pairs: with one, with two, and of an item's start and end (one tile of pairs 1300 cycles, two 2000).  Where units are few, they
 // start at a CTA's share each (which costs a CTA a unit at most): a CTA with the end of one and the start of another would be 5 000 cycles later than the others.
-constexpr int kCostOne = 2, kCostTwo = 3, kCostItem = 3, kFewUnits = kNumSMs / 4;
+constexpr int kCostOne = 2, kCostTwo = 3, kCostItem = 4, kFewUnits = kNumSMs / 4;
 
 struct PlanShared {
-  int64_t sums[2][kTreeThreads / 32];
-  int starts[kTreeThreads / 32], first, units;
+  int starts[kTreeThreads / 32], costs[2][kTreeThreads / 32], counts[kTreeThreads / 32], first, units;
   Kv8Cut cut;
 };
 static_assert(sizeof(PlanShared) <= 320, "shared memory");
 
-// exclusive scan over the CTA (one barrier; `sh` is used once); all: of everything
-template <typename T, typename F>
-__device__ __forceinline__ T plan_scan(T x, T none, F op, T* sh, T& all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+// Exclusive scan over the CTA, in two halves with a barrier between them: several go through one barrier, and a scan's shared memory is used once
+template <typename F>
+__device__ __forceinline__ int scan_warp(int x, F op, int* sh) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const T u = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x = op(x, u);
+    const int u = __shfl_up_sync(0xffffffffu, x, o);
+    if ((threadIdx.x & 31) >= o) x = op(x, u);
   }
-  if (lane == 31) sh[warp] = x;
-  const T left = __shfl_up_sync(0xffffffffu, x, 1);
-  __syncthreads();
-  T before = none;
-  all = none;
-#pragma unroll
-  for (int w = 0; w < kTreeThreads / 32; ++w) {
-    const T t = sh[w];
-    if (w < warp) before = op(before, t);
-    all = op(all, t);
-  }
-  return lane ? op(before, left) : before;
+  if ((threadIdx.x & 31) == 31) sh[threadIdx.x >> 5] = x;
+  return __shfl_up_sync(0xffffffffu, x, 1);
 }
-// x / y for quotients up to a few hundred
-__device__ __forceinline__ int small_quotient(int64_t x, int64_t y) {
-  int q = (int)__fdividef((float)x, (float)y);
-  while (q * y > x) --q;
-  while ((q + 1) * y <= x) ++q;
-  return q;
+template <typename F>
+__device__ __forceinline__ int scan_cta(int left, int none, F op, const int* sh, int& all) {
+  constexpr int kWarps = kTreeThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int t = lane < kWarps ? sh[lane] : none;
+#pragma unroll
+  for (int o = 1; o < kWarps; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, t, o);
+    if (lane >= o) t = op(t, u);
+  }
+  all = __shfl_sync(0xffffffffu, t, kWarps - 1);
+  const int before = __shfl_sync(0xffffffffu, t, max(warp - 1, 0));
+  return op(warp ? before : none, lane ? left : none);
 }
 
-// the CTA's units -> table or, where there are more than it holds, p.list; returns their number, and the place of the first in p.list (-1: in the table)
+// the CTA's units -> table or, where there are more than it holds, p.list; returns their number, and the place of the first in p.list (-1: in the table).  Costs of all units are below
+// 2^31 (tree_launch)
 __device__ __forceinline__ int2 tree_plan(const TreeParams& p, int R, int cta, int* scratch, PlanShared* sh, TreeWork* table) {
-  int *const clear = scratch, *const end = scratch + kMostRows, *const count = scratch + 2 * kMostRows;   // of the item that starts with a row (count 0: none does)
+  int *const ctx = scratch, *const end = scratch + kMostRows;   // of rows
+  int *const clear_of = end + kMostRows, *const end_of = clear_of + kMostRows, *const count_of = end_of + kMostRows;   // of the item that starts with a row (count 0: none does)
   const int tid = threadIdx.x, lane = tid & 31, each_rows = (p.T + kTreeThreads - 1) / kTreeThreads, ra = min(p.T, tid * each_rows), rb = min(p.T, ra + each_rows);
   const int tokens = (int)tree_tokens(p);
-  for (int r = ra; r < rb; ++r) {   // what is read below
-    asm volatile("prefetch.global.L1 [%0];" ::"l"(p.ctx_lens + r));
-    for (int w = 0; w < p.words; w += 8) asm volatile("prefetch.global.L1 [%0];" ::"l"(p.masks + (int64_t)r * p.words + w));
-  }
   auto seq_of = [&](int r) { return p.row_to_seq ? __ldg(p.row_to_seq + r) : r; };
+  auto most = [](int a, int b) { return max(a, b); };
+  auto plus = [](int a, int b) { return a + b; };
   if (tid == 0) sh->first = 0x7fffffff, sh->units = 0, sh->cut = {0, 0, 0, 0};
   int start = -1;   // the last row here that starts a run of one sequence
+#pragma unroll 1
   for (int r = ra; r < rb; ++r) {
-    clear[r] = 0x7fffffff, end[r] = 0, count[r] = 0;
-    if (r == 0 || seq_of(r) != seq_of(r - 1)) start = r;
+    const int mine = seq_of(r), before = r > 0 ? seq_of(r - 1) : mine;
+    int c = __ldg(p.ctx_lens + r), e = -1;
+    const uint32_t* m = p.masks + (int64_t)r * p.words;
+#pragma unroll 1
+    for (int w = 0; w < p.words; w += 8) {
+      uint32_t x[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[j] = w + j < p.words ? __ldg(m + w + j) : 0u;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (x[j]) e = 32 * (w + j) + 31 - __clz(x[j]);
+    }
+    c = min(max(c, 0), tokens);
+    ctx[r] = c, end[r] = min(c + e + 1, tokens);   // (tokens and a mask's bits are below 2^31 together)
+    clear_of[r] = 0x7fffffff, end_of[r] = 0, count_of[r] = 0;
+    if (r == 0 || mine != before) start = r;
   }
-  int any;
-  int run = plan_scan(start, -1, [](int a, int b) { return max(a, b); }, sh->starts, any);
-  const int each_max = __reduce_max_sync(0xffffffffu, rb - ra);
-  for (int k = 0; k < each_max; ++k) {
+  int all;
+  const int left = scan_warp(start, most, sh->starts);
+  __syncthreads();
+  int run = scan_cta(left, -1, most, sh->starts, all);
+#pragma unroll 1
+  for (int k = 0; k < each_rows; ++k) {
     const int r = ra + k;
     const bool in = r < rb;
     int r0 = -1, c = 0x7fffffff, e = 0;
     if (in) {
-      if (r == 0 || seq_of(r) != seq_of(r - 1)) run = r;
-      r0 = run + (r - run) / (2 * R) * (2 * R);   // its item's first row
-      c = (int)min((int64_t)max(__ldg(p.ctx_lens + r), 0), (int64_t)tokens);
-      e = c;
-      const uint32_t* m = p.masks + (int64_t)r * p.words;
-      for (int w = 0; w < p.words; w += 8) {
-        uint32_t x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] = w + j < p.words ? __ldg(m + w + j) : 0u;
-#pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (x[j]) e = (int)min((int64_t)c + 32 * (w + j) + 32 - __clz(x[j]), (int64_t)tokens);
-      }
+      if (each_rows == 1 ? start >= 0 : r == 0 || seq_of(r) != seq_of(r - 1)) run = r;
+      r0 = r - (r - run) % (2 * R);   // its item's first row
+      c = ctx[r], e = end[r];
     }
-    const int same = __shfl_sync(0xffffffffu, r0, 0);
-    if (__all_sync(0xffffffffu, r0 == same || !in)) {   // a warp's rows are one item's
+    if (__all_sync(0xffffffffu, r0 == __shfl_sync(0xffffffffu, r0, 0) || !in)) {   // a warp's rows are one item's
       c = __reduce_min_sync(0xffffffffu, c);
       e = __reduce_max_sync(0xffffffffu, e);
       const int n = __reduce_max_sync(0xffffffffu, in ? r - r0 + 1 : 0);
-      if (lane == 0 && in) atomicMin(clear + r0, c), atomicMax(end + r0, e), atomicMax(count + r0, n);
+      if (lane == 0 && in) atomicMin(clear_of + r0, c), atomicMax(end_of + r0, e), atomicMax(count_of + r0, n);
     } else if (in) {
-      atomicMin(clear + r0, c), atomicMax(end + r0, e), atomicMax(count + r0, r - r0 + 1);
+      atomicMin(clear_of + r0, c), atomicMax(end_of + r0, e), atomicMax(count_of + r0, r - r0 + 1);
     }
   }
   __syncthreads();
-  // costs in front (the upper 40 bits) and items (the lower 24)
-  auto tiles_of = [&](int r) { return (end[r] + kTreeKeys - 1) / kTreeKeys; };
-  auto each_of = [&](int r) { return count[r] > R ? kCostTwo : kCostOne; };
-  auto plus = [](int64_t a, int64_t b) { return a + b; };
-  int64_t sum = 0, all;
+  auto tiles_of = [&](int r) { return (end_of[r] + kTreeKeys - 1) / kTreeKeys; };
+  auto each_of = [&](int r) { return count_of[r] > R ? kCostTwo : kCostOne; };
+  int cost = 0, items = 0, n_items, total;
+#pragma unroll 1
   for (int r = ra; r < rb; ++r)
-    if (count[r] > 0) sum += ((int64_t)(kCostItem + max(tiles_of(r), 1) * each_of(r)) << 24) + 1;
-  const int64_t before = plan_scan(sum, (int64_t)0, plus, sh->sums[0], all);
-  const int n_items = (int)(all & 0xffffff), n_units = n_items * p.hkv;
-  int64_t total = (all >> 24) * p.hkv, mine = (before >> 24) * p.hkv, share;
+    if (count_of[r] > 0) cost += kCostItem + max(tiles_of(r), 1) * each_of(r), ++items;
+  const int left_cost = scan_warp(cost, plus, sh->costs[0]), left_items = scan_warp(items, plus, sh->counts);
+  __syncthreads();
+  int mine = scan_cta(left_cost, 0, plus, sh->costs[0], total);
+  const int item0 = scan_cta(left_items, 0, plus, sh->counts, n_items), n_units = n_items * p.hkv;
   const bool few = n_units <= kFewUnits;
-  const int gap = few ? 0 : kCostItem, widest = p.T > R ? kCostTwo : kCostOne;
+  const int gap = few ? 0 : kCostItem;
+  total *= p.hkv, mine *= p.hkv;
+  int share = max(gap + (p.T > R ? kCostTwo : kCostOne), (total + kNumSMs - 1) / kNumSMs);
   auto whole_of = [&](int r) {
-    const int64_t c = gap + (int64_t)max(tiles_of(r), 1) * each_of(r);
-    return few ? small_quotient(c + share - 1, share) * share : c;
+    const int c = gap + max(tiles_of(r), 1) * each_of(r);
+    return few ? (c + share - 1) / share * share : c;
   };
   if (few) {
-    total -= (int64_t)n_units * kCostItem;
-    share = max((int64_t)2 * kCostOne, (total + kNumSMs - n_units - 1) / (kNumSMs - n_units));   // (two groups of softmax warps: two key tiles at least)
-    sum = 0;
-    for (int r = ra; r < rb; ++r)
-      if (count[r] > 0) sum += whole_of(r) * p.hkv;
-    mine = plan_scan(sum, (int64_t)0, plus, sh->sums[1], total);
-  } else {
-    share = max((int64_t)(gap + widest), (total + kNumSMs - 1) / kNumSMs);
+    total -= n_units * kCostItem;
+    share = max(2 * kCostOne, (total + kNumSMs - n_units - 1) / (kNumSMs - n_units));   // (two groups of softmax warps: two key tiles at least)
+    if (n_items > 1) {   // (the only one is at 0)
+      cost = 0;
+#pragma unroll 1
+      for (int r = ra; r < rb; ++r)
+        if (count_of[r] > 0) cost += whole_of(r) * p.hkv;
+      const int left2 = scan_warp(cost, plus, sh->costs[1]);
+      __syncthreads();
+      mine = scan_cta(left2, 0, plus, sh->costs[1], total);
+    }
   }
-  const int64_t lo = cta * share, hi = lo + share;
-  auto emit = [&](auto put) {   // the CTA's units
-    int64_t front = mine;
-    int item = (int)(before & 0xffffff);
+  const int lo = cta * share, hi = lo + share;
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {   // the CTA's units: into the table, and once more, into the list, if they are too many
+    int front = mine, item = item0;
+#pragma unroll 1
     for (int r = ra; r < rb && front < hi; ++r) {
-      if (count[r] == 0) continue;
-      const int nt = tiles_of(r), each = each_of(r), behind = nt > 1 ? gap + (nt - 1) * each : 0;   // behind: of the last tile
-      const int64_t whole = whole_of(r);
-      auto first_tile = [&](int64_t x) {   // the first one, but for tile 0, at or behind this place of the unit's line
-        const uint32_t y = (uint32_t)(x - gap);
-        return x <= gap + each ? 1 : min(nt, (int)(each == kCostTwo ? (y + kCostTwo - 1) / kCostTwo : (y + kCostOne - 1) / kCostOne));
+      if (count_of[r] == 0) continue;
+      const int nt = tiles_of(r), each = each_of(r), behind = nt > 1 ? gap + (nt - 1) * each : 0, whole = whole_of(r);   // behind: of the last tile
+      auto first_tile = [&](int x) {   // the first one, but for tile 0, at or behind this place of the unit's line
+        const int y = x - gap;
+        return y <= each ? 1 : min(nt, each == kCostTwo ? (y + kCostTwo - 1) / kCostTwo : (y + kCostOne - 1) / kCostOne);
       };
-      for (int h = 0; h < p.hkv; ++h, front += whole) {
-        const int64_t last = front + behind;
-        if (front >= hi || last < lo) continue;
+      int u = item++ * p.hkv;
+      const int next = front + whole * p.hkv, skip = front < lo ? min(p.hkv, (lo - front) / whole) : 0;   // heads that end before the share
+      front += skip * whole, u += skip;
+#pragma unroll 1
+      for (int h = skip; h < p.hkv && front < hi; ++h, front += whole, ++u) {
+        const int last = front + behind;
+        if (last < lo) continue;
         TreeWork w;
-        w.rows = {r, count[r], seq_of(r), clear[r], end[r]};
+        w.rows = {r, count_of[r], seq_of(r), clear_of[r], end_of[r]};
         w.kvh = h;
         w.tile0 = front < lo ? first_tile(lo - front) : 0;
         w.tile1 = last < hi ? nt : first_tile(hi - front);
         w.parts = 1, w.slot = 0;
         if (front < lo || last >= hi) {
-          const int back = front < lo ? small_quotient(lo - front + share - 1, share) : 0, ahead = last >= hi ? small_quotient(last - lo, share) : 0;   // CTAs before, behind
+          const int back = front < lo ? (lo - front + share - 1) / share : 0, ahead = last >= hi ? (last - lo) / share : 0;   // CTAs before, behind
           w.parts = back + 1 + ahead;
           w.slot = 2 * cta + (back == 0);
-          if (back == 0) sh->cut = {r, count[r], h, w.parts};
+          if (back == 0) sh->cut = {r, count_of[r], h, w.parts};
         }
-        put(item * p.hkv + h, w);
+        if (pass == 0) {
+          const int place = atomicAdd(&sh->units, 1);
+          if (place < kTreeTable) table[place] = w;
+          atomicMin(&sh->first, u);
+        } else {
+          p.list[u + cta] = w;
+        }
       }
-      ++item;
+      front = next;
     }
-  };
-  emit([&](int u, const TreeWork& w) {
-    const int place = atomicAdd(&sh->units, 1);
-    if (place < kTreeTable) table[place] = w;
-    atomicMin(&sh->first, u);
-  });
-  __syncthreads();
-  const int units = sh->units;
-  if (units <= kTreeTable) return make_int2(units, -1);
-  emit([&](int u, const TreeWork& w) { p.list[u + cta] = w; });
-  __syncthreads();
-  return make_int2(units, sh->first + cta);
+    __syncthreads();
+    const int units = sh->units;
+    if (units <= kTreeTable) return make_int2(units, -1);
+    if (pass) return make_int2(units, sh->first + cta);
+  }
 }
 
 // ---- the walk ---------------------------------------------------------------------------------------------------------------------------
@@ -264,25 +273,32 @@ __device__ __noinline__ void tree_repair(const TreeParams& p, const TreeWork& w,
     const int64_t blk = __ldg(p.block_table + (int64_t)w.rows.seq * p.bt_stride + key / p.block_size);
     if (blk < 0 || blk >= p.n_blocks) return;
     const __nv_bfloat16* v = p.v + ((blk * p.hkv + w.kvh) * p.block_size + key % p.block_size) * kHeadDim + c;
+#pragma unroll 1
     for (int d = 0; d < 32; ++d) {
       const float x = __bfloat162float(v[d]);
       if (!(x - x == 0.f)) to[d] += x;
     }
   };
   bool nan = false;
+#pragma unroll 1
   for (int d = 0; d < 32; ++d) nan |= o[d] != o[d];
   if (nan) {
     float s[32];
+#pragma unroll 1
     for (int d = 0; d < 32; ++d) s[d] = 0.f;
     const int to = min(first, w.tile1) * kTreeKeys;
+#pragma unroll 1
     for (int key = w.tile0 * kTreeKeys; key < to; ++key) add(key, s);
+#pragma unroll 1
     for (int d = 0; d < 32; ++d)
       if (o[d] != o[d] && s[d] != 0.f) o[d] = s[d];
   }
   if (!taken_out) return;
+#pragma unroll 1
   for (int t = first; t < w.tile1; ++t) {
     uint32_t bits[2];
     tree_bits(r, t * kTreeKeys, bits);
+#pragma unroll 1
     for (int j = 0; j < kTreeKeys; ++j) {
       const bool known = t - first < kTrBad;
       if ((bits[j >> 5] >> (j & 31) & 1) && (!known || (bad[t - first][j >> 4] >> (2 * (j & 15)) & 3))) add(t * kTreeKeys + j, o);
@@ -802,11 +818,13 @@ extern "C" int b200_paged_attn_tree(const void* q, int64_t ldq, const void* k_ca
   B200_REQUIRE((reinterpret_cast<uintptr_t>(tree_masks) & 3) == 0, B200_ERR_INVALID, "paged_attn_tree: masks must be 4-byte aligned");
   B200_REQUIRE(scale > 0.f && scale - scale == 0.f, B200_ERR_INVALID, "paged_attn_tree: scale must be positive and finite");
   if (T == 0) return B200_OK;
+  const int64_t tiles = ((int64_t)bt_stride * block_size + kTreeKeys - 1) / kTreeKeys;
+  B200_REQUIRE(T <= kMostRows && (int64_t)T * hkv * (kCostItem + kCostTwo * tiles) < 0x7fffffffll - 4 * kCostTwo * tiles, B200_ERR_UNSUPPORTED,
+               "paged_attn_tree: %d rows of %d kv heads of up to %lld tokens (at most %d rows)", T, hkv, (long long)bt_stride * block_size, kMostRows);
   const int64_t need = b200_paged_attn_tree_workspace_bytes(T, hq, hkv);
   B200_REQUIRE(ws && aligned16(ws) && ws_bytes >= need, B200_ERR_INVALID, "paged_attn_tree: the workspace is 16-byte aligned and has at least %lld bytes (%lld)",
                (long long)need, (long long)ws_bytes);
   B200_REQUIRE(n_blocks * hkv * block_size <= 0x7fffffff - 256, B200_ERR_UNSUPPORTED, "paged_attn_tree: a cache of %lld rows", (long long)(n_blocks * hkv * block_size));
-  B200_REQUIRE(T <= kMostRows && (int64_t)T * hkv <= 0x7fffffff - 2 * kNumSMs, B200_ERR_UNSUPPORTED, "paged_attn_tree: %d rows of %d kv heads (at most %d rows)", T, hkv, kMostRows);
   TreeParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(q);
   p.k = static_cast<const __nv_bfloat16*>(k_cache_layer);
