@@ -52,21 +52,24 @@ __device__ __forceinline__ float entry_of(uint32_t o) {
 }
 constexpr uint32_t kNoEntry = 0x007fu;   // ordered(-inf)
 
+// 0xffff in the halves of x that reach (are above) y's
+__device__ __forceinline__ uint32_t reach(uint32_t x, uint32_t y) {
+  return __hge2_mask(*reinterpret_cast<const __nv_bfloat162*>(&x), *reinterpret_cast<const __nv_bfloat162*>(&y));
+}
+
 // candidates [row][slice][take]: an entry's index (-1: none) and its logit
 template <int J>
-__global__ void __launch_bounds__(kSliceThreads)
+__global__ void __launch_bounds__(kSliceThreads, J == 8 ? 4 : 6)
 beam_slices_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const int32_t* __restrict__ starts, int n_seqs, int n_slices, int vocab, int take,
                    SliceStat* __restrict__ stats, int2* __restrict__ cands) {
-  constexpr int kWarps = kSliceThreads / 32;
+  constexpr int kWarps = kSliceThreads / 32, kWords = 4 * J, kSets = (kWords + 15) / 16;
   __shared__ float sh_m[kWarps];
   __shared__ double sh_s[kWarps];
-  __shared__ int count;
+  __shared__ int count, sum_of[2];
   __shared__ uint2 list[kSliceList];   // ordered entry, index
-  __shared__ int sums[2];
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, slice = blockIdx.x % n_slices, row = blockIdx.x / n_slices;
-  if (row < starts[0] || row >= starts[n_seqs]) return;
   const __nv_bfloat16* l = logits + (int64_t)row * ld;
   const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7);   // groups of eight start at 16-byte addresses: entry i is at place i + shift
   uint4 v[J];
@@ -77,20 +80,27 @@ beam_slices_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const i
     v[j] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
     if (i >= 0 && i + 8 <= vocab) v[j] = ld_stream(l + i);
   }
+  const bool none = row < __ldg(starts) || row >= __ldg(starts + n_seqs);
+  // a group that crosses the row's ends: the first one's, or the last one's (a thread has one of them at most, or the one that is both)
+  const int last = (vocab - 1 - p0) / kLeastSlice;
+  const bool head = p0 < 0 && p0 + 8 > 0, tail = vocab - 1 >= p0 && last < J && p0 + last * kLeastSlice + 8 > vocab;
+  if (head || tail) {
+#pragma unroll 1
+    for (int side = 0; side < 2; ++side) {
+      const int g = side ? last : 0;
+      if (side ? !tail || (head && last == 0) : !head) continue;
+      uint32_t w[4] = {0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u};
 #pragma unroll
-  for (int j = 0; j < J; ++j) {
-    const int i = p0 + j * kLeastSlice;
-    if ((i < 0 && i + 8 > 0) || (i < vocab && i + 8 > vocab)) {   // a group that crosses the row's ends
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int a = i + 2 * k, b = a + 1;
-        const uint32_t x = a >= 0 && a < vocab ? __bfloat16_as_ushort(l[a]) : 0xff80u, y = b >= 0 && b < vocab ? __bfloat16_as_ushort(l[b]) : 0xff80u;
-        w[k] = x | y << 16;
+      for (int k = 0; k < 8; ++k) {
+        const int i = p0 + g * kLeastSlice + k;
+        if (i >= 0 && i < vocab) w[k >> 1] = k & 1 ? (w[k >> 1] & 0xffffu) | (uint32_t)__bfloat16_as_ushort(l[i]) << 16 : (w[k >> 1] & 0xffff0000u) | __bfloat16_as_ushort(l[i]);
       }
-      v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+#pragma unroll
+      for (int j = 0; j < J; ++j)
+        if (j == g) v[j] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   }
+  if (none) return;
   uint32_t h = 0xff80ff80u;
 #pragma unroll
   for (int j = 0; j < J; ++j) h = max2(h, max2(max2(v[j].x, v[j].y), max2(v[j].z, v[j].w)));
@@ -99,9 +109,9 @@ beam_slices_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const i
   if (lane == 0) sh_m[warp] = wm;
   if (tid == 0) count = 0;
   __syncthreads();
-  float m = sh_m[0];
+  float m = sh_m[lane & (kWarps - 1)];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, sh_m[w]);
+  for (int o = kWarps / 2; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   // exp(x - m) = 2^((x - m) log2 e): the difference is exact, or rounded once
   const uint64_t minus = f2::both(m > -INFINITY ? -m : 0.f), log2e = f2::both(1.4426950408889634f);
   uint64_t sum[2] = {0, 0};
@@ -130,78 +140,100 @@ beam_slices_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const i
   }
   if (enough > take) {
     uint32_t low = limit;
-    int reach = enough;
-    while (low < top && reach > take + (take >> 2) + 4) {
+    int got = enough;
+    while (low < top && got > take + (take >> 2) + 4) {
       const uint32_t mid = (low + top + 1) >> 1;
       const int n = __syncthreads_count(key >= mid);
-      if (n >= take) low = mid, reach = n;
+      if (n >= take) low = mid, got = n;
       else top = mid - 1;
     }
     limit = low;
   }
-  // entries that reach the limit -> the list
-  auto each = [&](auto f) {
+  // the entries that reach a number, as bits: 16 words to a set, the word's lower half in bit k, its upper half in bit 16 + k
+  auto reaching = [&](uint32_t least, uint32_t (&bits)[kSets]) {
+    const uint32_t y = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(entry_of(least))) * 0x10001u;
+#pragma unroll
+    for (int q = 0; q < kSets; ++q) bits[q] = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
       const uint32_t w[4] = {v[j].x, v[j].y, v[j].z, v[j].w};
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        f(bf16lo(w[k]), p0 + j * kLeastSlice + 2 * k);
-        f(bf16hi(w[k]), p0 + j * kLeastSlice + 2 * k + 1);
-      }
+      for (int k = 0; k < 4; ++k) bits[(4 * j + k) / 16] |= reach(w[k], y) & (0x10001u << ((4 * j + k) & 15));
     }
   };
-  auto collect = [&](uint32_t least, int most_index) {   // entries above `least`, and those at it up to an index
+  auto index_of = [&](int q, int b) {   // of bit b of set q
+    const int word = 16 * q + (b & 15);
+    return p0 + (word >> 2) * kLeastSlice + 2 * (word & 3) + (b >> 4);
+  };
+  // entries that reach `least`, those at it up to an index -> the list
+  auto collect = [&](uint32_t least, int most_index) {
     if (key >= least) {
-      const float bound = entry_of(least);
-      each([&](float x, int i) {
-        if (x > bound || (x == bound && i <= most_index)) {
-          const int at = atomicAdd(&count, 1);
-          if (at < kSliceList) list[at] = make_uint2(ordered(x), (uint32_t)i);
+      uint32_t bits[kSets];
+      reaching(least, bits);
+#pragma unroll
+      for (int q = 0; q < kSets; ++q)
+#pragma unroll 1
+        for (uint32_t rest = bits[q]; rest; rest &= rest - 1) {
+          const int i = index_of(q, __ffs(rest) - 1);
+          const uint32_t x = ordered(__bfloat162float(l[i]));
+          if (x > least || i <= most_index) {
+            const int at = atomicAdd(&count, 1);
+            if (at < kSliceList) list[at] = make_uint2(x, (uint32_t)i);
+          }
         }
-      });
     }
     __syncthreads();
   };
-  collect(limit, 0x7fffffff);
-  int n = count;
-  if (n > kSliceList) {
+  int from = 0x7fffffff;
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    collect(limit, from);
+    if (pass || count <= kSliceList) break;
     // many entries to a thread, or alike: the exact limit, and the index up to which entries at it count, bit by bit
-    auto total = [&](auto f) {
+    auto total = [&](uint32_t least, int most_index) {
+      uint32_t bits[kSets], above[kSets];
+      reaching(least, bits);
+      reaching(least + 1, above);
       int c = 0;
-      each([&](float x, int i) { c += f(x, i) ? 1 : 0; });
+#pragma unroll
+      for (int q = 0; q < kSets; ++q) {
+        c += __popc(above[q]);
+#pragma unroll 1
+        for (uint32_t rest = bits[q] & ~above[q]; rest; rest &= rest - 1) c += index_of(q, __ffs(rest) - 1) <= most_index;
+      }
       c = __reduce_add_sync(0xffffffffu, c);
       __syncthreads();
-      if (tid == 0) sums[0] = 0;
+      if (tid == 0) sum_of[0] = 0;
       __syncthreads();
-      if (lane == 0) atomicAdd(&sums[0], c);
+      if (lane == 0) atomicAdd(&sum_of[0], c);
       __syncthreads();
-      return sums[0];
+      return sum_of[0];
     };
     uint32_t low = limit, high = ordered(m);
-    while (low < high) {
+    int to = vocab;
+    from = 0;   // the smallest index that is enough
+#pragma unroll 1
+    while (low < high || from < to) {
+      const bool keys = low < high;
       const uint32_t mid = (low + high + 1) >> 1;
-      const float bound = entry_of(mid);
-      if (total([&](float x, int) { return x >= bound; }) >= take) low = mid;
-      else high = mid - 1;
+      const int at = (from + to) >> 1;
+      const bool is = total(keys ? mid : low, keys ? 0x7fffffff : at) >= take;
+      if (keys && is) low = mid;
+      else if (keys) high = mid - 1;
+      else if (is) to = at;
+      else from = at + 1;
     }
-    const float bound = entry_of(low);
-    int from = 0, to = vocab;   // the smallest index that is enough
-    while (from < to) {
-      const int mid = (from + to) >> 1;
-      if (total([&](float x, int i) { return x > bound || (x == bound && i <= mid); }) >= take) to = mid;
-      else from = mid + 1;
-    }
+    limit = low;
     if (tid == 0) count = 0;
     __syncthreads();
-    collect(low, from);
-    n = count;
   }
+  const int n = count;
   int2* out = cands + (int64_t)blockIdx.x * take;
   for (int e = tid; e < max(n, take); e += kSliceThreads) {
     if (e < n) {
       const uint2 x = list[e];
       int rank = 0;
+#pragma unroll 4
       for (int k = 0; k < n; ++k) {
         const uint2 y = list[k];
         rank += y.x > x.x || (y.x == x.x && y.y < x.y);
@@ -222,6 +254,22 @@ __device__ __forceinline__ uint64_t id_of(int row, float x, int entry) { return 
 __device__ __forceinline__ int row_of(uint64_t id) { return (int)(id >> 48); }
 __device__ __forceinline__ bool better(double s, uint64_t id, double t, uint64_t od) { return s > t || (s == t && id < od); }
 
+// the log-sum of a row, its largest logit at m: an eighth of the entries
+__device__ __noinline__ double row_part(const __nv_bfloat16* row, int from, int to, double m) {
+  double sum = 0.0;
+  for (int k = from + threadIdx.x; k < to; k += kMergeThreads) sum += exp((double)__bfloat162float(row[k]) - m);
+  return sum;
+}
+__device__ __noinline__ double row_base(const float* scores, int r, double m, double sum) {
+  const double base = (scores ? (double)scores[r] : 0.0) - (m + log(sum));
+  return base - base == 0.0 ? base : -INFINITY;
+}
+__device__ __forceinline__ uint32_t ordered_f32(float x) {
+  const uint32_t b = __float_as_uint(x);
+  return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float f32_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
+
 __global__ void __launch_bounds__(kMergeThreads) __cluster_dims__(kMergeCtas, 1, 1)
 beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const float* __restrict__ scores, const int32_t* __restrict__ starts, int n_rows, int n_slices,
                   int vocab, int take, const SliceStat* __restrict__ stats, const int2* __restrict__ cands, RowStat* rows, double* parts, int32_t* out_rows,
@@ -231,151 +279,179 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
   __shared__ uint64_t sh_id[kMergeList];
   __shared__ Best sorted[kMostTake + 1];
   __shared__ int need[2 * kMergeList], n_need, n_list, seen_all;
+  __shared__ uint32_t asked_for[kMergeList / 32];   // rows of the sequence that are in need (of the first kMergeList)
   __shared__ Best limit;
   pdl_wait();
   const cg::cluster_group cluster = cg::this_cluster();
   const int cta = (int)cluster.block_rank(), seq = blockIdx.x / kMergeCtas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int r0 = min(max(starts[seq], 0), n_rows), r1 = min(max(starts[seq + 1], r0), n_rows);
-  // log-sums of the rows
-  for (int r = r0 + warp; r < r1; r += kWarps) {
-    const SliceStat* st = stats + (int64_t)r * n_slices;
-    float m = -INFINITY;
-    for (int i = lane; i < n_slices; i += 32) m = fmaxf(m, st[i].m);
-    m = warp_max(m);
-    double s = 0.0;
-    for (int i = lane; i < n_slices; i += 32) s += st[i].sum * exp((double)st[i].m - (double)m);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (lane == 0) {
-      const double base = (scores ? (double)scores[r] : 0.0) - ((double)m + log(s));
-      rows[r] = {base - base == 0.0 ? base : -INFINITY, kNear};
-    }
-  }
-  __syncthreads();
   const int per_row = n_slices * take;
-  const int64_t n_cands = (int64_t)(r1 - r0) * per_row;
-  const int2* mine = cands + (int64_t)r0 * per_row;
-  bool exact = false;   // every row added up in fp64
-  for (;;) {
-    auto each = [&](auto f) {   // the thread's share of the candidates
-      for (int64_t i = tid; i < n_cands; i += kMergeThreads) {
-        const int2 c = mine[i];
-        const int r = r0 + (int)(i / per_row);
-        const double s = rows[r].base + (double)__int_as_float(c.y);
-        if (c.x >= 0 && s > -INFINITY) f(s, id_of(r, __int_as_float(c.y), c.x));
+  auto top_of = [&](int r) {   // a row's largest logit
+    float m = -INFINITY;
+#pragma unroll 1
+    for (int i = lane; i < n_slices; i += 32) m = fmaxf(m, stats[(int64_t)r * n_slices + i].m);
+    return warp_max(m);
+  };
+  if (cta == 0) {
+    // log-sums of the rows
+#pragma unroll 1
+    for (int r = r0 + warp; r < r1; r += kWarps) {
+      const SliceStat* st = stats + (int64_t)r * n_slices;
+      const float m = top_of(r);
+      double s = 0.0;
+#pragma unroll 1
+      for (int i = lane; i < n_slices; i += 32) {
+        const float d = st[i].m - m;   // (exact, or rounded once; both -inf: no number, as the sum of a row that has none)
+        s += st[i].sum * (double)tc::exp2_fast(d * 1.4426950408889634f);
       }
-    };
-    // the largest of each thread; what take + 1 of them reach, the take + 1 best reach
-    double s = -INFINITY;
-    uint64_t id = ~0ull;
-    each([&](double t, uint64_t od) {
-      if (better(t, od, s, id)) s = t, id = od;
-    });
-    sh_s[tid] = s, sh_id[tid] = id;
-    if (tid == 0) limit = {-INFINITY, ~0ull}, n_list = 0, n_need = 0, seen_all = 1;
-    __syncthreads();
-    int rank = 0;
-    for (int k = 0; k < kMergeThreads; ++k) rank += better(sh_s[k], sh_id[k], s, id);
-    if (rank == take && id != ~0ull) limit = {s, id};
-    __syncthreads();
-    double margin = exact ? 0.0 : 2 * kNear;
-    for (;;) {
-      const Best b = limit;
-      each([&](double t, uint64_t od) {
-        if (t > b.s - margin || !better(b.s, b.id, t, od)) {
-          const int at = atomicAdd(&n_list, 1);
-          if (at < kMergeList) sh_s[at] = t, sh_id[at] = od;
-        }
-      });
-      __syncthreads();
-      if (n_list <= kMergeList) break;
-      // too many: the entry behind the best `take` of those that found room is a limit nearer to the end.  Those next to it are not all seen
-      for (int e = tid; e < kMergeList; e += kMergeThreads) {
-        int before = 0;
-        for (int k = 0; k < kMergeList; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
-        if (before == take) limit = {sh_s[e], sh_id[e]};
-      }
-      __syncthreads();
-      if (tid == 0) n_list = 0, seen_all = margin == 0.0 && seen_all;
-      margin = 0.0;
-      __syncthreads();
-    }
-    const int n = n_list;
-    for (int e = tid; e < n; e += kMergeThreads) {
-      int before = 0;
-      for (int k = 0; k < n; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
-      if (before <= take) sorted[before] = {sh_s[e], sh_id[e]};
-    }
-    __syncthreads();
-    if (!exact) {
-      // candidates of two rows that are nearer to each other than their sums are good for
-      auto compare = [&](const Best& a, double t, uint64_t od) {
-        const int ra = row_of(a.id), rb = row_of(od);
-        if (ra == rb) return;
-        const double na = rows[ra].near, nb = rows[rb].near;
-        if (na + nb > 0.0 && fabs(a.s - t) <= na + nb) {
-          const int at = atomicAdd(&n_need, 2);
-          need[at] = na > 0.0 ? ra : -1, need[at + 1] = nb > 0.0 ? rb : -1;
-        }
-      };
-      if (tid < take && tid + 1 < n) compare(sorted[tid], sorted[tid + 1].s, sorted[tid + 1].id);
-      if (n > take)
-        for (int e = tid; e < n; e += kMergeThreads) {   // (those before the last one taken are compared above)
-          const Best last = sorted[take - 1];
-          if (better(last.s, last.id, sh_s[e], sh_id[e])) compare(last, sh_s[e], sh_id[e]);
-        }
-      __syncthreads();
-      const int wanted = seen_all ? n_need : r1 - r0;
-      if (wanted > 0) {   // (the same in every CTA of the cluster)
-        exact = !seen_all;
-        auto wanted_row = [&](int i) {   // -1: none, or one that came before
-          if (!seen_all) return r0 + i;
-          for (int k = 0; k < i; ++k)
-            if (need[k] == need[i]) return -1;
-          return need[i];
-        };
-        const int from = (int)((int64_t)vocab * cta / kMergeCtas), to = (int)((int64_t)vocab * (cta + 1) / kMergeCtas);
-        for (int i = 0; i < wanted; ++i) {
-          const int r = wanted_row(i);
-          if (r < 0) continue;
-          float m = -INFINITY;
-          for (int k = 0; k < n_slices; ++k) m = fmaxf(m, stats[(int64_t)r * n_slices + k].m);
-          double sum = 0.0;
-          for (int k = from + tid; k < to; k += kMergeThreads) sum += exp((double)__bfloat162float(logits[(int64_t)r * ld + k]) - (double)m);
 #pragma unroll
-          for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-          __syncthreads();
-          if (lane == 0) sh_sum[warp] = sum;
-          __syncthreads();
-          if (tid == 0) {
-            for (int w = 1; w < kWarps; ++w) sum += sh_sum[w];
-            parts[(int64_t)r * kMergeCtas + cta] = sum;
+      for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+      if (lane == 0) rows[r] = {row_base(scores, r, (double)m, s), kNear};
+    }
+    __syncthreads();
+  }
+  bool exact = false;   // every row added up in fp64
+#pragma unroll 1
+  for (;;) {
+    if (cta == 0) {
+      auto each = [&](auto f) {   // the thread's share of the candidates
+#pragma unroll 1
+        for (int r = r0; r < r1; ++r) {
+          const double base = rows[r].base;
+          if (base == -INFINITY) continue;
+          const int2* mine = cands + (int64_t)r * per_row;
+#pragma unroll 2
+          for (int i = tid; i < per_row; i += kMergeThreads) {
+            const int2 c = mine[i];
+            if (c.x >= 0) f(base + (double)__int_as_float(c.y), id_of(r, __int_as_float(c.y), c.x));
           }
         }
-        __threadfence();
-        cluster.sync();
-        for (int i = tid; i < wanted; i += kMergeThreads) {
-          const int r = wanted_row(i);
-          if (r < 0) continue;
-          float m = -INFINITY;
-          for (int k = 0; k < n_slices; ++k) m = fmaxf(m, stats[(int64_t)r * n_slices + k].m);
-          double sum = 0.0;
-          for (int k = 0; k < kMergeCtas; ++k) sum += __ldcg(parts + (int64_t)r * kMergeCtas + k);
-          const double base = (scores ? (double)scores[r] : 0.0) - ((double)m + log(sum));
-          rows[r] = {base - base == 0.0 ? base : -INFINITY, 0.0};
+      };
+      // the largest of each thread; a number that more than `take` of them reach, and few more, as fp32 (rounded down)
+      double best = -INFINITY;
+      each([&](double t, uint64_t) { best = fmax(best, t); });
+      const uint32_t key = ordered_f32(__double2float_rd(best));
+      if (tid == 0) n_list = 0, n_need = 0, seen_all = 1;
+      if (tid < kMergeList / 32) asked_for[tid] = 0;
+      uint32_t low = ordered_f32(-INFINITY) + 1, high = ordered_f32(INFINITY);
+      int got = __syncthreads_count(key >= low);
+      const bool limited = got > take;
+#pragma unroll 1
+      while (limited && low < high && got > take + 1 + (take >> 2) + 4) {
+        const uint32_t mid = low + ((high - low + 1) >> 1);
+        const int n = __syncthreads_count(key >= mid);
+        if (n > take) low = mid, got = n;
+        else high = mid - 1;
+      }
+      if (tid == 0) limit = {limited ? (double)f32_of(low) : -INFINITY, ~0ull};
+      __syncthreads();
+      double margin = exact ? 0.0 : 2 * kNear;
+#pragma unroll 1
+      for (;;) {
+        const Best b = limit;
+        each([&](double t, uint64_t od) {
+          if (t > b.s - margin || !better(b.s, b.id, t, od)) {
+            const int at = atomicAdd(&n_list, 1);
+            if (at < kMergeList) sh_s[at] = t, sh_id[at] = od;
+          }
+        });
+        __syncthreads();
+        if (n_list <= kMergeList) break;
+        // too many: the entry behind the best `take` of those that found room is a limit nearer to the end.  Those next to it are not all seen
+#pragma unroll 1
+        for (int e = tid; e < kMergeList; e += kMergeThreads) {
+          int before = 0;
+#pragma unroll 1
+          for (int k = 0; k < kMergeList; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
+          if (before == take) limit = {sh_s[e], sh_id[e]};
         }
-        cluster.sync();   // (nobody writes a row's parts again, or its numbers, while another reads)
-        continue;
+        __syncthreads();
+        if (tid == 0) n_list = 0, seen_all = margin == 0.0 && seen_all;
+        margin = 0.0;
+        __syncthreads();
+      }
+      const int n = n_list;
+#pragma unroll 1
+      for (int e = tid; e < n; e += kMergeThreads) {
+        int before = 0;
+#pragma unroll 2
+        for (int k = 0; k < n; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
+        if (before <= take) sorted[before] = {sh_s[e], sh_id[e]};
+      }
+      __syncthreads();
+      if (!exact) {
+        // candidates of two rows that are nearer to each other than their sums are good for: neighbours among those taken, and the last of them and whatever comes behind
+#pragma unroll 1
+        for (int e = tid; e < take + n; e += kMergeThreads) {
+          const int k = e < take ? e : take - 1;
+          if (k >= n || (e < take && e + 1 >= n)) continue;
+          const Best a = sorted[k], c = e < take ? sorted[e + 1] : Best{sh_s[e - take], sh_id[e - take]};
+          if (!better(a.s, a.id, c.s, c.id)) continue;
+          const int ra = row_of(a.id), rb = row_of(c.id);
+          const double na = rows[ra].near, nb = rows[rb].near;
+          if (ra != rb && na + nb > 0.0 && a.s - c.s <= na + nb) {
+#pragma unroll 1
+            for (int side = 0; side < 2; ++side) {
+              const int r = side ? rb : ra;
+              if (!((side ? nb : na) > 0.0)) continue;
+              const uint32_t bit = 1u << ((r - r0) & 31);
+              if (r - r0 < kMergeList && (atomicOr(&asked_for[(r - r0) >> 5], bit) & bit)) continue;
+              need[atomicAdd(&n_need, 1)] = r;   // (two for each of n entries at most)
+            }
+          }
+        }
+        __syncthreads();
+      }
+      const bool all_rows = !exact && !seen_all;
+      if (tid == 0 && all_rows) n_need = -1;
+      if (exact || (n_need == 0 && !all_rows)) {
+#pragma unroll 1
+        for (int k = tid; k < take; k += kMergeThreads) {
+          const int64_t at = (int64_t)seq * take + k;
+          out_rows[at] = k < n ? row_of(sorted[k].id) : -1;
+          out_tokens[at] = k < n ? (int)(uint32_t)sorted[k].id : -1;
+          out_scores[at] = k < n ? (float)sorted[k].s : -INFINITY;
+        }
+      }
+      exact = exact || all_rows;
+    }
+    cluster.sync();   // the other CTAs have waited here: their help is asked for where n_need is not 0 (-1: all rows)
+    const int* asked = cluster.map_shared_rank(&n_need, 0);
+    const int* list = cluster.map_shared_rank(need, 0);
+    const int wanted = *asked < 0 ? r1 - r0 : *asked;
+    const bool by_list = *asked >= 0;
+    const int from = (int)((int64_t)vocab * cta / kMergeCtas), to = (int)((int64_t)vocab * (cta + 1) / kMergeCtas);
+    auto wanted_row = [&](int i) { return by_list ? list[i] : r0 + i; };
+#pragma unroll 1
+    for (int i = 0; i < wanted; ++i) {
+      const int r = wanted_row(i);
+      double sum = row_part(logits + (int64_t)r * ld, from, to, (double)top_of(r));
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      __syncthreads();
+      if (lane == 0) sh_sum[warp] = sum;
+      __syncthreads();
+      if (tid == 0) {
+        for (int w = 1; w < kWarps; ++w) sum += sh_sum[w];
+        parts[(int64_t)r * kMergeCtas + cta] = sum;
       }
     }
-    if (cta == 0)
-      for (int k = tid; k < take; k += kMergeThreads) {
-        const int64_t at = (int64_t)seq * take + k;
-        out_rows[at] = k < n ? row_of(sorted[k].id) : -1;
-        out_tokens[at] = k < n ? (int)(uint32_t)sorted[k].id : -1;
-        out_scores[at] = k < n ? (float)sorted[k].s : -INFINITY;
+    __threadfence();
+    cluster.sync();   // (and nobody has left while another one reads its list)
+    if (wanted == 0) return;
+    if (cta == 0) {
+#pragma unroll 1
+      for (int i = warp; i < wanted; i += kWarps) {
+        const int r = wanted_row(i);
+        const float m = top_of(r);
+        if (lane == 0) {
+          double sum = 0.0;
+          for (int k = 0; k < kMergeCtas; ++k) sum += __ldcg(parts + (int64_t)r * kMergeCtas + k);
+          rows[r] = {row_base(scores, r, (double)m, sum), 0.0};
+        }
       }
-    return;
+      __syncthreads();
+    }
   }
 }
 
