@@ -63,14 +63,19 @@ accept_tree_kernel(const int32_t* __restrict__ target, const int32_t* __restrict
 
 // Moves of a group happen at once: whatever is read is what was there before.  A CTA takes pieces of rows ("units": a column range of a plane) of one group; all the
 // group's moves of a unit go through its shared memory, loads first, then, behind a barrier, stores.  Two halves of it: one batch of units is stored while the next is on its
-// way.  Bound by bytes, or by the launch where they are few.
-constexpr int kMoveThreads = 256, kMoveStage = 32768, kMostGroup = 1024, kMoveCtas = 3 * kNumSMs, kMoveColumns = 4096;
+// way.  A thread keeps its column and steps through (unit, move) by additions; where a unit lies is worked out once a batch (with divisions for every 16 bytes 2 MB states of 16 x 8
+// beams took 254 us).  Bound by bytes, or by the launch where they are few.
+constexpr int kMoveThreads = 256, kMoveStage = 32768, kMostGroup = 1024, kMoveUnits = 128, kMoveCtas = 3 * kNumSMs, kMoveColumns = 4096;
 
+struct MoveUnit {
+  unsigned char* base;
+  int64_t left;   // bytes of the row from here on
+};
 struct MoveParams {
   unsigned char *a, *b;
   int64_t layer_stride, row_bytes, slots;
   const int32_t *src, *dst, *starts;
-  int layers, heads, block_size, max_group, splits, columns;   // splits: CTAs of a group; columns: bytes of a unit's row
+  int layers, heads, block_size, max_group, splits, columns, piece_bits;   // splits: CTAs of a group; columns: bytes of a unit's row, 2^piece_bits pieces
 };
 
 template <int VEC>
@@ -87,10 +92,11 @@ __device__ __forceinline__ void move_out(unsigned char* to, const unsigned char*
 }
 
 template <int VEC>
-__global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const MoveParams p) {
-  extern __shared__ __align__(16) unsigned char stage[];   // two halves
-  __shared__ int64_t from[kMostGroup], to[kMostGroup];
+__global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const __grid_constant__ MoveParams p) {
+  extern __shared__ __align__(16) unsigned char stage[];   // two halves, then where moves come from and go to
+  __shared__ MoveUnit where[3][kMoveUnits];   // (of the batch that is stored, the next one, and of the one before, which a slow warp may still store)
   __shared__ int n_valid;
+  int64_t *const from = reinterpret_cast<int64_t*>(stage + 2 * kMoveStage), *const to = from + p.max_group;
   pdl_wait();
   pdl_launch_dependents();
   const int g = blockIdx.x / p.splits, part = blockIdx.x % p.splits, tid = threadIdx.x;
@@ -108,58 +114,61 @@ __global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const MovePara
   __syncthreads();
   const int m = n_valid;
   if (m == 0) return;
-  const int per_plane = (int)((p.row_bytes + p.columns - 1) / p.columns), pieces = p.columns / VEC;
-  const int units = (p.b ? 2 : 1) * p.layers * p.heads * per_plane;
+  const int per_plane = (int)((p.row_bytes + p.columns - 1) / p.columns), units = (p.b ? 2 : 1) * p.layers * p.heads * per_plane;
   const int u0 = (int)((int64_t)units * part / p.splits), u1 = (int)((int64_t)units * (part + 1) / p.splits);
-  const int batch = max(1, kMoveStage / (m * p.columns));
-  // item e of a batch: (unit, move, piece); its address in the caches, or null behind a row's end
-  auto item = [&](int u, int mv, int piece, const int64_t* where) -> unsigned char* {
-    const int plane = u / per_plane, head = plane % p.heads, layer = plane / p.heads;
-    const int64_t col = (int64_t)(u - plane * per_plane) * p.columns + piece * VEC;
-    if (col >= p.row_bytes) return nullptr;
-    unsigned char* base = layer < p.layers ? p.a + layer * p.layer_stride : p.b + (layer - p.layers) * p.layer_stride;
-    return base + (int64_t)head * p.block_size * p.row_bytes + where[mv] + col;
-  };
-  auto walk = [&](int u, int count, auto f) {
-    const int items = count * m * pieces;
-    for (int e = tid; e < items; e += kMoveThreads) {
-      const int piece = e % pieces, x = e / pieces;
-      f(e, u + x / m, x % m, piece);
+  const int batch = min(kMoveUnits, max(1, kMoveStage / (m * p.columns)));
+  // a thread's column (or columns, kMoveThreads pieces apart) and its steps through the pairs of unit and move
+  const int piece0 = tid & ((1 << p.piece_bits) - 1), lanes = max(1, kMoveThreads >> p.piece_bits), first = p.piece_bits < 31 ? tid >> p.piece_bits : 0;
+  const int unit_step = lanes / m, move_step = lanes % m, unit0 = first / m, move0 = first % m;
+  auto find = [&](int u, int count, MoveUnit* w) {
+    if (tid < count) {
+      const int plane = (u + tid) / per_plane, head = plane % p.heads, layer = plane / p.heads;
+      const int64_t col = (int64_t)(u + tid - plane * per_plane) * p.columns;
+      unsigned char* const base = layer < p.layers ? p.a + layer * p.layer_stride : p.b + (layer - p.layers) * p.layer_stride;
+      w[tid] = {base + (int64_t)head * p.block_size * p.row_bytes + col, p.row_bytes - col};
     }
   };
-  auto load = [&](int u, int count, unsigned char* half) {
-    walk(u, count, [&](int e, int unit, int mv, int piece) {
-      const unsigned char* src = item(unit, mv, piece, from);
-      if (src) move_in<VEC>(half + e * VEC, src);
-    });
+  auto walk = [&](int count, const MoveUnit* w, const int64_t* moves, auto f) {   // f(place in the half, address) for all of the thread's
+    for (int unit = unit0, mv = move0; unit < count;) {
+      const MoveUnit t = w[unit];
+      unsigned char* const at = t.base + moves[mv];
+      const int e = (unit * m + mv) << p.piece_bits;
+      for (int piece = piece0; piece < 1 << p.piece_bits; piece += kMoveThreads)
+        if (piece * VEC < t.left) f((e + piece) * VEC, at + piece * VEC);
+      unit += unit_step, mv += move_step;
+      if (mv >= m) mv -= m, ++unit;
+    }
+  };
+  auto load = [&](int count, const MoveUnit* w, int half) {
+    walk(count, w, from, [&](int e, const unsigned char* src) { move_in<VEC>(stage + half * kMoveStage + e, src); });
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-  auto count_at = [&](int u) { return min(batch, u1 - u); };
-  int half = 0;
-  if (u0 < u1) load(u0, count_at(u0), stage);
+  auto count_at = [&](int u) { return max(0, min(batch, u1 - u)); };
+  find(u0, count_at(u0), where[0]);
+  __syncthreads();
+  load(count_at(u0), where[0], 0);
+  int half = 0, w = 0;
   for (int u = u0; u < u1; u += batch, half ^= 1) {
-    const int next = u + batch;
-    if (next < u1) {
-      load(next, count_at(next), stage + (half ^ 1) * kMoveStage);
+    const int more = count_at(u + batch), next = w == 2 ? 0 : w + 1;
+    find(u + batch, more, where[next]);
+    __syncthreads();   // (the other half has been stored, and its units are there)
+    if (more) {
+      load(more, where[next], half ^ 1);
       asm volatile("cp.async.wait_group 1;" ::: "memory");
     } else {
       asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     __syncthreads();
-    const unsigned char* st = stage + half * kMoveStage;
-    walk(u, count_at(u), [&](int e, int unit, int mv, int piece) {
-      unsigned char* dst = item(unit, mv, piece, to);
-      if (dst) move_out<VEC>(dst, st + e * VEC);
-    });
-    __syncthreads();   // (the half is free again)
+    walk(count_at(u), where[w], to, [&](int e, unsigned char* dst) { move_out<VEC>(dst, stage + half * kMoveStage + e); });
+    w = next;
   }
 }
 
 template <int VEC>
 int move_launch(const MoveParams& p, int n_groups, cudaStream_t s) {
   static bool done[64] = {};
-  B200_CUDA(ensure_dynamic_smem(cache_move_kernel<VEC>, 2 * kMoveStage, done));
-  B200_CUDA(launch(cache_move_kernel<VEC>, dim3((unsigned)(n_groups * p.splits)), dim3(kMoveThreads), (size_t)(2 * kMoveStage), s, p));
+  B200_CUDA(ensure_dynamic_smem(cache_move_kernel<VEC>, 2 * kMoveStage + kMostGroup * 16, done));
+  B200_CUDA(launch(cache_move_kernel<VEC>, dim3((unsigned)(n_groups * p.splits)), dim3(kMoveThreads), (size_t)(2 * kMoveStage + p.max_group * 16), s, p));
   return B200_OK;
 }
 
@@ -197,10 +206,10 @@ extern "C" int b200_cache_move(void* cache_a, void* cache_b, int32_t n_layers, i
   const uint64_t all = reinterpret_cast<uintptr_t>(cache_a) | reinterpret_cast<uintptr_t>(cache_b) | (uint64_t)row_bytes | (n_layers > 1 ? (uint64_t)layer_stride : 0);
   const int vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
   MoveParams p = {static_cast<unsigned char*>(cache_a), static_cast<unsigned char*>(cache_b), layer_stride, row_bytes, n_blocks * block_size, src_slots, dst_slots, group_starts,
-                  n_layers, heads, block_size, max_group, 1, vec};
+                  n_layers, heads, block_size, max_group, 1, vec, 0};
   // a unit's row: as much of a row as leaves room for all moves of a group
   const int64_t room = std::min<int64_t>(kMoveStage / max_group, kMoveColumns);
-  while (2 * p.columns <= room && p.columns < row_bytes) p.columns *= 2;
+  while (2 * p.columns <= room && p.columns < row_bytes) p.columns *= 2, ++p.piece_bits;
   const __int128 units = (__int128)(cache_b ? 2 : 1) * n_layers * heads * ((row_bytes + p.columns - 1) / p.columns);
   B200_REQUIRE(units < 0x7fffffff, B200_ERR_UNSUPPORTED, "cache_move: rows of %lld bytes in %d planes", (long long)row_bytes, n_layers * heads);
   p.splits = (int)std::min<int64_t>((int64_t)units, std::max(1, kMoveCtas / n_groups));
