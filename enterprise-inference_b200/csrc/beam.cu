@@ -4,8 +4,8 @@
 // blocks: a warp takes 2 048 neighbouring logits, all in registers at once, and leaves their largest, m, and the sum of exp(x - m).  No barriers, nothing is selected.
 // merge: a cluster takes a sequence.  One of its CTAs joins the blocks' sums; a number that more than K blocks' largest scores reach bounds the K-th score from below, and only
 // the blocks that reach it, little more than K, are read again.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
-// is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in fp64 (an eighth
-// of the entries to a CTA) and the CTA picks again.  Entries of one row never need it.
+// is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in fp64 (half of the entries
+// to a CTA) and the CTA picks again.  Entries of one row never need it.
 // Bound by the bytes of the logits.
 #include <cooperative_groups.h>
 
@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kBlockThreads = 256, kBlockGroups = 8, kBlock = 32 * 8 * kBlockGroups, kBlockCtas = 4 * kNumSMs;
 constexpr int kMostTake = 128, kMostVocab = 393216;
-constexpr int kMergeThreads = 256, kMergeCtas = 8, kMergeList = 1024, kKnownRows = 64;
+constexpr int kMergeThreads = 1024, kMergeCtas = 2, kMergeList = 1024, kKnownRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 // What a row's log-sum may be off by: exponents of base 2 are rounded once (2^-24 of up to 17 in the mean over the weights, times ln 2: 7e-7) and have log2 e to 2^-26 (2e-7), the
 // hardware's exponential has 2^-22 (2.4e-7), for a term and for its block's largest, and nine sums and products follow one another in a lane (5e-7); behind them everything is fp64
@@ -154,7 +154,7 @@ __device__ __noinline__ double row_base(const float* scores, int r, double m, do
   const double base = (scores ? (double)scores[r] : 0.0) - (m + log(sum));
   return base - base == 0.0 ? base : -INFINITY;
 }
-__global__ void __launch_bounds__(kMergeThreads, 3) __cluster_dims__(kMergeCtas, 1, 1)
+__global__ void __launch_bounds__(kMergeThreads, 1) __cluster_dims__(kMergeCtas, 1, 1)
 beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const float* __restrict__ scores, const int32_t* __restrict__ starts, int n_rows, int per_row, int vocab, int take,
                   const float2* __restrict__ stats, RowStat* rows, double* parts, int32_t* out_rows, int32_t* out_tokens, float* out_scores) {
   constexpr int kWarps = kMergeThreads / 32;
@@ -212,9 +212,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         if (lane == 0) sh_sum[warp] = (double)wm;
         int got = __syncthreads_count(top > -INFINITY);
         if (got <= take) return -INFINITY;
-        float most = (float)sh_sum[lane & (kWarps - 1)];
-#pragma unroll
-        for (int o = kWarps / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, o));
+        const float most = warp_max_redux((float)sh_sum[lane & (kWarps - 1)]);
         uint32_t high = ordered_f32(most), low = high;
         float step = 0.5f;
         got = 0;
@@ -226,7 +224,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           got = __syncthreads_count(top >= f32_of(low));
         }
 #pragma unroll 1
-        while (low < high && got > take + 1 + (take >> 2) + 4) {
+        while (low < high && got > take + 1 + (take >> 1) + 8) {
           const uint32_t half = low + ((high - low + 1) >> 1);
           const int n = __syncthreads_count(top >= f32_of(half));
           if (n > take) low = half, got = n;
@@ -267,13 +265,17 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           uint32_t hot = 0;
 #pragma unroll
           for (int j = 0; j < kBlockGroups; ++j) hot |= (max8(v[j]) >= x0 ? 1u : 0u) << j;
-          // (few lanes have one: they read it again)
 #pragma unroll 1
-          for (; hot; hot &= hot - 1) {
-            const int i0 = p0 + (__ffs(hot) - 1) * 256;
+          for (; hot; hot &= hot - 1) {   // (few lanes have one)
+            const int g = __ffs(hot) - 1;
+            uint4 w = v[0];
+#pragma unroll
+            for (int j = 1; j < kBlockGroups; ++j)
+              if (j == g) w = v[j];
 #pragma unroll 1
-            for (int i = max(i0, 0); i < min(i0 + 8, vocab); ++i) {
-              const float x = __bfloat162float(logits[(int64_t)r * ld + i]);
+            for (int i = p0 + g * 256, end = i + 8; i < end; ++i) {   // (outside the row: -inf)
+              const float x = bf16lo(w.x);
+              w.x = __funnelshift_r(w.x, w.y, 16), w.y = __funnelshift_r(w.y, w.z, 16), w.z = __funnelshift_r(w.z, w.w, 16), w.w >>= 16;
               const double t = base + (double)x;
               if (x > -INFINITY && t >= least) f(t, id_of(r, x, i));
             }
@@ -316,7 +318,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
 #pragma unroll 1
       for (int e = tid; e < n; e += kMergeThreads) {
         int before = 0;
-#pragma unroll 2
+#pragma unroll 4
         for (int k = 0; k < n; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
         if (before <= take) sorted[before] = {sh_s[e], sh_id[e]};
       }
@@ -379,7 +381,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         parts[(int64_t)r * kMergeCtas + cta] = sum;
       }
     }
-    __threadfence();
+    if (wanted > 0) __threadfence();
     cluster.sync();   // (and nobody has left while another one reads its list)
     if (wanted == 0) return;
     if (cta == 0) {
@@ -423,7 +425,7 @@ extern "C" int b200_beam_select(const void* logits, int64_t ld, const float* sco
   B200_REQUIRE(vocab <= kMostVocab, B200_ERR_UNSUPPORTED, "beam_select: vocab=%d (at most %d)", vocab, kMostVocab);
   B200_REQUIRE(n_select <= kMostTake, B200_ERR_UNSUPPORTED, "beam_select: %d to select (at most %d)", n_select, kMostTake);
   B200_REQUIRE(n_rows <= 65535, B200_ERR_UNSUPPORTED, "beam_select: %d rows (at most 65535)", n_rows);
-  B200_REQUIRE(n_seqs <= 0x7fffffff / kMergeCtas, B200_ERR_UNSUPPORTED, "beam_select: %d sequences (at most %d)", n_seqs, 0x7fffffff / kMergeCtas);
+  B200_REQUIRE(n_seqs < 1 << 28, B200_ERR_UNSUPPORTED, "beam_select: %d sequences (at most 2^28 - 1)", n_seqs);
   if (n_seqs == 0) return B200_OK;
   const int64_t need = n_rows > 0 ? beam_select_workspace_bytes(n_rows, vocab) : 0;
   B200_REQUIRE(need == 0 || (ws && (reinterpret_cast<uintptr_t>(ws) & 15) == 0 && ws_bytes >= need), B200_ERR_INVALID,
