@@ -502,7 +502,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       uint32_t(*const bad)[4] = bad_keys + (item & 1) * kTrBad;
       const bool two = w.rows.nrows > R;
       const int row = (two ? x * R : 0) + r, t = w.rows.row0 + row;
-      const bool alive = r < R && row < w.rows.nrows;
+      const bool alive = r < R && row < w.rows.nrows, live = __any_sync(0xffffffffu, alive);   // a warp without a pair hands over whatever there is: its rows are never looked at
       const TreeRow see = {p.masks + (int64_t)t * p.words, alive ? tree_ctx(p, t) : 0, alive ? p.words : 0, w.rows.end, alive};
       const int masked = max(w.tile0, w.rows.clear / kTreeKeys);   // the first tile that not all rows see
       float mu = -INFINITY, l = 0.f;
@@ -510,58 +510,60 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       for (int i = w.tile0 + (two ? 0 : x); i < w.tile1; i += two ? 1 : 2, ++n) {
         mbar_wait(s_full + 2 * x + (n & 1), (n >> 1) & 1);
         fence_after();
-        const uint32_t s_addr = own + (n & 1) * kTreeKeys;
-        uint32_t s[64];
-        ld32(s_addr, s);
-        ld32(s_addr + 32, s + 32);
-        ld_wait<64>(s);
-        if (i >= masked) {
-          uint32_t bits[2];
-          tree_bits(see, i * kTreeKeys, bits);
+        if (live) {
+          const uint32_t s_addr = own + (n & 1) * kTreeKeys;
+          uint32_t s[64];
+          ld32(s_addr, s);
+          ld32(s_addr + 32, s + 32);
+          ld_wait<64>(s);
+          if (i >= masked) {
+            uint32_t bits[2];
+            tree_bits(see, i * kTreeKeys, bits);
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (!(bits[j >> 5] >> (j & 31) & 1)) s[j] = 0xff800000u;   // -inf
-        }
-        const float mx = max64(s);
-        const bool jump = (mx - mu) * sc2 > 8.f;   // also the first live key (mu = -inf)
-        if (__any_sync(0xffffffffu, jump)) {
-          const float mn = jump ? mx : mu, f = jump && mu != -INFINITY ? exp2_fast((mu - mn) * sc2) : 1.f;
-          if (n > n0 && __any_sync(0xffffffffu, f != 1.f)) {
-            mbar_wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
-            fence_after();
+            for (int j = 0; j < 64; ++j)
+              if (!(bits[j >> 5] >> (j & 31) & 1)) s[j] = 0xff800000u;   // -inf
+          }
+          const float mx = max64(s);
+          const bool jump = (mx - mu) * sc2 > 8.f;   // also the first live key (mu = -inf)
+          if (__any_sync(0xffffffffu, jump)) {
+            const float mn = jump ? mx : mu, f = jump && mu != -INFINITY ? exp2_fast((mu - mn) * sc2) : 1.f;
+            if (n > n0 && __any_sync(0xffffffffu, f != 1.f)) {
+              mbar_wait(o_full + 2 * x + ((n - 1) & 1), ((n - 1) >> 1) & 1);
+              fence_after();
 #pragma unroll 1
-            for (int c = 0; c < kHeadDim; c += 16) {
-              uint32_t o[16];
-              ld16(own + 128 + c, o);
-              ld_wait<16>(o);
+              for (int c = 0; c < kHeadDim; c += 16) {
+                uint32_t o[16];
+                ld16(own + 128 + c, o);
+                ld_wait<16>(o);
 #pragma unroll
-              for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
-              st16(own + 128 + c, o);
+                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * f);
+                st16(own + 128 + c, o);
+              }
             }
+            l *= f;
+            mu = mn;
           }
-          l *= f;
-          mu = mn;
-        }
-        // exponents as (score - maximum) x scale: a product less a rounded one would be off by 2^-24 of either, which is more than the exponent itself where scores are large
-        const uint64_t minus = f2::both(mu > -INFINITY ? -mu : 0.f), unit = f2::both(sc2);
-        uint64_t sum2[2] = {0, 0};
+          // exponents as (score - maximum) x scale: a product less a rounded one would be off by 2^-24 of either, which is more than the exponent itself where scores are large
+          const uint64_t minus = f2::both(mu > -INFINITY ? -mu : 0.f), unit = f2::both(sc2);
+          uint64_t sum2[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          uint32_t pk[32];
+          for (int c = 0; c < 2; ++c) {
+            uint32_t pk[32];
 #pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const uint64_t e = f2::mul(f2::add(f2::pack(__uint_as_float(s[c * 32 + 2 * j]), __uint_as_float(s[c * 32 + 2 * j + 1])), minus), unit);
-            const float p0 = exp2_fast(f2::lo(e)), p1 = exp2_fast(f2::hi(e));
-            // the high term truncated, the rest rounded
-            sum2[j & 1] = f2::add(sum2[j & 1], f2::pack(p0, p1));
-            pk[j] = pack_bf16(p0, p1);
-            const uint32_t h0 = pk[j] << 16, h1 = pk[j] & 0xffff0000u;
-            const uint64_t rest = f2::add(f2::pack(p0, p1), f2::pack(-__uint_as_float(h0), -__uint_as_float(h1)));
-            pk[16 + j] = pack_bf16(f2::lo(rest), f2::hi(rest));
+            for (int j = 0; j < 16; ++j) {
+              const uint64_t e = f2::mul(f2::add(f2::pack(__uint_as_float(s[c * 32 + 2 * j]), __uint_as_float(s[c * 32 + 2 * j + 1])), minus), unit);
+              const float p0 = exp2_fast(f2::lo(e)), p1 = exp2_fast(f2::hi(e));
+              // the high term truncated, the rest rounded
+              sum2[j & 1] = f2::add(sum2[j & 1], f2::pack(p0, p1));
+              pk[j] = pack_bf16(p0, p1);
+              const uint32_t h0 = pk[j] << 16, h1 = pk[j] & 0xffff0000u;
+              const uint64_t rest = f2::add(f2::pack(p0, p1), f2::pack(-__uint_as_float(h0), -__uint_as_float(h1)));
+              pk[16 + j] = pack_bf16(f2::lo(rest), f2::hi(rest));
+            }
+            st32(s_addr + c * 32, pk);
           }
-          st32(s_addr + c * 32, pk);
+          l += f2::sum(sum2[0]) + f2::sum(sum2[1]);
         }
-        l += f2::sum(sum2[0]) + f2::sum(sum2[1]);
         if (i >= masked && !(two && x)) {
           // 0 x NaN = NaN: what is no number leaves the value tile (two threads a key), everything behind the end does
           const int v_at = 2 * (done + i - w.tile0) + 1, vs = v_at % kTreeSlots, key = m >> 1;
@@ -630,7 +632,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
       if (w.parts > 1 && alive && c0 == 0) reinterpret_cast<float2*>(p.part + (int64_t)w.slot * p.pairs * kTrPart + (int64_t)p.pairs * kHeadDim)[row * G + g] = make_float2(mu, l);
       unsigned char* const st = ostage + warp * 2048;
 #pragma unroll 1
-      for (int c = c0; c < c1; c += 32) {
+      for (int c = live ? c0 : c1; c < c1; c += 32) {
         uint32_t o[32];
         if (any) {
           ld32(own + 128 + c, o);
