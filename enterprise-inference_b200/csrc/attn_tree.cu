@@ -697,16 +697,22 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // ---- parts -> out -----------------------------------------------------------------------------------------------------------------------
-// A warp takes 32 pairs of an item and eight columns: sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m) over its parts, in their order
-constexpr int kJoinThreads = 256, kJoinColumns = 8;
+// A warp takes 32 pairs of an item and eight columns: sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m) over its parts, in their order.  Bound by latency: two rounds of loads, for
+// which four CTAs an SM have the warps (one: 4 x 256 rows over 6000 tokens 192 us in all, four 164)
+constexpr int kJoinThreads = 256, kJoinColumns = 8, kJoinCtas = 4;
 
-__global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_constant__ TreeParams p) {
+__global__ void __launch_bounds__(kJoinThreads, kJoinCtas) tree_join_kernel(const __grid_constant__ TreeParams p) {
   __shared__ int front[kJoinThreads + 1], sh[kJoinThreads / 32];
+  __shared__ Kv8Cut cuts[kNumSMs];
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.hq / p.hkv;
-  const Kv8Cut mine = tid < kNumSMs ? p.cuts[tid] : Kv8Cut{0, 0, 0, 0};
-  int n = mine.parts < 2 ? 0 : (mine.nrows * G + 31) / 32 * (kHeadDim / kJoinColumns);
+  int n = 0;
+  if (tid < kNumSMs) {
+    const Kv8Cut cut = p.cuts[tid];
+    cuts[tid] = cut;
+    n = cut.parts < 2 ? 0 : (cut.nrows * G + 31) / 32 * (kHeadDim / kJoinColumns);
+  }
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, n, o);
@@ -714,27 +720,28 @@ __global__ void __launch_bounds__(kJoinThreads) tree_join_kernel(const __grid_co
   }
   if (lane == 31) sh[warp] = n;
   __syncthreads();
-  for (int w = 0; w < warp; ++w) n += sh[w];
+  int t = lane < kJoinThreads / 32 && lane < warp ? sh[lane] : 0;
+  n += __reduce_add_sync(0xffffffffu, t);
   front[tid + 1] = n;
   if (tid == 0) front[0] = 0;
   __syncthreads();
   const float unit = p.scale * 1.4426950408889634f;
   const int64_t slot = (int64_t)p.pairs * kTrPart;
+#pragma unroll 1
   for (int job = blockIdx.x * (kJoinThreads / 32) + warp; job < front[kJoinThreads]; job += gridDim.x * (kJoinThreads / 32)) {
     int k = 0;   // the last with front[k] <= job
 #pragma unroll
     for (int b = kJoinThreads / 2; b > 0; b >>= 1)
       if (front[k + b] <= job) k += b;
-    const Kv8Cut cut = p.cuts[k];
+    const Kv8Cut cut = cuts[k];
     const int at = job - front[k], c = at % (kHeadDim / kJoinColumns), pair = at / (kHeadDim / kJoinColumns) * 32 + lane;
     const bool alive = pair < cut.nrows * G;
     const float* part = p.part + (2 * k + 1) * slot;   // the first: behind it every other one
     auto part_of = [&](int i) { return part + (i ? 2 * i - 1 : 0) * slot; };
-    auto ml = [&](int i) { return __ldcg(reinterpret_cast<const float2*>(part_of(i) + (int64_t)p.pairs * kHeadDim) + pair); };
-    float m = -INFINITY, l = 0.f;
+    auto ml = [&](int i) { return reinterpret_cast<const float2*>(part_of(i) + (int64_t)p.pairs * kHeadDim)[pair]; };
+    float m = -INFINITY, l = 0.f, a[8] = {};
 #pragma unroll 8
     for (int i = 0; i < cut.parts; ++i) m = fmaxf(m, ml(i).x);
-    float a[8] = {};
 #pragma unroll 4
     for (int i = 0; i < cut.parts; ++i) {
       const float2 t = ml(i);
@@ -787,7 +794,7 @@ int tree_launch(TreeParams p, void* ws, cudaStream_t s) {
   B200_CUDA(ensure_dynamic_smem(attn_tree_kernel, kTrSmem, done));
   B200_CUDA(launch(attn_tree_kernel, dim3(kNumSMs), dim3(kTreeThreads), (size_t)kTrSmem, s, mq, mk, mv, p));
   const PdlScope after;
-  B200_CUDA(launch(tree_join_kernel, dim3(kNumSMs), dim3(kJoinThreads), (size_t)0, s, p));
+  B200_CUDA(launch(tree_join_kernel, dim3(kJoinCtas * kNumSMs), dim3(kJoinThreads), (size_t)0, s, p));
   return B200_OK;
 }
 
