@@ -524,7 +524,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
               if (!(bits[j >> 5] >> (j & 31) & 1)) s[j] = 0xff800000u;   // -inf
           }
           const float mx = max64(s);
-          const bool jump = (mx - mu) * sc2 > 8.f;   // also the first live key (mu = -inf)
+          const bool jump = alive && (mx - mu) * sc2 > 8.f;   // also the first live key (mu = -inf)
           if (__any_sync(0xffffffffu, jump)) {
             const float mn = jump ? mx : mu, f = jump && mu != -INFINITY ? exp2_fast((mu - mn) * sc2) : 1.f;
             if (n > n0 && __any_sync(0xffffffffu, f != 1.f)) {
