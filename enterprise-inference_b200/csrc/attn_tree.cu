@@ -30,6 +30,7 @@ constexpr int kTrBad = 64;                      // tiles of an item for which it
 constexpr int kTrPart = kHeadDim + 2;           // floats of a pair in a part: sums, their maximum (of the products q . k), the denominator
 constexpr int kTreeTable = 48;                  // units of a CTA in shared memory
 constexpr int kMostRows = 4096;                 // of a step: the plan's lists fit where the tiles come to lie
+constexpr int kMostTokens = 0x7fffffff - 4096;  // of a block table: places of a mask's last bit, and of tiles that are looked up ahead, are ints
 
 // rows [row0, row0 + nrows) of one sequence; clear, end: tokens that all of them see, up to the last one that any sees
 struct TreeItem {
@@ -135,7 +136,7 @@ __device__ __forceinline__ int2 tree_plan(const TreeParams& p, int R, int cta, i
         if (x[j]) e = 32 * (w + j) + 31 - __clz(x[j]);
     }
     c = min(max(c, 0), tokens);
-    ctx[r] = c, end[r] = min(c + e + 1, tokens);   // (tokens and a mask's bits are below 2^31 together)
+    ctx[r] = c, end[r] = min(c + e + 1, tokens);   // (tokens and a mask's bits: below 2^31 together)
     clear_of[r] = 0x7fffffff, end_of[r] = 0, count_of[r] = 0;
     if (r == 0 || mine != before) start = r;
   }
@@ -820,7 +821,7 @@ extern "C" int b200_paged_attn_tree(const void* q, int64_t ldq, const void* k_ca
   B200_REQUIRE(mask_words <= kMostWords, B200_ERR_UNSUPPORTED, "paged_attn_tree: %d mask words (at most %d)", mask_words, kMostWords);
   B200_REQUIRE(kv8_block_ok(block_size), B200_ERR_UNSUPPORTED, "paged_attn_tree: block_size=%d (16, 32, 64 or a multiple of 128)", block_size);
   B200_REQUIRE(kv8_rows_ok(n_blocks, hkv, block_size), B200_ERR_INVALID, "paged_attn_tree: %lld blocks", (long long)n_blocks);
-  B200_REQUIRE((int64_t)bt_stride * block_size <= 0x7fffffff - 256, B200_ERR_UNSUPPORTED, "paged_attn_tree: block tables of %lld tokens", (long long)bt_stride * block_size);
+  B200_REQUIRE((int64_t)bt_stride * block_size <= kMostTokens, B200_ERR_UNSUPPORTED, "paged_attn_tree: block tables of %lld tokens", (long long)bt_stride * block_size);
   B200_REQUIRE(ldq >= (int64_t)hq * kHeadDim && ldq % 8 == 0 && ldo >= (int64_t)hq * kHeadDim && ldo % 8 == 0, B200_ERR_INVALID,
                "paged_attn_tree: ldq and ldo are multiples of 8 that hold a row");
   B200_REQUIRE(aligned16(q) && aligned16(out) && aligned16(k_cache_layer) && aligned16(v_cache_layer), B200_ERR_INVALID, "paged_attn_tree: tensors must be 16-byte aligned");

@@ -30,6 +30,14 @@ def test_attention_refuses(kw, code):
     assert b"paged_attn_tree" in _lib().b200_last_error()
 
 
+def test_attention_refuses_tables_whose_places_are_no_ints():
+    """A mask's last bit lies up to 1024 tokens behind a context, tiles are looked up to 2048 tokens ahead."""
+    assert _attend(T=1, hq=1, hkv=1, ldq=128, ldo=128, stride=2 ** 24 - 16, block=128) == -3 and b"tokens" in _lib().b200_last_error()
+    assert _attend(T=1, hq=1, hkv=1, ldq=128, ldo=128, stride=2 ** 24 - 32, block=128) == -3 and b"tokens" in _lib().b200_last_error()
+    assert _attend(T=1, hq=1, hkv=1, ldq=128, ldo=128, stride=2 ** 24 - 33, block=128, size=0) == -1 and b"workspace" in _lib().b200_last_error()
+    assert _attend(T=4096, stride=2 ** 17, block=128) == -3 and b"rows" in _lib().b200_last_error()   # rows x heads x tiles
+
+
 def test_attention_of_no_rows_is_nothing():
     assert _attend(T=0, ws=None, size=0) == 0
     assert _lib().b200_paged_attn_tree_workspace_bytes(0, 32, 8) == 0 and _lib().b200_paged_attn_tree_workspace_bytes(5, 32, 0) == 0
