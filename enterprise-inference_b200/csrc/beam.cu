@@ -4,7 +4,7 @@
 // blocks: a warp takes 2 048 neighbouring logits, all in registers at once, and leaves their largest, m, and the sum of exp(x - m).  No barriers, nothing is selected.
 // merge: a cluster takes a sequence.  One of its CTAs joins the blocks' sums; a number that more than K blocks' largest scores reach bounds the K-th score from below, and only
 // the blocks that reach it, little more than K, are read again.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
-// is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in fp64 (half of the entries
+// is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in 64 bits (half of the entries
 // to a CTA) and the CTA picks again.  Entries of one row never need it.
 // Bound by the bytes of the logits.
 #include <cooperative_groups.h>
@@ -21,7 +21,7 @@ namespace cg = cooperative_groups;
 
 constexpr int kBlockThreads = 256, kBlockGroups = 8, kBlock = 32 * 8 * kBlockGroups, kBlockCtas = 4 * kNumSMs;
 constexpr int kMostTake = 128, kMostVocab = 393216;
-constexpr int kMergeThreads = 1024, kMergeCtas = 2, kMergeList = 1024, kKnownRows = 64;
+constexpr int kMergeThreads = 1024, kMergeCtas = 2, kMergeList = kMergeThreads, kKnownRows = 64;
 constexpr float kLog2e = 1.4426950408889634f;
 // What a row's log-sum may be off by: exponents of base 2 are rounded once (2^-24 of up to 17 in the mean over the weights, times ln 2: 7e-7) and have log2 e to 2^-26 (2e-7), the
 // hardware's exponential has 2^-22 (2.4e-7), for a term and for its block's largest, and nine sums and products follow one another in a lane (5e-7); behind them everything is fp64
@@ -136,9 +136,16 @@ __device__ __forceinline__ double exp2_series(double t) {
   e = fma(e, r, 1.0 / 24), e = fma(e, r, 1.0 / 6), e = fma(e, r, 0.5), e = fma(e, r, 1.0), e = fma(e, r, 1.0);
   return __hiloint2double(__double2hiint(e) + ((int)n << 20), __double2loint(e));
 }
-// of a row's sum of exp(x - m) what the entries [from, to) have
-__device__ __noinline__ double row_part(const __nv_bfloat16* row, int from, int to, double m) {
-  double sum[4] = {0.0, 0.0, 0.0, 0.0};
+// Sums of exp(x - m) in units of 2^-62, high and low 32 bits of the terms apart: exact whatever the order, so that rows of the same entries in other places stay alike (fp64 sums differ in
+// their last bit).  Units of 393 216 terms make 9e-14
+struct alignas(16) UnitSum {
+  unsigned long long high, low;
+};
+__device__ __forceinline__ void operator+=(UnitSum& a, const UnitSum& b) { a.high += b.high, a.low += b.low; }
+__device__ __forceinline__ double value_of(const UnitSum& a) { return (double)a.high * 0x1p-30 + (double)a.low * 0x1p-62; }
+// what the entries [from, to) of a row have
+__device__ __noinline__ UnitSum row_part(const __nv_bfloat16* row, int from, int to, double m) {
+  UnitSum sum = {0, 0};
 #pragma unroll 1
   for (int k0 = from + threadIdx.x; k0 < to; k0 += 4 * kMergeThreads) {
     float x[4];
@@ -146,9 +153,12 @@ __device__ __noinline__ double row_part(const __nv_bfloat16* row, int from, int 
     for (int j = 0; j < 4; ++j) x[j] = k0 + j * kMergeThreads < to ? __bfloat162float(row[k0 + j * kMergeThreads]) : -INFINITY;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (x[j] > -INFINITY) sum[j] += exp2_series(((double)x[j] - m) * 1.4426950408889634);
+      if (x[j] > -INFINITY) {
+        const unsigned long long t = (unsigned long long)__double2ll_rn(exp2_series(((double)x[j] - m) * 1.4426950408889634) * 0x1p62);
+        sum += {t >> 32, t & 0xffffffffu};
+      }
   }
-  return (sum[0] + sum[1]) + (sum[2] + sum[3]);
+  return sum;
 }
 __device__ __noinline__ double row_base(const float* scores, int r, double m, double sum) {
   const double base = (scores ? (double)scores[r] : 0.0) - (m + log(sum));
@@ -156,10 +166,11 @@ __device__ __noinline__ double row_base(const float* scores, int r, double m, do
 }
 __global__ void __launch_bounds__(kMergeThreads, 1) __cluster_dims__(kMergeCtas, 1, 1)
 beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const float* __restrict__ scores, const int32_t* __restrict__ starts, int n_rows, int per_row, int vocab, int take,
-                  const float2* __restrict__ stats, RowStat* rows, double* parts, int32_t* out_rows, int32_t* out_tokens, float* out_scores) {
+                  const float2* __restrict__ stats, RowStat* rows, UnitSum* parts, int32_t* out_rows, int32_t* out_tokens, float* out_scores) {
   constexpr int kWarps = kMergeThreads / 32;
   __shared__ double sh_s[kMergeList], sh_sum[kWarps];
   __shared__ uint64_t sh_id[kMergeList];
+  __shared__ UnitSum sh_part[kWarps];
   __shared__ Best sorted[kMostTake + 1];
   __shared__ int need[2 * kMergeList], blocks[kMergeList], n_need, n_list, n_blocks, seen_all;
   __shared__ uint32_t asked_for[kMergeList / 32];   // rows of the sequence that are in need (of the first kMergeList)
@@ -199,7 +210,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
     }
     __syncthreads();
   }
-  bool exact = false;   // every row added up in fp64
+  bool exact = false;   // every row added up in 64 bits
 #pragma unroll 1
   for (;;) {
     if (cta == 0) {
@@ -282,13 +293,30 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           }
         }
       };
-      bool by_threads = !(at.s > -INFINITY);   // too few blocks: a number that threads' largest entries reach
+      bool by_threads = !(at.s > -INFINITY), too_many = false;   // too few blocks: a number that threads' largest entries reach
 #pragma unroll 1
       for (;;) {
         if (by_threads) {
-          double own = -INFINITY;
-          each(at.s - margin, [&](double t, uint64_t) { own = fmax(own, t); });
-          at.s = fmax(at.s, (double)limit_of(own));
+          Best own = {-INFINITY, ~0ull - tid};   // (with none: behind all others, and no two alike)
+          each(at.s - margin, [&](double t, uint64_t od) {
+            if (better(t, od, own.s, own.id) && (!too_many || !better(at.s, at.id, t, od))) own = {t, od};
+          });
+          if (too_many) {
+            // the entry behind the best `take` threads' own is a limit nearer to the end (of 64 rows of 128 256 entries alike, the best rows last, the list would leave out a thousand at a
+            // time).  It leaves take + 1 threads with any: then it is the one behind the best `take` of those that found room, which leaves out all but `take` of them.  Either way
+            // fewer are left
+            if (__syncthreads_count(own.s > -INFINITY) > take + 1) sh_s[tid] = own.s, sh_id[tid] = own.id;
+            __syncthreads();
+            own = {sh_s[tid], sh_id[tid]};
+            int before = 0;
+#pragma unroll 1
+            for (int k = 0; k < kMergeList; ++k) before += better(sh_s[k], sh_id[k], own.s, own.id);
+            if (before == take) limit = own;
+            __syncthreads();
+            at = limit;
+          } else {
+            at.s = fmax(at.s, (double)limit_of(own.s));
+          }
           by_threads = false;
         }
         const double least = at.s - margin;
@@ -300,18 +328,10 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         });
         __syncthreads();
         if (n_list <= kMergeList) break;
-        // too many: the entry behind the best `take` of those that found room is a limit nearer to the end.  Those next to it are not all seen
-#pragma unroll 1
-        for (int e = tid; e < kMergeList; e += kMergeThreads) {
-          int before = 0;
-#pragma unroll 1
-          for (int k = 0; k < kMergeList; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
-          if (before == take) limit = {sh_s[e], sh_id[e]};
-        }
         __syncthreads();
-        at = limit;
-        if (tid == 0) n_list = 0, seen_all = margin == 0.0 && seen_all;
+        if (tid == 0) n_list = 0, seen_all = margin == 0.0 && seen_all;   // (those next to the limit will not all be seen)
         margin = 0.0;
+        by_threads = too_many = true;
         __syncthreads();
       }
       const int n = n_list;
@@ -370,14 +390,14 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
 #pragma unroll 1
     for (int i = 0; i < wanted; ++i) {
       const int r = wanted_row(i);
-      double sum = row_part(logits + (int64_t)r * ld, from, to, (double)top_of(r));
+      UnitSum sum = row_part(logits + (int64_t)r * ld, from, to, (double)top_of(r));
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      for (int o = 16; o > 0; o >>= 1) sum += {__shfl_xor_sync(0xffffffffu, sum.high, o), __shfl_xor_sync(0xffffffffu, sum.low, o)};
       __syncthreads();
-      if (lane == 0) sh_sum[warp] = sum;
+      if (lane == 0) sh_part[warp] = sum;
       __syncthreads();
       if (tid == 0) {
-        for (int w = 1; w < kWarps; ++w) sum += sh_sum[w];
+        for (int w = 1; w < kWarps; ++w) sum += sh_part[w];
         parts[(int64_t)r * kMergeCtas + cta] = sum;
       }
     }
@@ -390,9 +410,12 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         const int r = wanted_row(i);
         const float m = top_of(r);
         if (lane == 0) {
-          double sum = 0.0;
-          for (int k = 0; k < kMergeCtas; ++k) sum += __ldcg(parts + (int64_t)r * kMergeCtas + k);
-          const double base = row_base(scores, r, (double)m, sum);
+          UnitSum sum = {0, 0};
+          for (int k = 0; k < kMergeCtas; ++k) {
+            const ulonglong2 t = __ldcg(reinterpret_cast<const ulonglong2*>(parts) + (int64_t)r * kMergeCtas + k);
+            sum += {t.x, t.y};
+          }
+          const double base = row_base(scores, r, (double)m, value_of(sum));
           rows[r] = {base, 0.0};
           if (r - r0 < kKnownRows) known[r - r0] = base;
         }
@@ -407,7 +430,7 @@ int per_row_of(int vocab) { return (vocab + 7 + kBlock - 1) / kBlock; }   // blo
 }  // namespace
 
 int64_t beam_select_workspace_bytes(int n_rows, int vocab) {
-  return (int64_t)n_rows * (per_row_of(vocab) * (int64_t)sizeof(float2) + (int64_t)sizeof(RowStat) + kMergeCtas * (int64_t)sizeof(double)) + 64;
+  return (int64_t)n_rows * (per_row_of(vocab) * (int64_t)sizeof(float2) + (int64_t)sizeof(RowStat) + kMergeCtas * (int64_t)sizeof(UnitSum)) + 64;
 }
 
 }  // namespace b200
@@ -435,7 +458,7 @@ extern "C" int b200_beam_select(const void* logits, int64_t ld, const float* sco
   const __nv_bfloat16* l = static_cast<const __nv_bfloat16*>(logits);
   const int per_row = per_row_of(vocab);
   RowStat* rows = static_cast<RowStat*>(ws);
-  double* parts = reinterpret_cast<double*>(rows + n_rows);
+  UnitSum* parts = reinterpret_cast<UnitSum*>(rows + n_rows);
   float2* stats = reinterpret_cast<float2*>(parts + (int64_t)n_rows * kMergeCtas);
   if (n_rows > 0)
     B200_CUDA(launch(beam_blocks_kernel, dim3((unsigned)std::min(kBlockCtas, n_rows * per_row)), dim3(kBlockThreads), (size_t)0, s, l, ld, n_rows, per_row, vocab, stats));

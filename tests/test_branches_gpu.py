@@ -221,6 +221,26 @@ def test_long_contexts_and_many_tiles():
     step.check(step.run(), [0, 1, 35, 69, 70, 72, 73, 92])
 
 
+def test_thousands_of_short_sequences_beside_a_long_one():
+    """More walks of a CTA than its table holds; contexts of nothing among them."""
+    g = torch.Generator().manual_seed(16)
+    ctx = torch.randint(0, 90, (2000,), generator=g).tolist()
+    ctx[1234], ctx[0], ctx[1999] = 9000, 0, 65
+    step = Step([(c, [[] if c % 7 == 0 else [0]]) for c in ctx], 16, 8, 16, 16)
+    first = step.run()
+    step.check(first, [0, 1, 2, 500, 1000, 1233, 1234, 1235, 1998, 1999, *range(40, 1900, 97)])
+    assert torch.equal(step.run(ws=step.ws, dev=step.dev), first)
+
+
+@pytest.mark.parametrize("sizes", [(4096,), (1, 4000, 95), tuple(list(range(1, 90)) + [91])])
+def test_steps_of_the_most_rows(sizes):
+    g = torch.Generator().manual_seed(len(sizes))
+    assert sum(sizes) == 4096
+    seqs = [(int(torch.randint(0, 300, (1,), generator=g)), [torch.randperm(90, generator=g)[:int(torch.randint(0, 9, (1,), generator=g))].tolist() for _ in range(n)]) for n in sizes]
+    step = Step(seqs, 4, 2, 64, 17)
+    step.check(step.run(), [0, 1, 63, 64, 65, 127, 128, 1000, 2047, 4000, 4001, 4095, *range(300, 4000, 171)])
+
+
 def test_scores_far_apart():
     """Maxima that rise along the context, and fall: rescaling, and weights of nothing."""
     step = Step([(700, [[0, 1], [1], [0]]), (640, [[]] * 3)], 8, 2, 64, 14)
@@ -284,7 +304,7 @@ def test_captured_graphs_and_two_streams():
 
 # ---- selection over beams ---------------------------------------------------------------------------------------------------------
 
-def select(logits, scores, starts, take, ws=None, stream=None, ld=None, vocab=None):
+def select(logits, scores, starts, take, ws=None, stream=None, ld=None, vocab=None, at=None):
     lib, check = _lib()
     S, n = starts.shape[0] - 1, logits.shape[0]
     V, ld = vocab or logits.shape[1], ld or logits.stride(0)
@@ -292,7 +312,7 @@ def select(logits, scores, starts, take, ws=None, stream=None, ld=None, vocab=No
     ws = torch.full((size + 16,), 0xff, dtype=torch.uint8, device=DEV) if ws is None else ws
     rows, tokens = (torch.full((S, take), -9, dtype=I32, device=DEV) for _ in range(2))
     out = torch.full((S, take), 9.0, device=DEV)
-    check(lib.b200_beam_select(logits.data_ptr(), ld, _ptr(scores), starts.data_ptr(), S, n, V, take, rows.data_ptr(), tokens.data_ptr(), out.data_ptr(), ws.data_ptr(), size, stream))
+    check(lib.b200_beam_select((logits if at is None else at).data_ptr(), ld, _ptr(scores), starts.data_ptr(), S, n, V, take, rows.data_ptr(), tokens.data_ptr(), out.data_ptr(), ws.data_ptr(), size, stream))
     return rows, tokens, out
 
 
@@ -355,6 +375,30 @@ def test_select_between_rows_that_are_nearer_than_fp32_sums_tell():
     assert float((lse.max() - lse.min())) < 1e-3
     check_select(logits, None, _starts(12), 24)
     check_select(logits[:4].contiguous(), (lse - lse[0]).float()[:4], _starts(4), 24)   # nearer still: fp32's rounding of the scores apart
+
+
+@pytest.mark.parametrize("order", ["last", "first", "middle"])
+def test_select_among_more_alike_than_any_list_holds(order):
+    """Rows alike in every entry, whose scores differ by less than fp32 sums tell."""
+    logits = torch.zeros(64, 50000, dtype=BF)
+    scores = -1e-9 * torch.arange(64.0)
+    scores = {"first": scores, "last": scores.flip(0), "middle": scores[torch.randperm(64, generator=torch.Generator().manual_seed(3))]}[order]
+    check_select(logits, scores, _starts(64), 128)
+
+
+def test_select_between_many_rows_that_are_near():
+    """More rows than are kept at hand, all of them in need of 64 bits; in two sequences."""
+    g = torch.Generator().manual_seed(78)
+    base = (torch.randn(1, 3000, generator=g) * 2).to(BF)
+    logits = base.repeat(1300, 1)
+    logits[torch.arange(1300), torch.randint(0, 3000, (1300,), generator=g)] = -9.0
+    check_select(logits, None, _starts(100, 1200), 128)
+
+
+def test_select_without_rows():
+    starts = torch.zeros(4, dtype=I32, device=DEV)
+    for rows, tokens, out in (select(torch.zeros(0, 50, dtype=BF, device=DEV), None, starts, 5, ld=50, vocab=50, at=starts), select(torch.zeros(3, 50, dtype=BF, device=DEV), None, starts, 5)):
+        assert (rows == -1).all() and (tokens == -1).all() and (out == -INF).all()
 
 
 def test_select_without_candidates():
@@ -511,6 +555,56 @@ def test_moves_of_large_groups(n):
     da, ds, dd, st = _dev(a, src, dst, starts)
     move(da, None, ds, dd, st, n)
     assert torch.equal(da.cpu(), U.moved(a, src, dst, starts, n))
+
+
+@pytest.mark.parametrize("sizes,width", [((6, 3, 1, 6), 1 << 20), ((1,) * 9, 700000), ((40,), 300016)])
+def test_moves_of_large_states(sizes, width):
+    """Many batches to a CTA."""
+    g = torch.Generator().manual_seed(width)
+    n = sum(sizes) + 3
+    a, b = (torch.randint(0, 256, (2, n, 1, 1, width), generator=g).to(torch.uint8) for _ in range(2))
+    starts = _starts(*sizes)
+    da, db, ds = _dev(a, b, starts)
+    for _ in range(4):
+        src, dst = _moves(torch.randperm(n, generator=g)[:sum(sizes)], sizes, g, 0.1)
+        a, b = (U.moved(x, src, dst, starts, max(sizes)) for x in (a, b))
+        move(da, db, src.to(DEV), dst.to(DEV), ds, max(sizes))
+    assert torch.equal(da.cpu(), a) and torch.equal(db.cpu(), b)
+
+
+def test_walk_and_moves_captured_with_another_pair():
+    """Two graphs on streams of their own, replayed with other choices of the target at the same addresses."""
+    lib, check = _lib()
+    g = torch.Generator().manual_seed(6)
+    starts, n, B = _starts(9, 20, 1), 30, 32
+    parents = torch.tensor([p for s in (9, 20, 1) for p in _random_tree(s, g, 4)], dtype=I32)
+    slots = torch.arange(n, dtype=I32) * 3 + 1
+    runs = []
+    for _ in range(2):
+        cache = torch.randint(0, 99, (2, 3, 2, B, 64), generator=g).to(BF)
+        dev = _dev(torch.zeros(n, dtype=I32), torch.randint(0, 2, (n,), generator=g).to(I32), parents, starts, slots, cache)
+        out = [torch.full((n,), -9, dtype=I32, device=DEV) for _ in range(4)] + [torch.full((3,), -9, dtype=I32, device=DEV)]
+        graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            st, (t, d, p, f, sl, c) = torch.cuda.current_stream().cuda_stream, dev
+            check(lib.b200_accept_tree(t.data_ptr(), d.data_ptr(), p.data_ptr(), f.data_ptr(), sl.data_ptr(), 3, n, out[0].data_ptr(), out[1].data_ptr(), out[4].data_ptr(),
+                                       out[2].data_ptr(), out[3].data_ptr(), st))
+            check(lib.b200_cache_move(c.data_ptr(), None, 2, c.stride(0) * 2, 3, 2, B, 128, out[2].data_ptr(), out[3].data_ptr(), f.data_ptr(), 3, 20, st))
+        runs.append((graph, stream, dev, out, [cache]))
+    for _ in range(4):
+        for graph, stream, dev, out, cache in runs:
+            dev[0].copy_(torch.randint(0, 2, (n,), generator=g).to(I32))
+        torch.cuda.synchronize()
+        for graph, stream, *_ in runs:
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, stream, dev, out, cache in runs:
+            want = U.accept(dev[0].cpu(), dev[1].cpu(), parents, starts, slots)
+            assert all(torch.equal(out[i].cpu().long(), y) for i, y in zip((0, 1, 4, 2, 3), want))
+            cache[0] = U.moved(cache[0], want[3], want[4], starts, 20)
+            assert torch.equal(dev[5].cpu(), cache[0])
 
 
 def test_moves_outside_the_cache_and_behind_the_bound_are_not_made():
