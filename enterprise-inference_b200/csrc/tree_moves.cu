@@ -129,12 +129,21 @@ __global__ void __launch_bounds__(kMoveThreads) cache_move_kernel(const __grid_c
     }
   };
   auto walk = [&](int count, const MoveUnit* w, const int64_t* moves, auto f) {   // f(place in the half, address) for all of the thread's
+    if (lanes == 1) {
+      for (int piece = piece0; piece < 1 << p.piece_bits; piece += kMoveThreads)
+        for (int unit = 0; unit < count; ++unit) {
+          const MoveUnit t = w[unit];
+          if (piece * VEC >= t.left) continue;
+          unsigned char* const at = t.base + piece * VEC;
+          int e = unit * m * p.columns + piece * VEC;
+#pragma unroll 4
+          for (int mv = 0; mv < m; ++mv, e += p.columns) f(e, at + moves[mv]);
+        }
+      return;
+    }
     for (int unit = unit0, mv = move0; unit < count;) {
       const MoveUnit t = w[unit];
-      unsigned char* const at = t.base + moves[mv];
-      const int e = (unit * m + mv) << p.piece_bits;
-      for (int piece = piece0; piece < 1 << p.piece_bits; piece += kMoveThreads)
-        if (piece * VEC < t.left) f((e + piece) * VEC, at + piece * VEC);
+      if (piece0 * VEC < t.left) f((((unit * m + mv) << p.piece_bits) + piece0) * VEC, t.base + moves[mv] + piece0 * VEC);
       unit += unit_step, mv += move_step;
       if (mv >= m) mv -= m, ++unit;
     }
