@@ -339,8 +339,9 @@ B200_API int b200_verify_drafts(const void* target_logits, int64_t ldt, const vo
  * behind the bt_stride blocks of a block table do not exist; a row that sees none gives zeros; contexts below 0 count as 0.  What stands in a token that a row does not see is
  * never part of its result (an inf or a NaN there included); a block id outside [0, n_blocks) stands for keys and values of zero.  Rows of one sequence that follow one another
  * (row_to_seq; NULL: row t is sequence t) share its keys and values, whatever their contexts.  Up to 16 query heads to a kv head; block_size 16, 32, 64 or a multiple
- * of 128; n_blocks * n_kv_heads * block_size and a block table's tokens below 2^31 - 256; scale > 0.  Scores, softmax and sums in fp32, weights of 16 bits, one rounding.  The workspace has
- * no state between calls; calls that may run at the same time, two captured graphs among them, need one each.
+ * of 128; n_blocks * n_kv_heads * block_size up to 2^31 - 257; scale > 0.  Steps of more than 4096 rows, block tables of more than 2^31 - 4096 tokens and steps for which n_tokens *
+ * n_kv_heads * (4 + 3 tiles of 64 tokens of a block table) does not stay below 2^31 are refused (B200_ERR_UNSUPPORTED).  Scores, softmax and sums in fp32, weights of 16 bits, one
+ * rounding; the same bits every time.  The workspace (16-byte aligned) has no state between calls; calls that may run at the same time, two captured graphs among them, need one each.
  *
  * b200_beam_select: the n_select best continuations of a sequence's beams.  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1 of logits (bf16
  * [n_rows][ld]); with scores[r] a beam's sum of log-probabilities (NULL: zeros),
@@ -348,15 +349,16 @@ B200_API int b200_verify_drafts(const void* target_logits, int64_t ldt, const vo
  * in 64 bits where two candidates are near each other; out_rows, out_tokens, out_scores [n_seqs][n_select] (int32, int32, fp32) hold the rows (0 .. n_rows-1), entries and scores of
  * the best, the best first; alike scores: the lower row, then the larger logit, then the lower entry.  Logits of -inf are no candidates, nor is any entry of a row whose score or log-sum is not finite (a
  * beam that has ended: -inf; a NaN or +inf among its logits).  Where candidates run out, row and token are -1 and the score is -inf.  At most 128 to select, 65535 rows of 393216
- * entries, 2^28 - 1 sequences (B200_ERR_UNSUPPORTED).  The workspace has no state between calls; one for many rows does for fewer.
+ * entries, 2^28 - 1 sequences (B200_ERR_UNSUPPORTED).  The workspace has no state between calls; one for many rows does for fewer; calls that
+ * may run at the same time need one each.  Logits at any 2-byte address and any ld of vocab or more.
  *
  * b200_accept_tree: the way through a checked tree.  Sequence s owns rows row_starts[s] .. row_starts[s+1]-1: first its root (the last token that is certain), then drafted
  * nodes; parents[r] is the place of a node's parent in its sequence's rows (0: the root), in front of its own; the root's is not read.  target_tokens[r] is what the target chose behind
  * row r (b200_argmax or b200_sample of its logits: what is kept is distributed as the target's own draws).  From the root on, the first child whose draft is
  * the target's choice is taken.  out_tokens[n_rows]: per sequence the tokens chosen on that way (the kept drafts, then the token behind the last of them), then -1; out_rows[n_rows]:
- * the rows on it, the root's first, then -1; out_accepted[s]: drafts kept (0 for a sequence without rows).  With slot_mapping (the cache slots of the rows; else NULL, as
+ * the rows on it, the root's first, then -1; out_accepted[s]: drafts kept (0 for a sequence without rows).  With slot_mapping (the cache slots of the rows; else NULL, as are
  * move_src and move_dst): move_src, move_dst [n_rows] are the moves that bring the kept rows' keys and values to the slots of their sequence's first rows, -1 where there is nothing
- * to move.  Rows of no sequence stay as they are.
+ * to move: b200_cache_move makes them, with row_starts as its groups.  Rows of no sequence stay as they are.
  *
  * b200_cache_move: rows of caches, whole blocks or states to new places.  cache_a and cache_b (or NULL) each are n_layers times, layer_stride bytes apart,
  * [n_blocks][heads][block_size][row_bytes]; slot = block * block_size + place, as in slot_mapping.  The moves of group g, src_slots[i] -> dst_slots[i] for group_starts[g] <= i <
