@@ -48,6 +48,17 @@ __device__ __forceinline__ uint32_t ordered_f32(float x) {
 }
 __device__ __forceinline__ float f32_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
 
+// eight logits from entry i0 on, of which some lie outside the row (-inf), entry by entry
+__device__ __forceinline__ uint4 load_edge(const __nv_bfloat16* l, int i0, int vocab) {
+  uint4 w = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+  for (int q = 7; q >= 0; --q) {
+    const int i = i0 + q;
+    const uint32_t e = i >= 0 && i < vocab ? __bfloat16_as_ushort(l[i]) : 0xff80u;
+    w.w = w.w << 16 | w.z >> 16, w.z = w.z << 16 | w.y >> 16, w.y = w.y << 16 | w.x >> 16, w.x = w.x << 16 | e;
+  }
+  return w;
+}
 // a lane's eight groups of eight logits of a row's block (-inf outside the row); groups start at 16-byte addresses: entry i of a row is at place i + shift.  Returns the first one's index
 __device__ __forceinline__ int load_block(const __nv_bfloat16* l, int block, int vocab, uint4 (&v)[kBlockGroups]) {
   const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7), p0 = block * kBlock + (threadIdx.x & 31) * 8 - shift;
@@ -68,16 +79,10 @@ __device__ __forceinline__ int load_block(const __nv_bfloat16* l, int block, int
   for (int g = 0; g < kBlockGroups; ++g) {
     const int i0 = p0 + g * 256;
     if (!((i0 < 0 && i0 + 8 > 0) || (i0 < vocab && i0 + 8 > vocab))) continue;
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll 1
-    for (int q = 7; q >= 0; --q) {
-      const int i = i0 + q;
-      const uint32_t e = i >= 0 && i < vocab ? __bfloat16_as_ushort(l[i]) : 0xff80u;
-      w[3] = w[3] << 16 | w[2] >> 16, w[2] = w[2] << 16 | w[1] >> 16, w[1] = w[1] << 16 | w[0] >> 16, w[0] = w[0] << 16 | e;
-    }
+    const uint4 w = load_edge(l, i0, vocab);
 #pragma unroll
     for (int j = 0; j < kBlockGroups; ++j)
-      if (j == g) v[j] = make_uint4(w[0], w[1], w[2], w[3]);
+      if (j == g) v[j] = w;
   }
   return p0;
 }
@@ -119,24 +124,20 @@ beam_blocks_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, int n_r
   }
 }
 
+// scores as unsigned numbers in their order (compares of 64-bit integers; fp64's have several times the latency), zeros alike, and back
+__device__ __forceinline__ uint64_t ordered_f64(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x == 0.0 ? 0.0 : x);
+  return b ^ ((uint64_t)((int64_t)b >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double f64_of_ordered(uint64_t o) { return __longlong_as_double((long long)(o & 0x8000000000000000ull ? o ^ 0x8000000000000000ull : ~o)); }
 struct Best {
-  double s;
-  uint64_t id;
+  uint64_t score, id;
 };
 // what decides between scores that are alike: the lower row; within a row (where a log-sum may be large beside the logits) the larger logit, the lower entry
 __device__ __forceinline__ uint64_t id_of(int row, float x, int entry) { return (uint64_t)row << 48 | (uint64_t)(0xffffu - (ordered_f32(x) >> 16)) << 32 | (uint32_t)entry; }
 __device__ __forceinline__ int row_of(uint64_t id) { return (int)(id >> 48); }
-__device__ __forceinline__ bool better(double s, uint64_t id, double t, uint64_t od) { return s > t || (s == t && id < od); }
+__device__ __forceinline__ bool better(const Best& a, const Best& b) { return a.score > b.score || (a.score == b.score && a.id < b.id); }
 
-// 2^t for t <= 0 (2^-1000 below that): t = n + r, |r| <= 1 / 2, 2^r by the series of e^(r ln 2) up to the eleventh power, 1e-14 of it
-__device__ __forceinline__ double exp2_series(double t) {
-  t = fmax(t, -1000.0);
-  const double n = rint(t), r = (t - n) * 0.6931471805599453;
-  double e = 1.0 / 39916800;
-  e = fma(e, r, 1.0 / 3628800), e = fma(e, r, 1.0 / 362880), e = fma(e, r, 1.0 / 40320), e = fma(e, r, 1.0 / 5040), e = fma(e, r, 1.0 / 720), e = fma(e, r, 1.0 / 120);
-  e = fma(e, r, 1.0 / 24), e = fma(e, r, 1.0 / 6), e = fma(e, r, 0.5), e = fma(e, r, 1.0), e = fma(e, r, 1.0);
-  return __hiloint2double(__double2hiint(e) + ((int)n << 20), __double2loint(e));
-}
 // Sums of exp(x - m) in units of 2^-62, high and low 32 bits of the terms apart: exact whatever the order, so that rows of the same entries in other places stay alike (fp64 sums differ in
 // their last bit).  Units of 393 216 terms make 9e-14
 struct alignas(16) UnitSum {
@@ -144,20 +145,55 @@ struct alignas(16) UnitSum {
 };
 __device__ __forceinline__ void operator+=(UnitSum& a, const UnitSum& b) { a.high += b.high, a.low += b.low; }
 __device__ __forceinline__ double value_of(const UnitSum& a) { return (double)a.high * 0x1p-30 + (double)a.low * 0x1p-62; }
-// what the entries [from, to) of a row have
-__device__ __noinline__ UnitSum row_part(const __nv_bfloat16* row, int from, int to, double m) {
+// exp(d), d <= 0, in these units (0 below 2^-64): d = n ln 2 / 16 + r ln 2 / 16, |r| <= 1 / 2, 2^(n / 16) by its whole part and a table, 2^(r / 16) by its series up to the sixth power (5e-16
+// of it).  Conversions, which the hardware has at a quarter of its fp64 rate or less, are left out: n stands in the low word of a sum, the units are the shifted bits
+__constant__ double kSixteenths[16] = {1.0, 1.0442737824274138, 1.0905077326652577, 1.1387886347566916,
+                                       1.189207115002721, 1.241857812073484, 1.2968395546510096, 1.3542555469368927,
+                                       1.4142135623730951, 1.4768261459394993, 1.5422108254079407, 1.6104903319492543,
+                                       1.681792830507429, 1.7562521603732995, 1.8340080864093424, 1.9152065613971474};
+__device__ __forceinline__ unsigned long long units_of(double d, const double* table) {
+  if (!(d >= -45.0)) return 0;
+  constexpr double kScale = 23.083120654223414, kShift = 0x1.8p52;   // 16 / ln 2
+  const double k = fma(d, kScale, kShift), r = fma(d, kScale, kShift - k);
+  const int n = __double2loint(k);
+  double e = 9.181219573844438e-12;   // (ln 2 / 16)^6 / 6!, and so on
+  e = fma(e, r, 1.2715871950558131e-09), e = fma(e, r, 1.467610032291943e-07), e = fma(e, r, 1.3550807779497457e-05), e = fma(e, r, 0.0009383847928089872), e = fma(e, r, 0.04332169878499658);
+  e = fma(e, r, 1.0) * table[n & 15];
+  const int shift = (__double2hiint(e) >> 20) - 1023 + (n >> 4) + 10;   // 2^62 = 2^52 x 2^10
+  const unsigned long long bits = ((unsigned long long)__double_as_longlong(e) & 0xfffffffffffffull) | 0x10000000000000ull;
+  return shift >= 0 ? bits << shift : bits >> -shift;
+}
+// bf16 bits as fp64 (below the normal numbers: 0, next to which they are nothing in an exponent)
+__device__ __forceinline__ double f64_of(uint32_t b) {
+  return (b & 0x7fffu) < 0x80u ? 0.0 : __hiloint2double((int)((b & 0x8000u) << 16 | (((b & 0x7fffu) << 13) + (896u << 20))), 0);
+}
+// what a CTA's share of a row's entries has (of eight at a 16-byte address, four such loads at once); of a row with numbers that are none: anything
+__device__ __noinline__ UnitSum row_part(const __nv_bfloat16* l, int vocab, int cta, double m, const double* table) {
+  const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7), groups = (vocab + shift + 7) / 8;
+  const int from = (int)((int64_t)groups * cta / kMergeCtas), to = (int)((int64_t)groups * (cta + 1) / kMergeCtas);
   UnitSum sum = {0, 0};
 #pragma unroll 1
-  for (int k0 = from + threadIdx.x; k0 < to; k0 += 4 * kMergeThreads) {
-    float x[4];
+  for (int g0 = from + threadIdx.x; g0 < to; g0 += 4 * kMergeThreads) {
+    uint4 v[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) x[j] = k0 + j * kMergeThreads < to ? __bfloat162float(row[k0 + j * kMergeThreads]) : -INFINITY;
+    for (int j = 0; j < 4; ++j) {
+      const int g = g0 + j * kMergeThreads, i = g * 8 - shift;
+      v[j] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+      if (g < to) {
+        if (i >= 0 && i + 8 <= vocab) v[j] = ld_stream(l + i);
+        else v[j] = load_edge(l, i, vocab);
+      }
+    }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (x[j] > -INFINITY) {
-        const unsigned long long t = (unsigned long long)__double2ll_rn(exp2_series(((double)x[j] - m) * 1.4426950408889634) * 0x1p62);
+    for (int j = 0; j < 4; ++j) {
+#pragma unroll 1
+      for (int q = 0; q < 8; ++q) {
+        const uint32_t x = v[j].x & 0xffffu;
+        v[j].x = __funnelshift_r(v[j].x, v[j].y, 16), v[j].y = __funnelshift_r(v[j].y, v[j].z, 16), v[j].z = __funnelshift_r(v[j].z, v[j].w, 16), v[j].w >>= 16;
+        const unsigned long long t = x == 0xff80u ? 0ull : units_of(f64_of(x) - m, table);
         sum += {t >> 32, t & 0xffffffffu};
       }
+    }
   }
   return sum;
 }
@@ -169,14 +205,15 @@ __global__ void __launch_bounds__(kMergeThreads, 1) __cluster_dims__(kMergeCtas,
 beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const float* __restrict__ scores, const int32_t* __restrict__ starts, int n_rows, int per_row, int vocab, int take,
                   const float2* __restrict__ stats, RowStat* rows, UnitSum* parts, int32_t* out_rows, int32_t* out_tokens, float* out_scores) {
   constexpr int kWarps = kMergeThreads / 32;
-  __shared__ double sh_s[kMergeList], sh_sum[kWarps];
-  __shared__ uint64_t sh_id[kMergeList];
-  __shared__ UnitSum sh_part[kWarps];
+  __shared__ Best cand[kMergeList];
   __shared__ Best sorted[kMostTake + 1];
-  __shared__ int need[2 * kMergeList], blocks[kMergeList], n_need, n_list, n_blocks, seen_all;
-  __shared__ uint32_t asked_for[kMergeList / 32];   // rows of the sequence that are in need (of the first kMergeList)
-  __shared__ double known[kKnownRows];              // bases of the first rows
+  __shared__ float warp_tops[kWarps], block_tops[kMergeList];
+  __shared__ UnitSum sh_part[kWarps];
+  __shared__ double sixteenths[16], known[kKnownRows];   // known: bases of the first rows
+  __shared__ int need[2 * kMergeList], blocks[kMergeList], n_need, n_list, n_blocks, seen_all, asked;
+  __shared__ uint32_t asked_for[kMergeList / 32], exact_rows[kMergeList / 32];   // rows of the sequence that are in need, and that have been added up in 64 bits (of the first kMergeList)
   __shared__ Best limit;
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (before shared memory of the other CTA is written, it runs)
   pdl_wait();
   const cg::cluster_group cluster = cg::this_cluster();
   const int cta = (int)cluster.block_rank(), seq = blockIdx.x / kMergeCtas, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -189,18 +226,28 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
     return warp_max(m);
   };
   auto base_of = [&](int r) { return r - r0 < kKnownRows ? known[r - r0] : rows[r].base; };
+  auto near_of = [&](int r) { return r - r0 >= kMergeList ? rows[r].near : exact_rows[(r - r0) >> 5] >> ((r - r0) & 31) & 1 ? 0.0 : kNear; };
   if (cta == 0) {
-    // log-sums of the rows
+    if (tid < kMergeList / 32) exact_rows[tid] = 0;
+    // log-sums of the rows; the first kHeld x 32 blocks of a row stay in registers between the maximum and the sum
+    constexpr int kHeld = 4;
 #pragma unroll 1
     for (int r = r0 + warp; r < r1; r += kWarps) {
       const float2* st = stats + (int64_t)r * per_row;
-      const float m = top_of(r);
+      float2 held[kHeld];
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j) held[j] = 32 * j + lane < per_row ? st[32 * j + lane] : make_float2(-INFINITY, 0.f);
+      float m = fmaxf(fmaxf(held[0].x, held[1].x), fmaxf(held[2].x, held[3].x));
+#pragma unroll 1
+      for (int i = 32 * kHeld + lane; i < per_row; i += 32) m = fmaxf(m, st[i].x);
+      m = warp_max_redux(m);
       double s = 0.0;
-#pragma unroll 2
-      for (int i = lane; i < per_row; i += 32) {
-        const float2 t = st[i];
-        s += (double)t.y * (double)tc::exp2_fast((t.x - m) * kLog2e);   // (both -inf: no number, as the sum of a row that has none)
-      }
+      auto add = [&](const float2& t) { s += (double)t.y * (double)tc::exp2_fast((t.x - m) * kLog2e); };   // (both -inf: no number, as the sum of a row that has none)
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (32 * j + lane < per_row) add(held[j]);
+#pragma unroll 1
+      for (int i = 32 * kHeld + lane; i < per_row; i += 32) add(st[i]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
       if (lane == 0) {
@@ -211,20 +258,21 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
     }
     __syncthreads();
   }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   bool exact = false;   // every row added up in 64 bits
 #pragma unroll 1
   for (;;) {
     if (cta == 0) {
       double margin = exact ? 0.0 : 2 * kNear;
-      // a number that more than `take` threads' `best` reach, and not many more, as fp32 (rounded down): down from the largest in steps of four times the last, then by halves; -inf: there
-      // are no more than `take`
+      // a number that more than `take` threads' `best` reach, and not many more (of blocks, which a warp reads each), as fp32 (rounded down): down from the largest in steps of four times the last,
+      // then by halves; -inf: there are no more than `take`
       auto limit_of = [&](double best) {
         const float top = __double2float_rd(best), wm = warp_max_redux(top);
         __syncthreads();
-        if (lane == 0) sh_sum[warp] = (double)wm;
+        if (lane == 0) warp_tops[warp] = wm;
         int got = __syncthreads_count(top > -INFINITY);
         if (got <= take) return -INFINITY;
-        const float most = warp_max_redux((float)sh_sum[lane & (kWarps - 1)]);
+        const float most = warp_max_redux(warp_tops[lane & (kWarps - 1)]);
         uint32_t high = ordered_f32(most), low = high;
         float step = 0.5f;
         got = 0;
@@ -236,7 +284,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           got = __syncthreads_count(top >= f32_of(low));
         }
 #pragma unroll 1
-        while (low < high && got > take + 1 + (take >> 1) + 8) {
+        while (low < high && got > take + 1 + (take >> 2)) {
           const uint32_t half = low + ((high - low + 1) >> 1);
           const int n = __syncthreads_count(top >= f32_of(half));
           if (n > take) low = half, got = n;
@@ -247,19 +295,26 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
       // blocks by their largest entry
       if (tid == 0) n_list = 0, n_need = 0, n_blocks = 0, seen_all = 1;
       if (tid < kMergeList / 32) asked_for[tid] = 0;
-      double best = -INFINITY;
+      auto block_score = [&](int b, float& x) {
+        x = mine[b].x;
+        return base_of(r0 + b / per_row) + (double)x;
+      };
+      double best = -INFINITY, last_score = -INFINITY;
+      float last_top = -INFINITY;
 #pragma unroll 1
       for (int b = tid; b < all_blocks; b += kMergeThreads) {
-        const double t = base_of(r0 + b / per_row) + (double)mine[b].x;
-        if (t > best) best = t;
+        last_score = block_score(b, last_top);
+        if (last_score > best) best = last_score;
       }
-      Best at = {(double)limit_of(best), ~0ull};
+      Best at = {ordered_f64((double)limit_of(best)), ~0ull};
+      const double lowest = f64_of_ordered(at.score) - margin;
 #pragma unroll 1
       for (int b = tid; b < all_blocks; b += kMergeThreads) {
-        const double t = base_of(r0 + b / per_row) + (double)mine[b].x;
-        if (t > -INFINITY && t >= at.s - margin) {
+        float x = last_top;
+        const double t = all_blocks <= kMergeThreads ? last_score : block_score(b, x);
+        if (t > -INFINITY && t >= lowest) {
           const int k = atomicAdd(&n_blocks, 1);
-          if (k < kMergeList) blocks[k] = b;
+          if (k < kMergeList) blocks[k] = b, block_tops[k] = x;
         }
       }
       __syncthreads();
@@ -270,8 +325,8 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         for (int e = warp; e < (listed <= kMergeList ? listed : all_blocks); e += kWarps) {
           const int b = listed <= kMergeList ? blocks[e] : e, r = r0 + b / per_row;
           const double base = base_of(r);
-          const float x0 = __double2float_rd(least - base);   // (in the logits' own terms, a little less)
-          if (!(base > -INFINITY) || !(mine[b].x >= x0)) continue;
+          const float x0 = __double2float_rd(least - base - fabs(base) * 0x1p-50);   // (in the logits' own terms; where the sum is rounded to fp64, a little less)
+          if (!(base > -INFINITY) || !((listed <= kMergeList ? block_tops[e] : mine[b].x) >= x0)) continue;
           uint4 v[kBlockGroups];
           const int p0 = load_block(logits + (int64_t)r * ld, b - (r - r0) * per_row, vocab, v);
           uint32_t hot = 0;
@@ -288,43 +343,54 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
             for (int i = p0 + g * 256, end = i + 8; i < end; ++i) {   // (outside the row: -inf)
               const float x = bf16lo(w.x);
               w.x = __funnelshift_r(w.x, w.y, 16), w.y = __funnelshift_r(w.y, w.z, 16), w.z = __funnelshift_r(w.z, w.w, 16), w.w >>= 16;
+              if (!(x >= x0 && x > -INFINITY)) continue;
               const double t = base + (double)x;
-              if (x > -INFINITY && t >= least) f(t, id_of(r, x, i));
+              if (t >= least) f(Best{ordered_f64(t), id_of(r, x, i)});
             }
           }
         }
       };
-      bool by_threads = !(at.s > -INFINITY), too_many = false;   // too few blocks: a number that threads' largest entries reach
+      // f(entry, its place) for the first n of the list: a warp an entry
+      auto each_place = [&](int n, auto f) {
+#pragma unroll 1
+        for (int e = warp; e < n; e += kWarps) {
+          const Best x = cand[e];
+          int before = 0;
+#pragma unroll 1
+          for (int k = lane; k < n; k += 32) before += better(cand[k], x);
+          before = __reduce_add_sync(0xffffffffu, before);
+          if (lane == 0) f(x, before);
+        }
+      };
+      bool by_threads = !(f64_of_ordered(at.score) > -INFINITY), too_many = false;   // too few blocks: a number that threads' largest entries reach
 #pragma unroll 1
       for (;;) {
         if (by_threads) {
-          Best own = {-INFINITY, ~0ull - tid};   // (with none: behind all others, and no two alike)
-          each(at.s - margin, [&](double t, uint64_t od) {
-            if (better(t, od, own.s, own.id) && (!too_many || !better(at.s, at.id, t, od))) own = {t, od};
+          Best own = {0, ~0ull - tid};   // (with none: behind all others, and no two alike)
+          each(f64_of_ordered(at.score) - margin, [&](const Best& x) {
+            if (better(x, own) && (!too_many || !better(at, x))) own = x;
           });
           if (too_many) {
             // the entry behind the best `take` threads' own is a limit nearer to the end (of 64 rows of 128 256 entries alike, the best rows last, the list would leave out a thousand at a
             // time).  It leaves take + 1 threads with any: then it is the one behind the best `take` of those that found room, which leaves out all but `take` of them.  Either way
             // fewer are left
-            if (__syncthreads_count(own.s > -INFINITY) > take + 1) sh_s[tid] = own.s, sh_id[tid] = own.id;
+            if (__syncthreads_count(own.score > 0) > take + 1) cand[tid] = own;
             __syncthreads();
-            own = {sh_s[tid], sh_id[tid]};
-            int before = 0;
-#pragma unroll 1
-            for (int k = 0; k < kMergeList; ++k) before += better(sh_s[k], sh_id[k], own.s, own.id);
-            if (before == take) limit = own;
+            each_place(kMergeList, [&](const Best& x, int place) {
+              if (place == take) limit = x;
+            });
             __syncthreads();
             at = limit;
           } else {
-            at.s = fmax(at.s, (double)limit_of(own.s));
+            const uint64_t reached = ordered_f64((double)limit_of(own.score > 0 ? f64_of_ordered(own.score) : -INFINITY));
+            if (reached > at.score) at.score = reached;
           }
           by_threads = false;
         }
-        const double least = at.s - margin;
-        each(least, [&](double t, uint64_t od) {
-          if (t > least || !better(at.s, at.id, t, od)) {
+        each(f64_of_ordered(at.score) - margin, [&](const Best& x) {
+          if (margin > 0.0 || !better(at, x)) {
             const int k = atomicAdd(&n_list, 1);
-            if (k < kMergeList) sh_s[k] = t, sh_id[k] = od;
+            if (k < kMergeList) cand[k] = x;
           }
         });
         __syncthreads();
@@ -336,13 +402,9 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         __syncthreads();
       }
       const int n = n_list;
-#pragma unroll 1
-      for (int e = tid; e < n; e += kMergeThreads) {
-        int before = 0;
-#pragma unroll 4
-        for (int k = 0; k < n; ++k) before += better(sh_s[k], sh_id[k], sh_s[e], sh_id[e]);
-        if (before <= take) sorted[before] = {sh_s[e], sh_id[e]};
-      }
+      each_place(n, [&](const Best& x, int place) {
+        if (place <= take) sorted[place] = x;
+      });
       __syncthreads();
       if (!exact) {
         // candidates of two rows that are nearer to each other than their sums are good for: neighbours among those taken, and the last of them and whatever comes behind
@@ -350,11 +412,11 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         for (int e = tid; e < take + n; e += kMergeThreads) {
           const int k = e < take ? e : take - 1;
           if (k >= n || (e < take && e + 1 >= n)) continue;
-          const Best x = sorted[k], y = e < take ? sorted[e + 1] : Best{sh_s[e - take], sh_id[e - take]};
-          if (!better(x.s, x.id, y.s, y.id)) continue;
+          const Best x = sorted[k], y = e < take ? sorted[e + 1] : cand[e - take];
           const int ra = row_of(x.id), rb = row_of(y.id);
-          const double na = rows[ra].near, nb = rows[rb].near;
-          if (ra != rb && na + nb > 0.0 && x.s - y.s <= na + nb) {
+          if (ra == rb || !better(x, y)) continue;
+          const double na = near_of(ra), nb = near_of(rb);
+          if (na + nb > 0.0 && f64_of_ordered(x.score) - f64_of_ordered(y.score) <= na + nb) {
 #pragma unroll 1
             for (int side = 0; side < 2; ++side) {
               const int r = side ? rb : ra;
@@ -368,30 +430,31 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         __syncthreads();
       }
       const bool all_rows = !exact && !seen_all;
-      if (exact || (n_need == 0 && !all_rows)) {
+      const int wanted = exact ? 0 : all_rows ? -1 : n_need;
+      if (wanted == 0) {
 #pragma unroll 1
         for (int k = tid; k < take; k += kMergeThreads) {
           const int64_t to = (int64_t)seq * take + k;
-          out_rows[to] = k < n ? row_of(sorted[k].id) : -1;
-          out_tokens[to] = k < n ? (int)(uint32_t)sorted[k].id : -1;
-          out_scores[to] = k < n ? (float)sorted[k].s : -INFINITY;
+          const Best x = k < n ? sorted[k] : Best{0, 0};
+          out_rows[to] = k < n ? row_of(x.id) : -1;
+          out_tokens[to] = k < n ? (int)(uint32_t)x.id : -1;
+          out_scores[to] = k < n ? (float)f64_of_ordered(x.score) : -INFINITY;
         }
       }
-      __syncthreads();
-      if (tid == 0 && all_rows) n_need = -1;
+      if (tid < kMergeCtas) *cluster.map_shared_rank(&asked, tid) = wanted;
       exact = exact || all_rows;
     }
-    cluster.sync();   // the other CTAs have waited here: their help is asked for where n_need is not 0 (-1: all rows)
-    const int* asked = cluster.map_shared_rank(&n_need, 0);
+    cluster.sync();   // the other CTAs have waited here: their help is asked for where `asked` is not 0 (-1: all rows)
+    if (asked == 0) return;
+    const int wanted = asked < 0 ? r1 - r0 : asked;
     const int* list = cluster.map_shared_rank(need, 0);
-    const int wanted = *asked < 0 ? r1 - r0 : *asked;
-    const bool by_list = *asked >= 0;
-    const int from = (int)((int64_t)vocab * cta / kMergeCtas), to = (int)((int64_t)vocab * (cta + 1) / kMergeCtas);
-    auto wanted_row = [&](int i) { return by_list ? list[i] : r0 + i; };
+    auto wanted_row = [&](int i) { return asked < 0 ? r0 + i : list[i]; };
+    if (tid < 16) sixteenths[tid] = kSixteenths[tid];
+    __syncthreads();
 #pragma unroll 1
     for (int i = 0; i < wanted; ++i) {
       const int r = wanted_row(i);
-      UnitSum sum = row_part(logits + (int64_t)r * ld, from, to, (double)top_of(r));
+      UnitSum sum = row_part(logits + (int64_t)r * ld, vocab, cta, (double)top_of(r), sixteenths);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += {__shfl_xor_sync(0xffffffffu, sum.high, o), __shfl_xor_sync(0xffffffffu, sum.low, o)};
       __syncthreads();
@@ -402,9 +465,8 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         parts[(int64_t)r * kMergeCtas + cta] = sum;
       }
     }
-    if (wanted > 0) __threadfence();
-    cluster.sync();   // (and nobody has left while another one reads its list)
-    if (wanted == 0) return;
+    __threadfence();
+    cluster.sync();   // (and nobody goes on while another one reads its list)
     if (cta == 0) {
 #pragma unroll 1
       for (int i = warp; i < wanted; i += kWarps) {
@@ -416,9 +478,10 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
             const ulonglong2 t = __ldcg(reinterpret_cast<const ulonglong2*>(parts) + (int64_t)r * kMergeCtas + k);
             sum += {t.x, t.y};
           }
-          const double base = row_base(scores, r, (double)m, value_of(sum));
+          const double base = rows[r].base > -INFINITY ? row_base(scores, r, (double)m, value_of(sum)) : -INFINITY;   // (a row that is none stays none)
           rows[r] = {base, 0.0};
           if (r - r0 < kKnownRows) known[r - r0] = base;
+          if (r - r0 < kMergeList) atomicOr(&exact_rows[(r - r0) >> 5], 1u << ((r - r0) & 31));
         }
       }
       __syncthreads();

@@ -386,6 +386,14 @@ def test_select_among_more_alike_than_any_list_holds(order):
     check_select(logits, scores, _starts(64), 128)
 
 
+def test_select_among_alike_rows_beside_rows_that_are_none():
+    """The sums in 64 bits are asked for, and rows with a NaN, an infinity or nothing stay out of it."""
+    logits = torch.zeros(7, 30000, dtype=BF)
+    logits[0, 29999], logits[2, 77], logits[3], logits[5, :] = NAN, INF, -INF, 1e-39
+    check_select(logits, None, _starts(7), 100)
+    check_select(logits, torch.tensor([0.0, -1.0, 0.0, 0.0, -1.0, -1.0, NAN]), _starts(7), 100)
+
+
 def test_select_between_many_rows_that_are_near():
     """More rows than are kept at hand, all of them in need of 64 bits; in two sequences."""
     g = torch.Generator().manual_seed(78)
@@ -422,6 +430,8 @@ def test_select_of_logits_at_any_scale():
             check_select(logits[:1].contiguous(), None, _starts(1), 4)
         else:
             check_select(logits, torch.rand(8, generator=g) * -4, _starts(4, 4), 12)
+    below = -x.abs() - 0.5
+    check_select(below.to(BF), torch.full((8,), -1e30), _starts(4, 4), 100)   # (sums of which nothing but the beams' own is left)
     low = torch.full((4, 3000), -3.3895e38).to(BF)   # masked by the type's lowest value
     low[:, 5:9] = x[:4, 5:9].to(BF)
     check_select(low, None, _starts(2, 2), 3)
