@@ -204,10 +204,11 @@ __device__ __noinline__ double row_base(const float* scores, int r, double m, do
 __global__ void __launch_bounds__(kMergeThreads, 1) __cluster_dims__(kMergeCtas, 1, 1)
 beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const float* __restrict__ scores, const int32_t* __restrict__ starts, int n_rows, int per_row, int vocab, int take,
                   const float2* __restrict__ stats, RowStat* rows, UnitSum* parts, int32_t* out_rows, int32_t* out_tokens, float* out_scores) {
-  constexpr int kWarps = kMergeThreads / 32;
+  constexpr int kWarps = kMergeThreads / 32, kSteps = 512;
   __shared__ Best cand[kMergeList];
   __shared__ Best sorted[kMostTake + 1];
   __shared__ float warp_tops[kWarps], block_tops[kMergeList];
+  __shared__ int steps[kSteps + 32];
   __shared__ UnitSum sh_part[kWarps];
   __shared__ double sixteenths[16], known[kKnownRows];   // known: bases of the first rows
   __shared__ int need[2 * kMergeList], blocks[kMergeList], n_need, n_list, n_blocks, seen_all, asked;
@@ -264,33 +265,43 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
   for (;;) {
     if (cta == 0) {
       double margin = exact ? 0.0 : 2 * kNear;
-      // a number that more than `take` threads' `best` reach, and not many more (of blocks, which a warp reads each), as fp32 (rounded down): down from the largest in steps of four times the last,
-      // then by halves; -inf: there are no more than `take`
+      // a number that more than `take` threads' `best` reach, and not many more (of blocks, which a warp reads each), as fp32 (rounded down); -inf: there are no more than `take`.
+      // Threads are counted by their distance from the largest, in steps of a sixteenth of a power of two; the number is the far end of the step in which the count passes `take`
+      // (by halves, with a barrier for each, this took 3 000 cycles)
+      auto at_step = [](int k) { return k + k / (kSteps / 32); };   // (no bank conflicts)
       auto limit_of = [&](double best) {
         const float top = __double2float_rd(best), wm = warp_max_redux(top);
         __syncthreads();
         if (lane == 0) warp_tops[warp] = wm;
-        int got = __syncthreads_count(top > -INFINITY);
-        if (got <= take) return -INFINITY;
+        if (tid < kSteps) steps[at_step(tid)] = 0;
+        __syncthreads();
         const float most = warp_max_redux(warp_tops[lane & (kWarps - 1)]);
-        uint32_t high = ordered_f32(most), low = high;
-        float step = 0.5f;
-        got = 0;
-#pragma unroll 1
-        while (got <= take) {
-          if (low != high) high = low - 1;
-          low = step < 1e30f ? ordered_f32(most - step) : ordered_f32(-INFINITY) + 1;
-          step *= 4.f;
-          got = __syncthreads_count(top >= f32_of(low));
+        constexpr uint32_t kFirst = __builtin_bit_cast(uint32_t, 0x1p-23f) >> 19;
+        if (top > -INFINITY) {
+          const uint32_t far = __float_as_uint(most - top) >> 19;   // (by a sixteenth of a power of two each)
+          atomicAdd(&steps[at_step(far < kFirst ? 0 : min(far - kFirst + 1, kSteps - 1u))], 1);
         }
-#pragma unroll 1
-        while (low < high && got > take + 1 + (take >> 2)) {
-          const uint32_t half = low + ((high - low + 1) >> 1);
-          const int n = __syncthreads_count(top >= f32_of(half));
-          if (n > take) low = half, got = n;
-          else high = half - 1;
-        }
-        return f32_of(low);
+        __syncthreads();
+        auto scan = [&](int x) {
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += u;
+          }
+          return x;
+        };
+        int count = 0;   // a lane's kSteps / 32, then of one lane's
+#pragma unroll
+        for (int k = 0; k < kSteps / 32; ++k) count += steps[at_step(lane * (kSteps / 32) + k)];
+        const int until = scan(count);
+        const uint32_t past = __ballot_sync(0xffffffffu, until > take);
+        if (!past) return -INFINITY;
+        const int owner = __ffs(past) - 1, before = __shfl_sync(0xffffffffu, until - count, owner);
+        const int within = scan(lane < kSteps / 32 ? steps[at_step(owner * (kSteps / 32) + lane)] : 0);
+        const int step = owner * (kSteps / 32) + __ffs(__ballot_sync(0xffffffffu, before + within > take)) - 1;
+        if (step == kSteps - 1) return f32_of(ordered_f32(-INFINITY) + 1);   // (the last one has no end)
+        const float end = most - __uint_as_float((kFirst + step) << 19);
+        return end - (fabsf(most) + fabsf(end)) * 0x1p-22f;   // (distances are rounded)
       };
       // blocks by their largest entry
       if (tid == 0) n_list = 0, n_need = 0, n_blocks = 0, seen_all = 1;
