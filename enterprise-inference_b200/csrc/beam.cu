@@ -6,8 +6,9 @@
 // the blocks that reach it, little more than K, are read again.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
 // is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in 64 bits (half of the entries
 // to a CTA) and the CTA picks again.  Entries of one row never need it.
-// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.9 us, 32 sequences of up to 5 rows of 32 000 15.7, 512 rows of 128 256 (131 MB) 37.9, of which the merge takes some 7.  Logits through
-// shared memory by asynchronous copies, two or three blocks a warp ahead, are no faster (39 to 41 us): what is left beside the copy rate's 20 us is the first kernel's start and end.
+// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.3 us, 32 sequences of up to 5 rows of 32 000 12.4, 512 rows of 128 256 (131 MB) 35.2,
+// of which the merge takes some 6; 66 where one sequence has two rows that are near.  Logits through shared memory by asynchronous copies, two or three blocks a warp ahead, are no
+// faster (39 to 41 us against 38 then): what is left beside the copy rate's 20 us is the first kernel's start and end.
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -167,11 +168,16 @@ __device__ __forceinline__ unsigned long long units_of(double d, const double* t
 __device__ __forceinline__ double f64_of(uint32_t b) {
   return (b & 0x7fffu) < 0x80u ? 0.0 : __hiloint2double((int)((b & 0x8000u) << 16 | (((b & 0x7fffu) << 13) + (896u << 20))), 0);
 }
-// what a CTA's share of a row's entries has (of eight at a 16-byte address, four such loads at once); of a row with numbers that are none: anything
-__device__ __noinline__ UnitSum row_part(const __nv_bfloat16* l, int vocab, int cta, double m, const double* table) {
+// What a CTA's share of a row's entries has (of eight at a 16-byte address, four such loads at once); of a row with numbers that are none: anything.  bf16 has 4096 values from 2^-8 up to
+// 2^8: those are counted, and what each has goes into the sum as often (an exponential for every entry takes 80 issue slots of a warp); the few that are nearer to zero, or
+// further from it, by themselves
+constexpr uint32_t kCountFrom = (127 - 8) << 7, kCounted = 16 << 7;   // of either sign
+__device__ __noinline__ UnitSum row_part(const __nv_bfloat16* l, int vocab, int cta, double m, const double* table, uint32_t* counts) {
   const int shift = (int)((reinterpret_cast<uintptr_t>(l) >> 1) & 7), groups = (vocab + shift + 7) / 8;
   const int from = (int)((int64_t)groups * cta / kMergeCtas), to = (int)((int64_t)groups * (cta + 1) / kMergeCtas);
   UnitSum sum = {0, 0};
+  for (int i = threadIdx.x; i < 2 * (int)kCounted; i += kMergeThreads) counts[i] = 0;
+  __syncthreads();
 #pragma unroll 1
   for (int g0 = from + threadIdx.x; g0 < to; g0 += 4 * kMergeThreads) {
     uint4 v[4];
@@ -188,13 +194,26 @@ __device__ __noinline__ UnitSum row_part(const __nv_bfloat16* l, int vocab, int 
     for (int j = 0; j < 4; ++j) {
 #pragma unroll 1
       for (int q = 0; q < 8; ++q) {
-        const uint32_t x = v[j].x & 0xffffu;
+        const uint32_t x = v[j].x & 0xffffu, at = (x & 0x7fffu) - kCountFrom;
         v[j].x = __funnelshift_r(v[j].x, v[j].y, 16), v[j].y = __funnelshift_r(v[j].y, v[j].z, 16), v[j].z = __funnelshift_r(v[j].z, v[j].w, 16), v[j].w >>= 16;
-        const unsigned long long t = x == 0xff80u ? 0ull : units_of(f64_of(x) - m, table);
-        sum += {t >> 32, t & 0xffffffffu};
+        if (at < kCounted) {
+          atomicAdd(counts + (x >> 15) * kCounted + at, 1u);
+        } else if (x != 0xff80u) {
+          const unsigned long long t = units_of(f64_of(x) - m, table);
+          sum += {t >> 32, t & 0xffffffffu};
+        }
       }
     }
   }
+  __syncthreads();
+#pragma unroll 1
+  for (uint32_t i = threadIdx.x; i < 2 * kCounted; i += kMergeThreads) {
+    const unsigned long long n = counts[i];
+    if (n == 0) continue;
+    const unsigned long long t = units_of(f64_of(i < kCounted ? i + kCountFrom : 0x8000u | (i - kCounted + kCountFrom)) - m, table);
+    sum += {n * (t >> 32), n * (t & 0xffffffffu)};
+  }
+  __syncthreads();   // (before they are counted again)
   return sum;
 }
 __device__ __noinline__ double row_base(const float* scores, int r, double m, double sum) {
@@ -459,13 +478,15 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
     if (asked == 0) return;
     const int wanted = asked < 0 ? r1 - r0 : asked;
     const int* list = cluster.map_shared_rank(need, 0);
+    static_assert(sizeof(cand) == 8 * kCounted, "counts of a row's values lie where the list was");
+    uint32_t* const counts = reinterpret_cast<uint32_t*>(cand);
     auto wanted_row = [&](int i) { return asked < 0 ? r0 + i : list[i]; };
     if (tid < 16) sixteenths[tid] = kSixteenths[tid];
     __syncthreads();
 #pragma unroll 1
     for (int i = 0; i < wanted; ++i) {
       const int r = wanted_row(i);
-      UnitSum sum = row_part(logits + (int64_t)r * ld, vocab, cta, (double)top_of(r), sixteenths);
+      UnitSum sum = row_part(logits + (int64_t)r * ld, vocab, cta, (double)top_of(r), sixteenths, counts);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) sum += {__shfl_xor_sync(0xffffffffu, sum.high, o), __shfl_xor_sync(0xffffffffu, sum.low, o)};
       __syncthreads();
