@@ -36,6 +36,7 @@ constexpr uint32_t kLrTmO = 32;                // TMEM columns: two score buffer
 
 struct LrParams {
   const float* q;
+  const __nv_bfloat16* kc;
   const int32_t* block_table;
   const int32_t* row_to_seq;
   const int32_t* ctx_lens;
@@ -141,10 +142,12 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
   const float sk = threadIdx.x < 8 * kLrPairs && fh < n_heads && p.sink && p.n_splits == 1 ? p.sink[h0 + fh] * 1.4426950408889634f : -INFINITY;
 
   if (warp == 0) {
-    // ===== TMA: per tile the value columns two chunks a slot, then the other chunks; 64 keys a box, those past the context's last box left out =====
+    // ===== TMA: per tile the value columns two chunks a slot, then the other chunks; 64 keys a box, those past the context's last box left out.  A last chunk that is no whole one
+    // comes by the warp's own copies (tc.cuh), which end behind the tile's other loads =====
     const bool issuer = elect_one();
     if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     const int32_t* bt = p.block_table + (int64_t)(p.row_to_seq ? p.row_to_seq[t] : t) * p.bt_stride;
+    const int boxes = p.krow >> 6;   // whole chunks
     int st = 0, rs = 0;
     uint32_t st_ph = 1, rs_ph = 1;   // parity of the release that a slot's next load waits for (the first round finds it free)
     for (int i = tile_lo; i < tile_hi && !wait.stop(); ++i) {
@@ -158,19 +161,28 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
       auto load = [&](unsigned char* dst, int c, uint64_t* bar) {
         for (int x = 0; x < halves; ++x) tma_load_2d(dst + x * 8192, &map, c * 64, row[x], bar);
       };
+      auto tail = [&](unsigned char* dst, uint64_t* bar) {
+        for (int x = 0; x < halves; ++x) copy_tail_start(dst + x * 8192, p.kc + (int64_t)row[x] * p.krow + boxes * 64, p.krow, p.krow & 63);
+        copy_tail_end();
+        if (issuer) mbar_arrive(bar);
+      };
       for (int j = 0; j < p.vpairs; ++j) {
         wait(empty + st, st_ph);
+        const int n = min(2, vchunks - 2 * j), by_box = min(n, boxes - 2 * j);
         if (issuer) {
-          const int n = min(2, vchunks - 2 * j);
-          mbar_expect_tx(full + st, n * halves * 8192);
-          for (int c = 0; c < n; ++c) load(ring + (st * 2 + c) * kLrChunk, 2 * j + c, full + st);
+          if (by_box == n) mbar_expect_tx(full + st, n * halves * 8192);
+          else if (by_box) mbar_expect_more(full + st, by_box * halves * 8192);
+          for (int c = 0; c < by_box; ++c) load(ring + (st * 2 + c) * kLrChunk, 2 * j + c, full + st);
         }
         __syncwarp();
+        if (by_box < n) tail(ring + (st * 2 + by_box) * kLrChunk, full + st);
         if (++st == p.slots) st = 0, st_ph ^= 1;
       }
       for (int c = 0; c < p.rest; ++c) {
         wait(rest_empty + rs, rs_ph);
-        if (issuer) {
+        if (vchunks + c == boxes) {
+          tail(rest_ring + rs * kLrChunk, rest_full + rs);
+        } else if (issuer) {
           mbar_expect_tx(rest_full + rs, halves * 8192);
           load(rest_ring + rs * kLrChunk, vchunks + c, rest_full + rs);
         }
@@ -505,6 +517,7 @@ int latent_attn_rows(const float* q, const __nv_bfloat16* kc, const int32_t* blo
   const int rc = get_tensor_map_2d(kc, 1ull << 31, krow, krow, 64, &map);   // rows touched come from the block table
   if (rc) return rc;
   p.q = q;
+  p.kc = kc;
   p.block_table = block_table;
   p.row_to_seq = row_to_seq;
   p.ctx_lens = ctx_lens;

@@ -47,6 +47,7 @@ __host__ __device__ __forceinline__ int lt_own(int rank) { return rank > 256 ? (
 
 struct LtParams {
   const float* q;
+  const __nv_bfloat16* kc;
   const int32_t* block_table;
   const int32_t* row_to_seq;
   const int32_t* ctx_lens;
@@ -162,9 +163,11 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
   };
 
   if (warp == 0) {
-    // ===== TMA: per tile the chunks outside the half first (the scores take them first), then the half's own =====
+    // ===== TMA: per tile the chunks outside the half first (the scores take them first), then the half's own.  A last chunk that is no whole one comes by the warp's own copies
+    // (tc.cuh), whose end is waited for behind the tile's other loads =====
     const bool issuer = elect_one();
     if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
+    const int boxes = p.krow >> 6;   // whole chunks
     int st = 0, sl = 0;
     uint32_t st_ph = 1, sl_ph = 1;   // parity of the release that a slot's next load waits for (the first round finds it free)
     bool stop = false;
@@ -177,18 +180,27 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
         const int tok = i * kLtKeys;
         const int blk = __shfl_sync(0xffffffffu, __ldg(bt + tok / p.block_size), 0);
         const int row = blk * p.block_size + tok % p.block_size;
+        uint64_t* tail = nullptr;   // what the last chunk's own copies arrive at
+        auto load = [&](unsigned char* ring, uint64_t* bar, int n, auto chunk) {   // chunks chunk(0) .. chunk(n - 1); the last one may be no whole one
+          const int by_box = chunk(n - 1) < boxes ? n : n - 1;
+          if (issuer) {
+            if (by_box == n) mbar_expect_tx(bar, n * kLtChunk);
+            else if (by_box) mbar_expect_more(bar, by_box * kLtChunk);
+            for (int c = 0; c < by_box; ++c) tma_load_2d(ring + c * kLtChunk, &map, chunk(c) * 64, row, bar);
+          }
+          __syncwarp();
+          if (by_box < n) copy_tail_start(ring + by_box * kLtChunk, p.kc + (int64_t)row * p.krow + boxes * 64, p.krow, p.krow & 63), tail = bar;
+        };
         if (rest > 0) {
           mbar_wait(rest_free + sl, sl_ph);
-          if (issuer) {
-            mbar_expect_tx(rest_full + sl, rest * kLtChunk);
-            for (int c = 0; c < rest; ++c) tma_load_2d(rest_ring + (sl * rest + c) * kLtChunk, &map, (c < first ? c : c + own) * 64, row, rest_full + sl);
-          }
+          load(rest_ring + sl * rest * kLtChunk, rest_full + sl, rest, [&](int c) { return c < first ? c : c + own; });
           if (++sl == p.rest_stages) sl = 0, sl_ph ^= 1;
         }
         mbar_wait(own_free + st, st_ph);
-        if (issuer) {
-          mbar_expect_tx(own_full + st, own * kLtChunk);
-          for (int c = 0; c < own; ++c) tma_load_2d(own_ring + (st * own + c) * kLtChunk, &map, (first + c) * 64, row, own_full + st);
+        load(own_ring + st * own * kLtChunk, own_full + st, own, [&](int c) { return first + c; });
+        if (tail) {
+          copy_tail_end();
+          if (issuer) mbar_arrive(tail);
         }
         __syncwarp();
         if (++st == p.own_stages) st = 0, st_ph ^= 1;
@@ -555,6 +567,7 @@ int latent_attn_tc(const float* q, const __nv_bfloat16* kc, const int32_t* block
   if (rc) return rc;
   LtParams p = {};
   p.q = q;
+  p.kc = kc;
   p.block_table = block_table;
   p.row_to_seq = row_to_seq;
   p.ctx_lens = ctx_lens;

@@ -67,6 +67,27 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
       "l"(map), "r"(smem_u32(bar)), "r"(c0), "r"(c1)
       : "memory");
 }
+// The columns at the end of cached rows that are no whole box of 64, of 64 rows, by a warp: where a box would have put them (128-byte swizzle, `dst` at a multiple of 1024).  Boxes that
+// reach past a row's end are not used where a map declares more rows than the memory behind it has: steps with such rows (64 bytes under a box of 128) ended in illegal addresses
+// three times, each behind hundreds of other calls, and nothing else of them was out of range.  `src`: the first row's; ld and cols multiples of 16
+__device__ __forceinline__ void copy_tail_start(unsigned char* dst, const __nv_bfloat16* src, int ld, int cols) {
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int r = (threadIdx.x & 31) + 32 * h;
+    for (int x = 0; x < cols >> 3; ++x)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + r * 128 + ((x ^ (r & 7)) << 4))), "l"(src + (int64_t)r * ld + x * 8) : "memory");
+  }
+}
+// behind copy_tail_start: the columns are there for the tensor cores, once the warp has gone on from here
+__device__ __forceinline__ void copy_tail_end() {
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+  __syncwarp();
+}
+// bytes that copies will bring, without the arrival of mbar_expect_tx
+__device__ __forceinline__ void mbar_expect_more(uint64_t* bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+}
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
