@@ -3,10 +3,12 @@
 // score(r, i) = scores[r] + x_ri - log sum_j exp x_rj; a sequence takes the K largest of its rows and all their entries, ties by row, then by entry.
 // blocks: a warp takes 2 048 neighbouring logits, all in registers at once, and leaves their largest, m, and the sum of exp(x - m).  No barriers, nothing is selected.
 // merge: a cluster takes a sequence.  One of its CTAs joins the blocks' sums; a number that more than K blocks' largest scores reach bounds the K-th score from below, and only
-// the blocks that reach it, little more than K, are read again.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
+// the blocks that reach it, little more than K, are read again.  Where a sequence has less than kBlocksEach blocks for each of the K, their largest entries may lie far behind the K-th: groups of
+// eight entries give the limit then; and a list that is longer than K + kSpare is cut by a limit of its own entries (ranks take as long as the square of their number).  50 x 3 rows of 26 316
+// entries, 20 to take, 19.6 us, 37 to 296 without the two; 8 rows of 1 024, 64 to take, 22 and 134; they cost the others 0.3.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
 // is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in 64 bits (half of the entries
 // to a CTA) and the CTA picks again.  Entries of one row never need it.
-// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.3 us, 32 sequences of up to 5 rows of 32 000 12.4, 512 rows of 128 256 (131 MB) 35.2,
+// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.7 us, 32 sequences of up to 5 rows of 32 000 13.4, 512 rows of 128 256 (131 MB) 35.4,
 // of which the merge takes some 6; 66 where one sequence has two rows that are near.  Logits through shared memory by asynchronous copies, two or three blocks a warp ahead, are no
 // faster (39 to 41 us against 38 then): what is left beside the copy rate's 20 us is the first kernel's start and end.
 #include <cooperative_groups.h>
@@ -24,6 +26,7 @@ namespace cg = cooperative_groups;
 constexpr int kBlockThreads = 256, kBlockGroups = 8, kBlock = 32 * 8 * kBlockGroups, kBlockCtas = 4 * kNumSMs;
 constexpr int kMostTake = 128, kMostVocab = 393216;
 constexpr int kMergeThreads = 1024, kMergeCtas = 2, kMergeList = kMergeThreads, kKnownRows = 64;
+constexpr int kBlocksEach = 3, kSpare = 128;
 constexpr float kLog2e = 1.4426950408889634f;
 // What a row's log-sum may be off by: exponents of base 2 are rounded once (2^-24 of up to 17 in the mean over the weights, times ln 2: 7e-7) and have log2 e to 2^-26 (2e-7), the
 // hardware's exponential has 2^-22 (2.4e-7), for a term and for its block's largest, and nine sums and products follow one another in a lane (5e-7); behind them everything is fp64
@@ -220,10 +223,97 @@ __device__ __noinline__ double row_base(const float* scores, int r, double m, do
   const double base = (scores ? (double)scores[r] : 0.0) - (m + log(sum));
   return base - base == 0.0 ? base : -INFINITY;
 }
+// Limits: a number that more than `take` scores reach, and not many more, as fp32 (rounded down); -inf: there are no more than `take`.  Scores are counted by their distance from the
+// largest, in steps of a sixteenth of a power of two; the number is the far end of the step in which the count passes `take` (by halves, with a barrier for each, this took 3 000
+// cycles)
+constexpr int kSteps = 512;
+constexpr uint32_t kFirstStep = __builtin_bit_cast(uint32_t, 0x1p-23f) >> 19;
+__device__ __forceinline__ int at_step(int k) { return k + k / (kSteps / 32); }   // (no bank conflicts)
+__device__ __forceinline__ void count_step(int* steps, float most, float top) {
+  const uint32_t far = __float_as_uint(most - top) >> 19;   // (by a sixteenth of a power of two each)
+  atomicAdd(&steps[at_step(far < kFirstStep ? 0 : min(far - kFirstStep + 1, kSteps - 1u))], 1);
+}
+__device__ __forceinline__ float far_end(const int* steps, float most, int take) {
+  const int lane = threadIdx.x & 31;
+  auto scan = [&](int x) {
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += u;
+    }
+    return x;
+  };
+  int count = 0;   // a lane's kSteps / 32, then of one lane's
+#pragma unroll
+  for (int k = 0; k < kSteps / 32; ++k) count += steps[at_step(lane * (kSteps / 32) + k)];
+  const int until = scan(count);
+  const uint32_t past = __ballot_sync(0xffffffffu, until > take);
+  if (!past) return -INFINITY;
+  const int owner = __ffs(past) - 1, before = __shfl_sync(0xffffffffu, until - count, owner);
+  const int within = scan(lane < kSteps / 32 ? steps[at_step(owner * (kSteps / 32) + lane)] : 0);
+  const int step = owner * (kSteps / 32) + __ffs(__ballot_sync(0xffffffffu, before + within > take)) - 1;
+  if (step == kSteps - 1) return f32_of(ordered_f32(-INFINITY) + 1);   // (the last one has no end)
+  const float end = most - __uint_as_float((kFirstStep + step) << 19);
+  return end - (fabsf(most) + fabsf(end)) * 0x1p-22f;   // (distances are rounded)
+}
+// Where there are few blocks for those to take: the limit of the largest entries of groups of eight
+struct Listed {   // blocks whose scores reach `least`
+  const __nv_bfloat16* logits;
+  const float2* stats;   // of the sequence
+  const RowStat* rows;   // of the sequence
+  const int* blocks;     // NULL: all n
+  int64_t ld;
+  int n, per_row, vocab;
+  double least;
+};
+__device__ __noinline__ float limit_of_groups(const Listed& b, const double* known, int* steps, float* warp_tops, int take) {
+  constexpr int kWarps = kMergeThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < kSteps) steps[at_step(tid)] = 0;
+  float most = -INFINITY;
+  auto base_of = [&](int r) { return r < kKnownRows ? known[r] : b.rows[r].base; };
+  for (int e = tid; e < b.n; e += kMergeThreads) {
+    const int k = b.blocks ? b.blocks[e] : e;
+    most = fmaxf(most, __double2float_rd(base_of(k / b.per_row) + (double)b.stats[k].x));   // (no number: left out)
+  }
+  most = warp_max_redux(most);
+  if (lane == 0) warp_tops[warp] = most;
+  __syncthreads();
+  most = warp_max_redux(warp_tops[lane & (kWarps - 1)]);
+#pragma unroll 1
+  for (int e = warp; e < b.n; e += kWarps) {
+    const int k = b.blocks ? b.blocks[e] : e, r = k / b.per_row;
+    const double base = base_of(r);
+    if (!(base > -INFINITY)) continue;
+    uint4 v[kBlockGroups];
+    load_block(b.logits + (int64_t)r * b.ld, k - r * b.per_row, b.vocab, v);
+#pragma unroll
+    for (int j = 0; j < kBlockGroups; ++j) {
+      const double score = base + (double)max8(v[j]);
+      const float top = __double2float_rd(score);
+      if (score >= b.least && top > -INFINITY) count_step(steps, most, top);
+    }
+  }
+  __syncthreads();
+  return far_end(steps, most, take);
+}
+// The same of the first n of the list
+__device__ __noinline__ float limit_of_list(const Best* cand, int n, int* steps, float* warp_tops, int take) {
+  constexpr int kWarps = kMergeThreads / 32;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  if (tid < kSteps) steps[at_step(tid)] = 0;
+  const float top = tid < n ? __double2float_rd(f64_of_ordered(cand[tid].score)) : -INFINITY, wm = warp_max_redux(top);
+  if (lane == 0) warp_tops[warp] = wm;
+  __syncthreads();
+  const float most = warp_max_redux(warp_tops[lane & (kWarps - 1)]);
+  if (top > -INFINITY) count_step(steps, most, top);
+  __syncthreads();
+  return far_end(steps, most, take);
+}
 __global__ void __launch_bounds__(kMergeThreads, 1) __cluster_dims__(kMergeCtas, 1, 1)
 beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const float* __restrict__ scores, const int32_t* __restrict__ starts, int n_rows, int per_row, int vocab, int take,
                   const float2* __restrict__ stats, RowStat* rows, UnitSum* parts, int32_t* out_rows, int32_t* out_tokens, float* out_scores) {
-  constexpr int kWarps = kMergeThreads / 32, kSteps = 512;
+  constexpr int kWarps = kMergeThreads / 32;
   __shared__ Best cand[kMergeList];
   __shared__ Best sorted[kMostTake + 1];
   __shared__ float warp_tops[kWarps], block_tops[kMergeList];
@@ -284,10 +374,6 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
   for (;;) {
     if (cta == 0) {
       double margin = exact ? 0.0 : 2 * kNear;
-      // a number that more than `take` threads' `best` reach, and not many more (of blocks, which a warp reads each), as fp32 (rounded down); -inf: there are no more than `take`.
-      // Threads are counted by their distance from the largest, in steps of a sixteenth of a power of two; the number is the far end of the step in which the count passes `take`
-      // (by halves, with a barrier for each, this took 3 000 cycles)
-      auto at_step = [](int k) { return k + k / (kSteps / 32); };   // (no bank conflicts)
       auto limit_of = [&](double best) {
         const float top = __double2float_rd(best), wm = warp_max_redux(top);
         __syncthreads();
@@ -295,32 +381,9 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         if (tid < kSteps) steps[at_step(tid)] = 0;
         __syncthreads();
         const float most = warp_max_redux(warp_tops[lane & (kWarps - 1)]);
-        constexpr uint32_t kFirst = __builtin_bit_cast(uint32_t, 0x1p-23f) >> 19;
-        if (top > -INFINITY) {
-          const uint32_t far = __float_as_uint(most - top) >> 19;   // (by a sixteenth of a power of two each)
-          atomicAdd(&steps[at_step(far < kFirst ? 0 : min(far - kFirst + 1, kSteps - 1u))], 1);
-        }
+        if (top > -INFINITY) count_step(steps, most, top);
         __syncthreads();
-        auto scan = [&](int x) {
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, x, o);
-            if (lane >= o) x += u;
-          }
-          return x;
-        };
-        int count = 0;   // a lane's kSteps / 32, then of one lane's
-#pragma unroll
-        for (int k = 0; k < kSteps / 32; ++k) count += steps[at_step(lane * (kSteps / 32) + k)];
-        const int until = scan(count);
-        const uint32_t past = __ballot_sync(0xffffffffu, until > take);
-        if (!past) return -INFINITY;
-        const int owner = __ffs(past) - 1, before = __shfl_sync(0xffffffffu, until - count, owner);
-        const int within = scan(lane < kSteps / 32 ? steps[at_step(owner * (kSteps / 32) + lane)] : 0);
-        const int step = owner * (kSteps / 32) + __ffs(__ballot_sync(0xffffffffu, before + within > take)) - 1;
-        if (step == kSteps - 1) return f32_of(ordered_f32(-INFINITY) + 1);   // (the last one has no end)
-        const float end = most - __uint_as_float((kFirst + step) << 19);
-        return end - (fabsf(most) + fabsf(end)) * 0x1p-22f;   // (distances are rounded)
+        return far_end(steps, most, take);
       };
       // blocks by their largest entry
       if (tid == 0) n_list = 0, n_need = 0, n_blocks = 0, seen_all = 1;
@@ -392,30 +455,30 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           if (lane == 0) f(x, before);
         }
       };
-      bool by_threads = !(f64_of_ordered(at.score) > -INFINITY), too_many = false;   // too few blocks: a number that threads' largest entries reach
+      if (all_blocks < kBlocksEach * take || !(f64_of_ordered(at.score) > -INFINITY)) {
+        const Listed b = {logits + (int64_t)r0 * ld, mine, rows + r0, listed <= kMergeList ? blocks : nullptr, ld, listed <= kMergeList ? listed : all_blocks, per_row, vocab,
+                          f64_of_ordered(at.score) - margin};
+        at.score = max(at.score, ordered_f64((double)limit_of_groups(b, known, steps, warp_tops, take)));
+        __syncthreads();
+      }
+      bool too_many = false, closer = false;
 #pragma unroll 1
       for (;;) {
-        if (by_threads) {
+        if (too_many) {
           Best own = {0, ~0ull - tid};   // (with none: behind all others, and no two alike)
           each(f64_of_ordered(at.score) - margin, [&](const Best& x) {
-            if (better(x, own) && (!too_many || !better(at, x))) own = x;
+            if (better(x, own) && !better(at, x)) own = x;
           });
-          if (too_many) {
-            // the entry behind the best `take` threads' own is a limit nearer to the end (of 64 rows of 128 256 entries alike, the best rows last, the list would leave out a thousand at a
-            // time).  It leaves take + 1 threads with any: then it is the one behind the best `take` of those that found room, which leaves out all but `take` of them.  Either way
-            // fewer are left
-            if (__syncthreads_count(own.score > 0) > take + 1) cand[tid] = own;
-            __syncthreads();
-            each_place(kMergeList, [&](const Best& x, int place) {
-              if (place == take) limit = x;
-            });
-            __syncthreads();
-            at = limit;
-          } else {
-            const uint64_t reached = ordered_f64((double)limit_of(own.score > 0 ? f64_of_ordered(own.score) : -INFINITY));
-            if (reached > at.score) at.score = reached;
-          }
-          by_threads = false;
+          // the entry behind the best `take` threads' own is a limit nearer to the end (of 64 rows of 128 256 entries alike, the best rows last, the list would leave out a thousand at a
+          // time).  It leaves take + 1 threads with any: then it is the one behind the best `take` of those that found room, which leaves out all but `take` of them.  Either way
+          // fewer are left
+          if (__syncthreads_count(own.score > 0) > take + 1) cand[tid] = own;
+          __syncthreads();
+          each_place(kMergeList, [&](const Best& x, int place) {
+            if (place == take) limit = x;
+          });
+          __syncthreads();
+          at = limit;
         }
         each(f64_of_ordered(at.score) - margin, [&](const Best& x) {
           if (margin > 0.0 || !better(at, x)) {
@@ -424,11 +487,28 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           }
         });
         __syncthreads();
-        if (n_list <= kMergeList) break;
+        const int found = n_list;
+        if (found <= take + kSpare) break;
+        if (!closer) {   // a limit by those that found room: ranks take as long as the square of their number
+          closer = true;
+          const uint64_t reached = ordered_f64((double)limit_of_list(cand, min(found, kMergeList), steps, warp_tops, take));
+          if (reached > at.score) {
+            at.score = reached;
+            const Best x = cand[tid];
+            __syncthreads();
+            if (tid == 0) n_list = 0;
+            __syncthreads();
+            if (found > kMergeList) continue;   // from the blocks again
+            if (tid < found && f64_of_ordered(x.score) >= f64_of_ordered(reached) - margin) cand[atomicAdd(&n_list, 1)] = x;
+            __syncthreads();
+            break;
+          }
+        }
+        if (found <= kMergeList) break;
         __syncthreads();
         if (tid == 0) n_list = 0, seen_all = margin == 0.0 && seen_all;   // (those next to the limit will not all be seen)
         margin = 0.0;
-        by_threads = too_many = true;
+        too_many = true;
         __syncthreads();
       }
       const int n = n_list;

@@ -346,6 +346,15 @@ def test_select_at_many_sizes(seqs, beams, vocab, take):
     check_select(logits, -9 * torch.rand(seqs * beams, generator=g), _starts(*[beams] * seqs), take)
 
 
+@pytest.mark.parametrize("seqs,beams,vocab,take", [(5, 3, 26316, 20), (3, 3, 128256, 64), (2, 8, 32000, 128), (4, 1, 1024, 64), (3, 2, 300, 128), (2, 40, 2100, 128), (1, 2, 26316, 100)])
+@pytest.mark.parametrize("far", [0.0, 6.0, 40.0])
+def test_select_from_few_blocks(seqs, beams, vocab, take, far):
+    """Little more than as many blocks of logits as are to be taken, of rows that are far apart: the best row has thousands of entries in front of the other rows' best."""
+    g = torch.Generator().manual_seed(vocab + take)
+    logits = (torch.randn(seqs * beams, vocab, generator=g) * 2.5).to(BF)
+    check_select(logits, -far * torch.rand(seqs * beams, generator=g), _starts(*[beams] * seqs), take)
+
+
 @pytest.mark.parametrize("take", [1, 5, 16, 128])
 def test_select_among_ties(take):
     """Entries alike within a row and between rows: the lower row, then the lower entry; more of them than any list holds."""
