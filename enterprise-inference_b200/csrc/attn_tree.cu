@@ -16,8 +16,8 @@
 // (relative error 0.0017 over all; with the high term alone 0.0024, and a tenth faster with two tiles of pairs).  All else is fp32.
 //
 // Times on a B200, caches in HBM, 8 kv heads of 128 (its copy rate 6.56 TB/s, its bf16 rate 1670 TFLOP/s):
-//   8 nodes of a sequence of 600 tokens, 32 heads       16 us   latency: start and plan 4, walk and epilogue 4, launches and join 8
-//   64 nodes, 32 000 tokens, 32 heads                   57 us   131 MB: 2.3 TB/s; two tiles of pairs
+//   8 nodes of a sequence of 600 tokens, 32 heads       15 us   latency: start and plan 4, walk and epilogue 4, launches and join 7
+//   64 nodes, 32 000 tokens, 32 heads                   55 us   131 MB: 2.4 TB/s; two tiles of pairs
 //   32 x up to 25 nodes, 4 000 tokens, 32 heads        109 us   437 MB: 4.0 TB/s
 //   4 x 256 nodes, 6 000 tokens, 40 heads              160 us   tensor cores 64 % of their cycles; two tiles of pairs
 //   16 x 6 beams, 2 500 tokens, 64 heads, blocks of 16  55 us   133 MB: 2.4 TB/s (blocks of 128: 49)
@@ -711,13 +711,15 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 }
 
 // ---- parts -> out -----------------------------------------------------------------------------------------------------------------------
-// A warp takes 32 pairs of an item and eight columns: sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m) over its parts, in their order.  Bound by latency: two rounds of loads, for
-// which four CTAs an SM have the warps (one: 4 x 256 rows over 6000 tokens 192 us in all, four 164)
+// A job is 32 pairs of an item and eight columns: sum of a_i 2^(m_i - m) / sum of l_i 2^(m_i - m) over its parts, in their order.  Bound by latency, rounds of loads, for which four CTAs
+// an SM have the warps (one: 4 x 256 rows over 6000 tokens 192 us in all, four 164).  Where there are fewer jobs than warps, two, four or eight warps share a job's parts (a
+// tree of 30 nodes over 17 000 tokens, 4 heads over one, whose only item has 136 parts: 23 us in all, 65 with a warp a job; eight of 600 tokens, 32 over 8, 14.6 and 16.1; each part's loads of both rounds at once 15.4)
 constexpr int kJoinThreads = 256, kJoinColumns = 8, kJoinCtas = 4;
 
 __global__ void __launch_bounds__(kJoinThreads, kJoinCtas) tree_join_kernel(const __grid_constant__ TreeParams p) {
   __shared__ int front[kJoinThreads + 1], sh[kJoinThreads / 32];
   __shared__ Kv8Cut cuts[kNumSMs];
+  __shared__ float sums[10][kJoinThreads];   // maximum, denominator, columns
   pdl_wait();
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = p.hq / p.hkv;
@@ -741,31 +743,55 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinCtas) tree_join_kernel(cons
   __syncthreads();
   const float unit = p.scale * 1.4426950408889634f;
   const int64_t slot = (int64_t)p.pairs * kTrPart;
+  constexpr int kWarps = kJoinThreads / 32;
+  const int jobs = front[kJoinThreads];
+  int ways = 1;   // warps of a job
+  while (2 * ways <= kWarps && (int64_t)jobs * 2 * ways <= (int64_t)gridDim.x * kWarps) ways *= 2;
+  const int sub = warp % ways, step = gridDim.x * (kWarps / ways);
 #pragma unroll 1
-  for (int job = blockIdx.x * (kJoinThreads / 32) + warp; job < front[kJoinThreads]; job += gridDim.x * (kJoinThreads / 32)) {
+  for (int job0 = blockIdx.x * (kWarps / ways); job0 < jobs; job0 += step) {   // (the same in all warps; once, if several share a job)
+    const int job = job0 + warp / ways;
+    const bool in = job < jobs;
     int k = 0;   // the last with front[k] <= job
 #pragma unroll
     for (int b = kJoinThreads / 2; b > 0; b >>= 1)
       if (front[k + b] <= job) k += b;
-    const Kv8Cut cut = cuts[k];
+    const Kv8Cut cut = cuts[min(k, kNumSMs - 1)];
     const int at = job - front[k], c = at % (kHeadDim / kJoinColumns), pair = at / (kHeadDim / kJoinColumns) * 32 + lane;
-    const bool alive = pair < cut.nrows * G;
     const float* part = p.part + (2 * k + 1) * slot;   // the first: behind it every other one
     auto part_of = [&](int i) { return part + (i ? 2 * i - 1 : 0) * slot; };
     auto ml = [&](int i) { return reinterpret_cast<const float2*>(part_of(i) + (int64_t)p.pairs * kHeadDim)[pair]; };
     float m = -INFINITY, l = 0.f, a[8] = {};
+    const int each = (cut.parts + ways - 1) / ways, i0 = in ? sub * each : 0, i1 = in ? min(cut.parts, i0 + each) : 0;
 #pragma unroll 8
-    for (int i = 0; i < cut.parts; ++i) m = fmaxf(m, ml(i).x);
+    for (int i = i0; i < i1; ++i) m = fmaxf(m, ml(i).x);
 #pragma unroll 4
-    for (int i = 0; i < cut.parts; ++i) {
+    for (int i = i0; i < i1; ++i) {
       const float2 t = ml(i);
       const float4 *v = reinterpret_cast<const float4*>(part_of(i)) + (int64_t)(2 * c) * p.pairs + pair, x = __ldcg(v), y = __ldcg(v + p.pairs);
       const float f = t.x == m ? 1.f : exp2_fast((t.x - m) * unit);
       l += t.y * f;
       a[0] += x.x * f, a[1] += x.y * f, a[2] += x.z * f, a[3] += x.w * f, a[4] += y.x * f, a[5] += y.y * f, a[6] += y.z * f, a[7] += y.w * f;
     }
+    if (ways > 1) {
+      sums[0][tid] = m, sums[1][tid] = l;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sums[2 + j][tid] = a[j];
+      __syncthreads();
+      if (sub) return;
+      for (int w = 1; w < ways; ++w) m = fmaxf(m, sums[0][tid + 32 * w]);
+      l = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] = 0.f;
+      for (int w = 0; w < ways; ++w) {
+        const float own = sums[0][tid + 32 * w], f = own == m ? 1.f : exp2_fast((own - m) * unit);
+        l += sums[1][tid + 32 * w] * f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] += sums[2 + j][tid + 32 * w] * f;
+      }
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
-    if (alive)
+    if (in && pair < cut.nrows * G)
       *reinterpret_cast<uint4*>(p.out + (int64_t)(cut.row0 + pair / G) * p.ldo + (cut.kvh * G + pair % G) * kHeadDim + c * kJoinColumns) =
           make_uint4(pack_bf16(a[0] * inv, a[1] * inv), pack_bf16(a[2] * inv, a[3] * inv), pack_bf16(a[4] * inv, a[5] * inv), pack_bf16(a[6] * inv, a[7] * inv));
   }

@@ -221,6 +221,15 @@ def test_long_contexts_and_many_tiles():
     step.check(step.run(), [0, 1, 35, 69, 70, 72, 73, 92])
 
 
+@pytest.mark.parametrize("heads,hkv,nodes,ctx", [(4, 1, 30, 9000), (16, 1, 1, 12000), (4, 1, 51, 2600), (1, 1, 3, 9000), (32, 8, 8, 600), (32, 8, 40, 9000), (64, 8, 2, 5000)])
+def test_items_of_many_parts(heads, hkv, nodes, ctx):
+    """One sequence over all CTAs: parts of 2 to 140 CTAs are joined by one to eight warps a job."""
+    step = Step([(ctx, U.lines(_random_tree(nodes, torch.Generator().manual_seed(nodes))))], heads, hkv, 128, nodes + ctx)
+    out = step.run()
+    step.check(out, rows=sorted({0, nodes // 2, nodes - 1}))
+    assert torch.equal(out, step.run())
+
+
 def test_thousands_of_short_sequences_beside_a_long_one():
     """More walks of a CTA than its table holds; contexts of nothing among them."""
     g = torch.Generator().manual_seed(16)
