@@ -5,10 +5,10 @@
 // merge: a cluster takes a sequence.  One of its CTAs joins the blocks' sums; a number that more than K blocks' largest scores reach bounds the K-th score from below, and only
 // the blocks that reach it, little more than K, are read again.  Where a sequence has less than kBlocksEach blocks for each of the K, their largest entries may lie far behind the K-th: groups of
 // eight entries give the limit then; and a list that is longer than K + kSpare is cut by a limit of its own entries (ranks take as long as the square of their number).  50 x 3 rows of 26 316
-// entries, 20 to take, 19.6 us, 37 to 296 without the two; 8 rows of 1 024, 64 to take, 22 and 134; they cost the others 0.3.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
+// entries, 20 to take, 18 us, 37 to 296 without the two; 8 rows of 1 024, 64 to take, 21 and 134; they cost the others 0.3.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
 // is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in 64 bits (half of the entries
 // to a CTA) and the CTA picks again.  Entries of one row never need it.
-// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.7 us, 32 sequences of up to 5 rows of 32 000 13.4, 512 rows of 128 256 (131 MB) 35.4,
+// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.4 us, 32 sequences of up to 5 rows of 32 000 13.1, 512 rows of 128 256 (131 MB) 34.5,
 // of which the merge takes some 6; 66 where one sequence has two rows that are near.  Logits through shared memory by asynchronous copies, two or three blocks a warp ahead, are no
 // faster (39 to 41 us against 38 then): what is left beside the copy rate's 20 us is the first kernel's start and end.
 #include <cooperative_groups.h>
@@ -52,16 +52,12 @@ __device__ __forceinline__ uint32_t ordered_f32(float x) {
 }
 __device__ __forceinline__ float f32_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o); }
 
-// eight logits from entry i0 on, of which some lie outside the row (-inf), entry by entry
+// eight logits from entry i0 on, of which some lie outside the row (-inf), entry by entry, all asked for at once (one after another: 57 x 2 rows of 571 entries 19.8 us, 15.1 so)
 __device__ __forceinline__ uint4 load_edge(const __nv_bfloat16* l, int i0, int vocab) {
-  uint4 w = make_uint4(0, 0, 0, 0);
-#pragma unroll 1
-  for (int q = 7; q >= 0; --q) {
-    const int i = i0 + q;
-    const uint32_t e = i >= 0 && i < vocab ? __bfloat16_as_ushort(l[i]) : 0xff80u;
-    w.w = w.w << 16 | w.z >> 16, w.z = w.z << 16 | w.y >> 16, w.y = w.y << 16 | w.x >> 16, w.x = w.x << 16 | e;
-  }
-  return w;
+  uint32_t e[8];
+#pragma unroll
+  for (int q = 0; q < 8; ++q) e[q] = i0 + q >= 0 && i0 + q < vocab ? __bfloat16_as_ushort(l[i0 + q]) : 0xff80u;
+  return make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
 }
 // a lane's eight groups of eight logits of a row's block (-inf outside the row); groups start at 16-byte addresses: entry i of a row is at place i + shift.  Returns the first one's index
 __device__ __forceinline__ int load_block(const __nv_bfloat16* l, int block, int vocab, uint4 (&v)[kBlockGroups]) {
@@ -72,21 +68,24 @@ __device__ __forceinline__ int load_block(const __nv_bfloat16* l, int block, int
     for (int j = 0; j < kBlockGroups; ++j) v[j] = ld_stream(at + j * 256);
     return p0;
   }
+  // groups that cross the row's start (the first lane's first) or its end
+  const int lane = threadIdx.x & 31, place = vocab + shift, at = (place >> 3) - block * (kBlock / 8), end = (place & 7) && at >= 0 && at < kBlock / 8 && (at & 31) == lane ? at >> 5 : -1;
+  const bool start = block == 0 && lane == 0 && shift;
+  const int g = start ? 0 : end;
+  uint4 w = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+  if (g >= 0) w = load_edge(l, p0 + g * 256, vocab);
 #pragma unroll
   for (int j = 0; j < kBlockGroups; ++j) {
     const int i = p0 + j * 256;
     v[j] = make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
     if (i >= 0 && i + 8 <= vocab) v[j] = ld_stream(l + i);
+    else if (j == g) v[j] = w;
   }
-  // groups that cross the row's ends: entry by entry
-#pragma unroll 1
-  for (int g = 0; g < kBlockGroups; ++g) {
-    const int i0 = p0 + g * 256;
-    if (!((i0 < 0 && i0 + 8 > 0) || (i0 < vocab && i0 + 8 > vocab))) continue;
-    const uint4 w = load_edge(l, i0, vocab);
+  if (start && end > 0) {
+    w = load_edge(l, p0 + end * 256, vocab);
 #pragma unroll
     for (int j = 0; j < kBlockGroups; ++j)
-      if (j == g) v[j] = w;
+      if (j == end) v[j] = w;
   }
   return p0;
 }
