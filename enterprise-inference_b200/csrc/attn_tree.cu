@@ -40,6 +40,10 @@ constexpr int kTrChunk = kTreeKeys * 128;       // [64 keys][64 columns] bf16
 constexpr int kTrTile = 2 * kTrChunk;
 constexpr int kTrStage = 8 * 2048;              // output staging: 2 KiB per softmax warp
 constexpr int kTrBad = 64;                      // tiles of an item for which it is known which keys' values are no numbers
+// Items whose marks of such values are kept.  Of two tiles of pairs, a group may be two items with key tiles ahead of the other: the queries of item i + 2 wait for both groups' last scores of
+// item i + 1, which, if it has one or two key tiles, are issued before any of its weights, while the other group may still be at the end of item i.  Not three: its last scores of item i + 2 come
+// behind its weights of item i + 1, thus behind the end of item i
+constexpr int kTrMarks = 3;
 constexpr int kTrPart = kHeadDim + 2;           // floats of a pair in a part: sums, their maximum (of the products q . k), the denominator
 constexpr int kTreeTable = 48;                  // units of a CTA in shared memory
 constexpr int kMostRows = 4096;                 // of a step: the plan's lists fit where the tiles come to lie
@@ -77,7 +81,7 @@ struct TreeParams {
 __host__ __device__ __forceinline__ int64_t tree_tokens(const TreeParams& p) { return (int64_t)p.bt_stride * p.block_size; }
 __device__ __forceinline__ int tree_ctx(const TreeParams& p, int row) { return (int)min((int64_t)max(__ldg(p.ctx_lens + row), 0), tree_tokens(p)); }
 
-constexpr int kTrSmem = 1024 + 4 * kTrQChunk + kTreeSlots * kTrTile + kTrStage + 2 * 128 * 8 + 2 * kTrBad * 16 + (2 * kTreeSlots + 16) * 8 + 32 + kTreeTable * (int)sizeof(TreeWork) + 320;
+constexpr int kTrSmem = 1024 + 4 * kTrQChunk + kTreeSlots * kTrTile + kTrStage + 2 * 128 * 8 + kTrMarks * kTrBad * 16 + (2 * kTreeSlots + 16) * 8 + 32 + kTreeTable * (int)sizeof(TreeWork) + 320;
 static_assert(5 * kMostRows * 4 <= kTreeSlots * kTrTile, "the plan's lists");
 static_assert(kTrSmem <= 232448, "shared memory");
 
@@ -329,8 +333,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   unsigned char* ring = qs + 4 * kTrQChunk;        // [kTreeSlots][2][64 keys][64]: key and value tiles in turn
   unsigned char* ostage = ring + kTreeSlots * kTrTile;
   float2* exchange = reinterpret_cast<float2*>(ostage + kTrStage);                   // [group][pair] maximum, sum
-  uint32_t(*bad_keys)[4] = reinterpret_cast<uint32_t(*)[4]>(exchange + 2 * 128);    // [item's parity][tile][16 keys]: two bits a key
-  uint64_t* kv_full = reinterpret_cast<uint64_t*>(bad_keys + 2 * kTrBad);
+  uint32_t(*bad_keys)[4] = reinterpret_cast<uint32_t(*)[4]>(exchange + 2 * 128);    // [item % kTrMarks][tile][16 keys]: two bits a key
+  uint64_t* kv_full = reinterpret_cast<uint64_t*>(bad_keys + kTrMarks * kTrBad);
   uint64_t* kv_free = kv_full + kTreeSlots;
   uint64_t* s_full = kv_free + kTreeSlots;         // [group][2] the scores of its even / odd key tile are there
   uint64_t* p_ready = s_full + 4;                  // [group][2] their weights are
@@ -339,8 +343,8 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
   uint64_t* q_free = q_ready + 1;
   uint64_t* last = q_free + 1;                     // [group] the MMAs in flight when a wait ran out
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last + 2);   // and, behind it, the mark of a wait that ran out
-  int* taken_item = reinterpret_cast<int*>(tmem_slot + 2);       // [item's parity] the last one (counted from 1) with values that were taken out of a tile
-  TreeWork* table = reinterpret_cast<TreeWork*>((reinterpret_cast<uintptr_t>(taken_item + 2) + 15) & ~(uintptr_t)15);
+  int* taken_item = reinterpret_cast<int*>(tmem_slot + 2);       // [item % kTrMarks] the last one (counted from 1) with values that were taken out of a tile
+  TreeWork* table = reinterpret_cast<TreeWork*>((reinterpret_cast<uintptr_t>(taken_item + kTrMarks) + 15) & ~(uintptr_t)15);
   PlanShared* plan = reinterpret_cast<PlanShared*>(table + kTreeTable);
   const Waits mbar_wait(tmem_slot + 1, p.status);
   if (threadIdx.x == 0) {
@@ -358,7 +362,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     mbar_init(last, 1);
     mbar_init(last + 1, 1);
     tmem_slot[1] = 0;
-    taken_item[0] = taken_item[1] = 0;
+    for (int s = 0; s < kTrMarks; ++s) taken_item[s] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 9) {
@@ -509,11 +513,12 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
     const uint32_t base = tmem + ((uint32_t)(quad * 32) << 16), own = base + x * 256;
     const int r = m / G, g = m % G;
     const float sc2 = p.scale * 1.4426950408889634f;   // scores in the log2 domain
-    int n = 0, done = 0, item = 0, cleaned = 0;   // key tiles of this group so far; of all items before; items; tiles cleaned by group 0 for both
+    int n = 0, done = 0, item = 0, cleaned = 0;   // key tiles of this group so far; of all items before; items with key tiles; tiles cleaned by group 0 for both
     TreeWork w;
     while (next_work(w)) {
-      ++item;   // (a group is at most one item ahead of the other)
-      uint32_t(*const bad)[4] = bad_keys + (item & 1) * kTrBad;
+      if (w.tile1 > w.tile0) ++item;   // (nothing holds the groups together in the others, nor is anything marked)
+      const int marks = item % kTrMarks;
+      uint32_t(*const bad)[4] = bad_keys + marks * kTrBad;
       const bool two = w.rows.nrows > R;
       const int row = (two ? x * R : 0) + r, t = w.rows.row0 + row;
       const bool alive = r < R && row < w.rows.nrows, live = __any_sync(0xffffffffu, alive);   // a warp without a pair hands over whatever there is: its rows are never looked at
@@ -604,7 +609,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
           const uint32_t keys = __ballot_sync(0xffffffffu, found != 0 && !behind);
           if (lane == 0) {
             if (i - masked < kTrBad) bad[i - masked][quad] = keys;
-            if (keys) reinterpret_cast<volatile int*>(taken_item)[item & 1] = item;
+            if (keys) reinterpret_cast<volatile int*>(taken_item)[marks] = item;
           }
           fence_async_smem();
         }
@@ -639,7 +644,7 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
         l = l * f_own + o.y * f_other;
         mu = mn;
       }
-      const bool taken = reinterpret_cast<volatile int*>(taken_item)[item & 1] == item;
+      const bool taken = w.tile1 > w.tile0 && reinterpret_cast<volatile int*>(taken_item)[marks] == item;
       const int c0 = two ? 0 : x * 64, c1 = two ? kHeadDim : c0 + 64;
       const float inv = w.parts > 1 ? 1.f : l == 0.f ? 0.f : 1.f / l;
       float4* const part = reinterpret_cast<float4*>(p.part + (int64_t)w.slot * p.pairs * kTrPart) + row * G + g;

@@ -191,6 +191,37 @@ def test_values_that_are_no_numbers_reach_the_rows_that_see_them(what):
     assert torch.isfinite(out).all()
 
 
+@pytest.mark.parametrize("what", [NAN, INF, -INF])
+@pytest.mark.parametrize("contexts,idle", [((0,), 0), ((0, 40, 64), 0), ((0, 64), 2), ((10, 70, 130, 5), 1)])
+def test_values_that_are_no_numbers_in_walks_over_many_short_sequences(what, contexts, idle):
+    """A CTA walks many items of two tiles of pairs and one to four key tiles: every third sequence has values that are no numbers in tokens that only the second tile's rows see,
+    the others have none, and some sequences have rows that see nothing."""
+    g = torch.Generator().manual_seed(idle + len(contexts))
+    heads, hkv, n, seqs = 64, 16, 48, []   # 32 rows to a tile of pairs
+    kinds = [k for _ in range(85) for k in ["bad", "clean", "clean"] + ["idle"] * idle][:85]
+    for i, kind in enumerate(kinds):
+        seqs.append((0, [[]] * n) if kind == "idle" else (contexts[i % len(contexts)], U.lines(_random_tree(n, g, 6))))
+    step = Step(seqs, heads, hkv, 64, 40 + idle)
+    first, marked = 0, []
+    for s, (kind, (ctx, lines)) in enumerate(zip(kinds, seqs)):
+        if kind == "bad":
+            for j in range(32, n):
+                b, o = step.cache.token(s, ctx + j)
+                step.cache.v[b, :, o] = what
+            marked += range(first + 32, first + n)   # (each sees itself)
+        first += n
+    clean = sorted(set(range(step.T)) - set(marked))
+    out = step.run()
+    for _ in range(5):
+        got = out.view(step.T, heads * 128)
+        assert (torch.isnan(got[marked]) if what != what else got[marked] == what).all()
+        assert torch.isfinite(got[clean]).all()
+        again = step.run(ws=step.ws, dev=step.dev)
+        assert torch.equal(again[clean], out[clean])
+        out = again
+    step.check(out, [t for t in (*range(0, 2 * n, 7), *range(3 * n, 4 * n, 5)) if t in clean])
+
+
 def test_blocks_that_are_none_stand_for_zeros():
     step = Step([(300, [[0], [0, 1]]), (100, [[], [2]])], 8, 2, 64, 10)
     step.cache.bt[0, 1], step.cache.bt[0, 3], step.cache.bt[1, 0] = -1, step.cache.n_blocks, 2 ** 30
