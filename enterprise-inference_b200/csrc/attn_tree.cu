@@ -721,6 +721,17 @@ attn_tree_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constan
 // tree of 30 nodes over 17 000 tokens, 4 heads over one, whose only item has 136 parts: 23 us in all, 65 with a warp a job; eight of 600 tokens, 32 over 8, 14.6 and 16.1; each part's loads of both rounds at once 15.4)
 constexpr int kJoinThreads = 256, kJoinColumns = 8, kJoinCtas = 4;
 
+// sums += a part's times what brings them to the maximum of all.  Weights are above zero: what is no number stays, however little of it fp32 has (0 x inf would make a NaN of an infinity)
+__device__ __forceinline__ void join_part(float (&a)[8], const float (&x)[8], float f) {
+  if (f > 0.f || f != f) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] += x[j] * f;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) a[j] += x[j] - x[j] == 0.f ? 0.f : x[j];
+  }
+}
+
 __global__ void __launch_bounds__(kJoinThreads, kJoinCtas) tree_join_kernel(const __grid_constant__ TreeParams p) {
   __shared__ int front[kJoinThreads + 1], sh[kJoinThreads / 32];
   __shared__ Kv8Cut cuts[kNumSMs];
@@ -776,7 +787,7 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinCtas) tree_join_kernel(cons
       const float4 *v = reinterpret_cast<const float4*>(part_of(i)) + (int64_t)(2 * c) * p.pairs + pair, x = __ldcg(v), y = __ldcg(v + p.pairs);
       const float f = t.x == m ? 1.f : exp2_fast((t.x - m) * unit);
       l += t.y * f;
-      a[0] += x.x * f, a[1] += x.y * f, a[2] += x.z * f, a[3] += x.w * f, a[4] += y.x * f, a[5] += y.y * f, a[6] += y.z * f, a[7] += y.w * f;
+      join_part(a, {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w}, f);
     }
     if (ways > 1) {
       sums[0][tid] = m, sums[1][tid] = l;
@@ -791,8 +802,10 @@ __global__ void __launch_bounds__(kJoinThreads, kJoinCtas) tree_join_kernel(cons
       for (int w = 0; w < ways; ++w) {
         const float own = sums[0][tid + 32 * w], f = own == m ? 1.f : exp2_fast((own - m) * unit);
         l += sums[1][tid + 32 * w] * f;
+        float x[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) a[j] += sums[2 + j][tid + 32 * w] * f;
+        for (int j = 0; j < 8; ++j) x[j] = sums[2 + j][tid + 32 * w];
+        join_part(a, x, f);
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;

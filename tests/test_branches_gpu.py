@@ -222,6 +222,20 @@ def test_values_that_are_no_numbers_in_walks_over_many_short_sequences(what, con
     step.check(out, [t for t in (*range(0, 2 * n, 7), *range(3 * n, 4 * n, 5)) if t in clean])
 
 
+@pytest.mark.parametrize("what", [NAN, INF, -INF])
+@pytest.mark.parametrize("heads,hkv,nodes,ctx", [(8, 2, 3, 70), (8, 2, 3, 5000), (4, 1, 30, 9000), (32, 8, 40, 9000), (4, 1, 200, 3000)])
+def test_values_that_are_no_numbers_under_weights_of_next_to_nothing(what, heads, hkv, nodes, ctx):
+    """One of the last tokens has nearly all of the weight, by more than fp32 can tell; what is no number far in front of it is seen all the same, whatever the CTAs' shares."""
+    step = Step([(ctx, U.lines(_random_tree(nodes, torch.Generator().manual_seed(3))))], heads, hkv, 128, 50 + nodes)
+    b, o = step.cache.token(0, ctx - 1)
+    step.q[:] = step.q.abs()
+    step.cache.k[b, :, o] = 30.0   # scores of some hundreds, next to some units
+    b, o = step.cache.token(0, 5)
+    step.cache.v[b, hkv - 1, o, 7] = what
+    out = step.run().view(step.T, heads, 128)[:, heads - heads // hkv:, 7]
+    assert (torch.isnan(out) if what != what else out == what).all()
+
+
 def test_blocks_that_are_none_stand_for_zeros():
     step = Step([(300, [[0], [0, 1]]), (100, [[], [2]])], 8, 2, 64, 10)
     step.cache.bt[0, 1], step.cache.bt[0, 3], step.cache.bt[1, 0] = -1, step.cache.n_blocks, 2 ** 30
