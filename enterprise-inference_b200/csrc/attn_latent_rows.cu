@@ -156,13 +156,14 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
         const int k = tok + (x < halves ? x * 64 : 0);
-        row[x] = __shfl_sync(0xffffffffu, bt[k / p.block_size], 0) * p.block_size + k % p.block_size;
+        const int blk = __shfl_sync(0xffffffffu, bt[k / p.block_size], 0);
+        row[x] = blk < 0 ? -64 : blk * p.block_size + k % p.block_size;   // (in front of the cache: zeros)
       }
       auto load = [&](unsigned char* dst, int c, uint64_t* bar) {
         for (int x = 0; x < halves; ++x) tma_load_2d(dst + x * 8192, &map, c * 64, row[x], bar);
       };
       auto tail = [&](unsigned char* dst, uint64_t* bar) {
-        for (int x = 0; x < halves; ++x) copy_tail_start(dst + x * 8192, p.kc + (int64_t)row[x] * p.krow + boxes * 64, p.krow, p.krow & 63);
+        for (int x = 0; x < halves; ++x) copy_tail_start(dst + x * 8192, p.kc + boxes * 64, row[x], p.krow, p.krow & 63);
         copy_tail_end();
         if (issuer) mbar_arrive(bar);
       };

@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
       for (int i = w.tile_lo; i < w.tile_hi && !(stop = mbar_wait.stop()); ++i) {
         const int tok = i * kLtKeys;
         const int blk = __shfl_sync(0xffffffffu, __ldg(bt + tok / p.block_size), 0);
-        const int row = blk * p.block_size + tok % p.block_size;
+        const int row = blk < 0 ? -kLtKeys : blk * p.block_size + tok % p.block_size;   // (in front of the cache: zeros)
         uint64_t* tail = nullptr;   // what the last chunk's own copies arrive at
         auto load = [&](unsigned char* ring, uint64_t* bar, int n, auto chunk) {   // chunks chunk(0) .. chunk(n - 1); the last one may be no whole one
           const int by_box = chunk(n - 1) < boxes ? n : n - 1;
@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
             for (int c = 0; c < by_box; ++c) tma_load_2d(ring + c * kLtChunk, &map, chunk(c) * 64, row, bar);
           }
           __syncwarp();
-          if (by_box < n) copy_tail_start(ring + by_box * kLtChunk, p.kc + (int64_t)row * p.krow + boxes * 64, p.krow, p.krow & 63), tail = bar;
+          if (by_box < n) copy_tail_start(ring + by_box * kLtChunk, p.kc + boxes * 64, row, p.krow, p.krow & 63), tail = bar;
         };
         if (rest > 0) {
           mbar_wait(rest_free + sl, sl_ph);

@@ -69,13 +69,16 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, i
 }
 // The columns at the end of cached rows that are no whole box of 64, of 64 rows, by a warp: where a box would have put them (128-byte swizzle, `dst` at a multiple of 1024).  Boxes that
 // reach past a row's end are not used where a map declares more rows than the memory behind it has: steps with such rows (64 bytes under a box of 128) ended in illegal addresses
-// three times, each behind hundreds of other calls, and nothing else of them was out of range.  `src`: the first row's; ld and cols multiples of 16
-__device__ __forceinline__ void copy_tail_start(unsigned char* dst, const __nv_bfloat16* src, int ld, int cols) {
+// three times, each behind hundreds of other calls, and nothing else of them was out of range.  `row`: the first one, below 0 where a block is none: zeros, as boxes have them; ld and cols
+// multiples of 16, `from` the first row's columns
+__device__ __forceinline__ void copy_tail_start(unsigned char* dst, const __nv_bfloat16* from, int row, int ld, int cols) {
+  const __nv_bfloat16* const src = from + (int64_t)max(row, 0) * ld;
+  const int bytes = row < 0 ? 0 : 16;
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const int r = (threadIdx.x & 31) + 32 * h;
     for (int x = 0; x < cols >> 3; ++x)
-      asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst + r * 128 + ((x ^ (r & 7)) << 4))), "l"(src + (int64_t)r * ld + x * 8) : "memory");
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst + r * 128 + ((x ^ (r & 7)) << 4))), "l"(src + (int64_t)r * ld + x * 8), "r"(bytes) : "memory");
   }
 }
 // behind copy_tail_start: the columns are there for the tensor cores, once the warp has gone on from here

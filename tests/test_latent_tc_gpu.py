@@ -223,6 +223,36 @@ def test_latent_runs_of_every_count_of_chunks(rank, rd, splits):
     assert (got - want).abs().max() < 2.0 ** -8 * kc.float().abs().max() + 2.0 ** -9 * want.abs().max()
 
 
+# A block id below 0 inside a context stands for rows of zeros, in whole chunks of a key row and in a last one that is none: rows by themselves (one CTA, clusters), runs,
+# values that reach into the last chunk.
+@pytest.mark.parametrize("heads,rank,rd", [(16, 256, 32), (16, 256, 64), (16, 272, 16), (5, 80, 48), (1, 16, 16), (4, 304, 16)])
+@pytest.mark.parametrize("runs", [[1] * 3, [1] * 90, [150, 3, 40]])
+def test_latent_blocks_that_are_none_stand_for_zeros(heads, rank, rd, runs):
+    lib, check = pkg("_abi").lib(), pkg("_abi").check
+    bs, krow, S = 64, rank + rd, len(runs)
+    g = torch.Generator().manual_seed(krow + S)
+    seq, ctx = [s for s, n in enumerate(runs) for _ in range(n)], [90 + (37 * s) % 200 + i for s, n in enumerate(runs) for i in range(n)]
+    T, nb, scale = len(seq), 7, 0.6 / krow ** 0.5
+    kc = torch.randn(9, 1, bs, krow, generator=g).to(torch.bfloat16)
+    bt = torch.stack([torch.randperm(9, generator=g)[:nb] for _ in runs]).to(torch.int32)
+    bt[0::2, 0], bt[1::2, 1], bt[0::3, 2] = -1, -(1 << 31), -5
+    q = torch.randn(T, heads, krow, generator=g).to(torch.bfloat16).float()
+    seen = [torch.cat([kc[b, 0] if b >= 0 else torch.zeros(bs, krow, dtype=torch.bfloat16) for b in row.tolist()]).double() for row in bt]
+    want = torch.stack([_oracle(q[t].double(), seen[seq[t]], ctx[t], rank, scale, None, 0) for t in range(T)])
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)   # noqa: E731
+    kd, bd, qd, sq, cx = kc.to(DEV), bt.to(DEV), q.to(DEV), i32(seq), i32(ctx)
+    ws = torch.zeros(int(lib.b200_paged_attn_anydim_workspace_bytes(T)), dtype=torch.uint8, device=DEV)
+    out = torch.full((T, heads, rank), float("nan"), dtype=torch.bfloat16, device=DEV)
+    check(lib.b200_latent_attn(qd.data_ptr(), kd.data_ptr(), bd.data_ptr(), nb, sq.data_ptr(), cx.data_ptr(), out.data_ptr(), T, heads, krow, rank, bs, scale, None,
+                               ws.data_ptr(), 1, None, None))
+    torch.cuda.synchronize()
+    got = out.double().cpu()
+    assert torch.isfinite(got).all()
+    # (as above)
+    assert (got - want).norm() / want.norm() < 2.0 ** -8
+    assert (got - want).abs().max() < 2.0 ** -8 * kc.float().abs().max() + 2.0 ** -9 * want.abs().max()
+
+
 def test_latent_splits_of_halves_whose_maxima_part():
     """The halves of the value columns add a score's terms in different orders.  Here one of them follows the running maximum (17 units, just over the limit of
     2^8) and the other does not (16, what fp32 leaves of 2^24 + 17 - 2^24): the split's sums have to mean the same in both.  All values are 1."""
