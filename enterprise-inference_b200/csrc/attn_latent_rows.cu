@@ -143,7 +143,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
 
   if (warp == 0) {
     // ===== TMA: per tile the value columns two chunks a slot, then the other chunks; 64 keys a box, those past the context's last box left out.  A last chunk that is no whole one
-    // comes by the warp's own copies (tc.cuh), which end behind the tile's other loads =====
+    // comes by the warp's own copies (tc.cuh) =====
     const bool issuer = elect_one();
     if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     const int32_t* bt = p.block_table + (int64_t)(p.row_to_seq ? p.row_to_seq[t] : t) * p.bt_stride;
@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
       };
       auto tail = [&](unsigned char* dst, uint64_t* bar) {
         for (int x = 0; x < halves; ++x) copy_tail_start(dst + x * 8192, p.kc + boxes * 64, row[x], p.krow, p.krow & 63);
-        copy_tail_end();
+        copy_tail_arrive(bar);
         if (issuer) mbar_arrive(bar);
       };
       for (int j = 0; j < p.vpairs; ++j) {
@@ -205,6 +205,11 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
     const int nt = __shfl_sync(0xffffffffu, tile_hi - tile_lo, 0), keys = __shfl_sync(0xffffffffu, ctx - first - tile_lo * kLrKeys, 0);
     int st = 0, rs = 0, pv_st = 0;
     uint32_t st_ph = 0, rs_ph = 0;
+    auto arrived = [&](uint64_t* bar, uint32_t ph, int c, int n) {   // chunks c .. c + n - 1
+      wait(bar, ph);
+      if (c + n > p.krow >> 6) fence_async_smem();   // the last one's copied columns
+      fence_after();
+    };
     auto chunk = [&](uint32_t d, uint64_t da, int c) {
       const uint64_t dq = desc_q + (uint64_t)((c * kLrQChunk) >> 4);
       const int ks = min(4, ksteps - 4 * c);
@@ -219,14 +224,12 @@ __global__ void __launch_bounds__(kLrThreads, 1) latent_rows_kernel(const __grid
     auto scores = [&](int n) {
       const uint32_t d = tm + (n & 1) * kLrPairs;
       for (int j = 0; j < p.vpairs; ++j) {
-        wait(full + st, st_ph);
-        fence_after();
+        arrived(full + st, st_ph, 2 * j, min(2, vchunks - 2 * j));
         for (int c = 0; c < min(2, vchunks - 2 * j); ++c) chunk(d, desc_k + (uint64_t)(((st * 2 + c) * kLrChunk) >> 4), 2 * j + c);
         if (++st == p.slots) st = 0, st_ph ^= 1;
       }
       for (int c = 0; c < p.rest; ++c) {
-        wait(rest_full + rs, rs_ph);
-        fence_after();
+        arrived(rest_full + rs, rs_ph, vchunks + c, 1);
         chunk(d, desc_r + (uint64_t)((rs * kLrChunk) >> 4), vchunks + c);
         commit(one, rest_empty + rs);
         if (++rs == p.rest_slots) rs = 0, rs_ph ^= 1;

@@ -164,7 +164,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
 
   if (warp == 0) {
     // ===== TMA: per tile the chunks outside the half first (the scores take them first), then the half's own.  A last chunk that is no whole one comes by the warp's own copies
-    // (tc.cuh), whose end is waited for behind the tile's other loads =====
+    // (tc.cuh) =====
     const bool issuer = elect_one();
     if (issuer) asm volatile("prefetch.tensormap [%0];" ::"l"(&map) : "memory");
     const int boxes = p.krow >> 6;   // whole chunks
@@ -180,7 +180,6 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
         const int tok = i * kLtKeys;
         const int blk = __shfl_sync(0xffffffffu, __ldg(bt + tok / p.block_size), 0);
         const int row = blk < 0 ? -kLtKeys : blk * p.block_size + tok % p.block_size;   // (in front of the cache: zeros)
-        uint64_t* tail = nullptr;   // what the last chunk's own copies arrive at
         auto load = [&](unsigned char* ring, uint64_t* bar, int n, auto chunk) {   // chunks chunk(0) .. chunk(n - 1); the last one may be no whole one
           const int by_box = chunk(n - 1) < boxes ? n : n - 1;
           if (issuer) {
@@ -189,7 +188,11 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
             for (int c = 0; c < by_box; ++c) tma_load_2d(ring + c * kLtChunk, &map, chunk(c) * 64, row, bar);
           }
           __syncwarp();
-          if (by_box < n) copy_tail_start(ring + by_box * kLtChunk, p.kc + boxes * 64, row, p.krow, p.krow & 63), tail = bar;
+          if (by_box < n) {
+            copy_tail_start(ring + by_box * kLtChunk, p.kc + boxes * 64, row, p.krow, p.krow & 63);
+            copy_tail_arrive(bar);
+            if (issuer) mbar_arrive(bar);
+          }
         };
         if (rest > 0) {
           mbar_wait(rest_free + sl, sl_ph);
@@ -198,10 +201,6 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
         }
         mbar_wait(own_free + st, st_ph);
         load(own_ring + st * own * kLtChunk, own_full + st, own, [&](int c) { return first + c; });
-        if (tail) {
-          copy_tail_end();
-          if (issuer) mbar_arrive(tail);
-        }
         __syncwarp();
         if (++st == p.own_stages) st = 0, st_ph ^= 1;
       }
@@ -242,6 +241,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
         const uint32_t d = tm + kTmS + (m & 1) * kLtKeys;
         if constexpr (R > 0) {
           mbar_wait(rest_full + sl, sl_ph);
+          if (rest_tail < 4) fence_async_smem();   // (copied columns)
           fence_after();
           const uint64_t dr = desc_rest + (uint64_t)((sl * rest * kLtChunk) >> 4);
           auto step = [&](int j) {
@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(kLtThreads, 1) latent_attn_tc_kernel(const __g
           if (++sl == p.rest_stages) sl = 0, sl_ph ^= 1;
         }
         mbar_wait(own_full + st, st_ph);
+        if (own_tail < 4) fence_async_smem();
         fence_after();
         const uint64_t dk = desc_own + (uint64_t)((st * own * kLtChunk) >> 4);
         auto step = [&](int j) { mma_ts(one, d, tm + kTmQ + j * 8, dk + (uint64_t)(((j >> 2) * kLtChunk >> 4) + (j & 3) * 2), id_s, R > 0 || j ? 1u : 0u); };
