@@ -4,8 +4,9 @@
 // blocks: a warp takes 2 048 neighbouring logits, all in registers at once, and leaves their largest, m, and the sum of exp(x - m).  No barriers, nothing is selected.
 // merge: a cluster takes a sequence.  One of its CTAs joins the blocks' sums; a number that more than K blocks' largest scores reach bounds the K-th score from below, and only
 // the blocks that reach it, little more than K, are read again.  Where a sequence has less than kBlocksEach blocks for each of the K, their largest entries may lie far behind the K-th: groups of
-// eight entries give the limit then; and a list that is longer than K + kSpare is cut by a limit of its own entries (ranks take as long as the square of their number).  50 x 3 rows of 26 316
-// entries, 20 to take, 18 us, 37 to 296 without the two; 8 rows of 1 024, 64 to take, 21 and 134; they cost the others 0.3.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
+// eight entries give the limit then; and a list that is longer than K + kSpare is cut by a limit of its own entries (ranks take as long as the square of their number), one that has no room for
+// all by a limit of all: 40 000 entries near the limit in 4 rows of 32 768, 16 to take, 120 us, 88 with a limit of the 1 024 that found room, in 16 rows of 16 384 186 and 815.  50 x 3 rows of 26 316
+// entries, 20 to take, 17 us, 37 to 296 without the two; 8 rows of 1 024, 64 to take, 18 and 134; they cost the others 0.3.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
 // is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in 64 bits (half of the entries
 // to a CTA) and the CTA picks again.  Entries of one row never need it.
 // Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.4 us, 32 sequences of up to 5 rows of 32 000 13.1, 512 rows of 128 256 (131 MB) 34.5,
@@ -228,9 +229,9 @@ __device__ __noinline__ double row_base(const float* scores, int r, double m, do
 constexpr int kSteps = 512;
 constexpr uint32_t kFirstStep = __builtin_bit_cast(uint32_t, 0x1p-23f) >> 19;
 __device__ __forceinline__ int at_step(int k) { return k + k / (kSteps / 32); }   // (no bank conflicts)
-__device__ __forceinline__ void count_step(int* steps, float most, float top) {
+__device__ __forceinline__ void count_step(int* steps, float most, float top, int n = 1) {
   const uint32_t far = __float_as_uint(most - top) >> 19;   // (by a sixteenth of a power of two each)
-  atomicAdd(&steps[at_step(far < kFirstStep ? 0 : min(far - kFirstStep + 1, kSteps - 1u))], 1);
+  atomicAdd(&steps[at_step(far < kFirstStep ? 0 : min(far - kFirstStep + 1, kSteps - 1u))], n);
 }
 __device__ __forceinline__ float far_end(const int* steps, float most, int take) {
   const int lane = threadIdx.x & 31;
@@ -255,7 +256,8 @@ __device__ __forceinline__ float far_end(const int* steps, float most, int take)
   const float end = most - __uint_as_float((kFirstStep + step) << 19);
   return end - (fabsf(most) + fabsf(end)) * 0x1p-22f;   // (distances are rounded)
 }
-// Where there are few blocks for those to take: the limit of the largest entries of groups of eight
+// Limits from the blocks' entries: where there are few blocks for those to take, of the largest entries of groups of eight; where more entries reach the limit than the list holds, of all of
+// them (those that found room differ from call to call, and with a limit by them what has to be added up in 64 bits)
 struct Listed {   // blocks whose scores reach `least`
   const __nv_bfloat16* logits;
   const float2* stats;   // of the sequence
@@ -265,7 +267,8 @@ struct Listed {   // blocks whose scores reach `least`
   int n, per_row, vocab;
   double least;
 };
-__device__ __noinline__ float limit_of_groups(const Listed& b, const double* known, int* steps, float* warp_tops, int take) {
+template <bool kAll>
+__device__ __noinline__ float limit_of_entries(const Listed& b, const double* known, int* steps, float* warp_tops, int take) {
   constexpr int kWarps = kMergeThreads / 32;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if (tid < kSteps) steps[at_step(tid)] = 0;
@@ -286,6 +289,38 @@ __device__ __noinline__ float limit_of_groups(const Listed& b, const double* kno
     if (!(base > -INFINITY)) continue;
     uint4 v[kBlockGroups];
     load_block(b.logits + (int64_t)r * b.ld, k - r * b.per_row, b.vocab, v);
+    if constexpr (kAll) {
+      // neighbours alike, of which there may be thousands, are counted together
+      float last = -INFINITY;
+      int n = 0;
+      auto count = [&] {
+        const double score = base + (double)last;
+        const float top = __double2float_rd(score);
+        if (n > 0 && score >= b.least && top > -INFINITY) count_step(steps, most, top, n);
+      };
+#pragma unroll 1
+      for (int j = 0; j < kBlockGroups; ++j) {
+        uint4 w = v[0];
+#pragma unroll
+        for (int i = 1; i < kBlockGroups; ++i)
+          if (i == j) w = v[i];
+        if (!(base + (double)max8(w) >= b.least)) continue;
+        if (w.x == w.y && w.z == w.w && w.x == w.z && w.x == __funnelshift_l(w.x, w.x, 16)) {
+          if (bf16lo(w.x) != last) count(), last = bf16lo(w.x), n = 0;
+          n += 8;
+          continue;
+        }
+#pragma unroll 1
+        for (int q = 0; q < 8; ++q) {
+          const float x = bf16lo(w.x);
+          w.x = __funnelshift_r(w.x, w.y, 16), w.y = __funnelshift_r(w.y, w.z, 16), w.z = __funnelshift_r(w.z, w.w, 16), w.w >>= 16;
+          if (x != last) count(), last = x, n = 0;
+          ++n;
+        }
+      }
+      count();
+      continue;
+    }
 #pragma unroll
     for (int j = 0; j < kBlockGroups; ++j) {
       const double score = base + (double)max8(v[j]);
@@ -322,6 +357,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
   __shared__ int need[2 * kMergeList], blocks[kMergeList], n_need, n_list, n_blocks, seen_all, asked;
   __shared__ uint32_t asked_for[kMergeList / 32], exact_rows[kMergeList / 32];   // rows of the sequence that are in need, and that have been added up in 64 bits (of the first kMergeList)
   __shared__ Best limit;
+  __shared__ Listed reaching;
   asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");   // (before shared memory of the other CTA is written, it runs)
   pdl_wait();
   const cg::cluster_group cluster = cg::this_cluster();
@@ -454,12 +490,17 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
           if (lane == 0) f(x, before);
         }
       };
-      if (all_blocks < kBlocksEach * take || !(f64_of_ordered(at.score) > -INFINITY)) {
-        const Listed b = {logits + (int64_t)r0 * ld, mine, rows + r0, listed <= kMergeList ? blocks : nullptr, ld, listed <= kMergeList ? listed : all_blocks, per_row, vocab,
-                          f64_of_ordered(at.score) - margin};
-        at.score = max(at.score, ordered_f64((double)limit_of_groups(b, known, steps, warp_tops, take)));
+      // a limit by the entries of the blocks that reach this one
+      auto look = [&](auto limit_of_those) {
+        if (tid == 0)
+          reaching = {logits + (int64_t)r0 * ld, mine, rows + r0, listed <= kMergeList ? blocks : nullptr, ld, listed <= kMergeList ? listed : all_blocks, per_row, vocab,
+                      f64_of_ordered(at.score) - margin};
         __syncthreads();
-      }
+        const uint64_t reached = ordered_f64((double)limit_of_those(reaching, known, steps, warp_tops, take));
+        __syncthreads();
+        return reached;
+      };
+      if (all_blocks < kBlocksEach * take || !(f64_of_ordered(at.score) > -INFINITY)) at.score = max(at.score, look(limit_of_entries<false>));
       bool too_many = false, closer = false;
 #pragma unroll 1
       for (;;) {
@@ -488,9 +529,9 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
         __syncthreads();
         const int found = n_list;
         if (found <= take + kSpare) break;
-        if (!closer) {   // a limit by those that found room: ranks take as long as the square of their number
+        if (!closer) {   // a limit by these: ranks take as long as the square of their number
           closer = true;
-          const uint64_t reached = ordered_f64((double)limit_of_list(cand, min(found, kMergeList), steps, warp_tops, take));
+          const uint64_t reached = found > kMergeList ? look(limit_of_entries<true>) : ordered_f64((double)limit_of_list(cand, found, steps, warp_tops, take));
           if (reached > at.score) {
             at.score = reached;
             const Best x = cand[tid];

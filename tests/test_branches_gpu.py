@@ -457,6 +457,28 @@ def test_select_among_alike_rows_beside_rows_that_are_none():
     check_select(logits, torch.tensor([0.0, -1.0, 0.0, 0.0, -1.0, -1.0, NAN]), _starts(7), 100)
 
 
+@pytest.mark.parametrize("rows,blocks,take,second,first", [(4, 16, 16, 40000, 600), (4, 16, 16, 40000, 700), (4, 16, 16, 20000, 400), (8, 8, 16, 20000, 400), (8, 8, 16, 40000, 700),
+                                                           (4, 32, 8, 40000, 300), (4, 32, 8, 20000, 1000), (16, 8, 16, 20000, 200), (16, 8, 16, 40000, 1000)])
+def test_select_among_more_than_a_list_holds_has_the_same_bits_every_time(rows, blocks, take, second, first):
+    """One entry far in front, some hundreds a step behind it in few blocks, tens of thousands another step behind in all: a limit near the end depends on which of them are looked at, and
+    with it whether sums are wanted in 64 bits.  Scores next to zero, where fp32 shows the difference."""
+    g = torch.Generator().manual_seed(first + second)
+    V = blocks * 2048
+    x = (torch.randn(rows, V, generator=g) * 0.5 - 6).clamp(max=-3.0)
+    few = torch.randperm(rows * blocks, generator=g)[:take - 4]
+    x.view(-1)[torch.randperm(rows * V, generator=g)[:second]] = 2.0
+    places = (few[:, None] * 2048 + torch.arange(2048)).reshape(-1)
+    x.view(-1)[places[torch.randperm(len(places), generator=g)[:first]]] = 3.0
+    x[0, 5] = 11.0
+    logits = x.to(BF)
+    scores = (logits.double().logsumexp(1) - 3.0 + 0.01 * torch.arange(1, rows + 1)).float()
+    check_select(logits, scores, _starts(rows), take)
+    dev = _dev(logits, scores, _starts(rows))
+    want = select(*dev, take)
+    for _ in range(40):
+        assert all(torch.equal(a, b) for a, b in zip(select(*dev, take), want))
+
+
 def test_select_between_many_rows_that_are_near():
     """More rows than are kept at hand, all of them in need of 64 bits; in two sequences."""
     g = torch.Generator().manual_seed(78)
