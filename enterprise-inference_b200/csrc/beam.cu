@@ -34,7 +34,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 constexpr double kNear = 2e-6;
 
 struct RowStat {
-  double base, near;   // scores[r] - the log-sum (-inf: no candidates), and how far it may be off
+  double base, near;   // scores[r] - the log-sum (-inf: no candidates), and how far it may be off (below 0: as far, and asked for in 64 bits)
 };
 
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {
@@ -371,7 +371,7 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
     return warp_max(m);
   };
   auto base_of = [&](int r) { return r - r0 < kKnownRows ? known[r - r0] : rows[r].base; };
-  auto near_of = [&](int r) { return r - r0 >= kMergeList ? rows[r].near : exact_rows[(r - r0) >> 5] >> ((r - r0) & 31) & 1 ? 0.0 : kNear; };
+  auto near_of = [&](int r) { return r - r0 >= kMergeList ? fabs(rows[r].near) : exact_rows[(r - r0) >> 5] >> ((r - r0) & 31) & 1 ? 0.0 : kNear; };
   if (cta == 0) {
     if (tid < kMergeList / 32) exact_rows[tid] = 0;
     // log-sums of the rows; the first kHeld x 32 blocks of a row stay in registers between the maximum and the sum
@@ -572,7 +572,11 @@ beam_merge_kernel(const __nv_bfloat16* __restrict__ logits, int64_t ld, const fl
               const int r = side ? rb : ra;
               if (!((side ? nb : na) > 0.0)) continue;
               const uint32_t bit = 1u << ((r - r0) & 31);
-              if (r - r0 < kMergeList && (atomicOr(&asked_for[(r - r0) >> 5], bit) & bit)) continue;
+              if (r - r0 < kMergeList) {
+                if (atomicOr(&asked_for[(r - r0) >> 5], bit) & bit) continue;
+              } else if (__longlong_as_double((long long)atomicExch(reinterpret_cast<unsigned long long*>(&rows[r].near), (unsigned long long)__double_as_longlong(-kNear))) < 0.0) {
+                continue;
+              }
               need[atomicAdd(&n_need, 1)] = r;   // (two for each of n entries at most)
             }
           }
