@@ -13,7 +13,7 @@ import torch
 own = False
 BF16, F32, F64, I32, I64 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.int64
 DIM = 128
-_kept = {}   # the library and the workspace that a program keeps
+_kept = {}   # the library that a program keeps
 
 
 def listed():
@@ -359,10 +359,12 @@ def _library():
     return _kept["lib"], _kept["check"], _kept["ptr"]
 
 
-def _workspace(size):
-    if size > _kept.get("size", 0):
-        _kept.update(ws=torch.zeros(size, dtype=torch.uint8, device="cuda"), size=size)
-    return _kept["ws"].data_ptr(), _kept["size"]
+def _workspace(st, stream, size):
+    """One for each state and stream: passes that may run at the same time do not share one, and one that a captured pass writes to is there as long as its state."""
+    kept = st.setdefault("workspaces", {})
+    if stream not in kept:
+        kept[stream] = torch.empty(size, dtype=torch.uint8, device="cuda")
+    return kept[stream].data_ptr(), size
 
 
 def _own(st):
@@ -371,12 +373,12 @@ def _own(st):
     kind = case["kind"]
     if kind in ("tree", "beams"):
         hq, hkv = case["heads"], case["kv"]
-        ws = _workspace(lib.b200_paged_attn_tree_workspace_bytes(n, hq, hkv))
+        ws = _workspace(st, stream, lib.b200_paged_attn_tree_workspace_bytes(n, hq, hkv))
         check(lib.b200_paged_attn_tree(ptr(st.q), hq * DIM, ptr(st.k), ptr(st.v), st.n_blocks, ptr(st.bt), st.bt.shape[1], ptr(st.row_seq), ptr(st.ctx), ptr(st.masks),
                                        st.words, ptr(st.out), hq * DIM, n, hq, hkv, case["block"], st.scale, *ws, stream))
         return st.out
     if kind == "select":
-        ws = _workspace(lib.b200_beam_select_workspace_bytes(n, case["vocab"], case["take"]))
+        ws = _workspace(st, stream, lib.b200_beam_select_workspace_bytes(n, case["vocab"], case["take"]))
         check(lib.b200_beam_select(ptr(st.logits), case["vocab"], ptr(st.scores), ptr(st.starts), case["seqs"], n, case["vocab"], case["take"], ptr(st.rows),
                                    ptr(st.tokens), ptr(st.out), *ws, stream))
         return st.rows, st.tokens, st.out
