@@ -1,5 +1,8 @@
 """Several continuations of a sequence: attention by a mask per row, selection over beams, the walk through a checked tree and moves of cached rows, operator by operator
 and together, against branches_util's plain forms in 64 bits."""
+import importlib.util
+import os
+
 import pytest
 import torch
 
@@ -798,3 +801,32 @@ def test_a_beam_search_over_states():
         states = U.moved(states, src.cpu(), dst.cpu(), starts, W)
         assert torch.equal(dev.cpu(), states)
         d_scores, scores = out.flatten(), out.flatten().cpu()
+
+
+def test_captured_passes_over_the_cases_keep_their_workspaces():
+    """A pass that a graph has captured writes to memory that is its own, whatever passes over larger cases come behind it."""
+    spec = importlib.util.spec_from_file_location("more_operators", os.path.join(os.path.dirname(__file__), "..", "perf", "more_operators.py"))
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    m.own = True
+    cases = [{"kind": "tree", "seqs": 1, "nodes": 4, "even": True, "ctx": 300, "heads": 8, "kv": 2, "block": 16},
+             {"kind": "select", "seqs": 2, "rows": 3, "even": True, "vocab": 5000, "take": 4}]
+    states = [m.prepare(c, 1) for c in cases]
+    want = [[t.clone() for t in (r if isinstance(r, tuple) else (r,))] for r in map(m.run, states)]
+    graphs = []
+    for st in states:
+        torch.cuda.synchronize()
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1], stream=torch.cuda.Stream()):
+            m.run(st)
+    for c in ({"kind": "tree", "seqs": 8, "nodes": 64, "even": True, "ctx": 600, "heads": 32, "kv": 8, "block": 128}, {"kind": "select", "seqs": 20, "rows": 8, "even": True, "vocab": 128256, "take": 16}):
+        m.run(m.prepare(c, 2))
+    held = [torch.full((n,), 7, dtype=torch.uint8, device=DEV) for n in (1 << 10, 1 << 14, 1 << 18, 1 << 20, 3 << 20, 9 << 20, 30 << 20, 50 << 20) for _ in range(4)]
+    for st, graph, outs in zip(states, graphs, want):
+        for t in (st.out, *(st[k] for k in ("rows", "tokens") if k in st)):
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        got = (st.rows, st.tokens, st.out) if "rows" in st else (st.out,)
+        assert all(torch.equal(a, b) for a, b in zip(got, outs))
+    assert all((t == 7).all() for t in held)
