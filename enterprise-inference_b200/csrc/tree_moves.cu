@@ -213,6 +213,7 @@ extern "C" int b200_cache_move(void* cache_a, void* cache_b, int32_t n_layers, i
   B200_REQUIRE(plane < ((__int128)1 << 62), B200_ERR_INVALID, "cache_move: a layer of more bytes than there are");
   B200_REQUIRE(n_layers == 1 || layer_stride >= (int64_t)plane, B200_ERR_INVALID, "cache_move: layers of %lld bytes, %lld apart", (long long)plane, (long long)layer_stride);
   if (n_groups == 0 || max_group == 0) return B200_OK;
+  if (cache_b == cache_a) cache_b = nullptr;   // (values that are the keys: moved once, by one CTA a piece, or what is read might have been written already)
   const uint64_t all = reinterpret_cast<uintptr_t>(cache_a) | reinterpret_cast<uintptr_t>(cache_b) | (uint64_t)row_bytes | (n_layers > 1 ? (uint64_t)layer_stride : 0);
   const int vec = all % 16 == 0 ? 16 : all % 4 == 0 ? 4 : 1;
   MoveParams p = {static_cast<unsigned char*>(cache_a), static_cast<unsigned char*>(cache_b), layer_stride, row_bytes, n_blocks * block_size, src_slots, dst_slots, group_starts,

@@ -363,7 +363,7 @@ B200_API int b200_verify_drafts(const void* target_logits, int64_t ldt, const vo
  * b200_cache_move: rows of caches, whole blocks or states to new places.  cache_a and cache_b (or NULL) each are n_layers times, layer_stride bytes apart,
  * [n_blocks][heads][block_size][row_bytes]; slot = block * block_size + place, as in slot_mapping.  The moves of group g, src_slots[i] -> dst_slots[i] for group_starts[g] <= i <
  * group_starts[g+1], happen at once in all layers, heads and both caches: what is read is what stood there before the call, so beams may change places.  A move with a slot outside the
- * cache is none.  Destinations of one call differ, and no group reads what another one writes.  Groups have at most max_group moves (a HOST bound up to 1024; those behind
+ * cache is none.  cache_b may be cache_a (values that are the keys).  Destinations of one call differ, and no group reads what another one writes.  Groups have at most max_group moves (a HOST bound up to 1024; those behind
  * it are not made).  States, or blocks as a whole: heads = block_size = 1 and row_bytes their size.  Fastest where addresses, strides and row_bytes are multiples of 16. */
 B200_API int64_t b200_paged_attn_tree_workspace_bytes(int32_t n_tokens, int32_t n_q_heads, int32_t n_kv_heads);
 B200_API int b200_paged_attn_tree(const void* q, int64_t ldq, const void* k_cache_layer, const void* v_cache_layer, int64_t n_blocks,

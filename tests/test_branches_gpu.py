@@ -697,6 +697,19 @@ def test_moves_of_large_states(sizes, width):
     assert torch.equal(da.cpu(), a) and torch.equal(db.cpu(), b)
 
 
+def test_moves_of_keys_that_are_their_values():
+    """The same cache given twice: rows that change places do so once."""
+    g = torch.Generator().manual_seed(8)
+    a = torch.randint(0, 99, (4, 64, 1, 64, 576), generator=g).to(BF)
+    slots = torch.randperm(64 * 64, generator=g)[:2000]
+    src, dst, starts = slots.to(I32), slots.view(-1, 2).flip(1).reshape(-1).to(I32), _starts(*[40] * 50)   # pairs change places
+    da, ds, dd, st = _dev(a, src, dst, starts)
+    want = U.moved(a, src, dst, starts, 40)
+    for i in range(4):
+        move(da, da, ds, dd, st, 40)
+        assert torch.equal(da.cpu(), want if i % 2 == 0 else a)
+
+
 def test_walk_and_moves_captured_with_another_pair():
     """Two graphs on streams of their own, replayed with other choices of the target at the same addresses."""
     lib, check = _lib()
