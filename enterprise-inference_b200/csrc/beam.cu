@@ -9,7 +9,7 @@
 // entries, 20 to take, 17 us, 37 to 296 without the two; 8 rows of 1 024, 64 to take, 18 and 134; they cost the others 0.3.  (With a selection of its own in every slice of 16 384 logits the first kernel had twice the instructions.)  Order
 // is decided in 64 bits: sums of fp32 exponentials are good to kNear, so where two rows' candidates are nearer to each other than that, the cluster adds up those rows in 64 bits (half of the entries
 // to a CTA) and the CTA picks again.  Entries of one row never need it.
-// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.4 us, 32 sequences of up to 5 rows of 32 000 13.1, 512 rows of 128 256 (131 MB) 34.5,
+// Bound by the bytes of the logits, and where these are few by latency: 4 rows of 128 256 entries 10.2 us, 32 sequences of up to 5 rows of 32 000 12.9, 512 rows of 128 256 (131 MB) 33.8,
 // of which the merge takes some 6; 66 where one sequence has two rows that are near.  Logits through shared memory by asynchronous copies, two or three blocks a warp ahead, are no
 // faster (39 to 41 us against 38 then): what is left beside the copy rate's 20 us is the first kernel's start and end.
 #include <cooperative_groups.h>
